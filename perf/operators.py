@@ -236,11 +236,11 @@ def _signed(code, base):
 
 
 def _dither(n, seed, device):
-    x = torch.arange(n, dtype=torch.int64, device=device) * 0x9E3779B1 + seed & 0xFFFFFFFF
+    x = torch.arange(-(-n // 2), dtype=torch.int64, device=device) * 0x9E3779B1 + seed & 0xFFFFFFFF
     x = (x ^ x >> 15) * 0x6A09E667 & 0xFFFFFFFF
     x = (x ^ x >> 13) * 0xBB67AE85 & 0xFFFFFFFF
     x = x ^ x >> 16
-    return ((x & 0xFFFF) << 4 | 8).to(torch.int32), (x >> 16 << 4 | 8).to(torch.int32)
+    return (torch.stack([x & 0xFFFF, x >> 16], 1) << 4 | 8).view(-1)[:n].to(torch.int32)
 
 
 def _round8(x, dither, most, least):
@@ -320,9 +320,9 @@ def _plain_adamw_one(st, i):
     p.copy_(p * (1 - h["lr"] * h["weight_decay"]) - m / denom * (h["lr"] / (1 - h["beta1"] ** h["step"])))
     st["p16"][i].copy_(p)
     if bits == 8:
-        dm, dv = _dither(p.numel(), st["seeds"][i], p.device)
-        code, base = _round8(m.abs(), dm, 127, 0)
-        new = (code | torch.signbit(m).to(torch.uint8) * 128, base, *_round8(v, dv, 255, 1))
+        dither = _dither(p.numel(), st["seeds"][i], p.device)
+        code, base = _round8(m.abs(), dither, 127, 0)
+        new = (code | torch.signbit(m).to(torch.uint8) * 128, base, *_round8(v, dither, 255, 1))
     else:
         new = m, v
     return [old.copy_(x) for old, x in zip(moments, new)]
@@ -403,16 +403,17 @@ def _held(x, noise, most, least):
 
 
 def _noise(n, seed, device):
-    """The two halves of the hash of each position, in arithmetic modulo 2^32 on signed words."""
+    """Half of the hash of each pair of positions, in arithmetic modulo 2^32 on signed words."""
     def word(x):
         return torch.tensor(x - 2 ** 32 if x >= 2 ** 31 else x, dtype=torch.int32, device=device)
 
     def fold(x, k):
         return x ^ (x >> k & (1 << 32 - k) - 1)
 
-    x = torch.arange(n, device=device).to(torch.int32) * word(0x9E3779B1) + word(seed)
-    x = fold(fold(fold(x, 15) * word(0x6A09E667), 13) * word(0xBB67AE85), 16).to(torch.int64)
-    return x & 0xFFFF, x >> 16 & 0xFFFF
+    at = torch.arange(n, device=device)
+    x = (at >> 1).to(torch.int32) * word(0x9E3779B1) + word(seed)
+    x = fold(fold(fold(x, 15) * word(0x6A09E667), 13) * word(0xBB67AE85), 16)
+    return (x >> (at & 1).to(torch.int32) * 16).to(torch.int64) & 0xFFFF
 
 
 def _exact_adamw(st):
@@ -434,9 +435,9 @@ def _exact_adamw(st):
         p16.copy_(p)
         del mean, root, g
         if bits == 8:
-            nm, nv = _noise(n, st["seeds"][i], p.device)
-            m.copy_(torch.copysign(_held(m.abs(), nm, 127, 0), m))
-            v.copy_(_held(v.contiguous(), nv, 255, 1))
+            noise = _noise(n, st["seeds"][i], p.device)
+            m.copy_(torch.copysign(_held(m.abs(), noise, 127, 0), m))
+            v.copy_(_held(v.contiguous(), noise, 255, 1))
     return out
 
 
