@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import ref
+from .moments import decode
 
 _ACT_KINDS = {"gelu": 0, "gelu_new": 0, "gelu_tanh": 0, "relu": 1, "gelu_erf": 2}
 _FUSED_ACT_KINDS = {**_ACT_KINDS, "swiglu": 3}   # of the products with an activation in their epilogue
@@ -110,6 +111,20 @@ class RefOps(_EpilogueOps, _LaterOps):
         qkv.copy_(ref.rope(qkv, cs, S, nheads, d, backward))
         return qkv
 
+    def qk_norm_rope_fwd(self, qkv, wq, wk, cs, S, nq, nk, d, eps, keep=True):
+        """RMS norm of the nq query and nk key heads and their rotation by cs (None: none), in one pass.  keep: (a new tensor,
+        1 / rms of the heads); else (the result, which may be qkv itself, None)."""
+        out, rstd = ref.qk_norm_rope(qkv, wq, wk, cs, S, nq, nk, d, eps)
+        return out, rstd if keep else None
+
+    def qk_norm_rope_bwd(self, dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk):
+        """Its gradient, in place on the query and key heads of dqkv; the weights' are added to gwq and gwk."""
+        dx, dwq, dwk = ref.qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d)
+        dqkv[:, :(nq + nk) * d] = dx.to(dqkv.dtype)
+        gwq.add_(dwq.to(gwq.dtype))
+        gwk.add_(dwk.to(gwk.dtype))
+        return dqkv
+
     def attn_fwd(self, qkv, B, S, Hq, Hkv, D, causal=True, window=0):
         return ref.attention(qkv, B, S, Hq, Hkv, D, causal, window), None
 
@@ -143,12 +158,18 @@ class RefOps(_EpilogueOps, _LaterOps):
         return dx.to(x.dtype)
 
     # ---- embedding / loss / optimizer ------------------------------------------
-    def embedding_fwd(self, ids, table, pos_table=None, S=1, pos_offset=0):
-        return ref.embedding(ids, table, pos_table, S, pos_offset)
+    def embedding_fwd(self, ids, table, pos_table=None, S=1, pos_offset=0, scale=1.0):
+        return ref.embedding(ids, table, pos_table, S, pos_offset, scale)
 
-    def embedding_bwd(self, ids, dout, gtable, gpos=None, S=1, pos_offset=0):
+    def embedding_bwd(self, ids, dout, gtable, gpos=None, S=1, pos_offset=0, scale=1.0, by_token=False):
+        """Adds the gradients.  by_token (or a scale): the rows of a token are summed in their order and its row of the table
+        is written once."""
         ids = ids.reshape(-1)
-        gtable.index_add_(0, ids, dout.to(gtable.dtype))
+        if by_token or scale != 1.0:
+            sums = torch.zeros(gtable.shape, dtype=torch.promote_types(dout.dtype, torch.float32), device=dout.device)
+            gtable.copy_(gtable + sums.index_add_(0, ids, dout.to(sums.dtype)) * scale)
+        else:
+            gtable.index_add_(0, ids, dout.to(gtable.dtype))
         if gpos is not None:
             pos = torch.arange(ids.numel(), device=ids.device) % S + pos_offset
             gpos.index_add_(0, pos, dout.to(gpos.dtype))
@@ -173,6 +194,17 @@ class RefOps(_EpilogueOps, _LaterOps):
             p16.copy_(p)
         if zero_grad:
             g.zero_()
+
+    def adamw_step(self, p, moments, g, p16, *, step, seeds=None, **kw):
+        """AdamW over lists of tensors.  moments: a pair (m, v) in fp32 for each, or `Moments8` with a seed for each."""
+        steps = step if isinstance(step, (list, tuple)) else [step] * len(p)
+        for i, (x, mom, d, y) in enumerate(zip(p, moments, g, p16)):
+            ref.adamw_step(x, mom, d, step=steps[i], seed=0 if seeds is None else seeds[i], **kw)
+            if y is not None:
+                y.copy_(x)
+
+    def moment_values(self, moments, dtype=torch.float32):
+        return tuple(t.to(dtype) for t in decode(moments))
 
 
 def _decline(*args):
@@ -306,11 +338,22 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
     def patches(self, img, patch, kdim):
         return self.k.patches(img, patch, kdim)
 
-    def embedding_fwd(self, ids, table, pos_table=None, S=1, pos_offset=0):
+    def qk_norm_rope_fwd(self, qkv, wq, wk, cs, S, nq, nk, d, eps, keep=True):
+        return self.k.qk_norm_rope_fwd(qkv, wq, wk, cs, S, nq, nk, d, eps, keep)
+
+    def qk_norm_rope_bwd(self, dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk):
+        return self.k.qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk)
+
+    def embedding_fwd(self, ids, table, pos_table=None, S=1, pos_offset=0, scale=1.0):
+        if scale != 1.0:
+            return self.k.embedding_scaled(ids.reshape(-1), table, pos_table, S, pos_offset, scale)
         return self.k.embedding_fwd(ids.reshape(-1), table, pos_table, S, pos_offset)
 
-    def embedding_bwd(self, ids, dout, gtable, gpos=None, S=1, pos_offset=0):
-        self.k.embedding_bwd(ids.reshape(-1), dout, gtable, gpos, S, pos_offset)
+    def embedding_bwd(self, ids, dout, gtable, gpos=None, S=1, pos_offset=0, scale=1.0, by_token=False):
+        if by_token or scale != 1.0:
+            self.k.embedding_by_token(ids.reshape(-1), dout, gtable, gpos, S, pos_offset, scale)
+        else:
+            self.k.embedding_bwd(ids.reshape(-1), dout, gtable, gpos, S, pos_offset)
 
     def cross_entropy(self, logits, targets, grad_scale, want_grad=True):
         rows = self.k.cross_entropy(logits, targets, grad_scale, dlogits=logits if want_grad else None)
@@ -318,6 +361,12 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
 
     def adam_step(self, p, m, v, g, p16, **kw):
         self.k.adam_step(p, m, v, g, p16, **kw)
+
+    def adamw_step(self, p, moments, g, p16, **kw):
+        self.k.adamw_step(p, moments, g, p16, **kw)
+
+    def moment_values(self, moments, dtype=torch.float32):
+        return self.k.moment_values(moments, dtype)
 
 
 _cache: dict[str, object] = {}

@@ -12,6 +12,8 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from .moments import decode, dither, encode
+
 
 def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None) -> torch.Tensor:
     y = x @ w.t()
@@ -99,17 +101,52 @@ def attention(qkv: torch.Tensor, B: int, S: int, Hq: int, Hkv: int, D: int, caus
     return o.permute(0, 2, 1, 3).reshape(B * S, Hq * D).to(qkv.dtype)
 
 
+def _turn(x, cs, S: int, sign: float):
+    """Heads x [T, n, d] rotated by the angles of row t mod S of cs; None: as they are."""
+    if cs is None:
+        return x
+    h = x.shape[2] // 2
+    pos = torch.arange(x.shape[0], device=x.device) % S
+    cos, sin = cs[pos, None, :h], sign * cs[pos, None, h:]
+    return torch.cat([x[..., :h] * cos - x[..., h:] * sin, x[..., h:] * cos + x[..., :h] * sin], dim=-1)
+
+
+def _heads_and_weights(qkv, wq, wk, nq: int, nk: int, d: int):
+    x = qkv[:, : (nq + nk) * d].float().reshape(qkv.shape[0], nq + nk, d)
+    return x, torch.cat([wq.float().expand(nq, d), wk.float().expand(nk, d)])
+
+
+def qk_norm_rope(qkv, wq, wk, cs, S: int, nq: int, nk: int, d: int, eps: float):
+    """(qkv with query and key heads RMS-normalised and rotated, 1 / rms of these heads [T, nq + nk])."""
+    x, w = _heads_and_weights(qkv, wq, wk, nq, nk, d)
+    rstd = torch.rsqrt(x.pow(2).mean(-1) + eps)
+    y = _turn(x * rstd[..., None] * w, cs, S, 1.0).reshape(qkv.shape[0], (nq + nk) * d)
+    return torch.cat([y.to(qkv.dtype), qkv[:, (nq + nk) * d:]], dim=1), rstd
+
+
+def qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S: int, nq: int, nk: int, d: int):
+    """fp32 gradients of the query and key heads [T, (nq + nk) d], of wq and of wk."""
+    x, w = _heads_and_weights(qkv, wq, wk, nq, nk, d)
+    g = _turn(dqkv[:, : (nq + nk) * d].float().reshape(x.shape), cs, S, -1.0)
+    xh = x * rstd[..., None]
+    dw = (g * xh).sum(0)
+    dx = rstd[..., None] * (w * g - xh * (w * g * xh).mean(-1, keepdim=True))
+    return dx.reshape(qkv.shape[0], (nq + nk) * d), dw[:nq].sum(0), dw[nq:].sum(0)
+
+
 def cross_entropy_rows(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     return F.cross_entropy(logits.float(), targets, reduction="none")
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, pos_table: Optional[torch.Tensor] = None, S: int = 1,
-              pos_offset: int = 0) -> torch.Tensor:
+              pos_offset: int = 0, scale: float = 1.0) -> torch.Tensor:
     out = table[ids.reshape(-1)]
+    if scale != 1.0:
+        out = out.float() * scale
     if pos_table is not None:
         pos = torch.arange(ids.numel(), device=ids.device) % S + pos_offset
         out = out + pos_table[pos]
-    return out
+    return out.to(table.dtype)
 
 
 def adam_step(p, m, v, g, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0):
@@ -123,3 +160,17 @@ def adam_step(p, m, v, g, *, lr, beta1, beta2, eps, weight_decay, step, grad_sca
     bc2 = 1 - beta2 ** step
     denom = v.sqrt() / math.sqrt(bc2) + eps
     p.addcdiv_(m, denom, value=-lr / bc1)
+
+
+def adamw_step(p, moments, g, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0, seed=0):
+    """In-place AdamW (decoupled decay) on one fp32 tensor; moments: (m, v) in fp32, or `Moments8`, rounded with the dither of `seed`.
+    Every operation on the moments rounds by itself, as in the kernel."""
+    held = len(moments) == 4
+    m, v = decode(moments) if held else (t.reshape(-1) for t in moments)
+    x, g = p.view(-1), g.reshape(-1).float() * grad_scale
+    m = m * beta1 + g * (1 - beta1)
+    v = v * beta2 + g * (1 - beta2) * g
+    update = m / (v.sqrt() / math.sqrt(1 - beta2 ** step) + eps)
+    x.copy_(x * (1 - lr * weight_decay) - lr / (1 - beta1 ** step) * update)
+    for old, new in zip(moments, encode(m, v, dither(x.numel(), seed, x.device)) if held else (m, v)):
+        old.view(-1).copy_(new)

@@ -12,12 +12,15 @@ import ctypes
 import functools
 import math
 import os
+import struct
 import warnings
 from ctypes import c_float, c_int, c_long, c_void_p
 from pathlib import Path
 from typing import Optional
 
 import torch
+
+from .moments import BLOCK as MOMENT_BLOCK
 
 _LIB_PATH = Path(__file__).resolve().parents[1] / "_C" / "libzorse_sm100.so"
 _lib = None
@@ -48,6 +51,9 @@ _SIGNATURES = {
     "zb_cross_entropy": "ppppiilflp", "zb_adam": "ppppplfffffifiip",
     "zb_flash_fwd": "pppiiiiiiifipp", "zb_flash_fwd2": "pppiiiiiiifipp",
     "zb_flash_fwd4": "pppiiiiiiifipipip", "zb_flash_bwd3": "ppppppiiiiiiifpipip",
+    "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
+    "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
+    "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
 _CTYPES = {"p": c_void_p, "i": c_int, "l": c_long, "f": c_float}
 
@@ -185,6 +191,23 @@ def _bf16(t: torch.Tensor, name: str) -> None:
         raise TypeError(f"{name} must be a CUDA bf16 tensor, got {t.dtype} on {t.device}")
 
 
+def _on_current(t: torch.Tensor, name: str) -> None:
+    """A launch goes to the current device's stream: its operands have to be there."""
+    if not t.is_cuda or t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _workspace_size(fn, *sizes) -> int:
+    out = ctypes.c_long(0)
+    fn(*sizes, ctypes.addressof(out))
+    return out.value
+
+
 # --------------------------------------------------------------------------- GEMM
 @functools.lru_cache(maxsize=4096)
 def _gemm2_workspace(M: int, N: int, K: int, device: int) -> int:
@@ -301,6 +324,57 @@ def rope_(buf, cs, S: int, nheads: int, d: int, backward: bool = False):
     return buf
 
 
+def _qk_norm_operands(x, wq, wk, cs, S, nq, nk, d):
+    """Checks what forward and backward of the head norms have in common."""
+    _bf16(x, "qkv"); _bf16(wq, "wq"); _bf16(wk, "wk")
+    _on_current(x, "qkv")
+    T = x.shape[0]
+    _need(x.dim() == 2 and x.shape[1] == (nq + 2 * nk) * d and x.stride(1) == 1,
+          f"qkv is {tuple(x.shape)}, strides {x.stride()}: expected rows of ({nq} + 2 x {nk}) x {d}")
+    _need(wq.shape == (d,) and wk.shape == (d,) and wq.is_contiguous() and wk.is_contiguous(),
+          f"weights of {tuple(wq.shape)} and {tuple(wk.shape)} for heads of {d}")
+    if cs is not None:
+        _need(cs.dtype == torch.float32 and cs.device == x.device and cs.dim() == 2 and cs.is_contiguous() and cs.shape[1] == d
+              and cs.shape[0] >= min(S, T), f"table of {tuple(cs.shape)}, {cs.dtype}: expected fp32 [>= {min(S, T)}, {d}]")
+
+
+def qk_norm_rope_fwd(qkv, wq, wk, cs, S: int, nq: int, nk: int, d: int, eps: float, keep: bool = True):
+    """RMS norm of each of the nq query and nk key heads (weights wq / wk, [d]) of packed qkv [T, (nq + 2 nk) d], and the
+    rotate-half rotation by the row t mod S of cs ([S, d], None: no rotation).  keep: into a new tensor, which gets the
+    value heads too, with the heads' 1 / rms [T, nq + nk] for the backward pass; else in place, and None."""
+    _qk_norm_operands(qkv, wq, wk, cs, S, nq, nk, d)
+    T = qkv.shape[0]
+    out, rstd = qkv, None
+    if keep:
+        out = torch.empty(T, qkv.shape[1], dtype=qkv.dtype, device=qkv.device)
+        rstd = torch.empty(T, nq + nk, dtype=torch.float32, device=qkv.device)
+    _check(lib().zb_qk_norm_rope_fwd(_a(qkv), _a(out), _a(wq), _a(wk), _a(cs), _a(rstd), T, S, nq, nk, nk if keep else 0, d,
+                                     qkv.stride(0), out.stride(0), eps, _stream()), "qk_norm_rope_fwd")
+    return out, rstd
+
+
+def qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S: int, nq: int, nk: int, d: int, gwq, gwk):
+    """Gradient of `qk_norm_rope_fwd` in place on the query and key heads of dqkv (those of the values stay); qkv and rstd: the
+    raw projection and what the forward pass returned.  Adds the weights' gradients to gwq and gwk (fp32 or bf16)."""
+    _qk_norm_operands(qkv, wq, wk, cs, S, nq, nk, d)
+    _bf16(dqkv, "dqkv")
+    T = qkv.shape[0]
+    _need(dqkv.shape == qkv.shape and dqkv.stride(1) == 1 and dqkv.device == qkv.device, f"dqkv {tuple(dqkv.shape)}, qkv {tuple(qkv.shape)}")
+    _need(dqkv.data_ptr() != qkv.data_ptr() or T == 0, "the gradient is written in place: dqkv and qkv are the same memory")
+    _need(rstd.shape == (T, nq + nk) and rstd.dtype == torch.float32 and rstd.is_contiguous() and rstd.device == qkv.device,
+          f"rstd {tuple(rstd.shape)}, {rstd.dtype}: expected fp32 [{T}, {nq + nk}]")
+    _need(gwq.dtype == gwk.dtype and gwq.dtype in (torch.float32, torch.bfloat16) and gwq.shape == gwk.shape == (d,)
+          and gwq.is_contiguous() and gwk.is_contiguous() and gwq.device == gwk.device == qkv.device,
+          "gwq and gwk: both fp32 or both bf16, of the weights' shape")
+    L = lib()
+    partial = torch.empty(_workspace_size(L.zb_qk_norm_rope_workspace, T, nq, nk, d), dtype=torch.float32, device=qkv.device)
+    _check(L.zb_qk_norm_rope_bwd(_a(dqkv), _a(qkv), _a(wq), _a(wk), _a(rstd), _a(cs), _a(partial), _a(gwq), _a(gwk), T, S, nq, nk, d,
+                                 qkv.stride(0), dqkv.stride(0), int(gwq.dtype == torch.float32), _stream()), "qk_norm_rope_bwd")
+    global _launches
+    _launches += 1     # the sum over the CTAs
+    return dqkv
+
+
 def swiglu_fwd(gu):
     T, F2 = gu.shape
     out = torch.empty(T, F2 // 2, dtype=gu.dtype, device=gu.device)
@@ -357,6 +431,49 @@ def embedding_bwd(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int = 0)
                                   _stream()), "embedding_bwd")
 
 
+def _embedding_operands(ids, rows, table, what, pos_table, S, pos_offset):
+    T, H = ids.numel(), table.shape[1]
+    _on_current(table, what)
+    _need(ids.dtype == torch.int64 and ids.device == table.device and ids.is_contiguous(), f"ids: contiguous int64 on {table.device}")
+    _need(table.dim() == 2 and table.is_contiguous(), f"{what} {tuple(table.shape)}: expected contiguous rows")
+    if rows is not None:
+        _bf16(rows, "dout")
+        _need(rows.shape == (T, H) and rows.is_contiguous() and rows.device == table.device, f"dout {tuple(rows.shape)}: expected [{T}, {H}]")
+    if pos_table is not None:
+        _need(pos_table.dtype == table.dtype and pos_table.is_contiguous() and pos_table.shape[1] == H and S > 0 and pos_offset >= 0
+              and pos_table.shape[0] >= min(S, T) + pos_offset and pos_table.device == table.device,
+              f"positions {tuple(pos_table.shape)}: expected [>= {min(S, T) + pos_offset}, {H}] of {table.dtype}")
+
+
+def embedding_scaled(ids, table, pos_table=None, S: int = 1, pos_offset: int = 0, scale: float = 1.0):
+    """scale * table[ids] (+ positions), rounded once."""
+    _bf16(table, "table")
+    _embedding_operands(ids, None, table, "table", pos_table, S, pos_offset)
+    T = ids.numel()
+    V, H = table.shape
+    _need(V > 0 or T == 0, "an empty table")
+    out = torch.empty(T, H, dtype=table.dtype, device=table.device)
+    _check(lib().zb_embedding_scaled(_a(ids), _a(table), _a(pos_table), _a(out), T, H, V, S, pos_offset, scale, _stream()),
+           "embedding_scaled")
+    return out
+
+
+def embedding_by_token(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int = 0, scale: float = 1.0):
+    """dtable[v] += scale * the sum of dout's rows whose id is v, in their order, and dpos the sums by position; each row of a
+    table is read and written once.  The same bits on every run."""
+    _need(dtable.dtype in (torch.float32, torch.bfloat16), f"dtable: fp32 or bf16, got {dtable.dtype}")
+    _embedding_operands(ids, dout, dtable, "dtable", dpos, S, pos_offset)
+    T = ids.numel()
+    V, H = dtable.shape
+    _need(V > 0 or T == 0, "an empty table")
+    L = lib()
+    ws = torch.empty(_workspace_size(L.zb_embedding_by_token_workspace, T, H), dtype=torch.uint8, device=dtable.device)
+    _check(L.zb_embedding_by_token(_a(ids), _a(dout), _a(dtable), _a(dpos), _a(ws), T, H, V, S, pos_offset, scale,
+                                   int(dtable.dtype == torch.float32), _stream()), "embedding_by_token")
+    global _launches
+    _launches += (T > 0) + (T > 1) + (dpos is not None and T > 0)     # sums, their join, positions
+
+
 # --------------------------------------------------------------------------- loss
 def cross_entropy(logits, targets, grad_scale: float, dlogits=None, ignore_index: int = -100):
     """Returns per-row losses (fp32). Writes d(loss)/d(logits) * grad_scale into dlogits
@@ -375,6 +492,70 @@ def adam_step(p, m, v, g, p16, *, lr, beta1, beta2, eps, weight_decay, step, gra
     _check(lib().zb_adam(_a(p), _a(m), _a(v), _a(g), _a(p16), n, lr, beta1,
                          beta2, eps, weight_decay, step, grad_scale,
                          int(g.dtype == torch.float32), int(zero_grad), _stream()), "adam")
+
+
+def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step, grad_scale: float = 1.0,
+               seeds=None):
+    """AdamW over lists of tensors in one launch.  p: fp32, contiguous; moments: for each a pair (m, v) in fp32, or `Moments8`
+    (codes and bases of both; then `seeds` has the dither's seed of each tensor); g: fp32 or bf16, scaled by grad_scale first;
+    p16: the copies in bf16 to refresh, or None for a tensor that has none.  step: from 1, a number or one for each tensor."""
+    n = len(p)
+    _need(len(moments) == n and len(g) == n and len(p16) == n, f"lists of {n}, {len(moments)}, {len(g)} and {len(p16)} tensors")
+    if n == 0:
+        return
+    bits = 32 if len(moments[0]) == 2 else 8
+    _need(bits == 32 or (seeds is not None and len(seeds) == n), "moments in 8 bits need a seed for each tensor")
+    steps = step if isinstance(step, (list, tuple)) else [step] * n
+    _need(len(steps) == n and min(steps) >= 1, "step counts from 1, one for all tensors or one for each")
+    dev = p[0].device
+    _on_current(p[0], "p")
+    table, seen = [], set()
+    for i, (x, mom, d, y, k) in enumerate(zip(p, moments, g, p16, steps)):
+        num = x.numel()
+        _need(x.dtype == torch.float32 and x.is_contiguous() and x.device == dev, f"p[{i}]: contiguous fp32 on {dev}")
+        _need(d.numel() == num and d.is_contiguous() and d.dtype in (torch.float32, torch.bfloat16) and d.device == dev,
+              f"g[{i}]: {num} contiguous fp32 or bf16 on {dev}")
+        _need(y is None or (y.numel() == num and y.dtype == torch.bfloat16 and y.is_contiguous() and y.device == dev),
+              f"p16[{i}]: {num} contiguous bf16 on {dev}, or None")
+        if bits == 32:
+            m, v = mom
+            mb = vb = None
+            dtype = torch.float32
+        else:
+            m, mb, v, vb = mom
+            dtype, blocks = torch.uint8, -(-num // MOMENT_BLOCK)
+            _need(mb.dtype == vb.dtype == torch.int16 and mb.numel() == vb.numel() == blocks and mb.is_contiguous() and vb.is_contiguous()
+                  and mb.device == vb.device == dev, f"moments[{i}]: bases of {blocks} blocks, int16")
+        _need(m.dtype == v.dtype == dtype and m.numel() == v.numel() == num and m.is_contiguous() and v.is_contiguous()
+              and m.device == v.device == dev, f"moments[{i}]: {num} contiguous {dtype} on {dev}")
+        if num == 0:
+            continue
+        at = x.data_ptr()
+        _need(at not in seen, f"p[{i}] is in the list twice")
+        seen.add(at)
+        table += (at, m.data_ptr(), v.data_ptr(), _a(mb), _a(vb), d.data_ptr(), _a(y), num, lr / (1 - beta1 ** k),
+                  1 / math.sqrt(1 - beta2 ** k), seeds[i] & 0xFFFFFFFF if bits == 8 else 0, int(d.dtype == torch.float32))
+    count = len(seen)
+    if count == 0:
+        return
+    packed = struct.pack("8Qff2I" * count, *table)
+    _check(lib().zb_adamw_list(packed, count, bits, beta1, 1 - beta1, beta2, 1 - beta2, eps, 1 - lr * weight_decay, grad_scale,
+                               _stream()), "adamw")
+
+
+def moment_values(moments, dtype=torch.float32):
+    """What `Moments8` stand for: (m, v) as fp32 or bf16, either of which holds them exactly."""
+    m, mb, v, vb = moments
+    n, dev = m.numel(), m.device
+    _on_current(m, "m")
+    _need(dtype in (torch.float32, torch.bfloat16), f"values as fp32 or bf16, not {dtype}")
+    _need(m.dtype == v.dtype == torch.uint8 and v.numel() == n and m.is_contiguous() and v.is_contiguous() and v.device == dev, "codes: uint8, contiguous")
+    _need(mb.dtype == vb.dtype == torch.int16 and mb.numel() == vb.numel() == -(-n // MOMENT_BLOCK) and mb.is_contiguous()
+          and vb.is_contiguous() and mb.device == vb.device == dev, "bases: int16, one for each block")
+    out = torch.empty(n, dtype=dtype, device=dev), torch.empty(n, dtype=dtype, device=dev)
+    _check(lib().zb_moment_values(_a(m), _a(mb), _a(v), _a(vb), _a(out[0]), _a(out[1]), n, int(dtype == torch.float32), _stream()),
+           "moment_values")
+    return out
 
 
 # --------------------------------------------------------------------------- attention
