@@ -432,6 +432,22 @@ __device__ __forceinline__ uint4 ld_v4(const void* p) {
                : "l"(p));
   return v;
 }
+// 16 (or 8, 4) bytes from global to this thread's own place in shared memory; visible to it after ring_wait.
+__device__ __forceinline__ void ring_load16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void ring_load4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void ring_load8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ring_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Peer (or any coherent) 16-byte load that must not use the non-coherent path.
 __device__ __forceinline__ uint4 ld_v4_relaxed_sys(const void* p) {
   uint4 v;

@@ -9,147 +9,147 @@
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../norm/norm_common.cuh"
-#include <cooperative_groups.h>
 
 namespace zb {
-namespace cg = cooperative_groups;
-
-__device__ __forceinline__ int clamp_id(long id, int V) { return int(id < 0 ? 0 : id >= V ? V - 1 : id); }
+__device__ __forceinline__ int clamp_id(long id, int V) {
+  return static_cast<unsigned long>(id) < static_cast<unsigned long>(V) ? int(id) : id < 0 ? 0 : V - 1;
+}
 
 // ------------------------------- forward -------------------------------
-__global__ void __launch_bounds__(256) embedding_scaled_kernel(const long* ids, const __nv_bfloat16* table, const __nv_bfloat16* pos,
-                                                               __nv_bfloat16* out, int T, int H, int V, int S, int off, float scale) {
+// 2^shift lanes share a row (all 32 from 256 columns up), every lane up to four chunks of it at once: an id is read once for a
+// row and not for every chunk, and nothing is divided.
+__global__ void __launch_bounds__(128) embedding_scaled_kernel(const long* ids, const __nv_bfloat16* table, const __nv_bfloat16* pos,
+                                                               __nv_bfloat16* out, int T, int H, int V, int S, int off, float scale,
+                                                               int shift) {
   chain_trigger();
   chain_wait();
-  const int cpr = H >> 3;
-  const long total = long(T) * cpr;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
-    const int t = int(i / cpr), c = int(i - long(t) * cpr) * 8;
-    float a[8];
-    unpack8(ld_v4(table + size_t(clamp_id(ids[t], V)) * H + c), a);
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31, lanes = 1 << shift;
+  const long t = ((blockIdx.x * 4L + (threadIdx.x >> 5)) << (5 - shift)) + (lane >> shift);
+  if (t >= T) return;
+  const __nv_bfloat16* src = table + long(clamp_id(ids[t], V)) * H;
+  const __nv_bfloat16* add = pos == nullptr ? nullptr : pos + long(int(t) % S + off) * H;
+  for (int c0 = (lane & (lanes - 1)) * 8; c0 < H; c0 += U * lanes * 8) {
+    uint4 row[U], at[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] *= scale;
-    if (pos != nullptr) {
-      float b[8];
-      unpack8(ld_v4(pos + size_t(t % S + off) * H + c), b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] += b[j];
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * lanes * 8;
+      if (c >= H) break;
+      row[u] = ld_v4(src + c);
+      if (add != nullptr) at[u] = ld_v4(add + c);
     }
-    *reinterpret_cast<uint4*>(out + size_t(t) * H + c) = pack8(a);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * lanes * 8;
+      if (c >= H) break;
+      float a[8];
+      unpack8(row[u], a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] *= scale;
+      if (add != nullptr) {
+        float b[8];
+        unpack8(at[u], b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] += b[j];
+      }
+      *reinterpret_cast<uint4*>(out + t * H + c) = pack8(a);
+    }
   }
 }
 
 // ------------------------------- order of the ids -------------------------------
-// Stable radix sort of up to CLUSTER * SORT_MOST ids and their positions by one cluster, which holds them in the shared memory
-// of its CTAs: one launch, whatever the number of passes.  A pass: every warp ranks its ids among those of the same digit
-// (match), counts are added over warps and CTAs, and every id goes to its place in the CTA that owns it.
-constexpr int SORT_BITS = 9, SORT_BINS = 1 << SORT_BITS, SORT_MOST = 4096, SORT_CTAS = 8, SORT_CHUNK = SORT_CTAS * SORT_MOST;
-
+// Sorts the ids of a chunk together with their positions, equal ids in the order of their positions.  A CTA has `width` neighbouring
+// ids of the vocabulary and looks at the whole chunk: its own are ranked among those of the same id (by a warp's match, and counts
+// added over the warps), and how many ids are lower is counted on the way.  So no CTA needs another one, and there is one pass
+// over the chunk, from L2; a cluster of CTAs that sorted in their shared memory digit by digit took 15 us for 16384 ids of 15 bits.
+constexpr int SORT_BINS = 1024, SORT_ROUNDS = 32, SORT_CHUNK = SORT_ROUNDS * 1024;
 struct SortShared {
-  int key[2][SORT_MOST], at[2][SORT_MOST];
-  unsigned short count[32][SORT_BINS];          // of a warp's ids; then how many of its CTA's are in warps before it
-  int total[SORT_CTAS][SORT_BINS];              // of every CTA of the cluster
-  int base[SORT_BINS];
-  int scan[32];
+  unsigned short count[32][SORT_BINS];   // ids of a warp; then those of its CTA in warps before it
+  int base[SORT_BINS];                   // where a bin begins in the chunk
+  int scan[32], lower;
 };
-
-// order, sorted: [T]; chunk k of the ids (SORT_CHUNK of them) is sorted by cluster k.  `own`: ids per CTA, a multiple of 1024.
-__global__ void __launch_bounds__(1024) embedding_sort_kernel(const long* ids, int* order, int* sorted, int T, int V, int own, int passes,
-                                                              int bits) {
+// order, sorted: [T]
+__global__ void __launch_bounds__(1024) embedding_sort_kernel(const long* ids, int* order, int* sorted, int T, int V, int width, int ctas) {
   chain_trigger();
   chain_wait();
   extern __shared__ __align__(16) unsigned char raw[];
   SortShared& sh = *reinterpret_cast<SortShared*>(raw);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
-  const int first = int(blockIdx.x / ctas) * SORT_CHUNK, n = min(T - first, SORT_CHUNK);
-  const int mine = max(0, min(n - rank * own, own));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, per = own >> 10;   // 32 `per` ids in a row for each warp
-  cluster.sync();                               // no CTA writes to another that has not started
-  for (int i = tid; i < mine; i += 1024) {
-    sh.key[0][i] = clamp_id(ids[first + rank * own + i], V);
-    sh.at[0][i] = first + rank * own + i;
-  }
-  for (int pass = 0; pass < passes; ++pass) {
-    const int from = pass & 1, shift = pass * bits, bins = 1 << bits;
-    for (int i = tid; i < 32 * SORT_BINS / 2; i += 1024) reinterpret_cast<unsigned*>(sh.count)[i] = 0;
-    __syncthreads();
-    int digit[4], place[4];
+  const int chunk = blockIdx.x / ctas, lo = (blockIdx.x - chunk * ctas) * width, first = chunk * SORT_CHUNK, n = min(T - first, SORT_CHUNK);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rounds = (n + 1023) >> 10, e0 = warp * rounds * 32 + lane;     // 32 ids a round, a warp's rounds in a row
+  for (int i = lane * 8; i < width; i += 256) *reinterpret_cast<uint4*>(&sh.count[warp][i]) = make_uint4(0, 0, 0, 0);
+  if (tid == 0) sh.lower = 0;
+  int key[SORT_ROUNDS], below = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = (warp * per + k) * 32 + lane;
-      const bool there = k < per && e < mine;
-      const unsigned all = __ballot_sync(0xffffffffu, there);
-      digit[k] = there ? sh.key[from][e] >> shift & (bins - 1) : 0;
-      if (there) {
-        const unsigned same = __match_any_sync(all, digit[k]);
-        const int before = sh.count[warp][digit[k]];
-        place[k] = before + __popc(same & ((1u << lane) - 1));
-        __syncwarp(all);
-        if ((same & ((1u << lane) - 1)) == 0) sh.count[warp][digit[k]] = static_cast<unsigned short>(before + __popc(same));
-        __syncwarp(all);
-      }
-      __syncwarp();
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    const int e = e0 + r * 32;
+    key[r] = r < rounds && e < n ? clamp_id(ids[first + e], V) - lo : 1 << 30;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    if (r >= rounds) break;
+    below += key[r] < 0;
+    const bool mine = key[r] >= 0 && key[r] < width;
+    const unsigned all = __ballot_sync(0xffffffffu, mine);
+    if (all == 0) {
+      key[r] = -1;
+      continue;
     }
-    __syncthreads();
-    if (tid < bins) {
-      int sum = 0;
-      for (int w = 0; w < 32; ++w) {
-        const int c = sh.count[w][tid];
-        sh.count[w][tid] = static_cast<unsigned short>(sum);
-        sum += c;
-      }
-      for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(&sh, r)->total[rank][tid] = sum;
+    int place = 0;
+    if (mine) {
+      const unsigned same = __match_any_sync(all, key[r]), lower = same & ((1u << lane) - 1);
+      const int before = sh.count[warp][key[r]];
+      place = before + __popc(lower);
+      __syncwarp(all);
+      if (lower == 0) sh.count[warp][key[r]] = static_cast<unsigned short>(before + __popc(same));
     }
-    cluster.sync();
-    // base of a bin: everything of lower bins, and of this one in the CTAs before
-    int sum = 0, before = 0;
-    if (tid < bins) {
-      for (int r = 0; r < ctas; ++r) {
-        const int c = sh.total[r][tid];
-        sum += c;
-        before += r < rank ? c : 0;
-      }
+    __syncwarp();
+    key[r] = mine ? key[r] | place << 10 : -1;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
+  if (lane == 0 && below) atomicAdd(&sh.lower, below);      // (whole numbers: the order does not matter)
+  __syncthreads();
+  // bin `tid`: over the warps, then over the bins
+  int sum = 0;
+  if (tid < width) {
+#pragma unroll 8
+    for (int w = 0; w < 32; ++w) {
+      const int c = sh.count[w][tid];
+      sh.count[w][tid] = static_cast<unsigned short>(sum);
+      sum += c;
     }
-    int run = sum;
+  }
+  int run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  if (lane == 31) sh.scan[warp] = run;
+  __syncthreads();
+  if (warp == 0) {
+    const int self = sh.scan[lane];
+    int t = self;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += v;
+      const int v = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += v;
     }
-    if (lane == 31) sh.scan[warp] = run;
-    __syncthreads();
-    if (warp == 0) {
-      int s = sh.scan[lane];
-      const int self = s;
+    sh.scan[lane] = t - self;
+  }
+  __syncthreads();
+  sh.base[tid] = sh.lower + sh.scan[warp] + run - sum;
+  __syncthreads();
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += v;
-      }
-      sh.scan[lane] = s - self;
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    if (r >= rounds) break;
+    if (key[r] >= 0) {
+      const int bin = key[r] & (SORT_BINS - 1), pos = sh.base[bin] + sh.count[warp][bin] + (key[r] >> 10);
+      order[first + pos] = first + e0 + r * 32;
+      sorted[first + pos] = lo + bin;
     }
-    __syncthreads();
-    if (tid < bins) sh.base[tid] = sh.scan[warp] + run - sum + before;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = (warp * per + k) * 32 + lane;
-      if (k < per && e < mine) {
-        const int pos = sh.base[digit[k]] + sh.count[warp][digit[k]] + place[k];
-        const int key = sh.key[from][e], at = sh.at[from][e];
-        if (pass + 1 == passes) {
-          order[first + pos] = at;
-          sorted[first + pos] = key;
-        } else {
-          const int r = pos / own;
-          SortShared* to = cluster.map_shared_rank(&sh, r);
-          to->key[from ^ 1][pos - r * own] = key;
-          to->at[from ^ 1][pos - r * own] = at;
-        }
-      }
-    }
-    if (pass + 1 < passes) cluster.sync();
   }
 }
 
@@ -165,32 +165,80 @@ struct ByToken {
   float scale;
 };
 
+// A lane's columns of a slice of 256: eight neighbours for a bf16 table, twice four for an fp32 one, 128 apart, so that every
+// access of a warp is to whole 32-byte sectors (with eight fp32 neighbours a lane, sectors went by halves).
 template <typename GT>
-__device__ __forceinline__ void load_grad8(const GT* p, float (&f)[8]) {
-  if constexpr (sizeof(GT) == 4) {
-    const uint4 a = ld_v4(p), b = ld_v4(p + 4);
-    f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
-    f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
-  } else {
-    unpack8(ld_v4(p), f);
-  }
-}
-__device__ __forceinline__ void store_grad8(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-__device__ __forceinline__ void store_grad8(__nv_bfloat16* p, const float (&f)[8]) { *reinterpret_cast<uint4*>(p) = pack8(f); }
+constexpr int VEC = sizeof(GT) == 4 ? 4 : 8;
+template <typename GT>
+constexpr int PARTS = 8 / VEC<GT>;
 
+template <typename GT>
+__device__ __forceinline__ int parts_of(int col, int H) {       // of a lane whose first column is col
+  return col >= H ? 0 : PARTS<GT> == 2 && col + 128 < H ? 2 : 1;
+}
+__device__ __forceinline__ void unpack4(const uint4& u, float* f) {
+  f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack4(const uint2& u, float* f) {
+  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+}
+// A part of a table's row is 16 bytes; of a row of dout 8 or 16
+template <typename GT>
+__device__ __forceinline__ void unpack_grad(const uint4& u, float* f) {
+  if constexpr (sizeof(GT) == 4) unpack4(u, f);
+  else unpack8(u, f);
+}
+__device__ __forceinline__ void unpack_row(const uint2& u, float* f) { unpack4(u, f); }
+__device__ __forceinline__ void unpack_row(const uint4& u, float* f) { unpack8(u, f); }
+__device__ __forceinline__ void store_part(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+__device__ __forceinline__ void store_part(__nv_bfloat16* p, const float* f) { *reinterpret_cast<uint4*>(p) = pack8(f); }
+template <typename GT>
+struct RowPart;
+template <>
+struct RowPart<float> {
+  using type = uint2;
+};
+template <>
+struct RowPart<__nv_bfloat16> {
+  using type = uint4;
+};
+__device__ __forceinline__ void ring_load(uint4* to, const void* from) { ring_load16(to, from); }
+__device__ __forceinline__ void ring_load(uint2* to, const void* from) { ring_load8(to, from); }
+__device__ __forceinline__ uint2 ld_v2(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void load_row(uint2& u, const void* p) { u = ld_v2(p); }
+__device__ __forceinline__ void load_row(uint4& u, const void* p) { u = ld_v4(p); }
+// VEC sums in fp32, in shared memory or a workspace
+template <typename GT>
+__device__ __forceinline__ void store_sums(float* p, const float* f) {
+#pragma unroll
+  for (int k = 0; k < VEC<GT>; k += 4) store_part(p + k, f + k);
+}
+
+// Rows lie anywhere, so what bounds a warp is how many of them are on their way: every lane copies its parts of the rows to come
+// (and of the table's, which a run's end will add to) into its own places of a ring in shared memory.
+constexpr int PIECE_RING = 4;
+template <typename GT>
+struct PieceRing {
+  typename RowPart<GT>::type row[PIECE_RING][PARTS<GT>][256];
+  uint4 old[PIECE_RING][PARTS<GT>][256];
+};
 template <int K, typename GT>
 __global__ void __launch_bounds__(256) embedding_pieces_kernel(const ByToken a, GT* table) {
   chain_trigger();
   chain_wait();
-  constexpr int U = 4;
-  const int lane = threadIdx.x & 31, slices = (a.H + 255) >> 8, pieces = (a.n + K - 1) / K;
-  const int item = blockIdx.x * 8 + (threadIdx.x >> 5);
+  extern __shared__ __align__(16) unsigned char raw[];
+  PieceRing<GT>& ring = *reinterpret_cast<PieceRing<GT>*>(raw);
+  const int tid = threadIdx.x, lane = tid & 31, slices = (a.H + 255) >> 8, pieces = (a.n + K - 1) / K;
+  const int item = blockIdx.x * 8 + (tid >> 5);
   if (item >= pieces * slices) return;
-  const int piece = item / slices, col = (item - piece * slices) * 256 + lane * 8, j0 = piece * K, rows = min(K, a.n - j0);
-  const bool used = col < a.H;
+  constexpr int V = VEC<GT>, P = PARTS<GT>;
+  const int piece = item / slices, j0 = piece * K, rows = min(K, a.n - j0);
+  const int col = (item - piece * slices) * 256 + lane * V, parts = parts_of<GT>(col, a.H);
   const int id = lane < rows ? a.sorted[j0 + lane] : -1, at = lane < rows ? a.order[j0 + lane] : 0;
   const int prev = j0 > 0 ? a.sorted[j0 - 1] : -1, next = j0 + rows < a.n ? a.sorted[j0 + rows] : -1;
   int after = __shfl_down_sync(0xffffffffu, id, 1);
@@ -198,103 +246,144 @@ __global__ void __launch_bounds__(256) embedding_pieces_kernel(const ByToken a, 
   const unsigned ends = __ballot_sync(0xffffffffu, lane < rows && id != after);
   const bool goes_on = prev >= 0 && prev == __shfl_sync(0xffffffffu, id, 0);   // the first run began in an earlier piece
   const int first_end = goes_on ? __ffs(ends) - 1 : -1;
-  float acc[8] = {};
-  for (int j = 0; j < rows; j += U) {
-    uint4 row[U];
-    float old[U][8];
-    int to[U];
+  auto request = [&](int j, int slot) {
+    const int src = __shfl_sync(0xffffffffu, at, j & 31), to = __shfl_sync(0xffffffffu, id, j & 31);
+    if (j < rows) {
+      const __nv_bfloat16* row = a.dout + size_t(src) * a.H + col;
+      const GT* old = table + size_t(to) * a.H + col;
+      const bool add = (ends >> j & 1) && j != first_end;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int src = __shfl_sync(0xffffffffu, at, (j + u) & 31);
-      to[u] = __shfl_sync(0xffffffffu, id, (j + u) & 31);
-      row[u] = make_uint4(0, 0, 0, 0);
-      if (j + u < rows && used) {
-        row[u] = ld_v4(a.dout + size_t(src) * a.H + col);
-        if ((ends >> (j + u) & 1) && j + u != first_end) load_grad8(table + size_t(to[u]) * a.H + col, old[u]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[8];
-      unpack8(row[u], f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += f[k];
-      if (j + u < rows && (ends >> (j + u) & 1)) {
-        if (j + u == first_end) {
-          if (used) store_grad8(a.head + size_t(piece) * a.H + col, acc);
-        } else if (used) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) old[u][k] += a.scale * acc[k];
-          store_grad8(table + size_t(to[u]) * a.H + col, old[u]);
+      for (int k = 0; k < P; ++k) {
+        if (k < parts) {
+          ring_load(&ring.row[slot][k][tid], row + 128 * k);
+          if (add) ring_load16(&ring.old[slot][k][tid], old + 128 * k);
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] = 0.f;
       }
     }
+    ring_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < PIECE_RING - 1; ++j) request(j, j);
+  float acc[8] = {};
+  auto leave = [&](float* to) {
+#pragma unroll
+    for (int k = 0; k < P; ++k)
+      if (k < parts) store_sums<GT>(to + size_t(piece) * a.H + col + 128 * k, acc + V * k);
+  };
+  int slot = 0;
+  for (int j = 0; j < rows; ++j) {
+    request(j + PIECE_RING - 1, (slot + PIECE_RING - 1) % PIECE_RING);
+    ring_wait<PIECE_RING - 1>();
+    const int to = __shfl_sync(0xffffffffu, id, j);
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      if (k >= parts) break;
+      float f[V];
+      unpack_row(ring.row[slot][k][tid], f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[V * k + i] += f[i];
+    }
+    if (ends >> j & 1) {
+      if (j == first_end) {
+        leave(a.head);
+      } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          if (k >= parts) break;
+          float old[V];
+          unpack_grad<GT>(ring.old[slot][k][tid], old);
+#pragma unroll
+          for (int i = 0; i < V; ++i) old[i] += a.scale * acc[V * k + i];
+          store_part(table + size_t(to) * a.H + col + 128 * k, old);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    }
+    slot = (slot + 1) % PIECE_RING;
   }
-  if (used && !(ends >> (rows - 1) & 1))
-    store_grad8((goes_on && ends == 0 ? a.head : a.tail) + size_t(piece) * a.H + col, acc);
+  if (!(ends >> (rows - 1) & 1)) leave(goes_on && ends == 0 ? a.head : a.tail);
 }
 
 // Runs over several pieces: a CTA looks at eight pieces and 256 columns, a warp at one piece.  What begins in it and goes on is
 // its tail and the heads that follow, up to the run's last piece; runs over more than JOIN_ALONE pieces are added by the whole CTA,
 // each warp a stretch of the heads, the stretches in order.
 constexpr int JOIN_ALONE = 16;
+template <typename GT>
+__device__ __forceinline__ void add_to_row(GT* dst, const uint4 (&old)[2], int parts, float scale, const float (&acc)[8]) {
+#pragma unroll
+  for (int k = 0; k < PARTS<GT>; ++k) {
+    if (k >= parts) break;
+    float f[VEC<GT>];
+    unpack_grad<GT>(old[k], f);
+#pragma unroll
+    for (int i = 0; i < VEC<GT>; ++i) f[i] += scale * acc[VEC<GT> * k + i];
+    store_part(dst + 128 * k, f);
+  }
+}
+template <typename GT>
+__device__ __forceinline__ void load_old(const GT* src, int parts, uint4 (&old)[2]) {
+#pragma unroll
+  for (int k = 0; k < PARTS<GT>; ++k)
+    if (k < parts) old[k] = ld_v4(src + 128 * k);
+}
 template <int K, typename GT>
-__global__ void __launch_bounds__(256) embedding_join_kernel(const ByToken a, GT* table) {
+__global__ void __launch_bounds__(256, 4) embedding_join_kernel(const ByToken a, GT* table) {
   chain_trigger();
   chain_wait();
+  constexpr int V = VEC<GT>, P = PARTS<GT>;
   __shared__ int run_last[8];
   __shared__ __align__(16) float part[8][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slices = (a.H + 255) >> 8, pieces = (a.n + K - 1) / K;
-  const int group = blockIdx.x / slices, col = (blockIdx.x - group * slices) * 256 + lane * 8;
-  const bool used = col < a.H;
+  const int group = blockIdx.x / slices, col = (blockIdx.x - group * slices) * 256 + lane * V, parts = parts_of<GT>(col, a.H);
   int piece = group * 8 + warp, last = -1;
   if (piece < pieces - 1) {
-    const int end = (piece + 1) * K, id = a.sorted[end - 1];
-    if (a.sorted[end] == id && (piece == 0 || a.sorted[piece * K - 1] != id)) {
-      int lo = end, hi = a.n;                  // sorted[lo] == id; the first place behind the run is in (lo, hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.sorted[mid] == id) lo = mid;
-        else hi = mid;
+    const int end = (piece + 1) * K, id = a.sorted[end - 1], next = a.sorted[end], prev = piece == 0 ? -1 : a.sorted[piece * K - 1];
+    if (next == id && prev != id) {
+      // the run's last piece: the first one behind this that the run does not leave, 32 looked at together
+      for (last = piece + 1;; last += 32) {
+        const long behind = long(last + lane + 1) * K;
+        const unsigned stops = __ballot_sync(0xffffffffu, behind >= a.n || a.sorted[behind] != id);
+        if (stops) {
+          last += __ffs(stops) - 1;
+          break;
+        }
       }
-      last = lo / K;
     }
   }
-  auto sum_heads = [&](int from, int to, float (&acc)[8]) {
-    int q = from;
-    for (; q + 4 <= to; q += 4) {
-      float f[4][8];
+  auto add_rows = [&](const float* rows, int from, int to, float (&acc)[8]) {
+    constexpr int U = 4;
+    for (int q = from; q < to; q += U) {
+      uint4 u[U][2];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) load_grad8(a.head + size_t(q + u) * a.H + col, f[u]);
+      for (int i = 0; i < U; ++i) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+        for (int k = 0; k < 2; ++k) {
+          const bool there = q + i < to && (P == 2 ? k < parts : parts > 0);
+          u[i][k] = there ? ld_v4(rows + size_t(q + i) * a.H + col + (P == 2 ? 128 : 4) * k) : make_uint4(0, 0, 0, 0);
+        }
+      }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += f[u][k];
+      for (int i = 0; i < U; ++i) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float f[4];
+          unpack4(u[i][k], f);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[4 * k + x] += f[x];
+        }
       }
     }
-    for (; q < to; ++q) {
-      float f[8];
-      load_grad8(a.head + size_t(q) * a.H + col, f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += f[k];
-    }
-  };
-  auto add_to_table = [&](int p, const float (&acc)[8]) {
-    GT* dst = table + size_t(a.sorted[(p + 1) * K]) * a.H + col;
-    float f[8];
-    load_grad8(dst, f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] += a.scale * acc[k];
-    store_grad8(dst, f);
   };
   const bool together = last - piece > JOIN_ALONE;
-  if (last >= 0 && !together && used) {
-    float acc[8];
-    load_grad8(a.tail + size_t(piece) * a.H + col, acc);
-    sum_heads(piece + 1, last + 1, acc);
-    add_to_table(piece, acc);
+  if (last >= 0 && !together) {
+    GT* dst = table + size_t(a.sorted[(piece + 1) * K]) * a.H + col;
+    uint4 old[2];
+    load_old(dst, parts, old);
+    float acc[8] = {};
+    add_rows(a.tail, piece, piece + 1, acc);
+    add_rows(a.head, piece + 1, last + 1, acc);
+    add_to_row(dst, old, parts, a.scale, acc);
   }
   if (lane == 0) run_last[warp] = together && last >= 0 ? last : -1;
   __syncthreads();
@@ -304,19 +393,103 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const ByToken a, GT
     piece = group * 8 + w;
     const int heads = end - piece, stretch = (heads + 7) / 8, from = piece + 1 + warp * stretch;
     float acc[8] = {};
-    if (used) sum_heads(from, min(from + stretch, end + 1), acc);
-    if (used) store_grad8(&part[warp][lane * 8], acc);
-    __syncthreads();
-    if (warp == 0 && used) {
-      load_grad8(a.tail + size_t(piece) * a.H + col, acc);
-      for (int v = 0; v < 8; ++v) {
+    if (warp == 0) add_rows(a.tail, piece, piece + 1, acc);
+    add_rows(a.head, from, min(from + stretch, end + 1), acc);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] += part[v][lane * 8 + k];
+    for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = acc[k];
+    __syncthreads();
+    if (warp == 0) {
+      GT* dst = table + size_t(a.sorted[(piece + 1) * K]) * a.H + col;
+      uint4 old[2];
+      load_old(dst, parts, old);
+      for (int v = 1; v < 8; ++v) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += part[v][k * 32 + lane];
       }
-      add_to_table(piece, acc);
+      add_to_row(dst, old, parts, a.scale, acc);
     }
     __syncthreads();
   }
+}
+
+// Few tokens: no order is needed.  A CTA has one token and 256 columns, looks for the token's id among all ids and, where the token is
+// the first with it, adds up the rows of all, each warp a stretch of them.  One launch: 256 tokens of 512 columns SMALL_US us
+// against SORTED_US by sorting.
+constexpr int SMALL_T = 1024, SMALL_CTAS = 2048;
+template <typename GT>
+__global__ void __launch_bounds__(256) embedding_small_kernel(const long* ids, const __nv_bfloat16* dout, GT* table, int T, int H, int V,
+                                                              float scale) {
+  chain_trigger();
+  chain_wait();
+  constexpr int W = VEC<GT>, P = PARTS<GT>;
+  __shared__ unsigned found[SMALL_T / 32];
+  __shared__ unsigned short list[SMALL_T];
+  __shared__ __align__(16) float part[8][256];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, slices = (H + 255) >> 8;
+  const int t = blockIdx.x / slices, col = (blockIdx.x - t * slices) * 256 + lane * W, parts = parts_of<GT>(col, H);
+  const int id = clamp_id(ids[t], V);
+#pragma unroll
+  for (int r = 0; r < SMALL_T / 256; ++r) {
+    const int e = r * 256 + tid;
+    const unsigned m = __ballot_sync(0xffffffffu, e < T && clamp_id(ids[e < T ? e : 0], V) == id);
+    if (lane == 0) found[r * 8 + warp] = m;
+  }
+  __syncthreads();
+  // (every warp by itself) how many there are, and whether one lies before t
+  const unsigned word = found[lane];
+  const int at = lane * 32;
+  const unsigned early = at + 32 <= t ? word : at <= t ? word & ((1u << (t - at)) - 1) : 0;
+  if (__any_sync(0xffffffffu, early != 0)) return;                 // the same for the whole CTA
+  int run = __popc(word);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += v;
+  }
+  const int m = __shfl_sync(0xffffffffu, run, 31);
+  if (warp == 0) {
+    int k = run - __popc(word);
+    for (unsigned w = word; w; w &= w - 1) list[k++] = static_cast<unsigned short>(at + __ffs(w) - 1);
+  }
+  GT* dst = table + size_t(id) * H + col;
+  uint4 old[2];
+  if (warp == 0) load_old(dst, parts, old);
+  __syncthreads();
+  const int stretch = (m + 7) / 8, to = min((warp + 1) * stretch, m);
+  float acc[8] = {};
+  constexpr int U = 4;
+  for (int q = warp * stretch; q < to; q += U) {
+    typename RowPart<GT>::type u[U][P];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const __nv_bfloat16* row = dout + size_t(list[min(q + i, m - 1)]) * H + col;
+#pragma unroll
+      for (int k = 0; k < P; ++k)
+        if (k < parts) load_row(u[i][k], row + 128 * k);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        if (k >= parts || q + i >= to) break;
+        float f[W];
+        unpack_row(u[i][k], f);
+#pragma unroll
+        for (int x = 0; x < W; ++x) acc[W * k + x] += f[x];
+      }
+    }
+  }
+  if (m > 1) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[warp][k * 32 + lane] = acc[k];
+    __syncthreads();
+  }
+  if (warp != 0) return;
+  for (int v = 1; v < 8 && v * stretch < m; ++v) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] += part[v][k * 32 + lane];
+  }
+  add_to_row(dst, old, parts, scale, acc);
 }
 
 // gpos[p + off] += sum over the sequences of dout[b S + p], in order
@@ -324,21 +497,26 @@ template <typename GT>
 __global__ void __launch_bounds__(256) position_grad_kernel(const __nv_bfloat16* dout, GT* gpos, int T, int H, int S, int off) {
   chain_trigger();
   chain_wait();
-  const int cpr = H >> 3, rows = min(S, T);
+  constexpr int W = VEC<GT>;
+  const int cpr = H / W, rows = min(S, T);
   const long total = long(rows) * cpr;
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
-    const int p = int(i / cpr), c = int(i - long(p) * cpr) * 8;
-    float acc[8] = {}, f[8];
-    for (long t = p; t < T; t += S) {
-      unpack8(ld_v4(dout + t * H + c), f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k] += f[k];
-    }
+    const int p = int(i / cpr), c = int(i - long(p) * cpr) * W;
     GT* dst = gpos + size_t(p + off) * H + c;
-    load_grad8(dst, f);
+    const uint4 old = ld_v4(dst);
+    float acc[W] = {}, f[W];
+#pragma unroll 4
+    for (long t = p; t < T; t += S) {
+      typename RowPart<GT>::type u;
+      load_row(u, dout + t * H + c);
+      unpack_row(u, f);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] += acc[k];
-    store_grad8(dst, f);
+      for (int k = 0; k < W; ++k) acc[k] += f[k];
+    }
+    unpack_grad<GT>(old, f);
+#pragma unroll
+    for (int k = 0; k < W; ++k) f[k] += acc[k];
+    store_part(dst, f);
   }
 }
 
@@ -348,10 +526,19 @@ static int piece_rows(int n, int H) { return long(n) * ((H + 255) / 256) >= 32L 
 template <int K, typename GT>
 static int by_token(const ByToken& a, GT* table, cudaStream_t stream) {
   const int slices = (a.H + 255) / 256, pieces = (a.n + K - 1) / K;
-  ZB_CUDA_OK(launch_pass(embedding_pieces_kernel<K, GT>, (pieces * slices + 7) / 8, 256, 0, stream, a, table));
+  auto kern = embedding_pieces_kernel<K, GT>;
+  ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PieceRing<GT>))));
+  ZB_CUDA_OK(launch_pass(kern, (pieces * slices + 7) / 8, 256, sizeof(PieceRing<GT>), stream, a, table));
   if (pieces > 1) ZB_CUDA_OK(launch_pass(embedding_join_kernel<K, GT>, (pieces + 7) / 8 * slices, 256, 0, stream, a, table));
   return 0;
 }
+
+template <typename GT>
+static int small(const long* ids, const __nv_bfloat16* dout, GT* table, int T, int H, int V, float scale, cudaStream_t stream) {
+  ZB_CUDA_OK(launch_pass(embedding_small_kernel<GT>, T * ((H + 255) / 256), 256, 0, stream, ids, dout, table, T, H, V, scale));
+  return 0;
+}
+static bool is_small(int T, int H) { return T <= SMALL_T && long(T) * ((H + 255) / 256) <= SMALL_CTAS; }
 
 static int blocks_for(long items) {
   const long b = (items + 255) / 256, cap = long(num_sms()) * 16;
@@ -369,9 +556,11 @@ int zb_embedding_scaled(const long* ids, const void* table, const void* pos, voi
   if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(out)) & 15)
     ZB_FAIL(-1, "embedding: operands must be 16-byte aligned");
   if (T <= 0) return 0;
-  ZB_CUDA_OK(launch_pass(embedding_scaled_kernel, blocks_for(long(T) * (H / 8)), 256, 0, stream, ids,
-                         static_cast<const __nv_bfloat16*>(table), static_cast<const __nv_bfloat16*>(pos),
-                         static_cast<__nv_bfloat16*>(out), T, H, V, S, pos_offset, scale));
+  int shift = 0;
+  while (shift < 5 && (8 << shift) < H) ++shift;
+  const long warps = (long(T) + (32 >> shift) - 1) >> (5 - shift);
+  ZB_CUDA_OK(launch_pass(embedding_scaled_kernel, int((warps + 3) / 4), 128, 0, stream, ids, static_cast<const __nv_bfloat16*>(table),
+                         static_cast<const __nv_bfloat16*>(pos), static_cast<__nv_bfloat16*>(out), T, H, V, S, pos_offset, scale, shift));
   return 0;
 }
 
@@ -379,7 +568,7 @@ int zb_embedding_scaled(const long* ids, const void* table, const void* pos, voi
 int zb_embedding_by_token_workspace(int T, int H, long* bytes) {
   using namespace zb;
   const int n = T < SORT_CHUNK ? T : SORT_CHUNK, K = piece_rows(n, H);
-  *bytes = T > 0 ? ((8L * T + 15) / 16) * 16 + 8L * ((n + K - 1) / K) * H : 0;
+  *bytes = T > 0 && !is_small(T, H) ? ((8L * T + 15) / 16) * 16 + 8L * ((n + K - 1) / K) * H : 0;
   return 0;
 }
 
@@ -391,34 +580,40 @@ int zb_embedding_by_token(const long* ids, const void* dout, void* gtable, void*
        reinterpret_cast<uintptr_t>(workspace)) & 15)
     ZB_FAIL(-1, "embedding: operands must be 16-byte aligned");
   if (T <= 0) return 0;
-  int* order = static_cast<int*>(workspace);
-  int* sorted = order + T;
-  const int most = T < SORT_CHUNK ? T : SORT_CHUNK, K = piece_rows(most, H);
-  float* head = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((8L * T + 15) / 16) * 16);
-  float* tail = head + long((most + K - 1) / K) * H;
-  int bits = 1;
-  while (bits < 31 && (1L << bits) < V) ++bits;
-  const int passes = (bits + SORT_BITS - 1) / SORT_BITS, chunks = (T + SORT_CHUNK - 1) / SORT_CHUNK;
-  const int ctas = most >= SORT_CTAS * 1024 ? SORT_CTAS : (most + 1023) / 1024, own = ((most + ctas - 1) / ctas + 1023) / 1024 * 1024;
-  ZB_CUDA_OK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SortShared))));
-  ZB_CUDA_OK(launch_chained(embedding_sort_kernel, chunks * ctas, 1024, sizeof(SortShared), stream, ctas, ids, order, sorted, T, V, own,
-                            passes, (bits + passes - 1) / passes));
-  for (int c = 0; c < chunks; ++c) {
-    ByToken a = {static_cast<const __nv_bfloat16*>(dout), order + c * SORT_CHUNK, sorted + c * SORT_CHUNK, head, tail,
-                 T - c * SORT_CHUNK < SORT_CHUNK ? T - c * SORT_CHUNK : SORT_CHUNK, H, scale};
-    int rc;
-    if (grad_f32)
-      rc = K == 32 ? by_token<32>(a, static_cast<float*>(gtable), stream) : by_token<4>(a, static_cast<float*>(gtable), stream);
-    else
-      rc = K == 32 ? by_token<32>(a, static_cast<__nv_bfloat16*>(gtable), stream)
-                   : by_token<4>(a, static_cast<__nv_bfloat16*>(gtable), stream);
+  const __nv_bfloat16* rows = static_cast<const __nv_bfloat16*>(dout);
+  int rc = 0;
+  if (is_small(T, H)) {
+    rc = grad_f32 ? small(ids, rows, static_cast<float*>(gtable), T, H, V, scale, stream)
+                  : small(ids, rows, static_cast<__nv_bfloat16*>(gtable), T, H, V, scale, stream);
     if (rc) return rc;
+  } else {
+    int* order = static_cast<int*>(workspace);
+    int* sorted = order + T;
+    const int most = T < SORT_CHUNK ? T : SORT_CHUNK, K = piece_rows(most, H), chunks = (T + SORT_CHUNK - 1) / SORT_CHUNK;
+    float* head = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((8L * T + 15) / 16) * 16);
+    float* tail = head + long((most + K - 1) / K) * H;
+    // ids of a CTA: about as many CTAs as SMs, of at least 64 ids and at most SORT_BINS
+    int width = (V + num_sms() - 1) / num_sms();
+    width = width < 64 ? 64 : width > SORT_BINS ? SORT_BINS : width;
+    const int ctas = (V - 1) / width + 1;
+    if (long(ctas) * chunks > 0x7fffffffL) ZB_FAIL(-1, "embedding: %d tokens of a vocabulary of %d", T, V);
+    ZB_CUDA_OK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SortShared))));
+    ZB_CUDA_OK(launch_pass(embedding_sort_kernel, chunks * ctas, 1024, sizeof(SortShared), stream, ids, order, sorted, T, V, width, ctas));
+    for (int c = 0; c < chunks; ++c) {
+      ByToken a = {rows, order + c * SORT_CHUNK, sorted + c * SORT_CHUNK, head, tail, T - c * SORT_CHUNK < SORT_CHUNK ? T - c * SORT_CHUNK : SORT_CHUNK,
+                   H, scale};
+      if (grad_f32)
+        rc = K == 32 ? by_token<32>(a, static_cast<float*>(gtable), stream) : by_token<4>(a, static_cast<float*>(gtable), stream);
+      else
+        rc = K == 32 ? by_token<32>(a, static_cast<__nv_bfloat16*>(gtable), stream)
+                      : by_token<4>(a, static_cast<__nv_bfloat16*>(gtable), stream);
+      if (rc) return rc;
+    }
   }
   if (gpos != nullptr) {
-    const int grid = blocks_for(long(S < T ? S : T) * (H / 8));
-    const __nv_bfloat16* d = static_cast<const __nv_bfloat16*>(dout);
-    if (grad_f32) ZB_CUDA_OK(launch_pass(position_grad_kernel<float>, grid, 256, 0, stream, d, static_cast<float*>(gpos), T, H, S, pos_offset));
-    else ZB_CUDA_OK(launch_pass(position_grad_kernel<__nv_bfloat16>, grid, 256, 0, stream, d, static_cast<__nv_bfloat16*>(gpos), T, H, S, pos_offset));
+    const int grid = blocks_for(long(S < T ? S : T) * (H / (grad_f32 ? 4 : 8)));
+    if (grad_f32) ZB_CUDA_OK(launch_pass(position_grad_kernel<float>, grid, 256, 0, stream, rows, static_cast<float*>(gpos), T, H, S, pos_offset));
+    else ZB_CUDA_OK(launch_pass(position_grad_kernel<__nv_bfloat16>, grid, 256, 0, stream, rows, static_cast<__nv_bfloat16*>(gpos), T, H, S, pos_offset));
   }
   return 0;
 }

@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/SmallVector.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <utility>
@@ -55,6 +56,15 @@ struct Entry {
   int (*gemm2_rope_fwd)(const void*, const void*, const void*, const float*, void*, int, int, int, int, int, int, int, int, int*,
                         cudaStream_t);
   int (*column_sums)(const long*, int, int, cudaStream_t);
+  int (*qk_norm_rope_fwd)(const void*, void*, const void*, const void*, const float*, float*, int, int, int, int, int, int, long, long,
+                          float, cudaStream_t);
+  int (*qk_norm_rope_workspace)(int, int, int, int, long*);
+  int (*qk_norm_rope_bwd)(void*, const void*, const void*, const void*, float*, const float*, float*, void*, void*, int, int, int, int,
+                          int, long, long, int, cudaStream_t);
+  int (*embedding_scaled)(const long*, const void*, const void*, void*, int, int, int, int, int, float, cudaStream_t);
+  int (*embedding_by_token_workspace)(int, int, long*);
+  int (*embedding_by_token)(const long*, const void*, void*, void*, void*, int, int, int, int, int, float, int, cudaStream_t);
+  int (*adamw_list)(const void*, int, int, float, float, float, float, float, float, float, cudaStream_t);
   const char* (*last_error)();
 };
 Entry lib;
@@ -91,6 +101,8 @@ int* status_of(const Tensor& t) {
   const int d = t.get_device();
   return ready && d >= 0 && d < 64 && d == c10::cuda::current_device() ? status_words[d] : nullptr;
 }
+// Whether the tensor is on the current device, for launches that have no status word.
+bool here(const Tensor& t) { return ready && t.get_device() == c10::cuda::current_device(); }
 cudaStream_t stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) {
   return at::empty(sizes, like.options().dtype(type).requires_grad(false));
@@ -121,6 +133,11 @@ bool int_arg(PyObject* o, int64_t& v) {
   v = PyLong_Check(o) ? PyLong_AsLongLong(o) : -1;
   if (PyErr_Occurred()) { PyErr_Clear(); return false; }
   return PyLong_Check(o);
+}
+bool float_arg(PyObject* o, double& v) {
+  v = PyFloat_Check(o) || PyLong_Check(o) ? PyFloat_AsDouble(o) : 0.0;
+  if (PyErr_Occurred()) { PyErr_Clear(); return false; }
+  return PyFloat_Check(o) || PyLong_Check(o);
 }
 bool truth(PyObject* o) { return PyObject_IsTrue(o) == 1; }
 
@@ -672,6 +689,216 @@ PyObject* attn_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+struct HeadNorm {
+  const Tensor *qkv, *wq, *wk, *cs;
+  int64_t S, nq, nk, d;
+};
+// S, nq, nk, d from `sizes`, the operands that both directions have
+bool head_norm(const HeadNorm& given, PyObject* const* sizes, HeadNorm& a) {
+  a = given;
+  if (!int_arg(sizes[0], a.S) || !int_arg(sizes[1], a.nq) || !int_arg(sizes[2], a.nk) || !int_arg(sizes[3], a.d)) return false;
+  if (!fits(a.S) || a.nq < 0 || a.nk < 0 || a.nq + a.nk == 0 || a.nq + a.nk > 65536 || a.d < 1 || a.d > 512) return false;
+  if (!matrix(a.qkv, BF16) || a.qkv->size(1) != (a.nq + 2 * a.nk) * a.d || !fits(a.qkv->size(0)) || !here(*a.qkv)) return false;
+  for (const Tensor* w : {a.wq, a.wk})
+    if (!dense(w, BF16) || w->dim() != 1 || w->size(0) != a.d || !on(w, *a.qkv)) return false;
+  return a.cs == nullptr || (dense(a.cs, F32) && a.cs->dim() == 2 && a.cs->size(1) == a.d &&
+                             a.cs->size(0) >= std::min(a.S, a.qkv->size(0)) && on(a.cs, *a.qkv));
+}
+// qk_norm_rope_fwd(qkv, wq, wk, cs | None, S, nq, nk, d, eps, keep) -> (out, rstd), or (qkv, None) in place
+PyObject* qk_norm_rope_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(10)
+  HeadNorm a;
+  const Tensor* cs;
+  double eps;
+  if (!optional_tensor(args[3], cs) || !head_norm({tensor_of(args[0]), tensor_of(args[1]), tensor_of(args[2]), cs}, args + 4, a) ||
+      !float_arg(args[8], eps))
+    Py_RETURN_NONE;
+  const bool keep = truth(args[9]);
+  const int64_t T = a.qkv->size(0);
+  Tensor out, rstd;
+  if (keep) {
+    out = empty({T, a.qkv->size(1)}, *a.qkv, BF16);
+    rstd = empty({T, a.nq + a.nk}, *a.qkv, F32);
+  }
+  void* to = keep ? out.data_ptr() : ptr(a.qkv);
+  float* r = keep ? static_cast<float*>(rstd.data_ptr()) : nullptr;
+  const long ldx = a.qkv->stride(0), ldy = keep ? out.stride(0) : ldx;
+  const cudaStream_t s = stream();
+  if (!launch("qk_norm_rope_fwd", 1, [&] {
+        return lib.qk_norm_rope_fwd(ptr(a.qkv), to, ptr(a.wq), ptr(a.wk), static_cast<const float*>(ptr(a.cs)), r, int(T), int(a.S),
+                                    int(a.nq), int(a.nk), keep ? int(a.nk) : 0, int(a.d), ldx, ldy, float(eps), s);
+      }))
+    return nullptr;
+  if (!keep) return PyTuple_Pack(2, args[0], Py_None);
+  PyObject* pair = PyTuple_New(2);
+  if (pair == nullptr) return nullptr;
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(rstd)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+// qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs | None, S, nq, nk, d, gwq, gwk) -> dqkv
+PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(12)
+  HeadNorm a;
+  const Tensor *dy = tensor_of(args[0]), *rstd = tensor_of(args[4]), *gwq = tensor_of(args[10]), *gwk = tensor_of(args[11]), *cs;
+  if (!optional_tensor(args[5], cs) || !head_norm({tensor_of(args[1]), tensor_of(args[2]), tensor_of(args[3]), cs}, args + 6, a))
+    Py_RETURN_NONE;
+  const int64_t T = a.qkv->size(0);
+  if (!matrix(dy, BF16) || dy->sizes() != a.qkv->sizes() || !on(dy, *a.qkv) || ptr(dy) == ptr(a.qkv) || !dense(rstd, F32) ||
+      rstd->dim() != 2 || rstd->size(0) != T || rstd->size(1) != a.nq + a.nk || !on(rstd, *a.qkv) || !gradient(gwq) || !gradient(gwk) ||
+      gwq->scalar_type() != gwk->scalar_type() || gwq->dim() != 1 || gwk->dim() != 1 || gwq->size(0) != a.d || gwk->size(0) != a.d ||
+      !on(gwq, *a.qkv) || !on(gwk, *a.qkv))
+    Py_RETURN_NONE;
+  long floats = 0;
+  lib.qk_norm_rope_workspace(int(T), int(a.nq), int(a.nk), int(a.d), &floats);
+  const Tensor partial = empty({floats}, *a.qkv, F32);
+  const cudaStream_t s = stream();
+  if (!launch("qk_norm_rope_bwd", 2, [&] {
+        return lib.qk_norm_rope_bwd(ptr(dy), ptr(a.qkv), ptr(a.wq), ptr(a.wk), static_cast<float*>(ptr(rstd)),
+                                    static_cast<const float*>(ptr(a.cs)), static_cast<float*>(partial.data_ptr()), ptr(gwq), ptr(gwk),
+                                    int(T), int(a.S), int(a.nq), int(a.nk), int(a.d), a.qkv->stride(0), dy->stride(0),
+                                    gwq->scalar_type() == F32, s);
+      }))
+    return nullptr;
+  Py_INCREF(args[0]);
+  return args[0];
+  END_HANDLE_TH_ERRORS
+}
+
+// What the scaled embedding and its gradient have in common: ids, a table, positions of its type, S, offset, scale.
+struct Lookup {
+  const Tensor *ids, *table, *pos;
+  int64_t S, off;
+  double scale;
+  bool take(PyObject* const* rest) {   // positions | None, S, offset, scale
+    if (!optional_tensor(rest[0], pos) || !int_arg(rest[1], S) || !int_arg(rest[2], off) || !float_arg(rest[3], scale)) return false;
+    if (!gradient(table) || table->dim() != 2 || !fits(table->size(0)) || !fits(table->size(1)) || !here(*table) ||
+        !dense(ids, at::kLong) || !on(ids, *table) || !fits(ids->numel()) || !fits(S) || off < 0 || off > INT32_MAX / 2)
+      return false;
+    return pos == nullptr || (dense(pos, table->scalar_type()) && pos->dim() == 2 && pos->size(1) == table->size(1) &&
+                              pos->size(0) >= std::min(S, ids->numel()) + off && on(pos, *table));
+  }
+};
+// embedding_scaled(ids, table, positions | None, S, offset, scale) -> scale table[ids] (+ positions)
+PyObject* embedding_scaled(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(6)
+  Lookup a = {tensor_of(args[0]), tensor_of(args[1])};
+  if (!a.take(args + 2) || a.table->scalar_type() != BF16) Py_RETURN_NONE;
+  const int64_t T = a.ids->numel(), V = a.table->size(0), H = a.table->size(1);
+  Tensor out = empty({T, H}, *a.table, BF16);
+  const cudaStream_t s = stream();
+  if (!launch("embedding_scaled", 1, [&] {
+        return lib.embedding_scaled(static_cast<const long*>(ptr(a.ids)), ptr(a.table), ptr(a.pos), out.data_ptr(), int(T), int(H),
+                                    int(V), int(a.S), int(a.off), float(a.scale), s);
+      }))
+    return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+// embedding_by_token(ids, dout, dtable, dpositions | None, S, offset, scale) -> True
+PyObject* embedding_by_token(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(7)
+  Lookup a = {tensor_of(args[0]), tensor_of(args[2])};
+  const Tensor* dout = tensor_of(args[1]);
+  if (!a.take(args + 3)) Py_RETURN_NONE;
+  const int64_t T = a.ids->numel(), V = a.table->size(0), H = a.table->size(1);
+  if (!dense(dout, BF16) || dout->dim() != 2 || dout->size(0) != T || dout->size(1) != H || !on(dout, *a.table)) Py_RETURN_NONE;
+  long bytes = 0;
+  lib.embedding_by_token_workspace(int(T), int(H), &bytes);
+  const Tensor ws = empty({bytes}, *a.table, at::kByte);
+  const cudaStream_t s = stream();
+  if (!launch("embedding_by_token", 2 + (T > 1) + (a.pos != nullptr), [&] {
+        return lib.embedding_by_token(static_cast<const long*>(ptr(a.ids)), ptr(dout), ptr(a.table), ptr(a.pos), ws.data_ptr(), int(T),
+                                      int(H), int(V), int(a.S), int(a.off), float(a.scale), a.table->scalar_type() == F32, s);
+      }))
+    return nullptr;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// A list's tensors as zb_adamw_list reads them.
+struct AdamwTensor {
+  void *p, *m, *v, *mb, *vb, *g, *p16;
+  long n;
+  float step, inv_bc2;
+  unsigned seed, grad_f32;
+};
+// adamw_step(p, moments, g, p16, seeds | None, step, lr, beta1, beta2, eps, weight_decay, grad_scale) -> True; lists, step a number
+// or a list
+PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(12)
+  const Py_ssize_t n = PyList_Check(args[0]) ? PyList_GET_SIZE(args[0]) : 0;
+  auto list = [&](PyObject* o) { return PyList_Check(o) && PyList_GET_SIZE(o) == n; };
+  if (n == 0 || !list(args[1]) || !list(args[2]) || !list(args[3]) || !(args[4] == Py_None || list(args[4])) ||
+      !(PyLong_Check(args[5]) || list(args[5])))
+    Py_RETURN_NONE;
+  double h[6];   // lr, beta1, beta2, eps, weight_decay, grad_scale
+  for (int i = 0; i < 6; ++i)
+    if (!float_arg(args[6 + i], h[i])) Py_RETURN_NONE;
+  const Tensor* first = tensor_of(PyList_GET_ITEM(args[0], 0));
+  if (!dense(first, F32) || !here(*first)) Py_RETURN_NONE;
+  int bits = 0;
+  c10::SmallVector<AdamwTensor, 32> table;
+  c10::SmallVector<void*, 32> seen;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const Tensor *p = tensor_of(PyList_GET_ITEM(args[0], i)), *g = tensor_of(PyList_GET_ITEM(args[2], i)), *p16;
+    PyObject* mom = PyList_GET_ITEM(args[1], i);
+    int64_t k, seed = 0;
+    if (!optional_tensor(PyList_GET_ITEM(args[3], i), p16) || !PyTuple_Check(mom) ||
+        !int_arg(PyList_Check(args[5]) ? PyList_GET_ITEM(args[5], i) : args[5], k) || k < 1)
+      Py_RETURN_NONE;
+    const Py_ssize_t parts = PyTuple_GET_SIZE(mom);
+    if ((parts != 2 && parts != 4) || (bits != 0 && bits != (parts == 2 ? 32 : 8))) Py_RETURN_NONE;
+    bits = parts == 2 ? 32 : 8;
+    if (!dense(p, F32) || !gradient(g) || !on(p, *first) || !on(g, *first) || g->numel() != p->numel()) Py_RETURN_NONE;
+    const int64_t num = p->numel();
+    if (p16 != nullptr && (!dense(p16, BF16) || p16->numel() != num || !on(p16, *first))) Py_RETURN_NONE;
+    const Tensor* t[4];
+    for (Py_ssize_t j = 0; j < parts; ++j) {
+      t[j] = tensor_of(PyTuple_GET_ITEM(mom, j));
+      const bool base = parts == 4 && j % 2 == 1;
+      if (!dense(t[j], parts == 2 ? F32 : base ? at::kShort : at::kByte) || t[j]->numel() != (base ? (num + 255) / 256 : num) ||
+          !on(t[j], *first))
+        Py_RETURN_NONE;
+    }
+    if (bits == 8 && (args[4] == Py_None || !int_arg(PyList_GET_ITEM(args[4], i), seed))) Py_RETURN_NONE;
+    if (num == 0) continue;
+    AdamwTensor a = {};
+    a.p = ptr(p);
+    a.m = ptr(t[0]);
+    a.v = ptr(t[parts / 2]);
+    if (bits == 8) {
+      a.mb = ptr(t[1]);
+      a.vb = ptr(t[3]);
+    }
+    a.g = ptr(g);
+    a.p16 = ptr(p16);
+    a.n = num;
+    a.step = float(h[0] / (1 - std::pow(h[1], double(k))));
+    a.inv_bc2 = float(1 / std::sqrt(1 - std::pow(h[2], double(k))));
+    a.seed = static_cast<unsigned>(seed);
+    a.grad_f32 = g->scalar_type() == F32;
+    table.push_back(a);
+    seen.push_back(a.p);
+  }
+  std::sort(seen.begin(), seen.end());
+  if (table.empty() || std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+  const cudaStream_t s = stream();
+  if (!launch("adamw", 1, [&] {
+        return lib.adamw_list(table.data(), int(table.size()), bits, float(h[1]), float(1 - h[1]), float(h[2]), float(1 - h[2]),
+                              float(h[3]), float(1 - h[0] * h[4]), float(h[5]), s);
+      }))
+    return nullptr;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // init(addresses of the entry points in Entry's order, KernelError)
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ZB_ARGS(2)
@@ -708,6 +935,8 @@ PyMethodDef methods[] = {ZB_FN(init), ZB_FN(set_status), ZB_FN(launch_count), ZB
                          ZB_FN(linear_wgrad), ZB_FN(act_linear_fwd), ZB_FN(act_linear_dgrad), ZB_FN(linear_rope_fwd),
                          ZB_FN(norm_fwd), ZB_FN(norm_bwd), ZB_FN(finish), ZB_FN(rope), ZB_FN(swiglu_fwd),
                          ZB_FN(swiglu_bwd), ZB_FN(act_fwd), ZB_FN(act_bwd), ZB_FN(attn_fwd), ZB_FN(attn_bwd),
+                         ZB_FN(qk_norm_rope_fwd), ZB_FN(qk_norm_rope_bwd), ZB_FN(embedding_scaled), ZB_FN(embedding_by_token),
+                         ZB_FN(adamw_step),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "zorse_fastops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

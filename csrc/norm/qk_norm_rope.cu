@@ -20,36 +20,18 @@ struct QkNormArgs {
   float* partial;           // backward: [CTAs, 2, d]
   long ldx, ldy;
   int T, S, nq, nk, nv, d;  // nv: value heads to copy (forward into another tensor), else 0
-  float eps;
+  int span;                 // forward: units of a warp's item
+  float eps, inv_d;
 };
 
 // Sixteen values of a head per lane: eight from either half, so that a lane has both members of its pairs.
 struct HeadChunk {
   uint4 lo, hi;
 };
-__device__ __forceinline__ void unpack16(const HeadChunk& h, float (&f)[16]) {
-  unpack8(h.lo, f);
-  unpack8(h.hi, f + 8);
-}
-__device__ __forceinline__ HeadChunk pack16(const float (&f)[16]) { return {pack8(f), pack8(f + 8)}; }
 __device__ __forceinline__ HeadChunk load_head(const __nv_bfloat16* p, int half) { return {ld_v4(p), ld_v4(p + half)}; }
 __device__ __forceinline__ void store_head(__nv_bfloat16* p, int half, const HeadChunk& h) {
   *reinterpret_cast<uint4*>(p) = h.lo;
   *reinterpret_cast<uint4*>(p + half) = h.hi;
-}
-// f becomes R f (sign 1) or R^T f (sign -1); row: the cosines of the position
-__device__ __forceinline__ void rotate16(float (&f)[16], const float* row, int c, int half, float sign) {
-#pragma unroll
-  for (int k = 0; k < 8; k += 4) {
-    const float4 co = *reinterpret_cast<const float4*>(row + c + k), si = *reinterpret_cast<const float4*>(row + half + c + k);
-    const float cc[4] = {co.x, co.y, co.z, co.w}, ss[4] = {si.x, si.y, si.z, si.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a = f[k + j], b = f[8 + k + j], s = ss[j] * sign;
-      f[k + j] = a * cc[j] - b * s;
-      f[8 + k + j] = b * cc[j] + a * s;
-    }
-  }
 }
 template <int LANES>
 __device__ __forceinline__ float head_sum(float v) {
@@ -57,103 +39,268 @@ __device__ __forceinline__ float head_sum(float v) {
   for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-// LANES lanes share a head (a power of two, at least d / 16: for d = 96 two of eight idle); a warp takes 32 / LANES heads of a token.
-template <int LANES>
-__global__ void __launch_bounds__(256) qk_norm_rope_fwd_kernel(const QkNormArgs a) {
-  chain_trigger();
-  chain_wait();
-  constexpr int HEADS = 32 / LANES;
-  const int half = a.d >> 1, lane = threadIdx.x & 31, c = (lane % LANES) * 8;
-  const bool used = c < half;
-  const int nqk = a.nq + a.nk, heads = nqk + a.nv, groups = (heads + HEADS - 1) / HEADS;
-  const long items = long(a.T) * groups;
-  for (long i = blockIdx.x * 8L + (threadIdx.x >> 5); i < items; i += gridDim.x * 8L) {
-    const int t = int(i / groups), h = int(i - long(t) * groups) * HEADS + lane / LANES;
-    const bool live = used && h < heads;
-    const size_t col = size_t(h) * a.d + c;
-    HeadChunk u = {};
-    if (live) u = load_head(a.x + t * a.ldx + col, half);
-    float f[16], ss = 0.f;
-    unpack16(u, f);
+__device__ __forceinline__ void load_angles(const float* row, int half, float (&co)[8], float (&si)[8]) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) ss += f[j] * f[j];
-    const float rstd = rsqrtf(head_sum<LANES>(ss) / a.d + a.eps);
-    if (!live) continue;
-    if (h < nqk) {
-      const HeadChunk wu = load_head((h < a.nq ? a.wq : a.wk) + c, half);
-      float w[16];
-      unpack16(wu, w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) f[j] *= rstd * w[j];
-      if (a.cs != nullptr) rotate16(f, a.cs + size_t(t % a.S) * a.d, c, half, 1.f);
-      u = pack16(f);
-      if (a.rstd != nullptr && c == 0) a.rstd[long(t) * nqk + h] = rstd;
-    }
-    store_head(a.y + t * a.ldy + col, half, u);
+  for (int k = 0; k < 8; k += 4) {
+    *reinterpret_cast<float4*>(co + k) = *reinterpret_cast<const float4*>(row + k);
+    *reinterpret_cast<float4*>(si + k) = *reinterpret_cast<const float4*>(row + half + k);
   }
 }
 
-template <int LANES>
+// Bytes on the way bound these passes: with a unit's operands in registers, and a hundred of those a thread, an SM has too few
+// requests out.  So every thread copies its own chunks some units ahead into a ring of its own in shared memory.
+constexpr int QK_RING = 3;
+// Two values an instruction (fma.rn.f32x2 and the like): a head's arithmetic is most of what an SM issues here.
+struct Pair {
+  float a, b;
+};
+__device__ __forceinline__ Pair operator*(Pair x, Pair y) {
+  Pair r;
+  fmul2(r.a, r.b, x.a, x.b, y.a, y.b);
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair x, Pair y, Pair z) {
+  Pair r;
+  ffma2(r.a, r.b, x.a, x.b, y.a, y.b, z.a, z.b);
+  return r;
+}
+__device__ __forceinline__ Pair both(float v) { return {v, v}; }
+__device__ __forceinline__ Pair pair_of(uint32_t u) {
+  const float2 f = unpack_bf16x2(u);
+  return {f.x, f.y};
+}
+// A head chunk as pairs: 0 .. 3 of the low half, 4 .. 7 of the high one
+__device__ __forceinline__ void unpack_pairs(const HeadChunk& h, Pair (&p)[8]) {
+  p[0] = pair_of(h.lo.x); p[1] = pair_of(h.lo.y); p[2] = pair_of(h.lo.z); p[3] = pair_of(h.lo.w);
+  p[4] = pair_of(h.hi.x); p[5] = pair_of(h.hi.y); p[6] = pair_of(h.hi.z); p[7] = pair_of(h.hi.w);
+}
+__device__ __forceinline__ HeadChunk pack_pairs(const Pair (&p)[8]) {
+  HeadChunk h;
+  h.lo = make_uint4(pack_bf16x2(p[0].a, p[0].b), pack_bf16x2(p[1].a, p[1].b), pack_bf16x2(p[2].a, p[2].b), pack_bf16x2(p[3].a, p[3].b));
+  h.hi = make_uint4(pack_bf16x2(p[4].a, p[4].b), pack_bf16x2(p[5].a, p[5].b), pack_bf16x2(p[6].a, p[6].b), pack_bf16x2(p[7].a, p[7].b));
+  return h;
+}
+__device__ __forceinline__ float sum_of_squares(const Pair (&x)[8]) {
+  Pair s = x[0] * x[0];
+#pragma unroll
+  for (int j = 1; j < 8; ++j) s = fma2(x[j], x[j], s);
+  return s.a + s.b;
+}
+
+// LANES lanes share a head (a power of two, at least d / 16: for d = 96 two of eight idle); a warp takes 32 / LANES neighbouring
+// heads at a time, a unit.  A warp's item is `span` units of one token in a row.  The weights of a lane's kind of head and the
+// token's angles are multiplied once for all its heads: lo = x_lo a - x_hi b, hi = x_hi c + x_lo d, times rstd.
+template <int LANES, bool ROPE>
+__global__ void __launch_bounds__(128, 6) qk_norm_rope_fwd_kernel(const QkNormArgs a) {
+  chain_trigger();
+  chain_wait();
+  constexpr int HEADS = 32 / LANES;
+  __shared__ uint4 ring[QK_RING][2][128];
+  const int half = a.d >> 1, lane = threadIdx.x & 31, c = (lane % LANES) * 8;
+  const int nqk = a.nq + a.nk, units = (nqk + a.nv + HEADS - 1) / HEADS;
+  const unsigned parts = (units + a.span - 1) / a.span, i = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (i >= unsigned(a.T) * parts) return;
+  const int t = int(i / parts), first = int(i - t * parts) * a.span;
+  int h = first * HEADS + lane / LANES;                       // this lane's head, HEADS further on with every unit
+  const int end = c < half ? min(nqk + a.nv, (first + a.span) * HEADS) : 0;
+  const __nv_bfloat16* src = a.x + t * a.ldx + h * a.d + c;
+  __nv_bfloat16* dst = a.y + t * a.ldy + h * a.d + c;
+  const int step = HEADS * a.d;
+  int ahead = h;
+  auto request = [&](int slot) {
+    if (ahead < end) {
+      ring_load16(&ring[slot][0][threadIdx.x], src);
+      ring_load16(&ring[slot][1][threadIdx.x], src + half);
+      ahead += HEADS;
+      src += step;
+    }
+    ring_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < QK_RING - 1; ++k) request(k);
+  const float* angles = ROPE ? a.cs + size_t(t % a.S) * a.d + c : nullptr;
+  Pair lo_lo[4], lo_hi[4], hi_hi[4], hi_lo[4];
+  int kind = -1, slot = 0;
+  const int last = min(first + a.span, units);
+  for (int u = first; u < last; ++u) {
+    const int now = h < a.nq ? 0 : 1;
+    if (now != kind && h < nqk && c < half) {
+      kind = now;
+      Pair w[8];
+      unpack_pairs(load_head((now ? a.wk : a.wq) + c, half), w);
+      float co[8], si[8];
+      if (ROPE) load_angles(angles, half, co, si);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo_lo[j] = w[j];
+        hi_hi[j] = w[4 + j];
+        if (ROPE) {
+          const Pair cc = {co[2 * j], co[2 * j + 1]}, ss = {si[2 * j], si[2 * j + 1]};
+          lo_lo[j] = w[j] * cc;
+          hi_hi[j] = w[4 + j] * cc;
+          lo_hi[j] = w[4 + j] * Pair{-ss.a, -ss.b};
+          hi_lo[j] = w[j] * ss;
+        }
+      }
+    }
+    request((slot + QK_RING - 1) % QK_RING);
+    ring_wait<QK_RING - 1>();
+    HeadChunk out = {};
+    if (h < end) out = {ring[slot][0][threadIdx.x], ring[slot][1][threadIdx.x]};
+    slot = (slot + 1) % QK_RING;
+    Pair x[8];
+    unpack_pairs(out, x);
+    const float rstd = rsqrtf(head_sum<LANES>(sum_of_squares(x)) * a.inv_d + a.eps);
+    if (h < end) {
+      if (h < nqk) {
+        Pair y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const Pair lo = x[j] * both(rstd), hi = x[4 + j] * both(rstd);
+          y[j] = ROPE ? fma2(hi, lo_hi[j], lo * lo_lo[j]) : lo * lo_lo[j];
+          y[4 + j] = ROPE ? fma2(lo, hi_lo[j], hi * hi_hi[j]) : hi * hi_hi[j];
+        }
+        out = pack_pairs(y);
+        if (a.rstd != nullptr && c == 0) a.rstd[long(t) * nqk + h] = rstd;
+      }
+      store_head(dst, half, out);
+    }
+    h += HEADS;
+    dst += step;
+  }
+}
+
+struct QkRing {
+  uint4 chunk[QK_RING][4][256];    // x low, x high, gradient low, gradient high
+  float rstd[QK_RING][256];
+};
+// A warp takes an equal stretch of the units of all tokens, for either kind; the ring runs on over its tokens.
+template <int LANES, bool ROPE>
 __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs a) {
   chain_trigger();
   chain_wait();
   constexpr int HEADS = 32 / LANES;
+  extern __shared__ __align__(16) unsigned char raw[];
+  QkRing& ring = *reinterpret_cast<QkRing*>(raw);
   __shared__ float part[8][LANES * 16];
-  const int half = a.d >> 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (lane % LANES) * 8;
+  const int tid = threadIdx.x, half = a.d >> 1, lane = tid & 31, warp = tid >> 5, c = (lane % LANES) * 8, sub = lane / LANES;
   const bool used = c < half;
+  const int step = HEADS * a.d, nqk = a.nq + a.nk;
   for (int kind = 0; kind < 2; ++kind) {          // query heads, then key heads: one set of weight-gradient sums at a time
-    const int n = kind ? a.nk : a.nq, h0 = kind ? a.nq : 0, groups = (n + HEADS - 1) / HEADS;
-    float w[16], dw[16];
+    const int n = kind ? a.nk : a.nq, h0 = kind ? a.nq : 0, units = (n + HEADS - 1) / HEADS;
+    if (n == 0) {
+      for (int j = tid; j < a.d; j += 256) a.partial[(size_t(blockIdx.x) * 2 + kind) * a.d + j] = 0.f;
+      continue;
+    }
+    Pair w[8], dw[8];
     HeadChunk wu = {};
     if (used) wu = load_head((kind ? a.wk : a.wq) + c, half);
-    unpack16(wu, w);
+    unpack_pairs(wu, w);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) dw[j] = 0.f;
-    const long items = long(a.T) * groups;
-    for (long i = blockIdx.x * 8L + warp; i < items; i += gridDim.x * 8L) {
-      const int t = int(i / groups), k = int(i - long(t) * groups) * HEADS + lane / LANES, h = h0 + k;
-      const bool live = used && k < n;
-      const size_t col = size_t(h) * a.d + c;
-      HeadChunk xu = {}, gu = {};
-      float rstd = 0.f;
-      if (live) {
-        xu = load_head(a.x + t * a.ldx + col, half);
-        gu = load_head(a.y + t * a.ldy + col, half);
-        rstd = a.rstd[long(t) * (a.nq + a.nk) + h];
+    for (int j = 0; j < 8; ++j) dw[j] = both(0.f);
+    const long all = long(a.T) * units, me = blockIdx.x * 8 + warp, warps = gridDim.x * 8;
+    const long first = all * me / warps;
+    int left = int(all * (me + 1) / warps - first), to_ask = left;
+    unsigned t = unsigned(first / units);
+    int u = int(first - long(t) * units);
+    // the next unit to ask for: its number in the token, this lane's head among the kind's, and where that lies
+    int ask_u = u, ask_k = u * HEADS + sub;
+    size_t col = size_t(h0 + ask_k) * a.d + c;
+    const __nv_bfloat16 *ask_x = a.x + t * a.ldx + col, *ask_g = a.y + t * a.ldy + col;
+    __nv_bfloat16* dst = a.y + t * a.ldy + col;
+    const float* ask_r = a.rstd + size_t(t) * nqk + h0 + ask_k;
+    const long next_x = a.ldx - long(units) * step, next_g = a.ldy - long(units) * step;   // from behind a token's units to the next one's
+    auto request = [&](int slot) {
+      if (to_ask > 0) {
+        if (used && ask_k < n) {
+          ring_load16(&ring.chunk[slot][0][tid], ask_x);
+          ring_load16(&ring.chunk[slot][1][tid], ask_x + half);
+          ring_load16(&ring.chunk[slot][2][tid], ask_g);
+          ring_load16(&ring.chunk[slot][3][tid], ask_g + half);
+          ring_load4(&ring.rstd[slot][tid], ask_r);
+        }
+        --to_ask;
+        ask_x += step;
+        ask_g += step;
+        ask_r += HEADS;
+        ask_k += HEADS;
+        if (++ask_u == units) {
+          ask_u = 0;
+          ask_k = sub;
+          ask_x += next_x;
+          ask_g += next_g;
+          ask_r += nqk - units * HEADS;
+        }
       }
-      float x[16], g[16], along = 0.f;
-      unpack16(xu, x);
-      unpack16(gu, g);
-      if (a.cs != nullptr && live) rotate16(g, a.cs + size_t(t % a.S) * a.d, c, half, -1.f);
+      ring_commit();
+    };
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        x[j] *= rstd;
-        dw[j] += g[j] * x[j];
-        g[j] *= w[j];
-        along += g[j] * x[j];
+    for (int k = 0; k < QK_RING - 1; ++k) request(k);
+    int slot = 0, pos = int(t % unsigned(a.S));
+    while (left > 0) {
+      float co[8] = {}, si[8] = {};
+      if (ROPE && used) load_angles(a.cs + size_t(pos) * a.d + c, half, co, si);
+      const int here = min(left, units - u);
+      left -= here;
+      int k = u * HEADS + sub;
+      for (int i = 0; i < here; ++i) {
+        request((slot + QK_RING - 1) % QK_RING);
+        ring_wait<QK_RING - 1>();
+        const bool live = used && k < n;
+        HeadChunk xu = {}, gu = {};
+        float rstd = 0.f;
+        if (live) {
+          xu = {ring.chunk[slot][0][tid], ring.chunk[slot][1][tid]};
+          gu = {ring.chunk[slot][2][tid], ring.chunk[slot][3][tid]};
+          rstd = ring.rstd[slot][tid];
+        }
+        slot = (slot + 1) % QK_RING;
+        // with g = rstd R^T dy:  dw += g x,  dx = w g - x rstd^2 mean(w g x)
+        Pair x[8], g[8], along = both(0.f);
+        unpack_pairs(xu, x);
+        unpack_pairs(gu, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const Pair lo = g[j] * both(rstd), hi = g[4 + j] * both(rstd);
+          const Pair cc = {co[2 * j], co[2 * j + 1]}, ss = {si[2 * j], si[2 * j + 1]}, back = {-ss.a, -ss.b};
+          g[j] = ROPE ? fma2(hi, ss, lo * cc) : lo;
+          g[4 + j] = ROPE ? fma2(lo, back, hi * cc) : hi;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          dw[j] = fma2(g[j], x[j], dw[j]);
+          g[j] = g[j] * w[j];
+          along = fma2(g[j], x[j], along);
+        }
+        const float m = -head_sum<LANES>(along.a + along.b) * a.inv_d * (rstd * rstd);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = fma2(x[j], both(m), g[j]);
+        if (live) store_head(dst, half, pack_pairs(g));
+        k += HEADS;
+        dst += step;
       }
-      along = head_sum<LANES>(along) / a.d;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) g[j] = rstd * (g[j] - x[j] * along);
-      if (live) store_head(a.y + t * a.ldy + col, half, pack16(g));
+      u = 0;
+      dst += next_g;
+      pos = pos + 1 == a.S ? 0 : pos + 1;
     }
+    ring_wait<0>();
     // over the heads of a warp, then over its CTA's warps
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-#pragma unroll
-      for (int o = 16; o >= LANES; o >>= 1) dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], o);
-    }
     __syncthreads();
-    if (lane < LANES && used) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        part[warp][c + j] = dw[j];
-        part[warp][half + c + j] = dw[8 + j];
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int o = 16; o >= LANES; o >>= 1) {
+        dw[j].a += __shfl_xor_sync(0xffffffffu, dw[j].a, o);
+        dw[j].b += __shfl_xor_sync(0xffffffffu, dw[j].b, o);
+      }
+      if (lane < LANES && used) {
+        const int at = (j < 4 ? 0 : half) + c + 2 * (j & 3);
+        part[warp][at] = dw[j].a;
+        part[warp][at + 1] = dw[j].b;
       }
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < a.d; j += 256) {
+    for (int j = tid; j < a.d; j += 256) {
       float s = 0.f;
 #pragma unroll
       for (int v = 0; v < 8; ++v) s += part[v][j];
@@ -162,21 +309,23 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs 
   }
 }
 
-// slot[j] += sum over `rows` of partial[row][j], in a fixed order: 32 columns per CTA, eight warps over the rows.
+// slot[j] += sum over `rows` of partial[row][j], in a fixed order: 32 columns per CTA, its warps over the rows.
 template <typename GT>
-__global__ void __launch_bounds__(256) qk_norm_weight_grad_kernel(const float* partial, GT* gwq, GT* gwk, int rows, int d) {
+__global__ void __launch_bounds__(1024) qk_norm_weight_grad_kernel(const float* partial, GT* gwq, GT* gwk, int rows, int d) {
   chain_trigger();
   chain_wait();
-  __shared__ float part[8][32];
+  __shared__ float part[32][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (col < 2 * d)
-    for (int r = warp; r < rows; r += 8) s += partial[size_t(r) * 2 * d + col];
+  if (col < 2 * d) {
+#pragma unroll 8
+    for (int r = warp; r < rows; r += 32) s += partial[size_t(r) * 2 * d + col];
+  }
   part[warp][lane] = s;
   __syncthreads();
   if (warp != 0 || col >= 2 * d) return;
 #pragma unroll
-  for (int v = 1; v < 8; ++v) s += part[v][lane];
+  for (int v = 1; v < 32; ++v) s += part[v][lane];
   GT* slot = col < d ? gwq + col : gwk + (col - d);
   *slot = GT(float(*slot) + s);
 }
@@ -186,15 +335,23 @@ static int qk_norm_lanes(int d) {
   while (n * 16 < d) n *= 2;
   return n;
 }
+// Units to a warp's item: as many of a token's as leave `warps` warps with work, so that its angles are loaded and multiplied
+// out for many heads, but not for so many that the last items run alone.
+static int qk_norm_span(long T, int units, long warps, int most) {
+  const long s = T * units / warps;
+  return int(s < 1 ? 1 : s > most ? most : s);
+}
 static int qk_norm_bwd_ctas(int T, int nq, int nk, int d) {
   const int per = 32 / qk_norm_lanes(d), most = nq > nk ? nq : nk;
-  const long want = (long(T) * ((most + per - 1) / per) + 7) / 8, cap = long(num_sms()) * 3;
+  const long want = (long(T) * ((most + per - 1) / per) + 7) / 8, cap = long(num_sms()) * 2;
   return int(want < cap ? want : cap);
 }
 
 static int qk_norm_check(const QkNormArgs& a) {
   if (a.d % 16 != 0 || a.d < 16 || a.d > 512) ZB_FAIL(-1, "qk_norm_rope: head width %d is not a multiple of 16 up to 512", a.d);
   if (a.nq < 0 || a.nk < 0 || a.nv < 0 || a.S < 1) ZB_FAIL(-1, "qk_norm_rope: %d + %d heads, sequences of %d", a.nq, a.nk, a.S);
+  // units of all tokens, and what a warp of the last CTA counts up to behind them, in 32 bits
+  if (long(a.T) * (a.nq + a.nk + a.nv + 3) >= (1L << 31) - (1L << 20)) ZB_FAIL(-1, "qk_norm_rope: %d tokens of %d heads", a.T, a.nq + a.nk);
   if (a.ldx % 8 != 0 || a.ldy % 8 != 0) ZB_FAIL(-1, "qk_norm_rope: row strides %ld, %ld not a multiple of 8", a.ldx, a.ldy);
   if ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.wq) |
        reinterpret_cast<uintptr_t>(a.wk) | reinterpret_cast<uintptr_t>(a.cs)) & 15)
@@ -202,15 +359,21 @@ static int qk_norm_check(const QkNormArgs& a) {
   return 0;
 }
 
-#define QK_NORM_LAUNCH(KERNEL, GRID)                                                                        \
-  switch (qk_norm_lanes(a.d)) {                                                                             \
-    case 1: ZB_CUDA_OK(launch_pass(KERNEL<1>, GRID, 256, 0, stream, a)); break;                             \
-    case 2: ZB_CUDA_OK(launch_pass(KERNEL<2>, GRID, 256, 0, stream, a)); break;                             \
-    case 4: ZB_CUDA_OK(launch_pass(KERNEL<4>, GRID, 256, 0, stream, a)); break;                             \
-    case 8: ZB_CUDA_OK(launch_pass(KERNEL<8>, GRID, 256, 0, stream, a)); break;                             \
-    case 16: ZB_CUDA_OK(launch_pass(KERNEL<16>, GRID, 256, 0, stream, a)); break;                           \
-    default: ZB_CUDA_OK(launch_pass(KERNEL<32>, GRID, 256, 0, stream, a)); break;                           \
-  }
+template <int LANES>
+static int qk_norm_fwd_launch(const QkNormArgs& a, int grid, cudaStream_t stream) {
+  auto kern = qk_norm_rope_fwd_kernel<LANES, true>;
+  if (a.cs == nullptr) kern = qk_norm_rope_fwd_kernel<LANES, false>;
+  ZB_CUDA_OK(launch_pass(kern, grid, 128, 0, stream, a));
+  return 0;
+}
+template <int LANES>
+static int qk_norm_bwd_launch(const QkNormArgs& a, int grid, cudaStream_t stream) {
+  auto kern = qk_norm_rope_bwd_kernel<LANES, true>;
+  if (a.cs == nullptr) kern = qk_norm_rope_bwd_kernel<LANES, false>;
+  ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(QkRing))));
+  ZB_CUDA_OK(launch_pass(kern, grid, 256, sizeof(QkRing), stream, a));
+  return 0;
+}
 
 }  // namespace zb
 
@@ -223,15 +386,20 @@ int zb_qk_norm_rope_fwd(const void* x, void* y, const void* wq, const void* wk, 
   a.x = static_cast<const __nv_bfloat16*>(x); a.y = static_cast<__nv_bfloat16*>(y);
   a.wq = static_cast<const __nv_bfloat16*>(wq); a.wk = static_cast<const __nv_bfloat16*>(wk);
   a.cs = cs; a.rstd = rstd; a.ldx = ldx; a.ldy = ldy;
-  a.T = T; a.S = S; a.nq = nq; a.nk = nk; a.nv = nv; a.d = d; a.eps = eps;
+  a.T = T; a.S = S; a.nq = nq; a.nk = nk; a.nv = nv; a.d = d; a.eps = eps; a.inv_d = 1.f / d;
   if (int rc = qk_norm_check(a)) return rc;
-  const int per = 32 / qk_norm_lanes(d);
-  const long items = long(T) * ((nq + nk + nv + per - 1) / per);
-  if (items <= 0) return 0;
-  const long ctas = (items + 7) / 8, cap = long(num_sms()) * 16;
-  const int grid = int(ctas < cap ? ctas : cap);
-  QK_NORM_LAUNCH(qk_norm_rope_fwd_kernel, grid)
-  return 0;
+  const int per = 32 / qk_norm_lanes(d), units = (nq + nk + nv + per - 1) / per;
+  if (T <= 0 || units == 0) return 0;
+  a.span = qk_norm_span(T, units, long(num_sms()) * 48, 6);
+  const int grid = int((long(T) * ((units + a.span - 1) / a.span) + 3) / 4);
+  switch (qk_norm_lanes(d)) {
+    case 1: return qk_norm_fwd_launch<1>(a, grid, stream);
+    case 2: return qk_norm_fwd_launch<2>(a, grid, stream);
+    case 4: return qk_norm_fwd_launch<4>(a, grid, stream);
+    case 8: return qk_norm_fwd_launch<8>(a, grid, stream);
+    case 16: return qk_norm_fwd_launch<16>(a, grid, stream);
+    default: return qk_norm_fwd_launch<32>(a, grid, stream);
+  }
 }
 
 // *floats: what zb_qk_norm_rope_bwd wants as workspace
@@ -249,17 +417,26 @@ int zb_qk_norm_rope_bwd(void* dy, const void* x, const void* wq, const void* wk,
   a.x = static_cast<const __nv_bfloat16*>(x); a.y = static_cast<__nv_bfloat16*>(dy);
   a.wq = static_cast<const __nv_bfloat16*>(wq); a.wk = static_cast<const __nv_bfloat16*>(wk);
   a.cs = cs; a.rstd = rstd; a.partial = partial; a.ldx = ldx; a.ldy = ldy;
-  a.T = T; a.S = S; a.nq = nq; a.nk = nk; a.d = d;
+  a.T = T; a.S = S; a.nq = nq; a.nk = nk; a.d = d; a.inv_d = 1.f / d;
   if (int rc = qk_norm_check(a)) return rc;
   if (T <= 0 || nq + nk == 0) return 0;
   const int grid = qk_norm_bwd_ctas(T, nq, nk, d);
-  QK_NORM_LAUNCH(qk_norm_rope_bwd_kernel, grid)
+  int rc;
+  switch (qk_norm_lanes(d)) {
+    case 1: rc = qk_norm_bwd_launch<1>(a, grid, stream); break;
+    case 2: rc = qk_norm_bwd_launch<2>(a, grid, stream); break;
+    case 4: rc = qk_norm_bwd_launch<4>(a, grid, stream); break;
+    case 8: rc = qk_norm_bwd_launch<8>(a, grid, stream); break;
+    case 16: rc = qk_norm_bwd_launch<16>(a, grid, stream); break;
+    default: rc = qk_norm_bwd_launch<32>(a, grid, stream); break;
+  }
+  if (rc) return rc;
   const int columns = (2 * d + 31) / 32;
   if (grad_f32)
-    ZB_CUDA_OK(launch_pass(qk_norm_weight_grad_kernel<float>, columns, 256, 0, stream, partial, static_cast<float*>(gwq),
+    ZB_CUDA_OK(launch_pass(qk_norm_weight_grad_kernel<float>, columns, 1024, 0, stream, partial, static_cast<float*>(gwq),
                            static_cast<float*>(gwk), grid, d));
   else
-    ZB_CUDA_OK(launch_pass(qk_norm_weight_grad_kernel<__nv_bfloat16>, columns, 256, 0, stream, partial,
+    ZB_CUDA_OK(launch_pass(qk_norm_weight_grad_kernel<__nv_bfloat16>, columns, 1024, 0, stream, partial,
                            static_cast<__nv_bfloat16*>(gwq), static_cast<__nv_bfloat16*>(gwk), grid, d));
   return 0;
 }

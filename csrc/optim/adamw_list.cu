@@ -20,7 +20,7 @@
 namespace zb {
 
 constexpr int ADAMW_BLOCK = 256;                     // values with one base; a warp's work at a time
-constexpr int ADAMW_TILE = 8 * ADAMW_BLOCK;          // a CTA's
+constexpr int ADAMW_CTAS = 3;                        // on an SM
 
 struct AdamwTensor {                                 // as the caller packs it
   float* p;
@@ -38,47 +38,79 @@ struct AdamwHyper {
 template <int N>
 struct AdamwList {
   AdamwTensor t[N];
-  long end[N];                                       // tiles up to and with this tensor
+  long end[N];                                       // blocks up to and with this tensor
   int count;
   AdamwHyper h;
 };
 
-// one operation, rounded to nearest, subnormals kept
-__device__ __forceinline__ float mul1(float a, float b) {
-  float d;
-  asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
+// Two values an instruction, every operation rounded to nearest by itself, subnormals kept.  (A packed product and a packed sum
+// behind it come out as one fma in spite of their rounding modifiers; a scalar sum does not join a packed product.)
+struct Pair {
+  float a, b;
+};
+__device__ __forceinline__ Pair operator*(Pair x, Pair y) {
+  Pair r;
+  fmul2(r.a, r.b, x.a, x.b, y.a, y.b);
+  return r;
 }
-__device__ __forceinline__ float add1(float a, float b) {
-  float d;
-  asm("add.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
+__device__ __forceinline__ Pair operator+(Pair x, Pair y) {
+  Pair r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r.a) : "f"(x.a), "f"(y.a));
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r.b) : "f"(x.b), "f"(y.b));
+  return r;
 }
+__device__ __forceinline__ Pair fma2(Pair x, Pair y, Pair z) {
+  Pair r;
+  ffma2(r.a, r.b, x.a, x.b, y.a, y.b, z.a, z.b);
+  return r;
+}
+__device__ __forceinline__ Pair both(float v) { return {v, v}; }
 
-__device__ __forceinline__ unsigned adamw_hash(unsigned pair, unsigned seed) {
-  unsigned x = pair * 0x9E3779B1u + seed;
+__device__ __forceinline__ unsigned adamw_hash(unsigned pair_times_weyl_plus_seed) {
+  unsigned x = pair_times_weyl_plus_seed;
   x = (x ^ (x >> 15)) * 0x6A09E667u;
   x = (x ^ (x >> 13)) * 0xBB67AE85u;
   return x ^ (x >> 16);
 }
-__device__ __forceinline__ unsigned decode_bits(unsigned code, unsigned base) { return code ? (code + base) << 20 : 0u; }
-__device__ __forceinline__ float decode_m(unsigned byte, unsigned base) {
-  return __uint_as_float(decode_bits(byte & 0x7fu, base) | (byte & 0x80u) << 24);
+constexpr unsigned ADAMW_WEYL = 0x9E3779B1u;
+
+// Byte J of a word of codes, shifted to bits 20 .. 27
+template <int J>
+__device__ __forceinline__ unsigned code_at_20(unsigned word, unsigned mask) {
+  const unsigned t = word & (mask << (8 * J));
+  return J < 3 ? t << (20 - 8 * J) : t >> 4;
+}
+__device__ __forceinline__ bool has_zero_byte(unsigned w) { return ((w - 0x01010101u) & ~w & 0x80808080u) != 0; }
+// The patterns of four values from their codes; base20: the block's base, shifted.  ZEROS: some code may be 0
+template <bool ZEROS>
+__device__ __forceinline__ void decode4(unsigned word, unsigned mask, unsigned base20, unsigned (&u)[4]) {
+  u[0] = code_at_20<0>(word, mask); u[1] = code_at_20<1>(word, mask); u[2] = code_at_20<2>(word, mask); u[3] = code_at_20<3>(word, mask);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) u[j] = ZEROS && u[j] == 0 ? 0 : u[j] + base20;
+}
+__device__ __forceinline__ void decode_v4(unsigned word, unsigned base20, float (&f)[4]) {
+  unsigned u[4];
+  if (has_zero_byte(word)) decode4<true>(word, 0xffu, base20, u);
+  else decode4<false>(word, 0xffu, base20, u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(u[j]);
+}
+__device__ __forceinline__ void decode_m4(unsigned word, unsigned base20, float (&f)[4]) {
+  unsigned u[4];
+  if (has_zero_byte(word & 0x7f7f7f7fu)) decode4<true>(word, 0x7fu, base20, u);
+  else decode4<false>(word, 0x7fu, base20, u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(u[j] | (word << (24 - 8 * j) & 0x80000000u));
 }
 // The base of a block whose largest pattern is `top`: the highest code that a dither can give still fits
 __device__ __forceinline__ int code_base(unsigned top, int most) {
   const int b = int((top + 0xfffffu) >> 20) - most;
   return b > 0 ? b : 0;
 }
-constexpr unsigned ADAMW_TOP = 0x7fe00000u;          // NaNs are held as this one, and keep clear of the sign bit
+constexpr unsigned ADAMW_INF = 0x7f800000u, ADAMW_TOP = 0x7fe00000u;   // NaNs are held as the second one, clear of the sign bit
 
-__device__ __forceinline__ void adamw_moments(float g, float& m, float& v, const AdamwHyper& h) {
-  g = mul1(g, h.grad_scale);
-  m = add1(mul1(m, h.beta1), mul1(g, h.c1));
-  v = add1(mul1(v, h.beta2), mul1(mul1(g, h.c2), g));
-}
-__device__ __forceinline__ float adamw_param(float p, float m, float v, const AdamwTensor& t, const AdamwHyper& h) {
-  return p * h.keep - t.step * (m / (sqrtf(v) * t.inv_bc2 + h.eps));
+__device__ __forceinline__ unsigned bytes4(const int (&c)[4]) {
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
 // Four consecutive elements of a tensor, n of them there (4 but at its end)
@@ -134,60 +166,120 @@ __device__ __forceinline__ void store_codes(unsigned char* dst, int n, unsigned 
   }
 }
 
-// One warp, one block of 256: lane l has elements 4 l .. 4 l + 3 and 128 + 4 l ..
-template <int BITS, typename GT>
-__device__ __forceinline__ void adamw_block(const AdamwTensor& t, const AdamwHyper& h, long block, int lane) {
-  const long e0 = block * ADAMW_BLOCK + lane * 4;
+// What a lane has of a block of 256: elements 4 l .. 4 l + 3 and 128 + 4 l .., n of either there
+template <int BITS>
+struct AdamwLane {
   int n[2];
   float p[2][4], g[2][4], m[2][4], v[2][4];
   unsigned mu[2], vu[2];
+};
+template <int BITS, typename GT>
+__device__ __forceinline__ void adamw_load(AdamwLane<BITS>& x, const AdamwTensor& t, long e0) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const long e = e0 + k * 128, left = t.n - e;
-    n[k] = left >= 4 ? 4 : left > 0 ? int(left) : 0;
-    load4(t.p + e, n[k], p[k]);
-    load4(static_cast<const GT*>(t.g) + e, n[k], g[k]);
+    x.n[k] = left >= 4 ? 4 : left > 0 ? int(left) : 0;
+    load4(t.p + e, x.n[k], x.p[k]);
+    load4(static_cast<const GT*>(t.g) + e, x.n[k], x.g[k]);
     if constexpr (BITS == 32) {
-      load4(static_cast<const float*>(t.m) + e, n[k], m[k]);
-      load4(static_cast<const float*>(t.v) + e, n[k], v[k]);
+      load4(static_cast<const float*>(t.m) + e, x.n[k], x.m[k]);
+      load4(static_cast<const float*>(t.v) + e, x.n[k], x.v[k]);
     } else {
-      mu[k] = load_codes(static_cast<const unsigned char*>(t.m) + e, n[k]);
-      vu[k] = load_codes(static_cast<const unsigned char*>(t.v) + e, n[k]);
+      x.mu[k] = load_codes(static_cast<const unsigned char*>(t.m) + e, x.n[k]);
+      x.vu[k] = load_codes(static_cast<const unsigned char*>(t.v) + e, x.n[k]);
     }
   }
+}
+
+// Every lane copies its parts of its warp's blocks to come into its own places of a ring in shared
+// memory: with the loads in registers, too few bytes were on their way behind the arithmetic of the 8-bit form.  The last
+// block of a tensor, if it is not whole, is loaded when it is its turn.
+template <int BITS>
+struct AdamwRing {
+  static constexpr int SLOTS = 2, WIDE = BITS == 8 ? 4 : 8;
+  uint4 wide[SLOTS][WIDE][256];                   // p, g (8 bytes of bf16), and m, v in fp32
+  unsigned code[BITS == 8 ? SLOTS : 1][4][256];   // m, v in 8 bits
+};
+template <int BITS>
+__device__ __forceinline__ void adamw_request(AdamwRing<BITS>& ring, int slot, const AdamwTensor& t, long e0) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const long e = e0 + k * 128;
+    ring_load16(&ring.wide[slot][k][tid], t.p + e);
+    if (t.grad_f32) ring_load16(&ring.wide[slot][2 + k][tid], static_cast<const float*>(t.g) + e);
+    else ring_load8(&ring.wide[slot][2 + k][tid], static_cast<const __nv_bfloat16*>(t.g) + e);
+    if constexpr (BITS == 32) {
+      ring_load16(&ring.wide[slot][4 + k][tid], static_cast<const float*>(t.m) + e);
+      ring_load16(&ring.wide[slot][6 + k][tid], static_cast<const float*>(t.v) + e);
+    } else {
+      ring_load4(&ring.code[slot][k][tid], static_cast<const unsigned char*>(t.m) + e);
+      ring_load4(&ring.code[slot][2 + k][tid], static_cast<const unsigned char*>(t.v) + e);
+    }
+  }
+}
+__device__ __forceinline__ void floats4(const uint4& u, float (&f)[4]) {
+  f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+template <int BITS>
+__device__ __forceinline__ void adamw_take(AdamwLane<BITS>& x, const AdamwRing<BITS>& ring, int slot, bool grad_f32) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    x.n[k] = 4;
+    floats4(ring.wide[slot][k][tid], x.p[k]);
+    if (grad_f32) {
+      floats4(ring.wide[slot][2 + k][tid], x.g[k]);
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2*>(&ring.wide[slot][2 + k][tid]);
+      const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+      x.g[k][0] = a.x; x.g[k][1] = a.y; x.g[k][2] = b.x; x.g[k][3] = b.y;
+    }
+    if constexpr (BITS == 32) {
+      floats4(ring.wide[slot][4 + k][tid], x.m[k]);
+      floats4(ring.wide[slot][6 + k][tid], x.v[k]);
+    } else {
+      x.mu[k] = ring.code[slot][k][tid];
+      x.vu[k] = ring.code[slot][2 + k][tid];
+    }
+  }
+}
+
+// The step of one block by one warp; mb0, vb0: the block's bases
+template <int BITS, bool WHOLE>
+__device__ __forceinline__ void adamw_block(AdamwLane<BITS>& x, const AdamwTensor& t, const AdamwHyper& h, long block, int lane, int mb0,
+                                            int vb0) {
+  const long e0 = block * ADAMW_BLOCK + lane * 4;
+  auto &p = x.p, &g = x.g, &m = x.m, &v = x.v;
+  int n[2] = {WHOLE ? 4 : x.n[0], WHOLE ? 4 : x.n[1]};
   if constexpr (BITS == 8) {
-    const unsigned mb = unsigned(t.mb[block]), vb = unsigned(t.vb[block]);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[k][j] = decode_m(mu[k] >> (8 * j) & 0xffu, mb);
-        v[k][j] = __uint_as_float(decode_bits(vu[k] >> (8 * j) & 0xffu, vb));
-      }
+      decode_m4(x.mu[k], unsigned(mb0) << 20, m[k]);
+      decode_v4(x.vu[k], unsigned(vb0) << 20, v[k]);
     }
   }
   unsigned mtop = 0, vtop = 0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      adamw_moments(g[k][j], m[k][j], v[k][j], h);
-      p[k][j] = adamw_param(p[k][j], m[k][j], v[k][j], t, h);
-      if constexpr (BITS == 8) {
-        mtop = max(mtop, __float_as_uint(m[k][j]) & 0x7fffffffu);
-        vtop = max(vtop, __float_as_uint(v[k][j]) & 0x7fffffffu);
-      }
+    for (int j = 0; j < 4; j += 2) {
+      const Pair gs = Pair{g[k][j], g[k][j + 1]} * both(h.grad_scale);
+      const Pair mm = Pair{m[k][j], m[k][j + 1]} * both(h.beta1) + gs * both(h.c1);
+      const Pair vv = Pair{v[k][j], v[k][j + 1]} * both(h.beta2) + gs * both(h.c2) * gs;
+      m[k][j] = mm.a; m[k][j + 1] = mm.b;
+      v[k][j] = vv.a; v[k][j + 1] = vv.b;
+      const Pair denom = fma2({sqrtf(vv.a), sqrtf(vv.b)}, both(t.inv_bc2), both(h.eps));
+      const Pair up = {__fdividef(mm.a, denom.a), __fdividef(mm.b, denom.b)};
+      const Pair pp = fma2(up, both(-t.step), Pair{p[k][j], p[k][j + 1]} * both(h.keep));
+      p[k][j] = pp.a; p[k][j + 1] = pp.b;
     }
-  }
-  unsigned mb = 0, vb = 0;
-  if constexpr (BITS == 8) {
-    mtop = min(__reduce_max_sync(0xffffffffu, mtop), ADAMW_TOP);
-    vtop = min(__reduce_max_sync(0xffffffffu, vtop), ADAMW_TOP);
-    mb = code_base(mtop, 127);
-    vb = code_base(vtop, 255);
-    if (lane == 0) {
-      t.mb[block] = short(mb);
-      t.vb[block] = short(vb);
+    if constexpr (BITS == 8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mtop = max(mtop, __float_as_uint(m[k][j]) & 0x7fffffffu);
+        vtop = max(vtop, __float_as_uint(v[k][j]));           // (never negative; NaN as the canonical one)
+      }
     }
   }
 #pragma unroll
@@ -198,54 +290,143 @@ __device__ __forceinline__ void adamw_block(const AdamwTensor& t, const AdamwHyp
     if constexpr (BITS == 32) {
       store4(static_cast<float*>(t.m) + e, n[k], m[k]);
       store4(static_cast<float*>(t.v) + e, n[k], v[k]);
-    } else {
-      mu[k] = vu[k] = 0;
+    }
+  }
+  if constexpr (BITS == 8) {
+    mtop = __reduce_max_sync(0xffffffffu, mtop);
+    vtop = __reduce_max_sync(0xffffffffu, vtop);
+    if (max(mtop, vtop) > ADAMW_INF) {                        // a NaN somewhere in the block
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if ((__float_as_uint(m[k][j]) & 0x7fffffffu) > ADAMW_INF) m[k][j] = __uint_as_float(ADAMW_TOP);
+          if (__float_as_uint(v[k][j]) > ADAMW_INF) v[k][j] = __uint_as_float(ADAMW_TOP);
+        }
+      }
+      mtop = min(mtop, ADAMW_TOP);
+      vtop = min(vtop, ADAMW_TOP);
+    }
+    const int mb = code_base(mtop, 127), vb = code_base(vtop, 255);
+    if (lane == 0) {
+      t.mb[block] = short(mb);
+      t.vb[block] = short(vb);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const long e = e0 + k * 128;
+      const unsigned x = unsigned(e >> 1) * ADAMW_WEYL + t.seed, w0 = adamw_hash(x), w1 = adamw_hash(x + ADAMW_WEYL);
+      const unsigned dither[4] = {(w0 << 4 & 0xffff0u) | 8u, (w0 >> 12 & 0xffff0u) | 8u, (w1 << 4 & 0xffff0u) | 8u,
+                                  (w1 >> 12 & 0xffff0u) | 8u};
+      int mc[4], vc[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const unsigned word = adamw_hash(unsigned(e >> 1) + (j >> 1), t.seed);
-        const unsigned dither = (j & 1 ? word >> 16 : word & 0xffffu) << 4 | 8u;
-        const unsigned mbits = __float_as_uint(m[k][j]), vbits = min(__float_as_uint(v[k][j]) & 0x7fffffffu, ADAMW_TOP);
-        const unsigned mag = min(mbits & 0x7fffffffu, ADAMW_TOP);
-        const int mc = int((mag + dither) >> 20) - int(mb), vc = int((vbits + dither) >> 20) - int(vb);
-        mu[k] |= (unsigned(mag && mc > 0 ? mc : 0) | mbits >> 31 << 7) << (8 * j);
-        vu[k] |= unsigned(vbits ? max(vc, 1) : 0) << (8 * j);
+        const unsigned vbits = __float_as_uint(v[k][j]), mag = __float_as_uint(m[k][j]) & 0x7fffffffu;
+        mc[j] = max(int((mag + dither[j]) >> 20) - mb, 0);
+        vc[j] = max(int((vbits + dither[j]) >> 20) - vb, int(min(vbits, 1u)));
       }
-      store_codes(static_cast<unsigned char*>(t.m) + e, n[k], mu[k]);
-      store_codes(static_cast<unsigned char*>(t.v) + e, n[k], vu[k]);
+      // (the signs are the top bits of the patterns)
+      const unsigned tops = __byte_perm(__byte_perm(__float_as_uint(m[k][0]), __float_as_uint(m[k][1]), 0x0073),
+                                        __byte_perm(__float_as_uint(m[k][2]), __float_as_uint(m[k][3]), 0x0073), 0x5410);
+      store_codes(static_cast<unsigned char*>(t.m) + e, n[k], bytes4(mc) | (tops & 0x80808080u));
+      store_codes(static_cast<unsigned char*>(t.v) + e, n[k], bytes4(vc));
     }
   }
 }
 
 template <int N, int BITS>
-__global__ void __launch_bounds__(256) adamw_list_kernel(const __grid_constant__ AdamwList<N> list) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int i = 0;
-  for (long tile = blockIdx.x; tile < list.end[list.count - 1]; tile += gridDim.x) {
-    while (tile >= list.end[i]) ++i;
-    const AdamwTensor& t = list.t[i];
-    const long block = (tile - (i > 0 ? list.end[i - 1] : 0)) * 8 + warp;
-    if (block * ADAMW_BLOCK >= t.n) continue;
-    if (t.grad_f32) adamw_block<BITS, float>(t, list.h, block, lane);
-    else adamw_block<BITS, __nv_bfloat16>(t, list.h, block, lane);
+__global__ void __launch_bounds__(256, ADAMW_CTAS) adamw_list_kernel(const __grid_constant__ AdamwList<N> list) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  AdamwRing<BITS>& ring = *reinterpret_cast<AdamwRing<BITS>*>(raw);
+  constexpr int SLOTS = AdamwRing<BITS>::SLOTS;
+  const int lane = threadIdx.x & 31;
+  const long all = list.end[list.count - 1], stride = gridDim.x * 8L, first = blockIdx.x * 8L + (threadIdx.x >> 5);
+  // a block on its way: its tensor, its number in it, and its bases (m's below, v's above)
+  struct Asked {
+    int i, bases;
+    long block;
+  } queue[SLOTS - 1];
+  long ask = first;
+  int ask_i = 0;
+  // the tensor of the first block, looked for by halves; of later ones from there on
+  for (int top = list.count - 1; ask_i < top;) {
+    const int mid = (ask_i + top) >> 1;
+    if (ask >= list.end[mid]) ask_i = mid + 1;
+    else top = mid;
+  }
+  auto request = [&](int slot) {
+    Asked x = {0, 0, 0};
+    if (ask < all) {
+      while (ask >= list.end[ask_i]) ++ask_i;
+      const AdamwTensor& t = list.t[ask_i];
+      x.i = ask_i;
+      x.block = ask - (ask_i > 0 ? list.end[ask_i - 1] : 0);
+      if ((x.block + 1) * ADAMW_BLOCK <= t.n) adamw_request<BITS>(ring, slot, t, x.block * ADAMW_BLOCK + lane * 4);
+      if (BITS == 8) x.bases = int(static_cast<unsigned short>(t.mb[x.block])) | int(t.vb[x.block]) << 16;
+      ask += stride;
+    }
+    ring_commit();
+    return x;
+  };
+#pragma unroll
+  for (int k = 0; k < SLOTS - 1; ++k) queue[k] = request(k);
+  int slot = 0;
+  for (long at = first; at < all; at += stride) {
+    const Asked now = queue[0];
+#pragma unroll
+    for (int k = 0; k + 2 < SLOTS; ++k) queue[k] = queue[k + 1];
+    queue[SLOTS - 2] = request((slot + SLOTS - 1) % SLOTS);
+    ring_wait<SLOTS - 1>();
+    const AdamwTensor& t = list.t[now.i];
+    AdamwLane<BITS> x;
+    if ((now.block + 1) * ADAMW_BLOCK <= t.n) {
+      adamw_take<BITS>(x, ring, slot, t.grad_f32);
+      adamw_block<BITS, true>(x, t, list.h, now.block, lane, now.bases & 0xffff, now.bases >> 16);
+    } else {
+      if (t.grad_f32) adamw_load<BITS, float>(x, t, now.block * ADAMW_BLOCK + lane * 4);
+      else adamw_load<BITS, __nv_bfloat16>(x, t, now.block * ADAMW_BLOCK + lane * 4);
+      adamw_block<BITS, false>(x, t, list.h, now.block, lane, now.bases & 0xffff, now.bases >> 16);
+    }
+    slot = (slot + 1) % SLOTS;
   }
 }
 
-// out = what a tensor's codes stand for
+// out = what a tensor's codes stand for; eight of them a thread, n of the last thread's
 template <typename T>
 __global__ void __launch_bounds__(256) moment_values_kernel(const unsigned char* m, const short* mb, const unsigned char* v,
                                                             const short* vb, T* m_out, T* v_out, long n) {
-  for (long e = (blockIdx.x * 256L + threadIdx.x) * 4; e < n; e += gridDim.x * 1024L) {
-    const int k = n - e >= 4 ? 4 : int(n - e);
-    const unsigned mu = load_codes(m + e, k), vu = load_codes(v + e, k);
-    const unsigned bm = unsigned(mb[e / ADAMW_BLOCK]), bv = unsigned(vb[e / ADAMW_BLOCK]);
-    float a[4], b[4];
+  const long e = (blockIdx.x * 256L + threadIdx.x) * 8;
+  if (e >= n) return;
+  const unsigned bm = unsigned(mb[e / ADAMW_BLOCK]) << 20, bv = unsigned(vb[e / ADAMW_BLOCK]) << 20;
+  const int k[2] = {n - e >= 4 ? 4 : int(n - e), n - e >= 8 ? 4 : n - e > 4 ? int(n - e - 4) : 0};
+  unsigned mu[2], vu[2];
+  if (k[1] == 4) {
+    const uint2 a = *reinterpret_cast<const uint2*>(m + e), b = *reinterpret_cast<const uint2*>(v + e);
+    mu[0] = a.x; mu[1] = a.y; vu[0] = b.x; vu[1] = b.y;
+  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a[j] = decode_m(mu >> (8 * j) & 0xffu, bm);
-      b[j] = __uint_as_float(decode_bits(vu >> (8 * j) & 0xffu, bv));
+    for (int i = 0; i < 2; ++i) {
+      mu[i] = load_codes(m + e + 4 * i, k[i]);
+      vu[i] = load_codes(v + e + 4 * i, k[i]);
     }
-    store4(m_out + e, k, a);
-    store4(v_out + e, k, b);
+  }
+  float a[2][4], b[2][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    decode_m4(mu[i], bm, a[i]);
+    decode_v4(vu[i], bv, b[i]);
+  }
+  if (sizeof(T) == 2 && k[1] == 4) {
+    *reinterpret_cast<uint4*>(m_out + e) = make_uint4(pack_bf16x2(a[0][0], a[0][1]), pack_bf16x2(a[0][2], a[0][3]),
+                                                      pack_bf16x2(a[1][0], a[1][1]), pack_bf16x2(a[1][2], a[1][3]));
+    *reinterpret_cast<uint4*>(v_out + e) = make_uint4(pack_bf16x2(b[0][0], b[0][1]), pack_bf16x2(b[0][2], b[0][3]),
+                                                      pack_bf16x2(b[1][0], b[1][1]), pack_bf16x2(b[1][2], b[1][3]));
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    store4(m_out + e + 4 * i, k[i], a[i]);
+    store4(v_out + e + 4 * i, k[i], b[i]);
   }
 }
 
@@ -254,15 +435,17 @@ static int adamw_launch(const AdamwTensor* t, int count, const AdamwHyper& h, cu
   AdamwList<N> list;
   list.count = count;
   list.h = h;
-  long tiles = 0;
+  long blocks = 0;
   for (int i = 0; i < count; ++i) {
     list.t[i] = t[i];
-    tiles += (t[i].n + ADAMW_TILE - 1) / ADAMW_TILE;
-    list.end[i] = tiles;
+    blocks += (t[i].n + ADAMW_BLOCK - 1) / ADAMW_BLOCK;
+    list.end[i] = blocks;
   }
-  if (tiles == 0) return 0;
-  const long cap = long(num_sms()) * 8;
-  adamw_list_kernel<N, BITS><<<int(tiles < cap ? tiles : cap), 256, 0, stream>>>(list);
+  if (blocks == 0) return 0;
+  const long want = (blocks + 7) / 8, cap = long(num_sms()) * (ADAMW_CTAS);
+  auto kern = adamw_list_kernel<N, BITS>;
+  ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(AdamwRing<BITS>))));
+  kern<<<int(want < cap ? want : cap), 256, sizeof(AdamwRing<BITS>), stream>>>(list);
   ZB_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -299,11 +482,11 @@ int zb_moment_values(const void* m, const void* mb, const void* v, const void* v
                      cudaStream_t stream) {
   using namespace zb;
   if (n <= 0) return 0;
-  if (((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3) ||
+  if (((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 7) ||
       ((reinterpret_cast<uintptr_t>(m_out) | reinterpret_cast<uintptr_t>(v_out)) & 15))
-    ZB_FAIL(-1, "moment_values: codes must be 4-byte aligned, values 16");
-  const long ctas = (n + 1023) / 1024, cap = long(num_sms()) * 16;
-  const int grid = int(ctas < cap ? ctas : cap);
+    ZB_FAIL(-1, "moment_values: codes must be 8-byte aligned, values 16");
+  if ((n + 2047) / 2048 > 0x7fffffffL) ZB_FAIL(-1, "moment_values: %ld values", n);
+  const int grid = int((n + 2047) / 2048);
   const unsigned char *mc = static_cast<const unsigned char*>(m), *vc = static_cast<const unsigned char*>(v);
   const short *bm = static_cast<const short*>(mb), *bv = static_cast<const short*>(vb);
   if (out_f32)

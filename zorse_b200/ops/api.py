@@ -238,7 +238,8 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
         self._norm_bwd = fast.norm_bwd if default and sm100.NORM_BWD_VERSION == 2 else _decline
         self._attn_fwd = fast.attn_fwd if default and sm100.ATTN_FWD_VERSION == 0 else _decline
         self._attn_bwd = fast.attn_bwd if default and sm100.ATTN_BWD_VERSION == 0 else _decline
-        for name in ("rope", "swiglu_fwd", "swiglu_bwd", "act_fwd", "act_bwd"):
+        for name in ("rope", "swiglu_fwd", "swiglu_bwd", "act_fwd", "act_bwd", "qk_norm_rope_fwd", "qk_norm_rope_bwd",
+                     "embedding_scaled", "embedding_by_token", "adamw_step"):
             setattr(self, "_" + name, getattr(fast, name) if default else _decline)
 
     def linear_fwd(self, x, w, bias=None, addend=None):
@@ -339,19 +340,24 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
         return self.k.patches(img, patch, kdim)
 
     def qk_norm_rope_fwd(self, qkv, wq, wk, cs, S, nq, nk, d, eps, keep=True):
-        return self.k.qk_norm_rope_fwd(qkv, wq, wk, cs, S, nq, nk, d, eps, keep)
+        r = self._qk_norm_rope_fwd(qkv, wq, wk, cs, S, nq, nk, d, eps, keep)
+        return self.k.qk_norm_rope_fwd(qkv, wq, wk, cs, S, nq, nk, d, eps, keep) if r is None else r
 
     def qk_norm_rope_bwd(self, dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk):
-        return self.k.qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk)
+        if self._qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk) is None:
+            self.k.qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S, nq, nk, d, gwq, gwk)
+        return dqkv
 
     def embedding_fwd(self, ids, table, pos_table=None, S=1, pos_offset=0, scale=1.0):
         if scale != 1.0:
-            return self.k.embedding_scaled(ids.reshape(-1), table, pos_table, S, pos_offset, scale)
+            y = self._embedding_scaled(ids, table, pos_table, S, pos_offset, scale)
+            return self.k.embedding_scaled(ids.reshape(-1), table, pos_table, S, pos_offset, scale) if y is None else y
         return self.k.embedding_fwd(ids.reshape(-1), table, pos_table, S, pos_offset)
 
     def embedding_bwd(self, ids, dout, gtable, gpos=None, S=1, pos_offset=0, scale=1.0, by_token=False):
         if by_token or scale != 1.0:
-            self.k.embedding_by_token(ids.reshape(-1), dout, gtable, gpos, S, pos_offset, scale)
+            if self._embedding_by_token(ids, dout, gtable, gpos, S, pos_offset, scale) is None:
+                self.k.embedding_by_token(ids.reshape(-1), dout, gtable, gpos, S, pos_offset, scale)
         else:
             self.k.embedding_bwd(ids.reshape(-1), dout, gtable, gpos, S, pos_offset)
 
@@ -362,8 +368,10 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
     def adam_step(self, p, m, v, g, p16, **kw):
         self.k.adam_step(p, m, v, g, p16, **kw)
 
-    def adamw_step(self, p, moments, g, p16, **kw):
-        self.k.adamw_step(p, moments, g, p16, **kw)
+    def adamw_step(self, p, moments, g, p16, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0, seeds=None):
+        if self._adamw_step(p, moments, g, p16, seeds, step, lr, beta1, beta2, eps, weight_decay, grad_scale) is None:
+            self.k.adamw_step(p, moments, g, p16, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, step=step,
+                              grad_scale=grad_scale, seeds=seeds)
 
     def moment_values(self, moments, dtype=torch.float32):
         return self.k.moment_values(moments, dtype)
