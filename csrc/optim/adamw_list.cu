@@ -336,6 +336,8 @@ __device__ __forceinline__ void adamw_block(AdamwLane<BITS>& x, const AdamwTenso
 
 template <int N, int BITS>
 __global__ void __launch_bounds__(256, ADAMW_CTAS) adamw_list_kernel(const __grid_constant__ AdamwList<N> list) {
+  chain_trigger();
+  chain_wait();
   extern __shared__ __align__(16) unsigned char raw[];
   AdamwRing<BITS>& ring = *reinterpret_cast<AdamwRing<BITS>*>(raw);
   constexpr int SLOTS = AdamwRing<BITS>::SLOTS;
@@ -395,6 +397,8 @@ __global__ void __launch_bounds__(256, ADAMW_CTAS) adamw_list_kernel(const __gri
 template <typename T>
 __global__ void __launch_bounds__(256) moment_values_kernel(const unsigned char* m, const short* mb, const unsigned char* v,
                                                             const short* vb, T* m_out, T* v_out, long n) {
+  chain_trigger();
+  chain_wait();
   const long e = (blockIdx.x * 256L + threadIdx.x) * 8;
   if (e >= n) return;
   const unsigned bm = unsigned(mb[e / ADAMW_BLOCK]) << 20, bv = unsigned(vb[e / ADAMW_BLOCK]) << 20;
@@ -442,11 +446,10 @@ static int adamw_launch(const AdamwTensor* t, int count, const AdamwHyper& h, cu
     list.end[i] = blocks;
   }
   if (blocks == 0) return 0;
-  const long want = (blocks + 7) / 8, cap = long(num_sms()) * (ADAMW_CTAS);
+  const long want = (blocks + 7) / 8, cap = long(num_sms()) * ADAMW_CTAS;
   auto kern = adamw_list_kernel<N, BITS>;
   ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(AdamwRing<BITS>))));
-  kern<<<int(want < cap ? want : cap), 256, sizeof(AdamwRing<BITS>), stream>>>(list);
-  ZB_CUDA_OK(cudaGetLastError());
+  ZB_CUDA_OK(launch_pass(kern, int(want < cap ? want : cap), 256, sizeof(AdamwRing<BITS>), stream, list));
   return 0;
 }
 
@@ -490,11 +493,11 @@ int zb_moment_values(const void* m, const void* mb, const void* v, const void* v
   const unsigned char *mc = static_cast<const unsigned char*>(m), *vc = static_cast<const unsigned char*>(v);
   const short *bm = static_cast<const short*>(mb), *bv = static_cast<const short*>(vb);
   if (out_f32)
-    moment_values_kernel<float><<<grid, 256, 0, stream>>>(mc, bm, vc, bv, static_cast<float*>(m_out), static_cast<float*>(v_out), n);
+    ZB_CUDA_OK(launch_pass(moment_values_kernel<float>, grid, 256, 0, stream, mc, bm, vc, bv, static_cast<float*>(m_out),
+                           static_cast<float*>(v_out), n));
   else
-    moment_values_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(mc, bm, vc, bv, static_cast<__nv_bfloat16*>(m_out),
-                                                                  static_cast<__nv_bfloat16*>(v_out), n);
-  ZB_CUDA_OK(cudaGetLastError());
+    ZB_CUDA_OK(launch_pass(moment_values_kernel<__nv_bfloat16>, grid, 256, 0, stream, mc, bm, vc, bv,
+                           static_cast<__nv_bfloat16*>(m_out), static_cast<__nv_bfloat16*>(v_out), n));
   return 0;
 }
 

@@ -20,6 +20,16 @@ from ..utils.logger import init_logger
 from ..utils.pipeline_log import init_pipeline_logger
 
 
+def model_overrides(args) -> dict:
+    """Changes to the registered model that flags ask for."""
+    out = {"qk_norm": True} if args.qk_norm else {}
+    if args.embed_scale != 1.0:
+        out["embed_scale"] = args.embed_scale
+    if args.embed_by_token:
+        out["embed_by_token"] = True
+    return out
+
+
 def main(argv=None) -> int:
     args = parse_args_zorse(argv)
     log = init_logger(args.log_level)
@@ -35,6 +45,8 @@ def main(argv=None) -> int:
         activation_offload=True if args.offload_activations_to_host else None, lr=args.lr, seed=args.seed,
         backend=args.backend, pipeline_log=plog, shift_labels=args.shift_labels, defer_wgrad=args.defer_wgrad,
         defer_tail_wgrad=args.defer_tail_wgrad, prepost_recv=args.prepost_recv,
+        optimizer=args.optimizer, weight_decay=args.weight_decay, moment_bits=args.moment_bits,
+        model_overrides=model_overrides(args),
         p2p_timeout_s=args.p2p_timeout or None,
         p2p_fault_hooks=bool(args.inject_fault) and (":drop" in args.inject_fault or ":delay=" in args.inject_fault))
     if opt.defer_tail_wgrad < 0:

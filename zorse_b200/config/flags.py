@@ -68,6 +68,15 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--no_recompute", action="store_true", help="keep activations instead of recomputing layers")
     p.add_argument("--offload_activations_to_host", action="store_true")
     p.add_argument("--lr", type=float, default=1e-3)
+    p.add_argument("--optimizer", default="adam", choices=["adam", "adamw"],
+                   help="adam: weight decay through the gradient; adamw: decoupled weight decay, all units in one launch")
+    p.add_argument("--weight_decay", type=float, default=0.0)
+    p.add_argument("--moment_bits", type=int, default=32, choices=[8, 32],
+                   help="adamw: 8 holds both moments in two bytes a parameter instead of eight")
+    p.add_argument("--qk_norm", action="store_true", help="RMS norm of every query and key head ahead of its rotation")
+    p.add_argument("--embed_scale", type=float, default=1.0, help="factor on the token embedding")
+    p.add_argument("--embed_by_token", action="store_true",
+                   help="embedding gradient summed token by token: the same bits on every run")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--checkpoint_dir", type=str, default=None)
     p.add_argument("--checkpoint_every", type=int, default=0)

@@ -34,6 +34,7 @@ import torch
 import torch.distributed as dist
 
 from ..models.layers import ALIGN, Layer
+from ..ops.moments import Moments8, dither_seed
 from ..parallel.groups import Group
 from ..utils import stream_check as SC
 from ..utils.ranges import phase
@@ -68,6 +69,14 @@ class AdamConfig:
     beta2: float = 0.999
     eps: float = 1e-8
     weight_decay: float = 0.0
+    decoupled: bool = False    # AdamW: the decay acts on the parameters and not through the gradient
+    moment_bits: int = 32      # 8 (with `decoupled`): both moments in two bytes a parameter (ops/moments.py) instead of eight
+
+    def __post_init__(self):
+        if self.moment_bits not in (8, 32):
+            raise ValueError(f"moment_bits is 8 or 32, not {self.moment_bits}")
+        if self.moment_bits == 8 and not self.decoupled:
+            raise ValueError("moments in 8 bits are for AdamW (decoupled weight decay)")
 
 
 @dataclass
@@ -221,8 +230,16 @@ class ZeroUnit:
             layer.init_flat(full32, cfg.seed * 1000003 + gid)
         self.master = full32[lo:hi].clone()
         del full32
-        self.m = torch.zeros_like(self.master)
-        self.v = torch.zeros_like(self.master)
+        self.m = self.v = self.moments = None
+        if cfg.adam.moment_bits == 8:
+            if self.tp_group is not None:
+                # the blocks of values with one base hold neighbours that differ from slice to slice, so what the slices hold
+                # whole would not stay the same on all of them
+                raise ValueError("moments in 8 bits do not cover tensor-parallel lanes")
+            self.moments = Moments8.zeros(self.shard_n, device)
+        else:
+            self.m = torch.zeros_like(self.master)
+            self.v = torch.zeros_like(self.master)
         self.p_shard = self.master.to(cfg.compute_dtype)
         self.grad_shard: Optional[torch.Tensor] = None  # reduced gradients awaiting optimizer_step
         # ---- transient state -------------------------------------------------------
@@ -418,8 +435,11 @@ class ZeroUnit:
                    torch.empty(self.shard_n, dtype=self.cfg.compute_dtype, device=self.device))
         else:
             master, p16 = self.master, self.p_shard
-        self.ops.adam_step(master, self.m, self.v, g, p16, lr=cfg.lr, beta1=cfg.beta1, beta2=cfg.beta2, eps=cfg.eps,
-                           weight_decay=cfg.weight_decay, step=self.step_count, grad_scale=grad_scale)
+        if cfg.decoupled:
+            adamw_step([self], [master], [g], [p16], grad_scale)
+        else:
+            self.ops.adam_step(master, self.m, self.v, g, p16, lr=cfg.lr, beta1=cfg.beta1, beta2=cfg.beta2, eps=cfg.eps,
+                               weight_decay=cfg.weight_decay, step=self.step_count, grad_scale=grad_scale)
         self.counters.adam_steps += 1
         if offl:
             self.host_master.copy_(master, non_blocking=True)
@@ -535,7 +555,8 @@ class ZeroUnit:
 
     def state_tensors(self) -> dict[str, torch.Tensor]:
         mine = self.master if self.master is not None else self.host_master
-        return {"master": mine, "m": self.m, "v": self.v}
+        m, v = (self.m, self.v) if self.moments is None else self.ops.moment_values(self.moments)
+        return {"master": mine, "m": m, "v": v}
 
     def load_state(self, master: torch.Tensor, m: torch.Tensor, v: torch.Tensor, step: int) -> None:
         self._drop_master()
@@ -545,10 +566,25 @@ class ZeroUnit:
         else:
             self.master.copy_(master)
             self.p_shard.copy_(self.master.to(self.cfg.compute_dtype))
-        self.m.copy_(m)
-        self.v.copy_(v)
+        if self.moments is None:
+            self.m.copy_(m)
+            self.v.copy_(v)
+        else:
+            self.moments.load(m.to(self.device), v.to(self.device))
         self.step_count = step
         self._after_update()
+
+
+def adamw_step(units: list[ZeroUnit], masters: list, grads: list, copies: list, grad_scale: float) -> None:
+    """AdamW on the shards of several units in one launch; their step counts have been raised."""
+    cfg = units[0].cfg
+    a, seeds = cfg.adam, None
+    if a.moment_bits == 8:
+        # replicas of a shard (hybrid shard) round alike: their seeds are those of the shard
+        seeds = [dither_seed(cfg.seed, u.gid, u.lo, u.step_count) for u in units]
+    units[0].ops.adamw_step(masters, [u.moments if u.moments is not None else (u.m, u.v) for u in units], grads, copies, lr=a.lr,
+                            beta1=a.beta1, beta2=a.beta2, eps=a.eps, weight_decay=a.weight_decay,
+                            step=[u.step_count for u in units], grad_scale=grad_scale, seeds=seeds)
 
 
 class StageEngine:
@@ -568,6 +604,8 @@ class StageEngine:
                 and shard_ratios is None):
             from .fused import FusedZeroUnit
 
+            if cfg.adam.decoupled:
+                raise ValueError("the fused reduce-scatter kernel applies Adam: AdamW needs collectives=\"library\"")
             cls = FusedZeroUnit
         self.units = [cls(ly, gid, device=device, cfg=cfg, ops=ops, shard=shard, replicate=replicate, rank=rank,
                           streams=self.streams, zero_level=zero_level, counters=self.counters, meta_init=meta_init,
@@ -591,8 +629,32 @@ class StageEngine:
             u.prefetch()
 
     def optimizer_step(self) -> None:
-        for u in self.units:
-            u.optimizer_step()
+        units = [u for u in self.units if u.grad_shard is not None]
+        scales = {getattr(u, "grad_shard_scale", 1.0) for u in units}
+        if not self.cfg.adam.decoupled or len(scales) != 1:
+            for u in units:
+                u.optimizer_step()
+            return
+        cuda = self.device.type == "cuda"
+        if cuda:
+            cur = torch.cuda.current_stream()
+            for u in units:
+                if u.update_event is not None:
+                    cur.wait_event(u.update_event)
+        for u in units:
+            u.step_count += 1
+        with phase("zero.adam"):
+            adamw_step(units, [u.master for u in units], [u.grad_shard for u in units], [u.p_shard for u in units], scales.pop())
+        self.counters.adam_steps += len(units)
+        if cuda:
+            ev = torch.cuda.Event()
+            ev.record(cur)
+        for u in units:
+            u.grad_shard = None
+            if cuda:
+                SC.wrote(("shard", id(u)))
+                u.update_event = ev
+            u._after_update()
 
     def finish_step(self) -> None:
         for u in self.units:

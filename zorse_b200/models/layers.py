@@ -112,7 +112,9 @@ def _norm(ops, kind, x, w, b, eps):
 
 class TransformerBlock(Layer):
     """Generic block: {RMSNorm|LayerNorm} x {pre|post}-norm x {SwiGLU|GELU|ReLU} MLP x
-    {RoPE|none} x {causal|bidirectional} x optional sliding window, MHA or GQA.
+    {RoPE|none} x {causal|bidirectional} x optional sliding window, MHA or GQA.  `qk_norm`: every query and key
+    head is RMS-normalised ahead of its rotation, with one weight of the head's width for all query heads and one for
+    all key heads (the scores of attention then stay bounded however large the projections grow).
 
     Llama/Mistral: rms, pre, swiglu, rope, causal (reference models/llama_simple.py:391-518,
     models/mistral_simple.py:20); OPT/GPT: ln, pre or post, gelu/relu, biases, learned
@@ -123,8 +125,9 @@ class TransformerBlock(Layer):
 
     def __init__(self, hidden: int, heads: int, kv_heads: int, ffn: int, *, norm: str = "rms", pre_norm: bool = True,
                  act: str = "swiglu", bias: bool = False, rope_theta: Optional[float] = 10000.0, causal: bool = True,
-                 window: int = 0, eps: float = 1e-5, head_dim: Optional[int] = None, init_std: float = 0.02):
+                 window: int = 0, eps: float = 1e-5, head_dim: Optional[int] = None, init_std: float = 0.02, qk_norm: bool = False):
         super().__init__()
+        self.qk_norm = qk_norm
         self.H, self.Hq, self.Hkv, self.F = hidden, heads, kv_heads, ffn
         self.D = head_dim or hidden // heads
         self.norm, self.pre_norm, self.act, self.bias = norm, pre_norm, act, bias
@@ -141,6 +144,8 @@ class TransformerBlock(Layer):
         sp.append(ParamSpec("qkv_w", (qkv_w, H), std=self.std))
         if self.bias:
             sp.append(ParamSpec("qkv_b", (qkv_w,), "zeros"))
+        if self.qk_norm:
+            sp += [ParamSpec("qnorm_w", (D,), "ones"), ParamSpec("knorm_w", (D,), "ones")]
         sp.append(ParamSpec("o_w", (H, self.Hq * D), std=self.std))
         if self.bias:
             sp.append(ParamSpec("o_b", (H,), "zeros"))
@@ -163,6 +168,18 @@ class TransformerBlock(Layer):
             self._cs = ops.rope_table(S, self.D, self.rope_theta, device)
         return self._cs
 
+    def _head_norm_fwd(self, qkv, cs, S, ops, sv):
+        """Norm and rotation of the projection's query and key heads; the raw projection is kept for the backward pass."""
+        out, rstd = ops.qk_norm_rope_fwd(qkv, self.p["qnorm_w"], self.p["knorm_w"], cs, S, self.Hq, self.Hkv, self.D, self.eps,
+                                         keep=sv is not None)
+        if sv is not None:
+            sv.update(qkv_raw=qkv, qk_rstd=rstd)
+        return out
+
+    def _head_norm_bwd(self, dqkv, cs, S, ops, sv):
+        return ops.qk_norm_rope_bwd(dqkv, sv["qkv_raw"], self.p["qnorm_w"], self.p["knorm_w"], sv["qk_rstd"], cs, S, self.Hq,
+                                    self.Hkv, self.D, self.g["qnorm_w"], self.g["knorm_w"])
+
     # ---- sub-blocks ---------------------------------------------------------------
     def _attn_fwd(self, xin, resid, ctx, ops, sv):
         p, B, S = self.p, ctx["B"], ctx["S"]
@@ -170,12 +187,14 @@ class TransformerBlock(Layer):
         cs = self._rope(ops, S, xin.device)
         if ag is not None:
             qkv = ops.linear_fwd_gather(xin, "qkv_w", ag, p.get("qkv_b"))
-            if cs is not None:
+            if cs is not None and not self.qk_norm:
                 ops.rope_(qkv, cs, S, self.Hq + self.Hkv, self.D)
-        elif cs is not None:
+        elif cs is not None and not self.qk_norm:
             qkv = ops.linear_rope_fwd(xin, p["qkv_w"], p.get("qkv_b"), cs, S, self.Hq + self.Hkv, self.D)
         else:
             qkv = ops.linear_fwd(xin, p["qkv_w"], p.get("qkv_b"))
+        if self.qk_norm:
+            qkv = self._head_norm_fwd(qkv, cs, S, ops, sv)
         att, lse = ops.attn_fwd(qkv, B, S, self.Hq, self.Hkv, self.D, self.causal, self.window)
         out = ops.linear_fwd(att, p["o_w"], p.get("o_b"), addend=resid)
         if sv is not None:
@@ -190,7 +209,9 @@ class TransformerBlock(Layer):
         dqkv = ops.attn_bwd(datt, sv["qkv"], sv["att"], sv["lse"], B, S, self.Hq, self.Hkv, self.D, self.causal,
                             self.window)
         cs = self._rope(ops, S, dout.device)
-        if cs is not None:
+        if self.qk_norm:
+            self._head_norm_bwd(dqkv, cs, S, ops, sv)
+        elif cs is not None:
             ops.rope_(dqkv, cs, S, self.Hq + self.Hkv, self.D, backward=True)
         dxin = ops.linear_dgrad(dqkv, p["qkv_w"], addend=dres)
         ops.linear_wgrad(dqkv, xin, g["qkv_w"], g.get("qkv_b"), later=later)
@@ -254,13 +275,16 @@ class TransformerBlock(Layer):
 
 
 class EmbeddingLayer(Layer):
-    """Token embedding (+ learned positions, + LayerNorm for BERT-style models)."""
+    """Token embedding (+ learned positions, + LayerNorm for BERT-style models).  `scale` multiplies the token's row
+    (ahead of the positions); `by_token`: the gradient sums the rows of a token in their order and writes its row of the
+    table once, with the same bits on every run (a scaled embedding always does)."""
     kind = "embedding"
 
     def __init__(self, vocab: int, hidden: int, *, max_positions: int = 0, pos_offset: int = 0, post_norm: bool = False,
-                 eps: float = 1e-5, init_std: float = 0.02):
+                 eps: float = 1e-5, init_std: float = 0.02, scale: float = 1.0, by_token: bool = False):
         super().__init__()
         self.V, self.H, self.max_pos, self.pos_offset = vocab, hidden, max_positions, pos_offset
+        self.scale, self.by_token = float(scale), by_token
         self.post_norm, self.eps, self.std = post_norm, eps, init_std
 
     def param_specs(self):
@@ -273,7 +297,7 @@ class EmbeddingLayer(Layer):
 
     def forward(self, ids, ctx, ops, saved=None):
         S = ctx["S"]
-        e = ops.embedding_fwd(ids.reshape(-1), self.p["tok"], self.p.get("pos"), S, self.pos_offset)
+        e = ops.embedding_fwd(ids.reshape(-1), self.p["tok"], self.p.get("pos"), S, self.pos_offset, scale=self.scale)
         if self.post_norm:
             y, st = ops.norm_fwd(e, self.p["norm_w"], self.p["norm_b"], self.eps, True)
             if saved is not None:
@@ -286,7 +310,8 @@ class EmbeddingLayer(Layer):
     def backward(self, dy, ctx, ops, saved):
         if self.post_norm:
             dy = ops.norm_bwd(dy, saved["e"], self.p["norm_w"], saved["st"], None, self.g["norm_w"], self.g["norm_b"], True)
-        ops.embedding_bwd(saved["ids"].reshape(-1), dy, self.g["tok"], self.g.get("pos"), ctx["S"], self.pos_offset)
+        ops.embedding_bwd(saved["ids"].reshape(-1), dy, self.g["tok"], self.g.get("pos"), ctx["S"], self.pos_offset,
+                          scale=self.scale, by_token=self.by_token)
         return None
 
     def flops_per_token(self, S):

@@ -43,6 +43,9 @@ class ModelSpec:
     patch: int = 0
     classes: int = 0
     init_std: float = 0.02
+    qk_norm: bool = False          # RMS norm of every query and key head ahead of the rotation
+    embed_scale: float = 1.0       # factor on the token embedding
+    embed_by_token: bool = False   # its gradient summed token by token (the same bits on every run)
 
     @property
     def head_dim(self) -> int:
@@ -189,20 +192,23 @@ def make_block(spec: ModelSpec, tp: int = 1, tp_index: int = 0) -> TransformerBl
         from .tp_layers import TPTransformerBlock as cls
     return cls(spec.hidden, spec.heads, spec.n_kv, spec.ffn, norm=spec.norm, pre_norm=spec.pre_norm,
                act=spec.act, bias=spec.bias, rope_theta=spec.rope_theta, causal=spec.causal,
-               window=spec.window, eps=spec.eps, init_std=spec.init_std, **_tp_kw(tp, tp_index))
+               window=spec.window, eps=spec.eps, init_std=spec.init_std, qk_norm=spec.qk_norm, **_tp_kw(tp, tp_index))
 
 
 def make_embedding(spec: ModelSpec, seq_len: int, tp: int = 1, tp_index: int = 0) -> Layer:
     if spec.family == "vit":
         if tp > 1:
             raise NotImplementedError("tensor parallelism does not cover the ViT patch embedding")
+        if spec.embed_scale != 1.0 or spec.embed_by_token:
+            raise ValueError(f"{spec.name} embeds patches: embed_scale and embed_by_token are for token embeddings")
         return PatchEmbeddingLayer(spec.image, spec.patch, 3, spec.hidden, spec.init_std)
     maxpos = max(spec.max_positions, seq_len) if spec.max_positions else 0
     cls = EmbeddingLayer
     if tp > 1:
         from .tp_layers import SPEmbeddingLayer as cls
     return cls(spec.vocab, spec.hidden, max_positions=maxpos, pos_offset=spec.pos_offset,
-               post_norm=spec.embed_norm, eps=spec.eps, init_std=spec.init_std, **_tp_kw(tp, tp_index))
+               post_norm=spec.embed_norm, eps=spec.eps, init_std=spec.init_std, scale=spec.embed_scale,
+               by_token=spec.embed_by_token, **_tp_kw(tp, tp_index))
 
 
 def make_head(spec: ModelSpec, tp: int = 1, tp_index: int = 0) -> HeadLayer:

@@ -161,7 +161,9 @@ class TPTransformerBlock(TransformerBlock):
         p, B, S = self.p, ctx["B"], ctx["S"]
         qkv = ops.linear_fwd(xin_all, p["qkv_w"], p.get("qkv_b"))
         cs = self._rope(ops, S, xin_all.device)
-        if cs is not None:
+        if self.qk_norm:
+            qkv = self._head_norm_fwd(qkv, cs, S, ops, sv)
+        elif cs is not None:
             ops.rope_(qkv, cs, S, self.Hq + self.Hkv, self.D)
         att, lse = ops.attn_fwd(qkv, B, S, self.Hq, self.Hkv, self.D, self.causal, self.window)
         if sv is not None:
@@ -188,7 +190,9 @@ class TPTransformerBlock(TransformerBlock):
         dqkv = ops.attn_bwd(datt, sv["qkv"], sv["att"], sv["lse"], B, S, self.Hq, self.Hkv, self.D, self.causal,
                             self.window)
         cs = self._rope(ops, S, dout.device)
-        if cs is not None:
+        if self.qk_norm:
+            self._head_norm_bwd(dqkv, cs, S, ops, sv)
+        elif cs is not None:
             ops.rope_(dqkv, cs, S, self.Hq + self.Hkv, self.D, backward=True)
         dxin = tp.linear_rs(ops, dqkv, p["qkv_w"], False)
         ops.linear_wgrad(dqkv, tp.gather_rows(xin), g["qkv_w"], g.get("qkv_b"))

@@ -41,6 +41,9 @@ class TrainerOptions:
     activation_recompute: Optional[bool] = None
     activation_offload: Optional[bool] = None
     lr: float = 1e-3
+    optimizer: str = "adam"                # "adam" (decay through the gradient) | "adamw" (decoupled decay)
+    weight_decay: float = 0.0
+    moment_bits: int = 32                  # adamw: 8 keeps both moments in two bytes a parameter instead of eight
     seed: int = 0
     backend: Optional[str] = None          # torch.distributed backend override ("gloo" forces CPU)
     model_overrides: dict = field(default_factory=dict)
@@ -57,6 +60,8 @@ class Trainer:
     def __init__(self, cfg: PipelineConfig, opt: TrainerOptions):
         if opt.offload_model_params and not opt.optimizer_in_backward:
             raise ValueError("--offload_model_params requires --optimizer_in_backwards")
+        if opt.optimizer not in ("adam", "adamw"):
+            raise ValueError(f"optimizer is adam or adamw, not {opt.optimizer!r}")
         if opt.collectives == "fused":
             opt.optimizer_in_backward = True  # the fused reduce-scatter kernel applies Adam itself
         self.cfg, self.opt = cfg, opt
@@ -73,7 +78,8 @@ class Trainer:
             compute_dtype=compute, reduce_dtype=dtype_from_str(cfg.reduce_dtype),
             optimizer_in_backward=opt.optimizer_in_backward, offload_params=opt.offload_model_params,
             collectives=opt.collectives, grad_divide_by_group=cfg.grad_norm_compat == "reference",
-            adam=AdamConfig(lr=opt.lr), seed=opt.seed)
+            adam=AdamConfig(lr=opt.lr, weight_decay=opt.weight_decay, decoupled=opt.optimizer == "adamw",
+                            moment_bits=opt.moment_bits), seed=opt.seed)
         self.streams = Streams(self.device)
         # tensor parallelism: the config numbers lanes of tp processes; everything that follows the plan
         # (stages, microbatches, p2p peers) uses the lane number, the groups use process ranks
