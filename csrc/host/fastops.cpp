@@ -750,7 +750,7 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!matrix(dy, BF16) || dy->sizes() != a.qkv->sizes() || !on(dy, *a.qkv) || ptr(dy) == ptr(a.qkv) || !dense(rstd, F32) ||
       rstd->dim() != 2 || rstd->size(0) != T || rstd->size(1) != a.nq + a.nk || !on(rstd, *a.qkv) || !gradient(gwq) || !gradient(gwk) ||
       gwq->scalar_type() != gwk->scalar_type() || gwq->dim() != 1 || gwk->dim() != 1 || gwq->size(0) != a.d || gwk->size(0) != a.d ||
-      !on(gwq, *a.qkv) || !on(gwk, *a.qkv))
+      !on(gwq, *a.qkv) || !on(gwk, *a.qkv) || ptr(gwq) == ptr(gwk))
     Py_RETURN_NONE;
   long floats = 0;
   lib.qk_norm_rope_workspace(int(T), int(a.nq), int(a.nk), int(a.d), &floats);

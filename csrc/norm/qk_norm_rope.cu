@@ -5,6 +5,10 @@
 //   backward  g = R^T dy,  xh = x rstd,  dx = rstd (w g - xh mean(w g xh)),  dw += sum over tokens and heads of g xh
 // Sums and products are in fp32 and a value is rounded to bf16 once, at the end: as two passes the normalised heads would be
 // rounded in between.
+// Both directions are bound by memory: 16384 tokens of 32 + 8 + 8 heads of 128 forward into a new tensor 64 to 66 us, 6.2 TB/s or
+// 96 % of a copy's rate; 8192 tokens of 32 + 32 heads of 128 backward 72 us, 5.6 TB/s or 88 %, of which 3 are the sum over the
+// CTAs in a launch of its own.  Small ones are bound by their launches: 256 tokens of 8 + 2 x 8 heads of 64 2.2 us forward in a graph
+// and 4.6 backward, 5.7 and 7.2 called from Python.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "norm_common.cuh"
@@ -17,10 +21,11 @@ struct QkNormArgs {
   const __nv_bfloat16 *wq, *wk;
   const float* cs;          // [S, d] cosines | sines; null: no rotation
   float* rstd;              // [T, nq + nk]; forward: null if not kept
-  float* partial;           // backward: [CTAs, 2, d]
+  float* partial;           // backward: [CTAs, d]
   long ldx, ldy;
   int T, S, nq, nk, nv, d;  // nv: value heads to copy (forward into another tensor), else 0
   int span;                 // forward: units of a warp's item
+  int ctas_q;               // backward: CTAs of the query heads
   float eps, inv_d;
 };
 
@@ -48,7 +53,8 @@ __device__ __forceinline__ void load_angles(const float* row, int half, float (&
 }
 
 // Bytes on the way bound these passes: with a unit's operands in registers, and a hundred of those a thread, an SM has too few
-// requests out.  So every thread copies its own chunks some units ahead into a ring of its own in shared memory.
+// requests out.  So every thread copies its own chunks some units ahead into a ring of its own in shared memory (the two large
+// cases above 81 -> 66 us, with packed arithmetic and the angles kept for a token's heads, and 141 -> 74).
 constexpr int QK_RING = 3;
 // Two values an instruction (fma.rn.f32x2 and the like): a head's arithmetic is most of what an SM issues here.
 struct Pair {
@@ -174,7 +180,8 @@ struct QkRing {
   uint4 chunk[QK_RING][4][256];    // x low, x high, gradient low, gradient high
   float rstd[QK_RING][256];
 };
-// A warp takes an equal stretch of the units of all tokens, for either kind; the ring runs on over its tokens.
+// The first `ctas_q` CTAs have the query heads, the others the key heads: one set of weights and of weight-gradient sums a thread.
+// A warp takes an equal stretch of its kind's units of all tokens; the ring runs on over its tokens.
 template <int LANES, bool ROPE>
 __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs a) {
   chain_trigger();
@@ -185,149 +192,146 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs 
   __shared__ float part[8][LANES * 16];
   const int tid = threadIdx.x, half = a.d >> 1, lane = tid & 31, warp = tid >> 5, c = (lane % LANES) * 8, sub = lane / LANES;
   const bool used = c < half;
-  const int step = HEADS * a.d, nqk = a.nq + a.nk;
-  for (int kind = 0; kind < 2; ++kind) {          // query heads, then key heads: one set of weight-gradient sums at a time
-    const int n = kind ? a.nk : a.nq, h0 = kind ? a.nq : 0, units = (n + HEADS - 1) / HEADS;
-    if (n == 0) {
-      for (int j = tid; j < a.d; j += 256) a.partial[(size_t(blockIdx.x) * 2 + kind) * a.d + j] = 0.f;
-      continue;
-    }
-    Pair w[8], dw[8];
-    HeadChunk wu = {};
-    if (used) wu = load_head((kind ? a.wk : a.wq) + c, half);
-    unpack_pairs(wu, w);
+  const int step = HEADS * a.d, nqk = a.nq + a.nk, kind = int(blockIdx.x) >= a.ctas_q;
+  const int n = kind ? a.nk : a.nq, h0 = kind ? a.nq : 0, units = (n + HEADS - 1) / HEADS;
+  Pair w[8], dw[8];
+  HeadChunk wu = {};
+  if (used) wu = load_head((kind ? a.wk : a.wq) + c, half);
+  unpack_pairs(wu, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[j] = both(0.f);
-    const long all = long(a.T) * units, me = blockIdx.x * 8 + warp, warps = gridDim.x * 8;
-    const long first = all * me / warps;
-    int left = int(all * (me + 1) / warps - first), to_ask = left;
-    unsigned t = unsigned(first / units);
-    int u = int(first - long(t) * units);
-    // the next unit to ask for: its number in the token, this lane's head among the kind's, and where that lies
-    int ask_u = u, ask_k = u * HEADS + sub;
-    size_t col = size_t(h0 + ask_k) * a.d + c;
-    const __nv_bfloat16 *ask_x = a.x + t * a.ldx + col, *ask_g = a.y + t * a.ldy + col;
-    __nv_bfloat16* dst = a.y + t * a.ldy + col;
-    const float* ask_r = a.rstd + size_t(t) * nqk + h0 + ask_k;
-    const long next_x = a.ldx - long(units) * step, next_g = a.ldy - long(units) * step;   // from behind a token's units to the next one's
-    auto request = [&](int slot) {
-      if (to_ask > 0) {
-        if (used && ask_k < n) {
-          ring_load16(&ring.chunk[slot][0][tid], ask_x);
-          ring_load16(&ring.chunk[slot][1][tid], ask_x + half);
-          ring_load16(&ring.chunk[slot][2][tid], ask_g);
-          ring_load16(&ring.chunk[slot][3][tid], ask_g + half);
-          ring_load4(&ring.rstd[slot][tid], ask_r);
-        }
-        --to_ask;
-        ask_x += step;
-        ask_g += step;
-        ask_r += HEADS;
-        ask_k += HEADS;
-        if (++ask_u == units) {
-          ask_u = 0;
-          ask_k = sub;
-          ask_x += next_x;
-          ask_g += next_g;
-          ask_r += nqk - units * HEADS;
-        }
+  for (int j = 0; j < 8; ++j) dw[j] = both(0.f);
+  const long all = long(a.T) * units, me = (blockIdx.x - (kind ? a.ctas_q : 0)) * 8 + warp;
+  const long warps = (kind ? gridDim.x - a.ctas_q : a.ctas_q) * 8;
+  const long first = all * me / warps;
+  int left = int(all * (me + 1) / warps - first), to_ask = left;
+  unsigned t = unsigned(first / units);
+  int u = int(first - long(t) * units);
+  // the next unit to ask for: its number in the token, this lane's head among the kind's, and where that lies
+  int ask_u = u, ask_k = u * HEADS + sub;
+  size_t col = size_t(h0 + ask_k) * a.d + c;
+  const __nv_bfloat16 *ask_x = a.x + t * a.ldx + col, *ask_g = a.y + t * a.ldy + col;
+  __nv_bfloat16* dst = a.y + t * a.ldy + col;
+  const float* ask_r = a.rstd + size_t(t) * nqk + h0 + ask_k;
+  const long next_x = a.ldx - long(units) * step, next_g = a.ldy - long(units) * step;   // from behind a token's units to the next one's
+  auto request = [&](int slot) {
+    if (to_ask > 0) {
+      if (used && ask_k < n) {
+        ring_load16(&ring.chunk[slot][0][tid], ask_x);
+        ring_load16(&ring.chunk[slot][1][tid], ask_x + half);
+        ring_load16(&ring.chunk[slot][2][tid], ask_g);
+        ring_load16(&ring.chunk[slot][3][tid], ask_g + half);
+        ring_load4(&ring.rstd[slot][tid], ask_r);
       }
-      ring_commit();
-    };
-#pragma unroll
-    for (int k = 0; k < QK_RING - 1; ++k) request(k);
-    int slot = 0, pos = int(t % unsigned(a.S));
-    while (left > 0) {
-      float co[8] = {}, si[8] = {};
-      if (ROPE && used) load_angles(a.cs + size_t(pos) * a.d + c, half, co, si);
-      const int here = min(left, units - u);
-      left -= here;
-      int k = u * HEADS + sub;
-      for (int i = 0; i < here; ++i) {
-        request((slot + QK_RING - 1) % QK_RING);
-        ring_wait<QK_RING - 1>();
-        const bool live = used && k < n;
-        HeadChunk xu = {}, gu = {};
-        float rstd = 0.f;
-        if (live) {
-          xu = {ring.chunk[slot][0][tid], ring.chunk[slot][1][tid]};
-          gu = {ring.chunk[slot][2][tid], ring.chunk[slot][3][tid]};
-          rstd = ring.rstd[slot][tid];
-        }
-        slot = (slot + 1) % QK_RING;
-        // with g = rstd R^T dy:  dw += g x,  dx = w g - x rstd^2 mean(w g x)
-        Pair x[8], g[8], along = both(0.f);
-        unpack_pairs(xu, x);
-        unpack_pairs(gu, g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Pair lo = g[j] * both(rstd), hi = g[4 + j] * both(rstd);
-          const Pair cc = {co[2 * j], co[2 * j + 1]}, ss = {si[2 * j], si[2 * j + 1]}, back = {-ss.a, -ss.b};
-          g[j] = ROPE ? fma2(hi, ss, lo * cc) : lo;
-          g[4 + j] = ROPE ? fma2(lo, back, hi * cc) : hi;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          dw[j] = fma2(g[j], x[j], dw[j]);
-          g[j] = g[j] * w[j];
-          along = fma2(g[j], x[j], along);
-        }
-        const float m = -head_sum<LANES>(along.a + along.b) * a.inv_d * (rstd * rstd);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = fma2(x[j], both(m), g[j]);
-        if (live) store_head(dst, half, pack_pairs(g));
-        k += HEADS;
-        dst += step;
-      }
-      u = 0;
-      dst += next_g;
-      pos = pos + 1 == a.S ? 0 : pos + 1;
-    }
-    ring_wait<0>();
-    // over the heads of a warp, then over its CTA's warps
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-      for (int o = 16; o >= LANES; o >>= 1) {
-        dw[j].a += __shfl_xor_sync(0xffffffffu, dw[j].a, o);
-        dw[j].b += __shfl_xor_sync(0xffffffffu, dw[j].b, o);
-      }
-      if (lane < LANES && used) {
-        const int at = (j < 4 ? 0 : half) + c + 2 * (j & 3);
-        part[warp][at] = dw[j].a;
-        part[warp][at + 1] = dw[j].b;
+      --to_ask;
+      ask_x += step;
+      ask_g += step;
+      ask_r += HEADS;
+      ask_k += HEADS;
+      if (++ask_u == units) {
+        ask_u = 0;
+        ask_k = sub;
+        ask_x += next_x;
+        ask_g += next_g;
+        ask_r += nqk - units * HEADS;
       }
     }
-    __syncthreads();
-    for (int j = tid; j < a.d; j += 256) {
-      float s = 0.f;
+    ring_commit();
+  };
 #pragma unroll
-      for (int v = 0; v < 8; ++v) s += part[v][j];
-      a.partial[(size_t(blockIdx.x) * 2 + kind) * a.d + j] = s;
+  for (int k = 0; k < QK_RING - 1; ++k) request(k);
+  int slot = 0, pos = int(t % unsigned(a.S));
+  while (left > 0) {
+    float co[8] = {}, si[8] = {};
+    if (ROPE && used) load_angles(a.cs + size_t(pos) * a.d + c, half, co, si);
+    const int here = min(left, units - u);
+    left -= here;
+    int k = u * HEADS + sub;
+    for (int i = 0; i < here; ++i) {
+      request((slot + QK_RING - 1) % QK_RING);
+      ring_wait<QK_RING - 1>();
+      const bool live = used && k < n;
+      HeadChunk xu = {}, gu = {};
+      float rstd = 0.f;
+      if (live) {
+        xu = {ring.chunk[slot][0][tid], ring.chunk[slot][1][tid]};
+        gu = {ring.chunk[slot][2][tid], ring.chunk[slot][3][tid]};
+        rstd = ring.rstd[slot][tid];
+      }
+      slot = (slot + 1) % QK_RING;
+      // with g = rstd R^T dy:  dw += g x,  dx = w g - x rstd^2 mean(w g x)
+      Pair x[8], g[8], along = both(0.f);
+      unpack_pairs(xu, x);
+      unpack_pairs(gu, g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Pair lo = g[j] * both(rstd), hi = g[4 + j] * both(rstd);
+        const Pair cc = {co[2 * j], co[2 * j + 1]}, ss = {si[2 * j], si[2 * j + 1]}, back = {-ss.a, -ss.b};
+        g[j] = ROPE ? fma2(hi, ss, lo * cc) : lo;
+        g[4 + j] = ROPE ? fma2(lo, back, hi * cc) : hi;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dw[j] = fma2(g[j], x[j], dw[j]);
+        g[j] = g[j] * w[j];
+        along = fma2(g[j], x[j], along);
+      }
+      const float m = -head_sum<LANES>(along.a + along.b) * a.inv_d * (rstd * rstd);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = fma2(x[j], both(m), g[j]);
+      if (live) store_head(dst, half, pack_pairs(g));
+      k += HEADS;
+      dst += step;
     }
+    u = 0;
+    dst += next_g;
+    pos = pos + 1 == a.S ? 0 : pos + 1;
+  }
+  ring_wait<0>();
+  // over the heads of a warp, then over its CTA's warps
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int o = 16; o >= LANES; o >>= 1) {
+      dw[j].a += __shfl_xor_sync(0xffffffffu, dw[j].a, o);
+      dw[j].b += __shfl_xor_sync(0xffffffffu, dw[j].b, o);
+    }
+    if (lane < LANES && used) {
+      const int at = (j < 4 ? 0 : half) + c + 2 * (j & 3);
+      part[warp][at] = dw[j].a;
+      part[warp][at + 1] = dw[j].b;
+    }
+  }
+  __syncthreads();
+  for (int j = tid; j < a.d; j += 256) {
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) s += part[v][j];
+    a.partial[size_t(blockIdx.x) * a.d + j] = s;
   }
 }
 
-// slot[j] += sum over `rows` of partial[row][j], in a fixed order: 32 columns per CTA, its warps over the rows.
+// slot[j] += sum of partial[row][j] over a kind's rows, in a fixed order: 32 columns per CTA, its warps over the rows.
 template <typename GT>
-__global__ void __launch_bounds__(1024) qk_norm_weight_grad_kernel(const float* partial, GT* gwq, GT* gwk, int rows, int d) {
+__global__ void __launch_bounds__(1024) qk_norm_weight_grad_kernel(const float* partial, GT* gwq, GT* gwk, int ctas_q, int ctas, int d) {
   chain_trigger();
   chain_wait();
   __shared__ float part[32][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (col < 2 * d) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (d + 31) / 32, kind = int(blockIdx.x) >= per;
+  const int col = (blockIdx.x - kind * per) * 32 + lane, end = kind ? ctas : ctas_q;
+  GT* slot = (kind ? gwk : gwq) + col;
+  float s = 0.f, old = 0.f;
+  if (col < d) {
+    if (warp == 0) old = float(*slot);
 #pragma unroll 8
-    for (int r = warp; r < rows; r += 32) s += partial[size_t(r) * 2 * d + col];
+    for (int r = (kind ? ctas_q : 0) + warp; r < end; r += 32) s += partial[size_t(r) * d + col];
   }
   part[warp][lane] = s;
   __syncthreads();
-  if (warp != 0 || col >= 2 * d) return;
+  if (warp != 0 || col >= d) return;
 #pragma unroll
   for (int v = 1; v < 32; ++v) s += part[v][lane];
-  GT* slot = col < d ? gwq + col : gwk + (col - d);
-  *slot = GT(float(*slot) + s);
+  *slot = GT(old + s);
 }
 
 static int qk_norm_lanes(int d) {
@@ -341,10 +345,20 @@ static int qk_norm_span(long T, int units, long warps, int most) {
   const long s = T * units / warps;
   return int(s < 1 ? 1 : s > most ? most : s);
 }
-static int qk_norm_bwd_ctas(int T, int nq, int nk, int d) {
-  const int per = 32 / qk_norm_lanes(d), most = nq > nk ? nq : nk;
-  const long want = (long(T) * ((most + per - 1) / per) + 7) / 8, cap = long(num_sms()) * 2;
-  return int(want < cap ? want : cap);
+// CTAs of the backward pass for either kind of head: a unit for every warp, but no more than are on the GPU at once.  Those are dealt
+// out by the work on a token: its units, and its angles and place, which take as long as one more.  (One kind behind the other on all
+// CTAs: 256 tokens of 8 + 8 heads of 64 6.0 us instead of 4.6, 8192 of 32 + 8 heads of 128 46.7 instead of 46.1.)
+static void qk_norm_bwd_ctas(int T, int nq, int nk, int d, int* of_q, int* of_all) {
+  const int per = 32 / qk_norm_lanes(d);
+  const long uq = (nq + per - 1) / per, uk = (nk + per - 1) / per, cap = long(num_sms()) * 2;
+  long q = (T * uq + 7) / 8, k = (T * uk + 7) / 8;
+  if (q + k > cap) {
+    q = q == 0 ? 0 : k == 0 ? cap : cap * (uq + 1) / (uq + uk + 2);
+    q = uq > 0 && q < 1 ? 1 : uk > 0 && q > cap - 1 ? cap - 1 : q;
+    k = cap - q;
+  }
+  *of_q = int(q);
+  *of_all = int(q + k);
 }
 
 static int qk_norm_check(const QkNormArgs& a) {
@@ -405,7 +419,9 @@ int zb_qk_norm_rope_fwd(const void* x, void* y, const void* wq, const void* wk, 
 // *floats: what zb_qk_norm_rope_bwd wants as workspace
 int zb_qk_norm_rope_workspace(int T, int nq, int nk, int d, long* floats) {
   using namespace zb;
-  *floats = d > 0 && T > 0 ? 2L * d * qk_norm_bwd_ctas(T, nq, nk, d) : 0;
+  int of_q = 0, ctas = 0;
+  if (d > 0 && T > 0) qk_norm_bwd_ctas(T, nq, nk, d, &of_q, &ctas);
+  *floats = long(ctas) * d;
   return 0;
 }
 
@@ -420,7 +436,8 @@ int zb_qk_norm_rope_bwd(void* dy, const void* x, const void* wq, const void* wk,
   a.T = T; a.S = S; a.nq = nq; a.nk = nk; a.d = d; a.inv_d = 1.f / d;
   if (int rc = qk_norm_check(a)) return rc;
   if (T <= 0 || nq + nk == 0) return 0;
-  const int grid = qk_norm_bwd_ctas(T, nq, nk, d);
+  int grid = 0;
+  qk_norm_bwd_ctas(T, nq, nk, d, &a.ctas_q, &grid);
   int rc;
   switch (qk_norm_lanes(d)) {
     case 1: rc = qk_norm_bwd_launch<1>(a, grid, stream); break;
@@ -431,13 +448,13 @@ int zb_qk_norm_rope_bwd(void* dy, const void* x, const void* wq, const void* wk,
     default: rc = qk_norm_bwd_launch<32>(a, grid, stream); break;
   }
   if (rc) return rc;
-  const int columns = (2 * d + 31) / 32;
+  const int columns = 2 * ((d + 31) / 32);
   if (grad_f32)
     ZB_CUDA_OK(launch_pass(qk_norm_weight_grad_kernel<float>, columns, 1024, 0, stream, partial, static_cast<float*>(gwq),
-                           static_cast<float*>(gwk), grid, d));
+                           static_cast<float*>(gwk), a.ctas_q, grid, d));
   else
     ZB_CUDA_OK(launch_pass(qk_norm_weight_grad_kernel<__nv_bfloat16>, columns, 1024, 0, stream, partial,
-                           static_cast<__nv_bfloat16*>(gwq), static_cast<__nv_bfloat16*>(gwk), grid, d));
+                           static_cast<__nv_bfloat16*>(gwq), static_cast<__nv_bfloat16*>(gwk), a.ctas_q, grid, d));
   return 0;
 }
 

@@ -13,9 +13,14 @@
 // near 2^32 / golden ratio) through two rounds of shift-xor and multiplication by the fraction bits of sqrt 2 and sqrt 3.
 // m and v are computed by multiplications and additions that round one by one, so that the codes are a function of the
 // inputs and not of the compiler's contractions; encoding and decoding are integer operations.
+//
+// Bound by memory: 8 x 61 million parameters, fp32 gradients, 1.42 ms with moments in 8 bits (18 bytes a parameter, 6.2 TB/s or
+// 96 % of a copy's rate); the units of a 125M model, bf16 gradients, 0.755 ms with moments in fp32 (28 bytes, 94 %).  The 8-bit form
+// is near the issue limit as well (58 instructions a value; 76 with scalar arithmetic and codes handled one by one took 1.6 ms).
+// Blocks go to warps round robin, so that all warps work in one part of the tensors: in a stretch of its own for each warp, the
+// same kernel took 1.58 ms.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
-#include <type_traits>
 
 namespace zb {
 

@@ -103,7 +103,7 @@ def test_refusals_cpu(wrapper):
     g, rstd = torch.zeros(d), torch.ones(T, nq + nk)
     ok |= dict(dqkv=dy, rstd=rstd, gwq=g, gwk=g.clone())
     for wrong in (dict(dqkv=qkv), dict(dqkv=dy[:3]), dict(rstd=rstd[:, :2]), dict(rstd=rstd.double()), dict(gwq=g.bfloat16()),
-                  dict(gwq=g.double(), gwk=g.double()), dict(gwk=g[:32])):
+                  dict(gwq=g.double(), gwk=g.double()), dict(gwk=g[:32]), dict(gwk=g)):
         with pytest.raises(ValueError):
             wrapper.qk_norm_rope_bwd(**{**ok, **wrong})
 

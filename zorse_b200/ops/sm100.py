@@ -368,6 +368,7 @@ def qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S: int, nq: int, nk: int, d: i
     _need(gwq.dtype == gwk.dtype and gwq.dtype in (torch.float32, torch.bfloat16) and gwq.shape == gwk.shape == (d,)
           and gwq.is_contiguous() and gwk.is_contiguous() and gwq.device == gwk.device == qkv.device,
           "gwq and gwk: both fp32 or both bf16, of the weights' shape")
+    _need(gwq.data_ptr() != gwk.data_ptr(), "gwq and gwk are the same memory")
     L = lib()
     partial = torch.empty(_workspace_size(L.zb_qk_norm_rope_workspace, T, nq, nk, d), dtype=torch.float32, device=qkv.device)
     _check(L.zb_qk_norm_rope_bwd(_a(dqkv), _a(qkv), _a(wq), _a(wk), _a(rstd), _a(cs), _a(partial), _a(gwq), _a(gwk), T, S, nq, nk, d,
