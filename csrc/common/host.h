@@ -7,6 +7,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <string.h>
+#include <atomic>
 
 namespace zb {
 
@@ -139,6 +140,21 @@ template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pass(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
   return launch_chained(kern, grid, threads, smem, stream, 0, static_cast<Args&&>(args)...);
 }
+
+// Lets a kernel have more than 48 KB of shared memory, once on every device: asking the driver each time costs a fifth of a launch.
+struct SharedLimit {
+  std::atomic<unsigned long long> done{0};
+  template <typename K>
+  cudaError_t raise(K kern, size_t bytes) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+  }
+};
 
 inline int num_sms() {
   static int n[64] = {0};

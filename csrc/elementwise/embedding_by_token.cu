@@ -15,6 +15,7 @@
 #include "../norm/norm_common.cuh"
 
 namespace zb {
+
 __device__ __forceinline__ int clamp_id(long id, int V) {
   return static_cast<unsigned long>(id) < static_cast<unsigned long>(V) ? int(id) : id < 0 ? 0 : V - 1;
 }
@@ -552,7 +553,8 @@ template <int K, typename GT>
 static int by_token(const ByToken& a, GT* table, cudaStream_t stream) {
   const int slices = (a.H + 255) / 256, pieces = (a.n + K - 1) / K;
   auto kern = embedding_pieces_kernel<K, GT>;
-  ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PieceRing<GT>))));
+  static SharedLimit limit;
+  ZB_CUDA_OK(limit.raise(kern, sizeof(PieceRing<GT>)));
   ZB_CUDA_OK(launch_pass(kern, (pieces * slices + 7) / 8, 256, sizeof(PieceRing<GT>), stream, a, table));
   if (pieces > 1) ZB_CUDA_OK(launch_pass(embedding_join_kernel<K, GT>, (pieces + 7) / 8 * slices, 256, 0, stream, a, table));
   return 0;
@@ -637,7 +639,8 @@ int zb_embedding_by_token(const long* ids, const void* dout, void* gtable, void*
     auto kern = embedding_sort_kernel<32>;
     if (most <= 4 * 1024) kern = embedding_sort_kernel<4>;
     else if (most <= 16 * 1024) kern = embedding_sort_kernel<16>;
-    ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SortShared))));
+    static SharedLimit limit[3];
+    ZB_CUDA_OK(limit[most <= 4 * 1024 ? 0 : most <= 16 * 1024 ? 1 : 2].raise(kern, sizeof(SortShared)));
     ZB_CUDA_OK(launch_pass(kern, chunks * ctas, 1024, sizeof(SortShared), stream, ids, order, sorted, T, V, width, ctas));
     for (int c = 0; c < chunks; ++c) {
       ByToken a = {rows, order + c * SORT_CHUNK, sorted + c * SORT_CHUNK, head, tail, T - c * SORT_CHUNK < SORT_CHUNK ? T - c * SORT_CHUNK : SORT_CHUNK,

@@ -845,7 +845,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!dense(first, F32) || !here(*first)) Py_RETURN_NONE;
   int bits = 0;
   c10::SmallVector<AdamwTensor, 32> table;
-  c10::SmallVector<void*, 32> seen;
+  c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 64> written;
+  auto writes = [&](const void* p, int64_t bytes) {
+    if (p != nullptr) written.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + uintptr_t(bytes));
+  };
   for (Py_ssize_t i = 0; i < n; ++i) {
     const Tensor *p = tensor_of(PyList_GET_ITEM(args[0], i)), *g = tensor_of(PyList_GET_ITEM(args[2], i)), *p16;
     PyObject* mom = PyList_GET_ITEM(args[1], i);
@@ -885,12 +888,19 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.seed = static_cast<unsigned>(seed);
     a.grad_f32 = g->scalar_type() == F32;
     table.push_back(a);
-    seen.push_back(a.p);
+    writes(a.p, 4 * num);
+    writes(a.p16, 2 * num);
+    writes(a.m, num * (bits / 8));
+    writes(a.v, num * (bits / 8));
+    writes(a.mb, 2 * ((num + 255) / 256));
+    writes(a.vb, 2 * ((num + 255) / 256));
   }
-  std::sort(seen.begin(), seen.end());
-  if (table.empty() || std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second) Py_RETURN_NONE;
+  if (table.empty() || h[1] < 0 || h[1] >= 1 || h[2] < 0 || h[2] >= 1) Py_RETURN_NONE;
   const cudaStream_t s = stream();
-  if (!launch("adamw", 1, [&] {
+  if (!launch("adamw", int((table.size() + 255) / 256), [&] {
         return lib.adamw_list(table.data(), int(table.size()), bits, float(h[1]), float(1 - h[1]), float(h[2]), float(1 - h[2]),
                               float(h[3]), float(1 - h[0] * h[4]), float(h[5]), s);
       }))

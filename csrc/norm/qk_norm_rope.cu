@@ -384,7 +384,8 @@ template <int LANES>
 static int qk_norm_bwd_launch(const QkNormArgs& a, int grid, cudaStream_t stream) {
   auto kern = qk_norm_rope_bwd_kernel<LANES, true>;
   if (a.cs == nullptr) kern = qk_norm_rope_bwd_kernel<LANES, false>;
-  ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(QkRing))));
+  static SharedLimit limit[2];
+  ZB_CUDA_OK(limit[a.cs == nullptr].raise(kern, sizeof(QkRing)));
   ZB_CUDA_OK(launch_pass(kern, grid, 256, sizeof(QkRing), stream, a));
   return 0;
 }

@@ -453,7 +453,8 @@ static int adamw_launch(const AdamwTensor* t, int count, const AdamwHyper& h, cu
   if (blocks == 0) return 0;
   const long want = (blocks + 7) / 8, cap = long(num_sms()) * ADAMW_CTAS;
   auto kern = adamw_list_kernel<N, BITS>;
-  ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(AdamwRing<BITS>))));
+  static SharedLimit limit;
+  ZB_CUDA_OK(limit.raise(kern, sizeof(AdamwRing<BITS>)));
   ZB_CUDA_OK(launch_pass(kern, int(want < cap ? want : cap), 256, sizeof(AdamwRing<BITS>), stream, list));
   return 0;
 }

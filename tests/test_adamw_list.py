@@ -129,6 +129,8 @@ def test_refusals_cpu(monkeypatch):
                   dict(step=lambda s: [1]), dict(step=lambda s: [3, 0]), dict(p=swap(0, torch.zeros(300).double())),
                   dict(p=lambda p: [p[0], p[0][:40]]), dict(p=swap(0, torch.zeros(600)[::2])), dict(g=swap(1, torch.zeros(39))),
                   dict(g=swap(1, torch.zeros(40).half())), dict(p16=swap(0, torch.zeros(300))), dict(p16=swap(0, torch.zeros(299).bfloat16())),
+                  dict(beta1=lambda b: 1.0), dict(beta2=lambda b: -0.1), dict(p=lambda p: [p[0], p[0][100:140]]),
+                  dict(moments=lambda m: [m[0], (m[0][0][:40], torch.zeros(40))]),
                   dict(moments=swap(1, (torch.zeros(40), torch.zeros(41)))), dict(moments=swap(1, (torch.zeros(40).bfloat16(), torch.zeros(40))))):
         with pytest.raises(ValueError):
             call(**wrong)

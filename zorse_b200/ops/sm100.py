@@ -333,7 +333,7 @@ def _qk_norm_operands(x, wq, wk, cs, S, nq, nk, d):
     T = x.shape[0]
     _need(x.dim() == 2 and x.shape[1] == (nq + 2 * nk) * d and x.stride(1) == 1,
           f"qkv is {tuple(x.shape)}, strides {x.stride()}: expected rows of ({nq} + 2 x {nk}) x {d}")
-    _need(wq.shape == (d,) and wk.shape == (d,) and wq.is_contiguous() and wk.is_contiguous(),
+    _need(wq.shape == (d,) and wk.shape == (d,) and wq.is_contiguous() and wk.is_contiguous() and wq.device == wk.device == x.device,
           f"weights of {tuple(wq.shape)} and {tuple(wk.shape)} for heads of {d}")
     if cs is not None:
         _need(cs.dtype == torch.float32 and cs.device == x.device and cs.dim() == 2 and cs.is_contiguous() and cs.shape[1] == d
@@ -509,10 +509,11 @@ def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps
     bits = 32 if len(moments[0]) == 2 else 8
     _need(bits == 32 or (seeds is not None and len(seeds) == n), "moments in 8 bits need a seed for each tensor")
     steps = step if isinstance(step, (list, tuple)) else [step] * n
+    _need(0 <= beta1 < 1 and 0 <= beta2 < 1, f"betas {beta1}, {beta2} are not in [0, 1)")
     _need(len(steps) == n and min(steps) >= 1, "step counts from 1, one for all tensors or one for each")
     dev = p[0].device
     _on_current(p[0], "p")
-    table, seen = [], set()
+    table, written, count = [], [], 0
     for i, (x, mom, d, y, k) in enumerate(zip(p, moments, g, p16, steps)):
         num = x.numel()
         _need(x.dtype == torch.float32 and x.is_contiguous() and x.device == dev, f"p[{i}]: contiguous fp32 on {dev}")
@@ -533,17 +534,19 @@ def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps
               and m.device == v.device == dev, f"moments[{i}]: {num} contiguous {dtype} on {dev}")
         if num == 0:
             continue
-        at = x.data_ptr()
-        _need(at not in seen, f"p[{i}] is in the list twice")
-        seen.add(at)
-        table += (at, m.data_ptr(), v.data_ptr(), _a(mb), _a(vb), d.data_ptr(), _a(y), num, lr / (1 - beta1 ** k),
+        written += [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (x, m, v, mb, vb, y) if t is not None]
+        count += 1
+        table += (x.data_ptr(), m.data_ptr(), v.data_ptr(), _a(mb), _a(vb), d.data_ptr(), _a(y), num, lr / (1 - beta1 ** k),
                   1 / math.sqrt(1 - beta2 ** k), seeds[i] & 0xFFFFFFFF if bits == 8 else 0, int(d.dtype == torch.float32))
-    count = len(seen)
     if count == 0:
         return
+    written.sort()
+    _need(all(a[1] <= b[0] for a, b in zip(written, written[1:])), "tensors that the step writes overlap (one is in the list twice?)")
     packed = struct.pack("8Qff2I" * count, *table)
     _check(lib().zb_adamw_list(packed, count, bits, beta1, 1 - beta1, beta2, 1 - beta2, eps, 1 - lr * weight_decay, grad_scale,
                                _stream()), "adamw")
+    global _launches
+    _launches += (count - 1) // 256
 
 
 def moment_values(moments, dtype=torch.float32):
