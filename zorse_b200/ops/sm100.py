@@ -434,6 +434,9 @@ def embedding_bwd(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int = 0)
                                   _stream()), "embedding_bwd")
 
 
+EMBEDDING_CHUNK = 32768      # ids that are put in order together
+
+
 def _embedding_operands(ids, rows, table, what, pos_table, S, pos_offset):
     T, H = ids.numel(), table.shape[1]
     _on_current(table, what)
@@ -474,7 +477,7 @@ def embedding_by_token(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int
     _check(L.zb_embedding_by_token(_a(ids), _a(dout), _a(dtable), _a(dpos), _a(ws), T, H, V, S, pos_offset, scale,
                                    int(dtable.dtype == torch.float32), _stream()), "embedding_by_token")
     global _launches
-    _launches += (T > 0) + (T > 1) + (dpos is not None and T > 0)     # sums, their join, positions
+    _launches += (2 * -(-T // EMBEDDING_CHUNK) if ws.numel() else 0) + (dpos is not None and T > 0)   # sums and joined runs of a chunk, positions
 
 
 # --------------------------------------------------------------------------- loss
