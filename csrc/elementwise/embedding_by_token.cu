@@ -589,7 +589,7 @@ extern "C" {
 int zb_embedding_scaled(const long* ids, const void* table, const void* pos, void* out, int T, int H, int V, int S, int pos_offset,
                         float scale, cudaStream_t stream) {
   using namespace zb;
-  if (H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
+  if (H < 8 || H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
   if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(out)) & 15)
     ZB_FAIL(-1, "embedding: operands must be 16-byte aligned");
   if (T <= 0) return 0;
@@ -614,7 +614,7 @@ int zb_embedding_by_token_workspace(int T, int H, long* bytes) {
 int zb_embedding_by_token(const long* ids, const void* dout, void* gtable, void* gpos, void* workspace, int T, int H, int V, int S,
                           int pos_offset, float scale, int grad_f32, cudaStream_t stream) {
   using namespace zb;
-  if (H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
+  if (H < 8 || H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
   if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(gtable) | reinterpret_cast<uintptr_t>(gpos) |
        reinterpret_cast<uintptr_t>(workspace)) & 15)
     ZB_FAIL(-1, "embedding: operands must be 16-byte aligned");

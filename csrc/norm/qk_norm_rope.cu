@@ -366,6 +366,7 @@ static int qk_norm_check(const QkNormArgs& a) {
   if (a.nq < 0 || a.nk < 0 || a.nv < 0 || a.S < 1) ZB_FAIL(-1, "qk_norm_rope: %d + %d heads, sequences of %d", a.nq, a.nk, a.S);
   // units of all tokens, and what a warp of the last CTA counts up to behind them, in 32 bits
   if (long(a.T) * (a.nq + a.nk + a.nv + 3) >= (1L << 31) - (1L << 20)) ZB_FAIL(-1, "qk_norm_rope: %d tokens of %d heads", a.T, a.nq + a.nk);
+  if (a.T > 1 && a.ldy < long(a.nq + a.nk + a.nv) * a.d) ZB_FAIL(-1, "qk_norm_rope: rows to write lie over one another (stride %ld)", a.ldy);
   if (a.ldx % 8 != 0 || a.ldy % 8 != 0) ZB_FAIL(-1, "qk_norm_rope: row strides %ld, %ld not a multiple of 8", a.ldx, a.ldy);
   if ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.wq) |
        reinterpret_cast<uintptr_t>(a.wk) | reinterpret_cast<uintptr_t>(a.cs)) & 15)

@@ -177,6 +177,8 @@ def test_refused_by_the_library(ops):
     ids = torch.zeros(4, dtype=torch.long, device="cuda")
     with pytest.raises(KernelError):
         ops.embedding_fwd(ids, torch.zeros(5, 12, dtype=torch.bfloat16, device="cuda"), scale=2.0)
+    with pytest.raises(KernelError):
+        ops.embedding_bwd(ids, torch.zeros(4, 0, dtype=torch.bfloat16, device="cuda"), torch.zeros(5, 0, device="cuda"), by_token=True)
     dout = torch.zeros(4, 16, dtype=torch.bfloat16, device="cuda")
     off = torch.zeros(1 + 5 * 16, device="cuda")[1:].view(5, 16)
     with pytest.raises(KernelError):

@@ -94,7 +94,7 @@ def test_refusals_cpu(wrapper):
     qkv, wq, wk, cs, dy = _inputs(T, nq, nk, d, S)
     ok = dict(qkv=qkv, wq=wq, wk=wk, cs=cs, S=S, nq=nq, nk=nk, d=d, eps=1e-5)
     for wrong in (dict(qkv=qkv[:, :-8]), dict(qkv=qkv.t().contiguous().t()), dict(wq=wq[:32]), dict(wk=wk.repeat(2)[::2]),
-                  dict(cs=cs.double()), dict(cs=cs[:2]), dict(cs=cs[:, :32].contiguous()), dict(qkv=qkv.view(-1))):
+                  dict(cs=cs.double()), dict(cs=cs[:2]), dict(cs=cs[:, :32].contiguous()), dict(qkv=qkv.view(-1)), dict(S=0)):
         with pytest.raises(ValueError):
             wrapper.qk_norm_rope_fwd(**{**ok, **wrong})
     with pytest.raises(TypeError):
@@ -252,6 +252,8 @@ def test_refused_by_the_library(ops):
     with pytest.raises(KernelError):        # a head width that is no multiple of 16
         ops.qk_norm_rope_fwd(torch.zeros(4, 4 * 72, dtype=torch.bfloat16, device="cuda"), w, w, None, 4, 2, 1, 72, 1e-5)
     w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(KernelError):        # rows to write that lie over one another
+        ops.qk_norm_rope_fwd(x[:1, :256].expand(4, 256), w[:64], w[:64], None, 4, 2, 1, 64, 1e-5, keep=False)
     with pytest.raises(KernelError):        # rows off a 16-byte boundary
         ops.qk_norm_rope_fwd(x[:, 1:1 + 256], w, w, None, 4, 2, 1, 64, 1e-5)
     with pytest.raises(KernelError):        # a row stride that is no multiple of 8

@@ -330,11 +330,11 @@ def _qk_norm_operands(x, wq, wk, cs, S, nq, nk, d):
     """Checks what forward and backward of the head norms have in common."""
     _bf16(x, "qkv"); _bf16(wq, "wq"); _bf16(wk, "wk")
     _on_current(x, "qkv")
-    T = x.shape[0]
-    _need(x.dim() == 2 and x.shape[1] == (nq + 2 * nk) * d and x.stride(1) == 1,
+    _need(x.dim() == 2 and x.shape[0] < 2 ** 31 and 0 < S < 2 ** 31 and x.shape[1] == (nq + 2 * nk) * d and x.stride(1) == 1,
           f"qkv is {tuple(x.shape)}, strides {x.stride()}: expected rows of ({nq} + 2 x {nk}) x {d}")
     _need(wq.shape == (d,) and wk.shape == (d,) and wq.is_contiguous() and wk.is_contiguous() and wq.device == wk.device == x.device,
           f"weights of {tuple(wq.shape)} and {tuple(wk.shape)} for heads of {d}")
+    T = x.shape[0]
     if cs is not None:
         _need(cs.dtype == torch.float32 and cs.device == x.device and cs.dim() == 2 and cs.is_contiguous() and cs.shape[1] == d
               and cs.shape[0] >= min(S, T), f"table of {tuple(cs.shape)}, {cs.dtype}: expected fp32 [>= {min(S, T)}, {d}]")
@@ -440,6 +440,7 @@ EMBEDDING_CHUNK = 32768      # ids that are put in order together
 def _embedding_operands(ids, rows, table, what, pos_table, S, pos_offset):
     T, H = ids.numel(), table.shape[1]
     _on_current(table, what)
+    _need(max(T, *table.shape) < 2 ** 31, f"{T} ids, {what} {tuple(table.shape)}: sizes below 2^31")
     _need(ids.dtype == torch.int64 and ids.device == table.device and ids.is_contiguous(), f"ids: contiguous int64 on {table.device}")
     _need(table.dim() == 2 and table.is_contiguous(), f"{what} {tuple(table.shape)}: expected contiguous rows")
     if rows is not None:
