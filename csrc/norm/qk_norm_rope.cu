@@ -6,9 +6,9 @@
 // Sums and products are in fp32 and a value is rounded to bf16 once, at the end: as two passes the normalised heads would be
 // rounded in between.
 // Both directions are bound by memory: 16384 tokens of 32 + 8 + 8 heads of 128 forward into a new tensor 64 to 66 us, 6.2 TB/s or
-// 96 % of a copy's rate; 8192 tokens of 32 + 32 heads of 128 backward 72 us, 5.6 TB/s or 88 %, of which 3 are the sum over the
-// CTAs in a launch of its own.  Small ones are bound by their launches: 256 tokens of 8 + 2 x 8 heads of 64 2.2 us forward in a graph
-// and 4.6 backward, 5.7 and 7.2 called from Python.
+// 96 % of a copy's rate; 8192 tokens of 32 + 32 heads of 128 backward 71 us, 5.7 TB/s or 89 %, of which about 3 are the sum over
+// the CTAs in a launch of its own.  Small ones are bound by their launches: 256 tokens of 8 + 2 x 8 heads of 64 2.2 us forward in a
+// graph and 4.8 backward, 5.7 and 7.2 called from Python.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "norm_common.cuh"
@@ -323,8 +323,13 @@ __global__ void __launch_bounds__(1024) qk_norm_weight_grad_kernel(const float* 
   float s = 0.f, old = 0.f;
   if (col < d) {
     if (warp == 0) old = float(*slot);
-#pragma unroll 8
-    for (int r = (kind ? ctas_q : 0) + warp; r < end; r += 32) s += partial[size_t(r) * d + col];
+    for (int r = (kind ? ctas_q : 0) + warp; r < end; r += 8 * 32) {
+      float v[8];                        // (all asked for before the first is added)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = r + 32 * i < end ? partial[size_t(r + 32 * i) * d + col] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
   }
   part[warp][lane] = s;
   __syncthreads();

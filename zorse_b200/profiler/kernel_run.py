@@ -6,7 +6,8 @@ cases: gemm_fwd | gemm_dgrad | gemm_wgrad | gemm_act_fwd | gemm_act_bwd | gemm_r
        the epilogue) | wgrad_list (a block's weight gradients, bias and norm gradients from one list) | flash_fwd1 | flash_fwd2 | flash_fwd4 | flash_fwd4p | flash_fwd4q | flash_bwd1 | flash_bwd2 |
        flash_bwd | flash_bwd3 | flash_bwd3_dkv | flash_bwd3_dq (flash_bwd: the default version; the last three also as
        flash64_bwd3... on grouped heads of 64) | rmsnorm | rmsnorm_bwd | layernorm_bwd | rope | swiglu_fwd | swiglu_bwd |
-       embedding_fwd | embedding_bwd | adam | ce
+       embedding_fwd | embedding_bwd | adam | ce | qk_norm_rope_fwd | qk_norm_rope_bwd | embedding_scaled | embedding_by_token |
+       adamw_list | adamw_list8 | moment_values
 Prints the median CUDA-event time of the repetitions (a 256 MB write between them keeps operands out of L2).
 """
 from __future__ import annotations
@@ -109,6 +110,33 @@ def main(argv=None):
         p, m, v = (torch.zeros(n, device=dev) for _ in range(3))
         gr, p16 = rnd(n), torch.empty(n, device=dev, dtype=torch.bfloat16)
         fn = lambda: k.adam_step(p, m, v, gr, p16, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, step=1)
+    elif case in ("qk_norm_rope_fwd", "qk_norm_rope_bwd"):
+        T, S, nq, nk, d = 16384, 4096, 32, 8, 128                # 201 MB
+        from zorse_b200.ops.ref import rope_table
+
+        qkv, w, cs = rnd(T, (nq + 2 * nk) * d), rnd(d), rope_table(S, d, 1e4, dev)
+        _, rstd = k.qk_norm_rope_fwd(qkv, w, w, cs, S, nq, nk, d, 1e-5)
+        dqkv, gq, gk = rnd(T, (nq + 2 * nk) * d), torch.zeros(d, device=dev), torch.zeros(d, device=dev)
+        fn = ((lambda: k.qk_norm_rope_fwd(qkv, w, w, cs, S, nq, nk, d, 1e-5)) if case.endswith("fwd") else
+              (lambda: k.qk_norm_rope_bwd(dqkv, qkv, w, w, rstd, cs, S, nq, nk, d, gq, gk)))
+    elif case in ("embedding_scaled", "embedding_by_token"):
+        ids = torch.randint(0, 32000, (32768,), device=dev)
+        ids[torch.rand(32768, device=dev) < 0.2] = 7             # a padding token
+        table, dout, dtable = rnd(32000, 4096), rnd(32768, 4096), torch.zeros(32000, 4096, device=dev)
+        fn = (lambda: k.embedding_scaled(ids, table, scale=64.0)) if case.endswith("scaled") else (
+            lambda: k.embedding_by_token(ids, dout, dtable, scale=64.0))
+    elif case in ("adamw_list", "adamw_list8", "moment_values"):
+        from zorse_b200.ops.moments import Moments8
+
+        sizes = [16 * 1024 * 1024 + 64 * i for i in range(4)]
+        p, gr = [torch.zeros(n, device=dev) for n in sizes], [rnd(n).float() for n in sizes]
+        p16 = [torch.empty(n, device=dev, dtype=torch.bfloat16) for n in sizes]
+        mom = [Moments8.zeros(n, dev) if case != "adamw_list" else (torch.zeros(n, device=dev), torch.zeros(n, device=dev)) for n in sizes]
+        hyper = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.1, step=1)
+        if case == "moment_values":
+            k.adamw_step(p, mom, gr, p16, seeds=[1, 2, 3, 4], **hyper)
+        fn = (lambda: k.moment_values(mom[0], torch.bfloat16)) if case == "moment_values" else (
+            lambda: k.adamw_step(p, mom, gr, p16, seeds=[1, 2, 3, 4], **hyper))
     elif case == "ce":
         lg, tg = rnd(4096, 32000), torch.randint(0, 32000, (4096,), device=dev)
         fn = lambda: k.cross_entropy(lg, tg, 1.0, dlogits=lg)
