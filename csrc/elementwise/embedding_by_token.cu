@@ -340,7 +340,7 @@ __device__ __forceinline__ void load_old(const GT* src, int parts, uint4 (&old)[
     if (k < parts) old[k] = ld_v4(src + 128 * k);
 }
 template <int K, typename GT>
-__global__ void __launch_bounds__(256, 4) embedding_join_kernel(const ByToken a, GT* table) {
+__global__ void __launch_bounds__(256, 3) embedding_join_kernel(const ByToken a, GT* table) {
   chain_trigger();
   chain_wait();
   constexpr int P = PARTS<GT>;
@@ -543,10 +543,12 @@ __global__ void __launch_bounds__(256) position_grad_kernel(const __nv_bfloat16*
 
 // Rows to a piece: 4 to 32, as many as leave about as many warps as fit on the GPU at once.  Longer pieces cut fewer runs, shorter ones
 // wait for fewer rows one behind the other.  us with pieces of 4 / 8 / 16 / 32, fp32 table: 4096 tokens of 1024 columns 14.8 / 17.1 /
-// 18.9 / 32.5, 8192 of 2048 31.3 / 27.4 / 26.7 / 37.7, 16384 of 4096 104.8 / 82.3 / 72.6 / 69.9.
+// 18.9 / 32.5, 8192 of 2048 31.3 / 27.4 / 26.7 / 37.7, 16384 of 4096 104.8 / 82.3 / 72.6 / 69.9.  From 12288 tokens on not 4, however narrow the
+// rows: the parts of a token that occurs often would be too many for the CTA that adds them (16384 of 64, a fifth of them one token,
+// 36.5 / 28.9).
 static int piece_rows(int n, int H) {
   const long k = long(n) * ((H + 255) / 256) / (27L * num_sms());
-  return k >= 32 ? 32 : k >= 16 ? 16 : k >= 8 ? 8 : 4;
+  return k >= 32 ? 32 : k >= 16 ? 16 : k >= 8 || n >= 12288 ? 8 : 4;
 }
 
 template <int K, typename GT>
@@ -631,9 +633,9 @@ int zb_embedding_by_token(const long* ids, const void* dout, void* gtable, void*
     const int most = T < SORT_CHUNK ? T : SORT_CHUNK, K = piece_rows(most, H), chunks = (T + SORT_CHUNK - 1) / SORT_CHUNK;
     float* head = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((8L * T + 15) / 16) * 16);
     float* tail = head + long((most + K - 1) / K) * H;
-    // ids of a CTA: about as many CTAs as SMs, of at least 64 ids and at most SORT_BINS
+    // ids of a CTA: about as many CTAs as SMs, of at least 8 ids and at most SORT_BINS
     int width = (V + num_sms() - 1) / num_sms();
-    width = width < 64 ? 64 : width > SORT_BINS ? SORT_BINS : width;
+    width = width < 8 ? 8 : width > SORT_BINS ? SORT_BINS : width;
     const int ctas = (V - 1) / width + 1;
     if (long(ctas) * chunks > 0x7fffffffL) ZB_FAIL(-1, "embedding: %d tokens of a vocabulary of %d", T, V);
     auto kern = embedding_sort_kernel<32>;

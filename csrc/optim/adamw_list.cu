@@ -16,7 +16,8 @@
 //
 // Bound by memory: 8 x 61 million parameters, fp32 gradients, 1.42 ms with moments in 8 bits (18 bytes a parameter, 6.2 TB/s or
 // 96 % of a copy's rate); the units of a 125M model, bf16 gradients, 0.755 ms with moments in fp32 (28 bytes, 94 %).  The 8-bit form
-// is near the issue limit as well (58 instructions a value; 76 with scalar arithmetic and codes handled one by one took 1.6 ms).
+// is near the issue limit as well (70 % of its slots are taken; with scalar arithmetic, codes handled one by one and no block ahead it
+// took 1.6 ms).
 // Blocks go to warps round robin, so that all warps work in one part of the tensors: in a stretch of its own for each warp, the
 // same kernel took 1.58 ms.
 #include "../common/host.h"
@@ -196,14 +197,13 @@ __device__ __forceinline__ void adamw_load(AdamwLane<BITS>& x, const AdamwTensor
   }
 }
 
-// Every lane copies its parts of its warp's blocks to come into its own places of a ring in shared
-// memory: with the loads in registers, too few bytes were on their way behind the arithmetic of the 8-bit form.  The last
-// block of a tensor, if it is not whole, is loaded when it is its turn.
+// Every lane copies its parts of its warp's next block into its own places in shared memory while it works on this one: with the
+// loads in registers, too few bytes were on their way behind the arithmetic of the 8-bit form.  The last block of a tensor, if it
+// is not whole, is loaded when it is its turn.
 template <int BITS>
 struct AdamwRing {
-  static constexpr int SLOTS = 2, WIDE = BITS == 8 ? 4 : 8;
-  uint4 wide[SLOTS][WIDE][256];                   // p, g (8 bytes of bf16), and m, v in fp32
-  unsigned code[BITS == 8 ? SLOTS : 1][4][256];   // m, v in 8 bits
+  uint4 wide[2][BITS == 8 ? 4 : 8][256];      // p, g (8 bytes of bf16), and m, v in fp32
+  unsigned code[BITS == 8 ? 2 : 1][4][256];   // m, v in 8 bits
 };
 template <int BITS>
 __device__ __forceinline__ void adamw_request(AdamwRing<BITS>& ring, int slot, const AdamwTensor& t, long e0) {
@@ -345,14 +345,13 @@ __global__ void __launch_bounds__(256, ADAMW_CTAS) adamw_list_kernel(const __gri
   chain_wait();
   extern __shared__ __align__(16) unsigned char raw[];
   AdamwRing<BITS>& ring = *reinterpret_cast<AdamwRing<BITS>*>(raw);
-  constexpr int SLOTS = AdamwRing<BITS>::SLOTS;
   const int lane = threadIdx.x & 31;
   const long all = list.end[list.count - 1], stride = gridDim.x * 8L, first = blockIdx.x * 8L + (threadIdx.x >> 5);
   // a block on its way: its tensor, its number in it, and its bases (m's below, v's above)
   struct Asked {
     int i, bases;
     long block;
-  } queue[SLOTS - 1];
+  };
   long ask = first;
   int ask_i = 0;
   // the tensor of the first block, looked for by halves; of later ones from there on
@@ -375,15 +374,12 @@ __global__ void __launch_bounds__(256, ADAMW_CTAS) adamw_list_kernel(const __gri
     ring_commit();
     return x;
   };
-#pragma unroll
-  for (int k = 0; k < SLOTS - 1; ++k) queue[k] = request(k);
+  Asked next = request(0);
   int slot = 0;
   for (long at = first; at < all; at += stride) {
-    const Asked now = queue[0];
-#pragma unroll
-    for (int k = 0; k + 2 < SLOTS; ++k) queue[k] = queue[k + 1];
-    queue[SLOTS - 2] = request((slot + SLOTS - 1) % SLOTS);
-    ring_wait<SLOTS - 1>();
+    const Asked now = next;
+    next = request(slot ^ 1);
+    ring_wait<1>();
     const AdamwTensor& t = list.t[now.i];
     AdamwLane<BITS> x;
     if ((now.block + 1) * ADAMW_BLOCK <= t.n) {
@@ -394,7 +390,7 @@ __global__ void __launch_bounds__(256, ADAMW_CTAS) adamw_list_kernel(const __gri
       else adamw_load<BITS, __nv_bfloat16>(x, t, now.block * ADAMW_BLOCK + lane * 4);
       adamw_block<BITS, false>(x, t, list.h, now.block, lane, now.bases & 0xffff, now.bases >> 16);
     }
-    slot = (slot + 1) % SLOTS;
+    slot ^= 1;
   }
 }
 
