@@ -217,6 +217,24 @@ def test_steps_in_a_row_and_neighbours(ops, bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_that_follow_at_once_on_other_processors(ops, bits):
+    """Launches that begin under the end of the one before: blocks that share lines of bases, and whole tensors, go to other
+    processors from step to step (the list turned round), with nothing in between."""
+    sizes = [400000, 90000, 257, 130000]
+    p, moments, g, p16 = _tensors(sizes, bits, torch.float32, fresh=True)
+    dev = [_to(x, "cuda") for x in (p, moments, g, p16)]
+    steps = [(k, [dither_seed(k, i) for i in range(4)] if bits == 8 else None) for k in range(1, 9)]
+    for k, seeds in steps:
+        turn = slice(None, None, -1 if k % 2 else 1)
+        ops.adamw_step(*(x[turn] for x in dev), step=k, seeds=seeds and seeds[turn], **HYPER)
+    for k, seeds in steps:
+        get_ops("ref").adamw_step(p, moments, g, p16, step=k, seeds=seeds, **HYPER)
+    for a, b in zip(dev[1], moments):
+        assert all(torch.equal(x.cpu(), y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
 def test_special_gradients(ops):
     """Infinities and NaN show in the moments that they reach and in no other block."""
     n = 3 * BLOCK

@@ -136,6 +136,23 @@ def test_small_sums_are_exact(ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,V,H", [(20000, 500, 64), (700, 300, 256), (4000, 9000, 520)])
+@pytest.mark.parametrize("grads", [torch.float32, torch.bfloat16])
+def test_calls_that_follow_at_once(ops, T, V, H, grads):
+    """Microbatches into one table, each call begun under the end of the one before: whole numbers small enough to be exact."""
+    table, want, calls = torch.zeros(V, H, dtype=grads, device="cuda"), torch.zeros(V, H), []
+    for i in range(6):
+        ids = _ids(T, V, ("any", "runs", "few")[i % 3], seed=i)
+        dout = (torch.rand(T, H, generator=torch.Generator().manual_seed(i)) < 0.002).to(torch.bfloat16)
+        want.index_add_(0, ids, dout.float())
+        calls.append((ids.cuda(), dout.cuda()))
+    assert want.max() <= 256
+    for ids, dout in calls:
+        ops.embedding_bwd(ids, dout, table, by_token=True)
+    assert torch.equal(table.float().cpu(), want)
+
+
+@pytest.mark.gpu
 def test_ids_outside_the_table_count_as_the_nearest(ops):
     V, H = 11, 32
     ids = torch.tensor([-5, 0, 10, 11, 2 ** 40, -2 ** 40, 3])
