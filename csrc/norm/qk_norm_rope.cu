@@ -176,14 +176,18 @@ __global__ void __launch_bounds__(128, 6) qk_norm_rope_fwd_kernel(const QkNormAr
   }
 }
 
+// Tokens beside one another in a unit of the backward pass (9068 tokens of 4 + 1 heads of 64 12.1 -> 8.0 us, 8192 of 4 + 1 of 128 12.4 -> 10.6)
+__host__ __device__ constexpr int qk_norm_side(int n, int heads) { return n > 0 && n < heads && heads % n == 0 ? heads / n : 1; }
+
 struct QkRing {
   uint4 chunk[QK_RING][4][256];    // x low, x high, gradient low, gradient high
   float rstd[QK_RING][256];
 };
 // The first `ctas_q` CTAs have the query heads, the others the key heads: one set of weights and of weight-gradient sums a thread.
-// A warp takes an equal stretch of its kind's units of all tokens; the ring runs on over its tokens.
+// A warp takes an equal stretch of its kind's units of all tokens; the ring runs on over its tokens.  Where a token has fewer heads of a
+// kind than a unit, `side` tokens lie side by side in one.
 template <int LANES, bool ROPE>
-__global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs a) {
+__global__ void __launch_bounds__(256, 2) qk_norm_rope_bwd_kernel(const QkNormArgs a) {
   chain_trigger();
   chain_wait();
   constexpr int HEADS = 32 / LANES;
@@ -193,29 +197,31 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs 
   const int tid = threadIdx.x, half = a.d >> 1, lane = tid & 31, warp = tid >> 5, c = (lane % LANES) * 8, sub = lane / LANES;
   const bool used = c < half;
   const int step = HEADS * a.d, nqk = a.nq + a.nk, kind = int(blockIdx.x) >= a.ctas_q;
-  const int n = kind ? a.nk : a.nq, h0 = kind ? a.nq : 0, units = (n + HEADS - 1) / HEADS;
+  const int n = kind ? a.nk : a.nq, h0 = kind ? a.nq : 0, units = (n + HEADS - 1) / HEADS, side = qk_norm_side(n, HEADS);
+  const int beside = side > 1 ? sub / n : 0, sub_head = sub - beside * n;      // this lane's token of those, and head
   Pair w[8], dw[8];
   HeadChunk wu = {};
   if (used) wu = load_head((kind ? a.wk : a.wq) + c, half);
   unpack_pairs(wu, w);
 #pragma unroll
   for (int j = 0; j < 8; ++j) dw[j] = both(0.f);
-  const long all = long(a.T) * units, me = (blockIdx.x - (kind ? a.ctas_q : 0)) * 8 + warp;
+  const long all = long((a.T + side - 1) / side) * units, me = (blockIdx.x - (kind ? a.ctas_q : 0)) * 8 + warp;
   const long warps = (kind ? gridDim.x - a.ctas_q : a.ctas_q) * 8;
   const long first = all * me / warps;
   int left = int(all * (me + 1) / warps - first), to_ask = left;
-  unsigned t = unsigned(first / units);
+  int t = int(first / units);
   int u = int(first - long(t) * units);
-  // the next unit to ask for: its number in the token, this lane's head among the kind's, and where that lies
-  int ask_u = u, ask_k = u * HEADS + sub;
+  t = t * side + beside;
+  // the next unit to ask for: its number in the token, this lane's token, its head among the kind's, and where that lies
+  int ask_u = u, ask_t = t, ask_k = u * HEADS + sub_head;
   size_t col = size_t(h0 + ask_k) * a.d + c;
   const __nv_bfloat16 *ask_x = a.x + t * a.ldx + col, *ask_g = a.y + t * a.ldy + col;
   __nv_bfloat16* dst = a.y + t * a.ldy + col;
   const float* ask_r = a.rstd + size_t(t) * nqk + h0 + ask_k;
-  const long next_x = a.ldx - long(units) * step, next_g = a.ldy - long(units) * step;   // from behind a token's units to the next one's
+  const long next_x = side * a.ldx - long(units) * step, next_g = side * a.ldy - long(units) * step;   // from behind a token's units to the next one's
   auto request = [&](int slot) {
     if (to_ask > 0) {
-      if (used && ask_k < n) {
+      if (used && ask_k < n && ask_t < a.T) {
         ring_load16(&ring.chunk[slot][0][tid], ask_x);
         ring_load16(&ring.chunk[slot][1][tid], ask_x + half);
         ring_load16(&ring.chunk[slot][2][tid], ask_g);
@@ -229,27 +235,29 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs 
       ask_k += HEADS;
       if (++ask_u == units) {
         ask_u = 0;
-        ask_k = sub;
+        ask_t += side;
+        ask_k = sub_head;
         ask_x += next_x;
         ask_g += next_g;
-        ask_r += nqk - units * HEADS;
+        ask_r += side * nqk - units * HEADS;
       }
     }
     ring_commit();
   };
 #pragma unroll
   for (int k = 0; k < QK_RING - 1; ++k) request(k);
-  int slot = 0, pos = int(t % unsigned(a.S));
+  int slot = 0, pos = t % a.S;
   while (left > 0) {
+    const bool there = used && t < a.T;
     float co[8] = {}, si[8] = {};
-    if (ROPE && used) load_angles(a.cs + size_t(pos) * a.d + c, half, co, si);
+    if (ROPE && there) load_angles(a.cs + size_t(pos) * a.d + c, half, co, si);
     const int here = min(left, units - u);
     left -= here;
-    int k = u * HEADS + sub;
+    int k = u * HEADS + sub_head;
     for (int i = 0; i < here; ++i) {
       request((slot + QK_RING - 1) % QK_RING);
       ring_wait<QK_RING - 1>();
-      const bool live = used && k < n;
+      const bool live = there && k < n;
       HeadChunk xu = {}, gu = {};
       float rstd = 0.f;
       if (live) {
@@ -283,8 +291,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_bwd_kernel(const QkNormArgs 
       dst += step;
     }
     u = 0;
+    t += side;
     dst += next_g;
-    pos = pos + 1 == a.S ? 0 : pos + 1;
+    pos += side;
+    if (pos >= a.S) pos %= a.S;
   }
   ring_wait<0>();
   // over the heads of a warp, then over its CTA's warps
@@ -354,11 +364,12 @@ static int qk_norm_span(long T, int units, long warps, int most) {
 // out by the work on a token: its units, and its angles and place, which take as long as one more.  (One kind behind the other on all
 // CTAs: 256 tokens of 8 + 8 heads of 64 6.0 us instead of 4.6, 8192 of 32 + 8 heads of 128 46.7 instead of 46.1.)
 static void qk_norm_bwd_ctas(int T, int nq, int nk, int d, int* of_q, int* of_all) {
-  const int per = 32 / qk_norm_lanes(d);
+  const int per = 32 / qk_norm_lanes(d), side_q = qk_norm_side(nq, per), side_k = qk_norm_side(nk, per);
   const long uq = (nq + per - 1) / per, uk = (nk + per - 1) / per, cap = long(num_sms()) * 2;
-  long q = (T * uq + 7) / 8, k = (T * uk + 7) / 8;
+  long q = ((T + side_q - 1) / side_q * uq + 7) / 8, k = ((T + side_k - 1) / side_k * uk + 7) / 8;
   if (q + k > cap) {
-    q = q == 0 ? 0 : k == 0 ? cap : cap * (uq + 1) / (uq + uk + 2);
+    const long of_token_q = (uq + 1) * side_k, of_token_k = (uk + 1) * side_q;
+    q = q == 0 ? 0 : k == 0 ? cap : cap * of_token_q / (of_token_q + of_token_k);
     q = uq > 0 && q < 1 ? 1 : uk > 0 && q > cap - 1 ? cap - 1 : q;
     k = cap - q;
   }
