@@ -8,7 +8,7 @@
 // Both directions are bound by memory: 16384 tokens of 32 + 8 + 8 heads of 128 forward into a new tensor 64 to 66 us, 6.2 TB/s or
 // 96 % of a copy's rate; 8192 tokens of 32 + 32 heads of 128 backward 71 us, 5.7 TB/s or 89 %, of which about 3 are the sum over
 // the CTAs in a launch of its own.  Small ones are bound by their launches: 256 tokens of 8 + 2 x 8 heads of 64 2.2 us forward in a
-// graph and 4.8 backward, 5.7 and 7.2 called from Python.
+// graph and 4.9 backward, 5.3 and 6.7 called from Python.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "norm_common.cuh"
