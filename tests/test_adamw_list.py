@@ -218,6 +218,21 @@ def test_steps_in_a_row_and_neighbours(ops, bits):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_of_both_types_in_one_list_and_empty_tensors(ops, bits):
+    sizes = [700, 0, 5000, 256, 33]
+    p, moments, g, p16 = _tensors(sizes, bits, torch.float32)
+    g = [x.bfloat16() if i % 2 else x for i, x in enumerate(g)]
+    g[2] = g[2].bfloat16()
+    seeds = [3, 4, 5, 6, 7] if bits == 8 else None
+    dev = [_to(x, "cuda") for x in (p, moments, g, p16)]
+    ops.adamw_step(*dev, step=2, seeds=seeds, **HYPER)
+    get_ops("ref").adamw_step(p, moments, g, p16, step=2, seeds=seeds, **HYPER)
+    for a, b in zip(dev[1], moments):
+        assert all(torch.equal(x.cpu(), y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
 def test_steps_that_follow_at_once_on_other_processors(ops, bits):
     """Launches that begin under the end of the one before: blocks that share lines of bases, and whole tensors, go to other
     processors from step to step (the list turned round), with nothing in between."""

@@ -90,7 +90,7 @@ def test_forward(ops, T, S, V, H, off, positions):
 
 
 SHAPES = [  # T, S, V, H
-    (1, 1, 1, 8), (2, 2, 3, 64), (5, 5, 1000, 256), (33, 33, 7, 264), (256, 128, 32000, 512), (1000, 500, 600, 128),
+    (1, 1, 1, 8), (2, 2, 3, 64), (5, 9, 40, 64), (5, 5, 1000, 256), (3000, 4000, 700, 40), (33, 33, 7, 264), (256, 128, 32000, 512), (1000, 500, 600, 128),
     (1025, 205, 129, 72), (3000, 1000, 50257, 768), (9000, 4500, 128256, 64), (20000, 20000, 300, 32),
     (16500, 5500, 3000, 1032), (32000, 8000, 5000, 1032), (32768, 4096, 4096, 16), (32769, 32769, 70000, 24), (70001, 70001, 262145, 8),
 ]

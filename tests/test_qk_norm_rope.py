@@ -39,7 +39,7 @@ def _fwd64(qkv, wq, wk, cs, S, nq, nk, d, eps):
 SHAPES = [  # T, q heads, kv heads, width, S
     (1, 1, 1, 64, 1), (3, 2, 1, 128, 3), (130, 8, 8, 64, 65), (257, 5, 3, 96, 257), (64, 4, 2, 256, 16), (19, 3, 1, 16, 7),
     (33, 2, 2, 512, 33), (40, 7, 1, 48, 50), (2000, 32, 8, 128, 1000),
-    (37, 4, 1, 64, 3), (1001, 2, 2, 128, 333), (5, 1, 1, 32, 9), (613, 8, 4, 64, 613), (4099, 1, 1, 16, 2),
+    (50, 3, 0, 64, 50), (50, 0, 2, 128, 25), (37, 4, 1, 64, 3), (1001, 2, 2, 128, 333), (5, 1, 1, 32, 9), (613, 8, 4, 64, 613), (4099, 1, 1, 16, 2),
 ]
 
 

@@ -51,6 +51,20 @@ def test_gradients_match_autograd(model, more, schedule, recompute):
         assert (got - want).abs().max() <= 2e-4 * want.abs().max() + 1e-8
 
 
+@pytest.mark.parametrize("how", [dict(defer_wgrad=True), dict(defer_tail_wgrad=2)])
+def test_held_back_weight_gradients_change_nothing(how):
+    """Schedules that hold weight gradients back leave those of the head norms and the embedding where they are."""
+    states = []
+    for more in ({}, how):
+        tr = Trainer(_one_rank(), TrainerOptions(schedule="1f1b", ops="ref", model_overrides={"layers": 2, **OVERRIDES}, optimizer="adamw", **more))
+        batch = tr.synthetic_batch()
+        for _ in range(2):
+            tr.train_step_from_host(batch)
+        states.append(_state(tr))
+    for a, b in zip(*states):
+        torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-7)
+
+
 @pytest.mark.parametrize("in_backward", [False, True])
 def test_adamw_follows_torch(in_backward):
     cfg = _one_rank()
