@@ -758,7 +758,7 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       !on(gwq, *a.qkv) || !on(gwk, *a.qkv) || ptr(gwq) == ptr(gwk))
     Py_RETURN_NONE;
   long floats = 0;
-  lib.qk_norm_rope_workspace(int(T), int(a.nq), int(a.nk), int(a.d), &floats);
+  if (lib.qk_norm_rope_workspace(int(T), int(a.nq), int(a.nk), int(a.d), &floats) != 0) Py_RETURN_NONE;
   const Tensor partial = fresh({floats}, *a.qkv, F32);
   const cudaStream_t s = stream();
   if (!launch("qk_norm_rope_bwd", 2, [&] {
@@ -814,7 +814,7 @@ PyObject* embedding_by_token(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   const int64_t T = a.ids->numel(), V = a.table->size(0), H = a.table->size(1);
   if (!dense(dout, BF16) || dout->dim() != 2 || dout->size(0) != T || dout->size(1) != H || !on(dout, *a.table)) Py_RETURN_NONE;
   long bytes = 0;
-  lib.embedding_by_token_workspace(int(T), int(H), &bytes);
+  if (lib.embedding_by_token_workspace(int(T), int(H), &bytes) != 0) Py_RETURN_NONE;
   const Tensor ws = fresh({bytes}, *a.table, at::kByte);
   const cudaStream_t s = stream();
   // order, and of every 32768 ids the sums and the runs over several pieces, or all in one; positions

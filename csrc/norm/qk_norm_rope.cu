@@ -377,9 +377,15 @@ static void qk_norm_bwd_ctas(int T, int nq, int nk, int d, int* of_q, int* of_al
   *of_all = int(q + k);
 }
 
+// What has to hold before anything is counted in heads: the lanes and units of other widths mean nothing.
+static int qk_norm_heads_check(int nq, int nk, int d) {
+  if (d % 16 != 0 || d < 16 || d > 512) ZB_FAIL(-1, "qk_norm_rope: head width %d is not a multiple of 16 up to 512", d);
+  if (nq < 0 || nk < 0) ZB_FAIL(-1, "qk_norm_rope: %d + %d heads", nq, nk);
+  return 0;
+}
 static int qk_norm_check(const QkNormArgs& a) {
-  if (a.d % 16 != 0 || a.d < 16 || a.d > 512) ZB_FAIL(-1, "qk_norm_rope: head width %d is not a multiple of 16 up to 512", a.d);
-  if (a.nq < 0 || a.nk < 0 || a.nv < 0 || a.S < 1) ZB_FAIL(-1, "qk_norm_rope: %d + %d heads, sequences of %d", a.nq, a.nk, a.S);
+  if (int rc = qk_norm_heads_check(a.nq, a.nk, a.d)) return rc;
+  if (a.S < 1) ZB_FAIL(-1, "qk_norm_rope: sequences of %d", a.S);
   // units of all tokens, and what a warp of the last CTA counts up to behind them, in 32 bits
   if (long(a.T) * (a.nq + a.nk + a.nv + 3) >= (1L << 31) - (1L << 20)) ZB_FAIL(-1, "qk_norm_rope: %d tokens of %d heads", a.T, a.nq + a.nk);
   if (a.T > 1 && a.ldy < long(a.nq + a.nk + a.nv) * a.d) ZB_FAIL(-1, "qk_norm_rope: rows to write lie over one another (stride %ld)", a.ldy);
@@ -439,7 +445,8 @@ int zb_qk_norm_rope_fwd(const void* x, void* y, const void* wq, const void* wk, 
 int zb_qk_norm_rope_workspace(int T, int nq, int nk, int d, long* floats) {
   using namespace zb;
   int of_q = 0, ctas = 0;
-  if (d > 0 && T > 0) qk_norm_bwd_ctas(T, nq, nk, d, &of_q, &ctas);
+  if (int rc = qk_norm_heads_check(nq, nk, d)) return rc;
+  if (T > 0) qk_norm_bwd_ctas(T, nq, nk, d, &of_q, &ctas);
   *floats = long(ctas) * d;
   return 0;
 }

@@ -206,7 +206,8 @@ def _need(ok: bool, what: str) -> None:
 
 def _workspace_size(fn, *sizes) -> int:
     out = ctypes.c_long(0)
-    fn(*sizes, ctypes.addressof(out))
+    if fn(*sizes, ctypes.addressof(out)):
+        raise KernelError(f"workspace: {lib().zb_last_error().decode()}")
     return out.value
 
 
