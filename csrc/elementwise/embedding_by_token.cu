@@ -577,6 +577,14 @@ static int small(const long* ids, const __nv_bfloat16* dout, GT* table, int T, i
   ZB_CUDA_OK(launch_pass(embedding_small_kernel<GT>, T * ((H + 255) / 256), 256, 0, stream, ids, dout, table, T, H, V, scale));
   return 0;
 }
+// (columns and positions are counted in 32 bits, some way beyond the last one)
+static int embedding_check(int H, int V, int S, int off) {
+  if (H < 8 || H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
+  if (H > 1 << 30) ZB_FAIL(-1, "embedding: H=%d above 2^30", H);
+  if (V < 0 || S < 0 || off < 0) ZB_FAIL(-1, "embedding: a vocabulary of %d, sequences of %d, positions from %d", V, S, off);
+  return 0;
+}
+
 static bool is_small(int T, int H) { return T <= SMALL_T && long(T) * ((H + 255) / 256) <= SMALL_CTAS; }
 
 static int blocks_for(long items) {
@@ -591,7 +599,7 @@ extern "C" {
 int zb_embedding_scaled(const long* ids, const void* table, const void* pos, void* out, int T, int H, int V, int S, int pos_offset,
                         float scale, cudaStream_t stream) {
   using namespace zb;
-  if (H < 8 || H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
+  if (int rc = embedding_check(H, V, S, pos_offset)) return rc;
   if ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(pos) | reinterpret_cast<uintptr_t>(out)) & 15)
     ZB_FAIL(-1, "embedding: operands must be 16-byte aligned");
   if (T <= 0) return 0;
@@ -616,7 +624,7 @@ int zb_embedding_by_token_workspace(int T, int H, long* bytes) {
 int zb_embedding_by_token(const long* ids, const void* dout, void* gtable, void* gpos, void* workspace, int T, int H, int V, int S,
                           int pos_offset, float scale, int grad_f32, cudaStream_t stream) {
   using namespace zb;
-  if (H < 8 || H % 8 != 0) ZB_FAIL(-1, "embedding: H=%d not a multiple of 8", H);
+  if (int rc = embedding_check(H, V, S, pos_offset)) return rc;
   if ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(gtable) | reinterpret_cast<uintptr_t>(gpos) |
        reinterpret_cast<uintptr_t>(workspace)) & 15)
     ZB_FAIL(-1, "embedding: operands must be 16-byte aligned");

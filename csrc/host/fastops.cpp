@@ -781,7 +781,8 @@ struct Lookup {
   bool take(PyObject* const* rest) {   // positions | None, S, offset, scale
     if (!optional_tensor(rest[0], pos) || !int_arg(rest[1], S) || !int_arg(rest[2], off) || !float_arg(rest[3], scale)) return false;
     if (!gradient(table) || table->dim() != 2 || !fits(table->size(0)) || !fits(table->size(1)) || !here(*table) ||
-        !dense(ids, at::kLong) || !on(ids, *table) || !fits(ids->numel()) || !fits(S) || off < 0 || off > INT32_MAX / 2)
+        !dense(ids, at::kLong) || !on(ids, *table) || !fits(ids->numel()) || !fits(S) || off < 0 || off > INT32_MAX ||
+        std::min(S, ids->numel()) + off > INT32_MAX)
       return false;
     return pos == nullptr || (dense(pos, table->scalar_type()) && pos->dim() == 2 && pos->size(1) == table->size(1) &&
                               pos->size(0) >= std::min(S, ids->numel()) + off && on(pos, *table));

@@ -1,0 +1,38 @@
+"""Scaled embedding and its gradient by token: sizes that do not fit into 32 bits are refused, and sums over many tokens."""
+import pytest
+import torch
+
+from zorse_b200.ops import sm100 as k
+
+
+@pytest.fixture()
+def no_launch(monkeypatch):
+    class Lib:
+        def __getattr__(self, name):
+            raise AssertionError(f"{name} was reached")
+
+    monkeypatch.setattr(k, "_lib", Lib())
+    monkeypatch.setattr(k, "_bf16", lambda t, name: None)
+    monkeypatch.setattr(k, "_on_current", lambda t, name: None)
+
+
+@pytest.mark.parametrize("S,off", [(2 ** 31, 0), (2 ** 32, 0), (2 ** 32 + 6, 2), (6, 2 ** 31), (6, 2 ** 32), (6, 2 ** 31 - 3)])
+def test_sequences_and_offsets_beyond_32_bits_are_refused_cpu(no_launch, S, off):
+    ids, table, dout = torch.zeros(6, dtype=torch.long), torch.zeros(10, 16, dtype=torch.bfloat16), torch.zeros(6, 16, dtype=torch.bfloat16)
+    # (a table of positions as long as asked for, on no device)
+    pos = torch.zeros(1, 16, dtype=torch.bfloat16).expand(max(8, min(S, 6) + off), 16)
+    pos = type("Rows", (), dict(dtype=pos.dtype, shape=pos.shape, device=pos.device, is_contiguous=lambda self: True,
+                                data_ptr=lambda self: 0))()
+    with pytest.raises(ValueError, match="2\\^31"):
+        k.embedding_scaled(ids, table, pos, S, off, scale=2.0)
+    with pytest.raises(ValueError, match="2\\^31"):
+        k.embedding_by_token(ids, dout, table, pos, S, off)
+
+
+def test_the_library_refuses_sizes_it_does_not_count_cpu():
+    """Before anything is launched, and before it looks at an address."""
+    L = k.lib()
+    for H, V, S, off in ((2 ** 31 - 8, 4, 4, 0), (2 ** 30 + 8, 4, 4, 0), (12, 4, 4, 0), (16, -1, 4, 0), (16, 4, -2 ** 31, 0), (16, 4, 4, -1)):
+        for call, args in ((L.zb_embedding_scaled, (0, 0, 0, 0, 1, H, V, S, off, 1.0, 0)),
+                           (L.zb_embedding_by_token, (0, 0, 0, 0, 0, 1, H, V, S, off, 1.0, 1, 0))):
+            assert call(*args) != 0 and L.zb_last_error().startswith(b"embedding: ")
