@@ -386,9 +386,12 @@ static int qk_norm_heads_check(int nq, int nk, int d) {
 static int qk_norm_check(const QkNormArgs& a) {
   if (int rc = qk_norm_heads_check(a.nq, a.nk, a.d)) return rc;
   if (a.S < 1) ZB_FAIL(-1, "qk_norm_rope: sequences of %d", a.S);
+  // a token's elements, and the heads that a warp's last item counts up to behind them (six units of 32 at most), in 32 bits
+  const long heads = long(a.nq) + a.nk + a.nv;
+  if ((heads + 192) * a.d >= 1L << 31) ZB_FAIL(-1, "qk_norm_rope: rows of %ld heads of %d", heads, a.d);
   // units of all tokens, and what a warp of the last CTA counts up to behind them, in 32 bits
-  if (long(a.T) * (a.nq + a.nk + a.nv + 3) >= (1L << 31) - (1L << 20)) ZB_FAIL(-1, "qk_norm_rope: %d tokens of %d heads", a.T, a.nq + a.nk);
-  if (a.T > 1 && a.ldy < long(a.nq + a.nk + a.nv) * a.d) ZB_FAIL(-1, "qk_norm_rope: rows to write lie over one another (stride %ld)", a.ldy);
+  if (a.T * (heads + 3) >= (1L << 31) - (1L << 20)) ZB_FAIL(-1, "qk_norm_rope: %d tokens of %d heads", a.T, a.nq + a.nk);
+  if (a.T > 1 && a.ldy < heads * a.d) ZB_FAIL(-1, "qk_norm_rope: rows to write lie over one another (stride %ld)", a.ldy);
   if (a.ldx % 8 != 0 || a.ldy % 8 != 0) ZB_FAIL(-1, "qk_norm_rope: row strides %ld, %ld not a multiple of 8", a.ldx, a.ldy);
   if ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.wq) |
        reinterpret_cast<uintptr_t>(a.wk) | reinterpret_cast<uintptr_t>(a.cs)) & 15)

@@ -54,6 +54,30 @@ def test_the_workspace_of_widths_it_takes_cpu():
         assert floats.value > 0 and floats.value % d == 0
 
 
+@pytest.mark.parametrize("T,nq,nk,d", [(1, 2 ** 23, 0, 512), (1, 2 ** 22 - 192, 0, 512), (2, 2 ** 21, 2 ** 21, 512), (1, 2 ** 30, 2 ** 30, 16)])
+def test_rows_beyond_32_bits_are_refused_cpu(T, nq, nk, d):
+    """Before anything is launched, and before the library looks at an address."""
+    L = k.lib()
+    for rc in (L.zb_qk_norm_rope_fwd(0, 0, 0, 0, 0, 0, T, 1, nq, nk, nk, d, 2 ** 40, 2 ** 40, 1e-5, 0),
+               L.zb_qk_norm_rope_bwd(0, 0, 0, 0, 0, 0, 0, 0, 0, T, 1, nq, nk, d, 2 ** 40, 2 ** 40, 1, 0)):
+        assert rc == -1 and b" heads" in L.zb_last_error()
+
+
+def test_heads_beyond_32_bits_are_refused_cpu(monkeypatch):
+    """The wrapper: a number of heads that would reach the library as another one."""
+    monkeypatch.setattr(k, "_bf16", lambda t, name: None)
+    monkeypatch.setattr(k, "_on_current", lambda t, name: None)
+    monkeypatch.setattr(k, "_lib", None)
+    monkeypatch.setattr(k, "lib", lambda: pytest.fail("the library was reached"))
+    w = torch.ones(16, dtype=torch.bfloat16)
+    for nq, nk in ((2 ** 32 + 2, 0), (2 ** 31, 0), (-2, 2), (4, -1)):
+        n = (nq + 2 * nk) * 16
+        x = type("Rows", (), dict(shape=torch.Size((1, n)), dtype=torch.bfloat16, device=w.device, dim=lambda self: 2,
+                                  stride=lambda self, i=None: (n, 1) if i is None else (n, 1)[i]))()
+        with pytest.raises(ValueError, match="2\\^31"):
+            k.qk_norm_rope_fwd(x, w, w, None, 1, nq, nk, 16, 1e-5)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [528, 1024, 72])
 def test_both_passes_refuse_other_widths(d):

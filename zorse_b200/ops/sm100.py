@@ -333,6 +333,7 @@ def _qk_norm_operands(x, wq, wk, cs, S, nq, nk, d):
     _on_current(x, "qkv")
     _need(x.dim() == 2 and x.shape[0] < 2 ** 31 and 0 < S < 2 ** 31 and x.shape[1] == (nq + 2 * nk) * d and x.stride(1) == 1,
           f"qkv is {tuple(x.shape)}, strides {x.stride()}: expected rows of ({nq} + 2 x {nk}) x {d}")
+    _need(x.shape[1] < 2 ** 31 and 0 <= nq < 2 ** 31 and 0 <= nk < 2 ** 31, f"rows of {x.shape[1]} elements, {nq} + {nk} heads: sizes below 2^31")
     _need(wq.shape == (d,) and wk.shape == (d,) and wq.is_contiguous() and wk.is_contiguous() and wq.device == wk.device == x.device,
           f"weights of {tuple(wq.shape)} and {tuple(wk.shape)} for heads of {d}")
     T = x.shape[0]
