@@ -694,6 +694,21 @@ PyObject* attn_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether two vectors or matrices of one shape and type (rows of any distance, each contiguous) share memory: as the wrapper's
+// _rows_overlap.
+bool rows_overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0) return false;
+  const int64_t size = a.element_size(), width = a.size(-1) * size, rows = a.dim() == 2 ? a.size(0) : 1;
+  int64_t step = rows > 1 ? a.stride(0) * size : width, other = rows > 1 ? b.stride(0) * size : width;
+  uintptr_t lo = reinterpret_cast<uintptr_t>(a.data_ptr()), hi = reinterpret_cast<uintptr_t>(b.data_ptr());
+  if (lo > hi) {
+    std::swap(lo, hi);
+    std::swap(step, other);
+  }
+  if (hi >= lo + uintptr_t((rows - 1) * step + width)) return false;
+  const int64_t between = step == other && step > 0 ? int64_t((hi - lo) % uintptr_t(step)) : 0;
+  return !(width <= between && between <= step - width);
+}
 struct HeadNorm {
   const Tensor *qkv, *wq, *wk, *cs;
   int64_t S, nq, nk, d;
@@ -752,10 +767,10 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!optional_tensor(args[5], cs) || !head_norm({tensor_of(args[1]), tensor_of(args[2]), tensor_of(args[3]), cs}, args + 6, a))
     Py_RETURN_NONE;
   const int64_t T = a.qkv->size(0);
-  if (!matrix(dy, BF16) || dy->sizes() != a.qkv->sizes() || !on(dy, *a.qkv) || ptr(dy) == ptr(a.qkv) || !dense(rstd, F32) ||
+  if (!matrix(dy, BF16) || dy->sizes() != a.qkv->sizes() || !on(dy, *a.qkv) || rows_overlap(*dy, *a.qkv) || !dense(rstd, F32) ||
       rstd->dim() != 2 || rstd->size(0) != T || rstd->size(1) != a.nq + a.nk || !on(rstd, *a.qkv) || !gradient(gwq) || !gradient(gwk) ||
       gwq->scalar_type() != gwk->scalar_type() || gwq->dim() != 1 || gwk->dim() != 1 || gwq->size(0) != a.d || gwk->size(0) != a.d ||
-      !on(gwq, *a.qkv) || !on(gwk, *a.qkv) || ptr(gwq) == ptr(gwk))
+      !on(gwq, *a.qkv) || !on(gwk, *a.qkv) || rows_overlap(*gwq, *gwk))
     Py_RETURN_NONE;
   long floats = 0;
   if (lib.qk_norm_rope_workspace(int(T), int(a.nq), int(a.nk), int(a.d), &floats) != 0) Py_RETURN_NONE;

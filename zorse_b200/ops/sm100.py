@@ -204,6 +204,23 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two vectors or matrices of one shape and type (rows of any distance, each contiguous) share memory.  Rows of one
+    distance may lie between one another, as two halves of wider rows do; with different distances, stretches that meet count."""
+    if a.numel() == 0:
+        return False
+    size = a.element_size()
+    width, rows = a.shape[-1] * size, a.shape[0] if a.dim() == 2 else 1
+    step_a, step_b = (t.stride(0) * size if rows > 1 else width for t in (a, b))
+    lo, hi = a.data_ptr(), b.data_ptr()
+    if lo > hi:
+        lo, hi, step_a, step_b = hi, lo, step_b, step_a
+    if hi >= lo + (rows - 1) * step_a + width:
+        return False
+    between = (hi - lo) % step_a if step_a == step_b and step_a > 0 else 0
+    return not width <= between <= step_a - width
+
+
 def _workspace_size(fn, *sizes) -> int:
     out = ctypes.c_long(0)
     if fn(*sizes, ctypes.addressof(out)):
@@ -364,13 +381,13 @@ def qk_norm_rope_bwd(dqkv, qkv, wq, wk, rstd, cs, S: int, nq: int, nk: int, d: i
     _bf16(dqkv, "dqkv")
     T = qkv.shape[0]
     _need(dqkv.shape == qkv.shape and dqkv.stride(1) == 1 and dqkv.device == qkv.device, f"dqkv {tuple(dqkv.shape)}, qkv {tuple(qkv.shape)}")
-    _need(dqkv.data_ptr() != qkv.data_ptr() or T == 0, "the gradient is written in place: dqkv and qkv are the same memory")
+    _need(not _rows_overlap(dqkv, qkv), "the gradient is written in place: dqkv and qkv share memory")
     _need(rstd.shape == (T, nq + nk) and rstd.dtype == torch.float32 and rstd.is_contiguous() and rstd.device == qkv.device,
           f"rstd {tuple(rstd.shape)}, {rstd.dtype}: expected fp32 [{T}, {nq + nk}]")
     _need(gwq.dtype == gwk.dtype and gwq.dtype in (torch.float32, torch.bfloat16) and gwq.shape == gwk.shape == (d,)
           and gwq.is_contiguous() and gwk.is_contiguous() and gwq.device == gwk.device == qkv.device,
           "gwq and gwk: both fp32 or both bf16, of the weights' shape")
-    _need(gwq.data_ptr() != gwk.data_ptr(), "gwq and gwk are the same memory")
+    _need(not _rows_overlap(gwq, gwk), "gwq and gwk share memory")
     L = lib()
     partial = torch.empty(_workspace_size(L.zb_qk_norm_rope_workspace, T, nq, nk, d), dtype=torch.float32, device=qkv.device)
     _check(L.zb_qk_norm_rope_bwd(_a(dqkv), _a(qkv), _a(wq), _a(wk), _a(rstd), _a(cs), _a(partial), _a(gwq), _a(gwk), T, S, nq, nk, d,
