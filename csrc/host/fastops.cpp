@@ -868,9 +868,14 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!dense(first, F32) || !here(*first)) Py_RETURN_NONE;
   int bits = 0;
   c10::SmallVector<AdamwTensor, 32> table;
-  c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 64> written;
-  auto writes = [&](const void* p, int64_t bytes) {
-    if (p != nullptr) written.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + uintptr_t(bytes));
+  struct Stretch {
+    uintptr_t lo, hi;
+    Py_ssize_t owner;
+  };
+  c10::SmallVector<Stretch, 64> written;
+  c10::SmallVector<Stretch, 32> read;
+  auto stretch = [](const void* p, int64_t bytes, Py_ssize_t i) {
+    return Stretch{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + uintptr_t(bytes), i};
   };
   for (Py_ssize_t i = 0; i < n; ++i) {
     const Tensor *p = tensor_of(PyList_GET_ITEM(args[0], i)), *g = tensor_of(PyList_GET_ITEM(args[2], i)), *p16;
@@ -911,16 +916,23 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     a.seed = static_cast<unsigned>(seed);
     a.grad_f32 = g->scalar_type() == F32;
     table.push_back(a);
-    writes(a.p, 4 * num);
-    writes(a.p16, 2 * num);
-    writes(a.m, num * (bits / 8));
-    writes(a.v, num * (bits / 8));
-    writes(a.mb, 2 * ((num + 255) / 256));
-    writes(a.vb, 2 * ((num + 255) / 256));
+    const int64_t bases = 2 * ((num + 255) / 256);
+    for (const auto& [at, bytes] : {std::pair<void*, int64_t>{a.p, 4 * num}, {a.p16, 2 * num}, {a.m, num * (bits / 8)},
+                                    {a.v, num * (bits / 8)}, {a.mb, bases}, {a.vb, bases}})
+      if (at != nullptr) written.push_back(stretch(at, bytes, i));
+    read.push_back(stretch(a.g, num * (a.grad_f32 ? 4 : 2), i));
   }
-  std::sort(written.begin(), written.end());
+  std::sort(written.begin(), written.end(), [](const Stretch& x, const Stretch& y) { return x.lo < y.lo; });
   for (size_t i = 1; i < written.size(); ++i)
-    if (written[i].first < written[i - 1].second) Py_RETURN_NONE;
+    if (written[i].lo < written[i - 1].hi) Py_RETURN_NONE;
+  // a gradient may lie in the memory of a tensor of its own, element on element, and in no other that is written
+  for (const Stretch& r : read) {
+    auto next = std::upper_bound(written.begin(), written.end(), r.lo, [](uintptr_t lo, const Stretch& x) { return lo < x.lo; });
+    if (next != written.end() && next->lo < r.hi) Py_RETURN_NONE;
+    if (next == written.begin()) continue;
+    const Stretch& w = *(next - 1);
+    if (w.hi > r.lo && !(w.lo == r.lo && w.hi == r.hi && w.owner == r.owner)) Py_RETURN_NONE;
+  }
   if (table.empty() || h[1] < 0 || h[1] >= 1 || h[2] < 0 || h[2] >= 1) Py_RETURN_NONE;
   const cudaStream_t s = stream();
   if (!launch("adamw", int((table.size() + 255) / 256), [&] {

@@ -8,6 +8,7 @@ the import of the library raises.  Tensors are passed as raw device pointers.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 import functools
 import math
@@ -522,6 +523,11 @@ def adam_step(p, m, v, g, p16, *, lr, beta1, beta2, eps, weight_decay, step, gra
                          int(g.dtype == torch.float32), int(zero_grad), _stream()), "adam")
 
 
+def _stretch(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses of a contiguous tensor."""
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+
 def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step, grad_scale: float = 1.0,
                seeds=None):
     """AdamW over lists of tensors in one launch.  p: fp32, contiguous; moments: for each a pair (m, v) in fp32, or `Moments8`
@@ -538,7 +544,7 @@ def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps
     _need(len(steps) == n and min(steps) >= 1, "step counts from 1, one for all tensors or one for each")
     dev = p[0].device
     _on_current(p[0], "p")
-    table, written, count = [], [], 0
+    table, written, read, count = [], [], [], 0
     for i, (x, mom, d, y, k) in enumerate(zip(p, moments, g, p16, steps)):
         num = x.numel()
         _need(x.dtype == torch.float32 and x.is_contiguous() and x.device == dev, f"p[{i}]: contiguous fp32 on {dev}")
@@ -559,7 +565,8 @@ def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps
               and m.device == v.device == dev, f"moments[{i}]: {num} contiguous {dtype} on {dev}")
         if num == 0:
             continue
-        written += [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (x, m, v, mb, vb, y) if t is not None]
+        written += [(*_stretch(t), i) for t in (x, m, v, mb, vb, y) if t is not None]
+        read.append((*_stretch(d), i))
         count += 1
         table += (x.data_ptr(), m.data_ptr(), v.data_ptr(), _a(mb), _a(vb), d.data_ptr(), _a(y), num, lr / (1 - beta1 ** k),
                   1 / math.sqrt(1 - beta2 ** k), seeds[i] & 0xFFFFFFFF if bits == 8 else 0, int(d.dtype == torch.float32))
@@ -567,6 +574,11 @@ def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps
         return
     written.sort()
     _need(all(a[1] <= b[0] for a, b in zip(written, written[1:])), "tensors that the step writes overlap (one is in the list twice?)")
+    for lo, hi, i in read:
+        at = bisect.bisect_left(written, (lo + 1,)) - 1       # the last one that begins no later
+        # a gradient may lie in the memory of a tensor of its own, element on element: those are read before they are written
+        _need((at < 0 or written[at][1] <= lo or written[at] == (lo, hi, i)) and (at + 1 == len(written) or written[at + 1][0] >= hi),
+              f"g[{i}] overlaps a tensor that the step writes")
     packed = struct.pack("8Qff2I" * count, *table)
     _check(lib().zb_adamw_list(packed, count, bits, beta1, 1 - beta1, beta2, 1 - beta2, eps, 1 - lr * weight_decay, grad_scale,
                                _stream()), "adamw")
