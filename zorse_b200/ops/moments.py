@@ -13,7 +13,7 @@ import torch
 
 BLOCK = 256
 _M_MOST, _V_MOST = 127, 255
-_INF, _TOP = 0x7F800000, 0x7FE00000       # NaNs, whatever their pattern, are held as the second one
+_TOP = 0x7FE00000                       # NaNs, whatever their pattern, are held as this one
 
 
 class Moments8(NamedTuple):
@@ -54,7 +54,7 @@ def decode(moments) -> tuple[torch.Tensor, torch.Tensor]:
 def _encode(x, add, most, least):
     n = x.numel()
     bits = x.contiguous().view(torch.int32)
-    bits = torch.where(bits > _INF, _TOP, bits)
+    bits = torch.where(torch.isnan(x), _TOP, bits)       # (a NaN may have its sign bit set, and be a negative number here)
     blocks = torch.nn.functional.pad(bits, (0, -n % BLOCK)).view(-1, BLOCK)
     base = ((blocks.amax(1) + 0xFFFFF >> 20) - most).clamp_(min=0)
     code = ((bits + add >> 20) - _spread(base, n)).clamp_(min=least)
