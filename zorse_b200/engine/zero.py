@@ -631,7 +631,8 @@ class StageEngine:
     def optimizer_step(self) -> None:
         units = [u for u in self.units if u.grad_shard is not None]
         scales = {getattr(u, "grad_shard_scale", 1.0) for u in units}
-        if not self.cfg.adam.decoupled or len(scales) != 1:
+        # (parked parameters come to the GPU unit by unit, for the time of their step: they are not there as one list)
+        if not self.cfg.adam.decoupled or len(scales) != 1 or any(u.host_master is not None for u in units):
             for u in units:
                 u.optimizer_step()
             return
