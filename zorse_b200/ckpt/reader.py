@@ -87,6 +87,31 @@ def _whole_block(directory, meta, offsets, saved: dict, gid: int, which: int, sp
     return whole
 
 
+def _check_units(trainer, saved: dict, saved_tp: int) -> None:
+    """Every unit of this process was saved from a layer of the size that the model has at the saved width, in each of the slices
+    it will be read from: a flat tensor of another layout would be cut in the wrong places without a word."""
+    from ..models import registry
+
+    now_tp, now_t = trainer.cfg.tensor_parallel_size, getattr(trainer, "tp_index", 0)
+    sizes = {}                       # of a block's slices at the saved width
+    for st in trainer.stages:
+        for u in st.engine.units:
+            recut = u.layer.kind == "block" and saved_tp != now_tp
+            for t in range(saved_tp) if recut else [now_t if saved_tp == now_tp else 0]:
+                su = saved.get((u.gid, t))
+                if su is None:
+                    raise CheckpointError(f"checkpoint has no unit {u.gid}" + (f", slice {t}" if t else ""))
+                want = u.layer.layout()[1]
+                if recut:
+                    if t not in sizes:
+                        sizes[t] = registry.make_block(trainer.spec, saved_tp, t).layout()[1]
+                    want = sizes[t]
+                kind = su.get("kind", u.layer.kind)
+                if kind != u.layer.kind or su["numel"] != want:
+                    raise CheckpointError(f"unit {u.gid}: {kind} of {su['numel']} elements saved, the model has "
+                                          f"{u.layer.kind} of {want}" + (f" at tensor parallelism {saved_tp}" if recut else ""))
+
+
 def load_checkpoint(trainer, directory: str) -> int:
     """Loads master weights and Adam state into the trainer's units; returns the saved step."""
     meta = read_meta(directory)
@@ -97,16 +122,13 @@ def load_checkpoint(trainer, directory: str) -> int:
     saved_tp = int(meta.get("tensor_parallel_size", 1))
     now_tp, now_t = trainer.cfg.tensor_parallel_size, getattr(trainer, "tp_index", 0)
     offsets = _file_offsets(meta)
+    _check_units(trainer, saved, saved_tp)
     for st in trainer.stages:
         for u in st.engine.units:
-            if (u.gid, 0) not in saved:
-                raise CheckpointError(f"checkpoint has no unit {u.gid}")
             lo, hi = u.lo, u.hi
             recut = u.layer.kind == "block" and saved_tp != now_tp
             # layers that are not cut (embedding, head) are whole in every slice: read slice 0's copy
             su = saved[(u.gid, now_t if saved_tp == now_tp else 0)]
-            if not recut and su["numel"] != u.layer.layout()[1]:
-                raise CheckpointError(f"unit {u.gid}: {su['numel']} elements saved, model has {u.layer.layout()[1]}")
             parts = []
             for which in range(3):
                 t = torch.zeros(u.shard_n, dtype=torch.float32)
