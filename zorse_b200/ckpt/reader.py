@@ -87,6 +87,42 @@ def _whole_block(directory, meta, offsets, saved: dict, gid: int, which: int, sp
     return whole
 
 
+# of the model's description: what only the start of a job or the order of a sum depends on
+_FREE = ("name", "init_std", "embed_by_token")
+
+
+def _check_job(trainer, meta: dict) -> None:
+    """The job goes on with the model and the optimizer that were saved.  (Checkpoints from before these were recorded have neither.
+    Moments may be held in other bits: the files have their values.)"""
+    from dataclasses import asdict
+
+    now = asdict(trainer.spec)
+    for key, value in meta.get("model", {}).items():
+        if key in now and key not in _FREE and now[key] != value:
+            raise CheckpointError(f"{key}: the checkpoint's model has {value}, the job's {now[key]}")
+    opt = meta.get("optimizer", trainer.opt.optimizer)
+    if opt != trainer.opt.optimizer:
+        raise CheckpointError(f"optimizer: the checkpoint was trained with {opt}, the job has {trainer.opt.optimizer}")
+
+
+def flags_of(meta: dict) -> list[str]:
+    """The trainer's flags that a job needs to go on with this checkpoint's model and optimizer."""
+    model, out = meta.get("model", {}), []
+    if model.get("qk_norm"):
+        out.append("--qk_norm")
+    if model.get("embed_scale", 1.0) != 1.0:
+        out += ["--embed_scale", repr(model["embed_scale"])]
+    if model.get("embed_by_token"):
+        out.append("--embed_by_token")
+    if meta.get("optimizer", "adam") != "adam":
+        out += ["--optimizer", meta["optimizer"]]
+    if meta.get("weight_decay", 0.0) != 0.0:
+        out += ["--weight_decay", repr(meta["weight_decay"])]
+    if meta.get("moment_bits", 32) != 32:
+        out += ["--moment_bits", str(meta["moment_bits"])]
+    return out
+
+
 def _check_units(trainer, saved: dict, saved_tp: int) -> None:
     """Every unit of this process was saved from a layer of the size that the model has at the saved width, in each of the slices
     it will be read from: a flat tensor of another layout would be cut in the wrong places without a word."""
@@ -122,6 +158,7 @@ def load_checkpoint(trainer, directory: str) -> int:
     saved_tp = int(meta.get("tensor_parallel_size", 1))
     now_tp, now_t = trainer.cfg.tensor_parallel_size, getattr(trainer, "tp_index", 0)
     offsets = _file_offsets(meta)
+    _check_job(trainer, meta)
     _check_units(trainer, saved, saved_tp)
     for st in trainer.stages:
         for u in st.engine.units:

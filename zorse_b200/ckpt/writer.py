@@ -1,7 +1,8 @@
 """Checkpoint writer (the reference has no checkpointing at all; this format is new).
 
 Layout: `<dir>/step_<n>/meta.json` + one flat binary per (stage, rank) `stage<s>_rank<r>.bin`.
-`meta.json` holds the training config, the step, seeds, dtypes and, per stage, the unit table:
+`meta.json` holds the training config, the model as it was built (overrides and flags included), the optimizer and the bits of its
+moments, the step, seeds, dtypes and, per stage, the unit table:
 global unit id, kind, unpadded and padded element counts, shard-group ranks and the element
 offsets of their shards (equal or, with `shard_ratio`, unequal) and, with tensor parallelism, which
 slice of the layer the entry is (`tp_index`; ranks are process ranks).  A rank file is the concatenation, per unit in table order, of the fp32 master
@@ -12,6 +13,7 @@ from __future__ import annotations
 
 import json
 import os
+from dataclasses import asdict
 
 import torch
 import torch.distributed as dist
@@ -73,6 +75,8 @@ def save_checkpoint(trainer, directory: str, step: int) -> str:
         meta = {"format_version": FORMAT_VERSION, "step": step, "seed": trainer.opt.seed,
                 "training_config": to_dict(trainer.cfg), "compute_dtype": trainer.cfg.autocast_dtype,
                 "world_size": trainer.world, "tensor_parallel_size": trainer.cfg.tensor_parallel_size,
+                "model": asdict(trainer.spec), "optimizer": trainer.opt.optimizer, "weight_decay": trainer.opt.weight_decay,
+                "moment_bits": trainer.opt.moment_bits,
                 "units": sorted(units, key=lambda e: (e["stage"], e["gid"], e.get("tp_index", 0)))}
         _atomic_write(os.path.join(d, "meta.json"), json.dumps(meta, indent=1).encode())
     trainer.barrier()

@@ -8,7 +8,8 @@ after it.  It picks the newest checkpoint directory that is complete (`meta.json
 last), takes the model, batch, sequence length and dtypes from it, removes the failed GPUs from
 the cluster description (renumbering the rest), runs the planner on what is left and writes the
 new training config.  The checkpoint reader re-shards, so the job resumes under the new plan with
-`zorse.py --config_file <output> --resume <checkpoint>`; the command is printed.
+`zorse.py --config_file <output> --resume <checkpoint>`; the command is printed, with the flags that the
+checkpoint's model and optimizer need.
 
 There is no in-place elastic resizing: a changed world is a new job that starts from a
 checkpoint.  (The reference has neither checkpoints nor recovery.)
@@ -116,7 +117,7 @@ def main(argv=None) -> int:
     ap.add_argument("--exclude_ranks", default="", help="comma-separated global ranks of the GPUs that failed")
     ap.add_argument("--output", default="training_config.json")
     a = ap.parse_args(argv)
-    from ..ckpt.reader import read_meta
+    from ..ckpt.reader import flags_of, read_meta
 
     ck = latest_checkpoint(a.checkpoint_dir)
     if ck is None:
@@ -136,7 +137,8 @@ def main(argv=None) -> int:
 
     n = min(n, parse_pipeline_dict(cfg).world_size)
     print(f"checkpoint {ck} (step {meta['step']}), {n} GPUs left, plan written to {a.output}")
-    print(f"python -m torch.distributed.run --nproc-per-node {n} zorse.py --config_file {a.output} --resume {ck}")
+    print(f"python -m torch.distributed.run --nproc-per-node {n} zorse.py --config_file {a.output} --resume {ck}"
+          + "".join(f" {x}" for x in flags_of(meta)))
     return 0
 
 
