@@ -833,8 +833,8 @@ PyObject* embedding_by_token(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (lib.embedding_by_token_workspace(int(T), int(H), &bytes) != 0) Py_RETURN_NONE;
   const Tensor ws = fresh({bytes}, *a.table, at::kByte);
   const cudaStream_t s = stream();
-  // order, and of every 32768 ids the sums and the runs over several pieces, or all in one; positions
-  const int n = 1 + (bytes > 0 ? 2 * int((T + 32767) / 32768) : 0) + (a.pos != nullptr);
+  // order (of more than 32768 ids in two), sums and the runs over several pieces, or all in one; positions
+  const int n = 1 + (bytes > 0 ? 2 + (T > 32768) : 0) + (a.pos != nullptr);
   if (!launch("embedding_by_token", n, [&] {
         return lib.embedding_by_token(static_cast<const long*>(ptr(a.ids)), ptr(dout), ptr(a.table), ptr(a.pos), ws.data_ptr(), int(T),
                                       int(H), int(V), int(a.S), int(a.off), float(a.scale), a.table->scalar_type() == F32, s);

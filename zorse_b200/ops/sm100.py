@@ -500,7 +500,7 @@ def embedding_by_token(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int
     _check(L.zb_embedding_by_token(_a(ids), _a(dout), _a(dtable), _a(dpos), _a(ws), T, H, V, S, pos_offset, scale,
                                    int(dtable.dtype == torch.float32), _stream()), "embedding_by_token")
     global _launches
-    _launches += (2 * -(-T // EMBEDDING_CHUNK) if ws.numel() else 0) + (dpos is not None and T > 0)   # sums and joined runs of a chunk, positions
+    _launches += (2 + (T > EMBEDDING_CHUNK) if ws.numel() else 0) + (dpos is not None and T > 0)   # sums, joined runs, chunks put together; positions
 
 
 # --------------------------------------------------------------------------- loss
