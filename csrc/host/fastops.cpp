@@ -788,6 +788,11 @@ PyObject* qk_norm_rope_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// Whether two contiguous tensors share memory.
+bool meet(const Tensor& a, const Tensor& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.data_ptr()), y = reinterpret_cast<uintptr_t>(b.data_ptr());
+  return a.nbytes() > 0 && b.nbytes() > 0 && x < y + b.nbytes() && y < x + a.nbytes();
+}
 // What the scaled embedding and its gradient have in common: ids, a table, positions of its type, S, offset, scale.
 struct Lookup {
   const Tensor *ids, *table, *pos;
@@ -829,6 +834,7 @@ PyObject* embedding_by_token(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (!a.take(args + 3)) Py_RETURN_NONE;
   const int64_t T = a.ids->numel(), V = a.table->size(0), H = a.table->size(1);
   if (!dense(dout, BF16) || dout->dim() != 2 || dout->size(0) != T || dout->size(1) != H || !on(dout, *a.table)) Py_RETURN_NONE;
+  if (meet(*dout, *a.table) || (a.pos != nullptr && meet(*dout, *a.pos))) Py_RETURN_NONE;
   long bytes = 0;
   if (lib.embedding_by_token_workspace(int(T), int(H), &bytes) != 0) Py_RETURN_NONE;
   const Tensor ws = fresh({bytes}, *a.table, at::kByte);

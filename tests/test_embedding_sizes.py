@@ -36,3 +36,33 @@ def test_the_library_refuses_sizes_it_does_not_count_cpu():
         for call, args in ((L.zb_embedding_scaled, (0, 0, 0, 0, 1, H, V, S, off, 1.0, 0)),
                            (L.zb_embedding_by_token, (0, 0, 0, 0, 0, 1, H, V, S, off, 1.0, 1, 0))):
             assert call(*args) != 0 and L.zb_last_error().startswith(b"embedding: ")
+
+
+def _shared(call, device):
+    buf = torch.zeros(4096, dtype=torch.bfloat16, device=device)
+    ids, dout, table = torch.zeros(6, dtype=torch.long, device=device), buf[1024:1120].view(6, 16), torch.zeros(10, 16, dtype=torch.bfloat16, device=device)
+    for over in (buf[1024:1184].view(10, 16), buf[1112:1272].view(10, 16), buf[872:1032].view(10, 16), buf[1000:1320].view(torch.float32).view(10, 16)):
+        with pytest.raises(ValueError, match="share memory"):
+            call(ids, dout, over, None, 6, 0)
+    with pytest.raises(ValueError, match="share memory"):
+        call(ids, dout, table, buf[1104:1200].view(6, 16), 6, 0)
+    return ids, dout, buf[1120:1280].view(10, 16), buf[928:1024].view(6, 16)
+
+
+def test_a_gradient_in_the_memory_of_its_rows_is_refused_cpu(no_launch):
+    args = _shared(k.embedding_by_token, "cpu")
+    with pytest.raises(AssertionError, match="was reached"):     # neighbours are not refused
+        k.embedding_by_token(*args, 6, 0)
+
+
+@pytest.mark.gpu
+def test_a_gradient_in_the_memory_of_its_rows_is_refused():
+    from zorse_b200.ops.api import get_ops
+
+    ops = get_ops("sm100")
+
+    def call(ids, dout, table, pos, S, off):
+        ops.embedding_bwd(ids, dout, table, pos, S, off, by_token=True)
+
+    ids, dout, table, pos = _shared(call, "cuda")
+    assert ops._embedding_by_token(ids, dout, table, pos, 6, 0, 1.0) is True

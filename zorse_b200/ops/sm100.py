@@ -222,6 +222,17 @@ def _rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return not width <= between <= step_a - width
 
 
+def _stretch(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses of a contiguous tensor."""
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    (lo, hi), (from_, to) = _stretch(a), _stretch(b)
+    return lo < to and from_ < hi and lo < hi and from_ < to
+
+
 def _workspace_size(fn, *sizes) -> int:
     out = ctypes.c_long(0)
     if fn(*sizes, ctypes.addressof(out)):
@@ -492,6 +503,8 @@ def embedding_by_token(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int
     table is read and written once.  The same bits on every run."""
     _need(dtable.dtype in (torch.float32, torch.bfloat16), f"dtable: fp32 or bf16, got {dtable.dtype}")
     _embedding_operands(ids, dout, dtable, "dtable", dpos, S, pos_offset)
+    for t, name in ((dtable, "dtable"), (dpos, "dpos")):
+        _need(t is None or not _meet(dout, t), f"{name} is added to while dout is read: they share memory")
     T = ids.numel()
     V, H = dtable.shape
     _need(V > 0 or T == 0, "an empty table")
@@ -521,11 +534,6 @@ def adam_step(p, m, v, g, p16, *, lr, beta1, beta2, eps, weight_decay, step, gra
     _check(lib().zb_adam(_a(p), _a(m), _a(v), _a(g), _a(p16), n, lr, beta1,
                          beta2, eps, weight_decay, step, grad_scale,
                          int(g.dtype == torch.float32), int(zero_grad), _stream()), "adam")
-
-
-def _stretch(t: torch.Tensor) -> tuple[int, int]:
-    """The addresses of a contiguous tensor."""
-    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
 
 
 def adamw_step(p, moments, g, p16, *, lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step, grad_scale: float = 1.0,
