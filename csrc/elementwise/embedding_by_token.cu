@@ -8,8 +8,10 @@
 // Ids outside [0, V) count as the nearest inside, as in the gather without a scale.
 // The gather of 32768 rows of 2048 columns takes 36 us: 134 MB written and as many read, most of them from L2, 7.5 TB/s.  The
 // gradient of 16384 tokens of 4096 columns into an fp32 table of 32000, a fifth of them one token, takes 71 us: 45 the sums
-// themselves (296 MB, 6.5 TB/s), the rest the order of the ids and the runs over several pieces, both bound by latency.  With atomics
-// the same gradient takes 143, and with ids spread evenly 130 against 104.
+// themselves (296 MB, 6.5 TB/s), the rest the order of the ids and the runs over several pieces, both bound by latency.
+// Against atomics, in a graph, us by atomics / by token: into fp32 tables 16384 tokens of 4096 columns with ids spread evenly 130 / 103,
+// 16384 of 256 with a fifth one token 66 / 29, but 8192 of 2048 spread evenly 22 / 26 and 16384 of 64 3.1 / 15.5; into bf16 tables, where
+// atomics take half the traffic and round at every occurrence, 16384 of 4096 56 / 71 and 16384 of 64 2.3 / 16.8.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "../norm/norm_common.cuh"
@@ -463,8 +465,9 @@ __global__ void __launch_bounds__(256, 3) embedding_join_kernel(const ByToken a,
 }
 
 // Few tokens: no order is needed.  A CTA has one token and 256 columns, looks for the token's id among all ids and, where the token is
-// the first with it, adds up the rows of all, each warp a stretch of them.  One launch: 256 tokens of 512 columns 3.1 us against
-// 10.0 by sorting, 1024 of 512, a fifth of them one token, 6.9 against 12.4; 1024 of 2048, four times as many CTAs, 16.1 against 12.1.
+// the first with it, adds up the rows of all, each warp a stretch of them.  One launch: in a graph 256 tokens of 512 columns 3.0 us
+// against 10.0 by sorting, 1024 of 512, a fifth of them one token, 6.9 against 12.4; 1024 of 2048, four times as many CTAs, 16.1
+// against 12.1.
 constexpr int SMALL_T = 1024, SMALL_CTAS = 2048;
 template <typename GT>
 __global__ void __launch_bounds__(256) embedding_small_kernel(const long* ids, const __nv_bfloat16* dout, GT* table, int T, int H, int V,
