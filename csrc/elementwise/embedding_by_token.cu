@@ -651,6 +651,7 @@ int zb_embedding_scaled(const long* ids, const void* table, const void* pos, voi
 // for each piece
 int zb_embedding_by_token_workspace(int T, int H, long* bytes) {
   using namespace zb;
+  if (int rc = embedding_check(H, 0, 0, 0)) return rc;
   const int K = piece_rows(T, H);
   *bytes = T > 0 && !is_small(T, H) ? order_bytes(T) + 8L * ((T - 1L) / K + 1) * H : 0;
   return 0;

@@ -66,3 +66,26 @@ def test_a_gradient_in_the_memory_of_its_rows_is_refused():
 
     ids, dout, table, pos = _shared(call, "cuda")
     assert ops._embedding_by_token(ids, dout, table, pos, 6, 0, 1.0) is True
+
+
+@pytest.mark.gpu
+def test_without_positions_their_sizes_do_not_matter():
+    from zorse_b200.ops.api import get_ops
+
+    ops = get_ops("sm100")
+    ids = torch.tensor([3, 1, 3], device="cuda")
+    table, dout = torch.randn(5, 16, device="cuda").bfloat16(), torch.ones(3, 16, dtype=torch.bfloat16, device="cuda")
+    for S, off in ((0, 0), (2 ** 31, 0), (2 ** 32, -1), (7, 2 ** 40)):
+        assert torch.equal(ops.embedding_fwd(ids, table, None, S, off, scale=2.0), (table[ids].float() * 2).bfloat16())
+        got = torch.zeros(5, 16, device="cuda")
+        ops.embedding_bwd(ids, dout, got, None, S, off, by_token=True)
+        assert torch.equal(got.sum(1).cpu(), torch.tensor([0.0, 16, 0, 32, 0]))
+
+
+def test_the_workspace_of_sizes_it_does_not_count_is_refused_cpu():
+    import ctypes
+
+    out = ctypes.c_long(-1)
+    for H in (2 ** 31 - 8, 12, 0):
+        assert k.lib().zb_embedding_by_token_workspace(4096, H, ctypes.addressof(out)) == -1 and out.value == -1
+    assert k.lib().zb_embedding_by_token_workspace(4096, 64, ctypes.addressof(out)) == 0 and out.value > 0

@@ -486,9 +486,10 @@ def _embedding_operands(ids, rows, table, what, pos_table, S, pos_offset):
 
 
 def embedding_scaled(ids, table, pos_table=None, S: int = 1, pos_offset: int = 0, scale: float = 1.0):
-    """scale * table[ids] (+ positions), rounded once."""
+    """scale * table[ids] (+ positions), rounded once.  S and pos_offset are those of the positions."""
     _bf16(table, "table")
     _embedding_operands(ids, None, table, "table", pos_table, S, pos_offset)
+    S, pos_offset = (1, 0) if pos_table is None else (S, pos_offset)
     T = ids.numel()
     V, H = table.shape
     _need(V > 0 or T == 0, "an empty table")
@@ -503,6 +504,7 @@ def embedding_by_token(ids, dout, dtable, dpos=None, S: int = 1, pos_offset: int
     table is read and written once.  The same bits on every run."""
     _need(dtable.dtype in (torch.float32, torch.bfloat16), f"dtable: fp32 or bf16, got {dtable.dtype}")
     _embedding_operands(ids, dout, dtable, "dtable", dpos, S, pos_offset)
+    S, pos_offset = (1, 0) if dpos is None else (S, pos_offset)
     for t, name in ((dtable, "dtable"), (dpos, "dpos")):
         _need(t is None or not _meet(dout, t), f"{name} is added to while dout is read: they share memory")
     T = ids.numel()
