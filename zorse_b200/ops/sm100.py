@@ -481,8 +481,8 @@ def _embedding_operands(ids, rows, table, what, pos_table, S, pos_offset):
         _need(pos_table.dtype == table.dtype and pos_table.is_contiguous() and pos_table.shape[1] == H and S > 0 and pos_offset >= 0
               and pos_table.shape[0] >= min(S, T) + pos_offset and pos_table.device == table.device,
               f"positions {tuple(pos_table.shape)}: expected [>= {min(S, T) + pos_offset}, {H}] of {table.dtype}")
-    # the kernels count in 32 bits: a longer S would reach them as another one, 0 among them
-    _need(S < 2 ** 31 and min(S, T) + pos_offset < 2 ** 31, f"sequences of {S}, positions from {pos_offset}: sizes below 2^31")
+        # the kernels count in 32 bits: a longer S would reach them as another one, 0 among them
+        _need(S < 2 ** 31 and min(S, T) + pos_offset < 2 ** 31, f"sequences of {S}, positions from {pos_offset}: sizes below 2^31")
 
 
 def embedding_scaled(ids, table, pos_table=None, S: int = 1, pos_offset: int = 0, scale: float = 1.0):
