@@ -20,10 +20,13 @@
 //
 // Warps 0-7: compute (0-3: query columns 0-63, 4-7: columns 64-127; each warp covers 32 key
 // lanes), warp 8: TMA producer, warp 9: MMA issuer + TMEM owner.
+// PACKED (packed.cuh; with the two-kernel form): sequences of different lengths in one stream of S tokens.  Tiles stay on the grid of
+// 128 rows, and every key has its own range of queries.
 // With TRACE the first `trace_ctas` CTAs record (clock64, code) per warp at phase boundaries.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "attn_bwd_common.h"
+#include "packed.cuh"
 #include <type_traits>
 
 namespace zb {
@@ -77,14 +80,15 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t cta) {
 // CL > 1 (DQ = false): a cluster of CL CTAs shares a key tile, each taking its part of the query heads of the GQA group;
 // the fp32 sums are added up through distributed shared memory, in rank order, at the end.  One CTA per key tile leaves
 // 2048 tokens with 8 kv heads at 128 CTAs of 4 to 64 steps: the time is that of the longest.
-template <int D, bool TRACE, bool DQ, int CL>
+template <int D, bool TRACE, bool DQ, int CL, bool PACKED>
 __global__ void __launch_bounds__(32 * BWD2_WARPS, 1)
 flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                   const __grid_constant__ CUtensorMap tmap_dk, const __grid_constant__ CUtensorMap tmap_dv,
                   const AttnBwdParams p, const float* stats, int s_pad,
-                  unsigned long long* trace, int trace_ctas) {
+                  unsigned long long* trace, int trace_ctas, const PackedView packed) {
   using Cfg = AttnBwd2Cfg<D>;
+  static_assert(!PACKED || !DQ, "packed sequences: dQ has a kernel of its own");
   constexpr int BM = 128, BN = 128, QS = Cfg::QS, DB = D / 64;
   // With d = 64 tensor memory has room for a second S^T (without the dQ part): the scores of the next step are then formed
   // ahead of this step's P^T, and the compute warps go from one step's dS^T to the next step's exponentials without
@@ -117,17 +121,18 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // grid = (kv heads, key tiles, batch): x-fastest dispatch starts every head's heaviest key tile
   // (tile 0 sees all query tiles under a causal mask) before any light one
-  const int jt = blockIdx.y, kv_head = blockIdx.x / CL, batch = blockIdx.z;
+  const int kv_head = blockIdx.x / CL, batch = blockIdx.z;
   const int cl_rank = blockIdx.x % CL;      // rank in the cluster
-  const int kv0 = jt * BN;
+  int kv0 = int(blockIdx.y) * BN;
   const int rep = p.Hq / p.Hkv / CL;        // query heads this CTA walks over
   const int head0 = kv_head * (p.Hq / p.Hkv) + cl_rank * rep;
   const int n_qt = (p.S + BM - 1) / BM;
-  const int i_lo = p.causal ? (kv0 / BM) : 0;
+  int i_lo = p.causal ? (kv0 / BM) : 0;
   int i_hi = n_qt;
   if (p.window > 0) i_hi = min(n_qt, (kv0 + BN - 1 + p.window - 1) / BM + 1);
-  const int per_head = max(i_hi - i_lo, 0);
-  const int n_iters = per_head * rep;
+  int n_iters = max(i_hi - i_lo, 0) * rep;
+  [[maybe_unused]] int total = p.S;                 // PACKED: the end of the last sequence
+  [[maybe_unused]] int all_lo = 0, all_hi = 0;      // PACKED: queries that see every key of the tile
   WaitCtx wctx{abort_flag, p.status};
 
   const int cta_lin = int(blockIdx.x) + int(gridDim.x) * (int(blockIdx.y) + int(gridDim.y) * int(blockIdx.z));
@@ -170,6 +175,17 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   if constexpr (!DQ) {
     chain_wait();
     chain_trigger();   // behind the wait: the dQ kernel starts on this, under the last CTAs here (chain_late in ptx.cuh)
+  }
+  if constexpr (PACKED) {
+    kv0 = packed.order_keys[blockIdx.y] * BN;
+    total = packed.total();
+    const int2 first = packed.bounds[kv0], last = packed.bounds[kv0 + BN - 1];
+    const KeyRange r = query_range(first, last, kv0, p.causal, p.window);
+    i_lo = r.lo / BM;
+    i_hi = r.hi > r.lo ? (r.hi + BM - 1) / BM : i_lo;
+    n_iters = (i_hi - i_lo) * rep;
+    all_lo = p.causal ? kv0 + BN - 1 : last.x;
+    all_hi = p.window > 0 ? min(first.y, kv0 + p.window) : first.y;
   }
 
   if (warp == 8) {
@@ -248,7 +264,16 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const uint32_t r_dp = tmem_base + Cfg::DP_COL;
       auto r_s = [&](int it) { return tmem_base + (NSB == 2 && (it & 1) ? uint32_t(Cfg::S1_COL) : 0u); };
       bool ok = mbar_wait_warp(k_full, 0, wctx, ST_TIMEOUT_FULL);
+      [[maybe_unused]] int tile_a = i_lo, tile_b = i_lo;   // PACKED: query tiles of the next A and the next B
+      // PACKED: what lies behind the last sequence (Q, dO, V) meets weights of 0 in products, and 0 times a NaN is one
+      auto clear_next = [&](uint32_t addr, int& tile) {
+        if constexpr (PACKED) {
+          clear_tail_rows<D>(addr, total - tile * BM, lane);
+          if (++tile == i_hi) tile = i_lo;
+        }
+      };
       auto issue_a = [&](int it) {  // S^T = K Q^T
+        clear_next(smem_u32(sQ + (it % QS) * Cfg::TILE_BYTES), tile_a);
         if (elected) {
           const uint32_t q_addr = smem_u32(sQ + (it % QS) * Cfg::TILE_BYTES), d = r_s(it);
 #pragma unroll
@@ -261,6 +286,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         __syncwarp();
       };
       auto issue_b = [&](uint32_t do_addr) {  // dP^T = V dO^T
+        clear_next(do_addr, tile_b);
         if (elected) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -280,6 +306,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (ok) ok = mbar_wait_warp(&do_full[0], 0, wctx, ST_TIMEOUT_FULL);
       if (ok) {
         tc_fence_after();
+        if constexpr (PACKED) clear_tail_rows<D>(v_addr, total - kv0, lane);
         issue_b(smem_u32(sDO));
         tr(TB_MMA_B_ISSUED);
       }
@@ -396,6 +423,12 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const uint32_t lane_addr = tmem_base + (uint32_t((warp & 3) * 32) << 16);
     const int key = kv0 + t;
     const bool key_ok = key < p.S;
+    [[maybe_unused]] int see_lo = 0, see_hi = 0;       // PACKED: queries that see this key
+    if constexpr (PACKED) {
+      const int2 b = packed.bounds[key];
+      see_lo = p.causal ? max(key, b.x) : b.x;
+      see_hi = p.window > 0 ? min(b.y, key + p.window) : b.y;
+    }
     uint8_t* ds_row = sDS + half * BLK + t * 128;  // this thread's 128-byte row of its 64-query block
     bool ok = true;
     int head = head0, qt = i_lo - 1;   // (counted along: two divisions per step otherwise)
@@ -411,15 +444,16 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if constexpr (!DQ) {
         if (!__all_sync(0xffffffffu, mbar_wait(&q_full[it % QS], uint32_t(it / QS) & 1, wctx, ST_TIMEOUT_FULL))) { ok = false; break; }
       }
-      const bool need_mask = (p.causal && kv0 + BN - 1 > q0) || (p.window > 0 && kv0 < q0 + BM - p.window) ||
-                             (kv0 + BN > p.S) || (q0 + BM > p.S);
+      const bool need_mask = PACKED ? q0 < all_lo || q0 + BM > all_hi
+                                    : (p.causal && kv0 + BN - 1 > q0) || (p.window > 0 && kv0 < q0 + BM - p.window) ||
+                                          (kv0 + BN > p.S) || (q0 + BM > p.S);
       // ---- C1: P^T = exp2(S^T c - lse_q), kept as packed bf16 pairs (queries 2i, 2i+1) ----
       if (!__all_sync(0xffffffffu, mbar_wait(&s_full[it % NSB], uint32_t(it / NSB) & 1, wctx, ST_TIMEOUT_TMEM_FULL))) { ok = false; break; }
       tr(TB_S_READY);
       tc_fence_after();
       // queries of this half that this thread's key is seen by: columns [vis_lo, vis_lo + vis_n)
-      const int vis_lo = p.causal ? max(key - qc0, 0) : 0;
-      const int vis_hi = min((p.window > 0 ? min(key + p.window, p.S) : p.S) - qc0, 64);
+      const int vis_lo = PACKED ? max(see_lo - qc0, 0) : p.causal ? max(key - qc0, 0) : 0;
+      const int vis_hi = min((PACKED ? see_hi : p.window > 0 ? min(key + p.window, p.S) : p.S) - qc0, 64);
       const uint32_t vis_n = key_ok ? uint32_t(max(vis_hi - vis_lo, 0)) : 0u;
       if constexpr (!DQ) {
         // P stays in fp32 registers between its two uses; two-wide fp32 math; the softmax scale of dS is applied to
@@ -742,7 +776,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 template <int D>
 __global__ void __launch_bounds__(256)
 attn_bwd2_stats_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o,
-                       const float* lse, float* stats, int S, int Hq, int s_pad, int o_vec) {
+                       const float* lse, float* stats, int S, int Hq, int s_pad, int o_vec, const int2* bounds) {
   chain_trigger();
   chain_wait();
   constexpr int LANES = D / 8, GROUPS = 256 / LANES, N = 64 / GROUPS;   // lanes per token, tokens at a time, tokens per group
@@ -783,19 +817,21 @@ attn_bwd2_stats_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o,
   if (threadIdx.x < 64) {   // (the padding too: its P is masked, but 0 times what lies there has to be 0)
     const size_t bh = size_t(b) * Hq + h;
     float* row = stats + bh * 2 * size_t(s_pad);
-    row[s] = s < S ? lse[bh * S + s] * -1.4426950408889634f : 0.f;
-    row[s_pad + s] = -sm[threadIdx.x];
+    bool in = s < S;
+    if (in && bounds != nullptr) in = bounds[s].x < bounds[s].y;   // packed sequences: nor what a token of none holds
+    row[s] = in ? lse[bh * S + s] * -1.4426950408889634f : 0.f;
+    row[s_pad + s] = in ? -sm[threadIdx.x] : 0.f;
   }
 }
 
 static int launch_stats(const __nv_bfloat16* o, const __nv_bfloat16* d_o, const float* lse, float* stats, int B, int S, int Hq,
-                        int D, int s_pad, cudaStream_t stream) {
+                        int D, int s_pad, cudaStream_t stream, const int2* bounds = nullptr) {
   const dim3 grid(s_pad / 64, Hq, B);
   const int o_vec = (reinterpret_cast<uintptr_t>(o) & 15) == 0;   // (dO is fetched by TMA and aligned anyway)
   if (reinterpret_cast<uintptr_t>(d_o) & 15) ZB_FAIL(-4, "attention: dO not 16-byte aligned");
   if (D == 128) ZB_CUDA_OK(launch_pass(attn_bwd2_stats_kernel<128>, grid, 256, 0, stream, o, d_o, lse, stats, S, Hq, s_pad,
-                                       o_vec));
-  else ZB_CUDA_OK(launch_pass(attn_bwd2_stats_kernel<64>, grid, 256, 0, stream, o, d_o, lse, stats, S, Hq, s_pad, o_vec));
+                                       o_vec, bounds));
+  else ZB_CUDA_OK(launch_pass(attn_bwd2_stats_kernel<64>, grid, 256, 0, stream, o, d_o, lse, stats, S, Hq, s_pad, o_vec, bounds));
   ZB_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -808,9 +844,9 @@ static int make_head_tmap_bwd2(CUtensorMap* out, const __nv_bfloat16* base, int 
   return make_tmap_nd_bf16(out, base, 4, dims, strides, box);
 }
 
-template <int D, bool TRACE, bool DQ = true, int CL = 1>
+template <int D, bool TRACE, bool DQ = true, int CL = 1, bool PACKED = false>
 static int launch_bwd2(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const AttnBwdParams& p, const float* stats,
-                       int s_pad, unsigned long long* trace, int trace_ctas, cudaStream_t stream) {
+                       int s_pad, unsigned long long* trace, int trace_ctas, cudaStream_t stream, const PackedView& packed = {}) {
   using Cfg = AttnBwd2Cfg<D>;
   const int width = (p.Hq + 2 * p.Hkv) * D;
   CUtensorMap tq, tk, tv, tdo, tdk, tdv;
@@ -821,18 +857,15 @@ static int launch_bwd2(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const
   if ((rc = make_head_tmap_bwd2(&tk, qkv + size_t(p.Hq) * D, p.B, p.S, p.Hkv, D, width))) return rc;
   if ((rc = make_head_tmap_bwd2(&tv, qkv + size_t(p.Hq + p.Hkv) * D, p.B, p.S, p.Hkv, D, width))) return rc;
   if ((rc = make_head_tmap_bwd2(&tdo, d_o, p.B, p.S, p.Hq, D, p.Hq * D))) return rc;
-  auto kern = flash_bwd2_kernel<D, TRACE, DQ, CL>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
-    attr_set = true;
-  }
+  auto kern = flash_bwd2_kernel<D, TRACE, DQ, CL, PACKED>;
+  static SharedLimit limit;
+  ZB_CUDA_OK(limit.raise(kern, Cfg::SMEM_BYTES));
   dim3 grid(p.Hkv * CL, (p.S + 127) / 128, p.B);
   if constexpr (!DQ) {
     ZB_CUDA_OK(launch_chained(kern, grid, 32 * BWD2_WARPS, Cfg::SMEM_BYTES, stream, CL > 1 ? CL : 0, tq, tk, tv, tdo, tdk, tdv, p, stats,
-                              s_pad, trace, trace_ctas));
+                              s_pad, trace, trace_ctas, packed));
   } else {
-    kern<<<grid, 32 * BWD2_WARPS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, tdo, tdk, tdv, p, stats, s_pad, trace, trace_ctas);
+    kern<<<grid, 32 * BWD2_WARPS, Cfg::SMEM_BYTES, stream>>>(tq, tk, tv, tdo, tdk, tdv, p, stats, s_pad, trace, trace_ctas, packed);
     ZB_CUDA_OK(cudaGetLastError());
   }
   return 0;
@@ -851,7 +884,7 @@ static int bwd_cluster(int B, int S, int Hq, int Hkv) {
 }
 
 int attn_bwd_dq(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const AttnBwdParams& p, const float* stats, int s_pad,
-                int D, int late, cudaStream_t stream);   // flash_bwd_dq.cu
+                int D, int late, cudaStream_t stream, const PackedView* packed = nullptr);   // flash_bwd_dq.cu
 
 }  // namespace zb
 
@@ -937,6 +970,42 @@ int zb_flash_bwd3(const void* d_o, const void* qkv, const void* o, const float* 
   }
   if (rc) return rc;
   return (parts & 2) ? attn_bwd_dq(QKV, DO, p, stats, s_pad, D, parts == 3, stream) : 0;
+}
+
+// The same three kernels for sequences of different lengths (packed.cu): d_o, o [T, Hq D], qkv and dqkv [T, (Hq + 2 Hkv) D], lse
+// [Hq, T].  The gradient of tokens of no sequence is 0, whatever they hold.  Scratch: stats fp32 [Hq * 2 * T rounded up to 128].
+int zb_packed_attn_bwd(const void* d_o, const void* qkv, const void* o, const float* lse, void* dqkv, float* stats, const void* bounds,
+                       const int* order_tiles, const int* order_keys, int T, int Hq, int Hkv, int D, int causal, int window,
+                       float softmax_scale, int* status, cudaStream_t stream) {
+  using namespace zb;
+  if (T <= 0 || Hq <= 0) return 0;
+  if (int rc = packed_check(T, Hq, Hkv, D)) return rc;
+  auto DO = static_cast<const __nv_bfloat16*>(d_o);
+  auto O = static_cast<const __nv_bfloat16*>(o);
+  auto QKV = static_cast<const __nv_bfloat16*>(qkv);
+  const int s_pad = (T + 127) / 128 * 128;
+  PackedView view = packed_view(bounds, T);
+  view.order_tiles = order_tiles;
+  view.order_keys = order_keys;
+  if (int rc = launch_stats(O, DO, lse, stats, 1, T, Hq, D, s_pad, stream, view.bounds)) return rc;
+  AttnBwdParams p;
+  p.lse = lse; p.delta = nullptr; p.dq_acc = nullptr;
+  p.dqkv = static_cast<__nv_bfloat16*>(dqkv);
+  p.B = 1; p.S = T; p.Hq = Hq; p.Hkv = Hkv;
+  p.window = window; p.causal = causal;
+  p.scale = softmax_scale;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.status = status;
+  auto run = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    switch (bwd_cluster(1, T, Hq, Hkv)) {
+      case 4: return launch_bwd2<DD, false, false, 4, true>(QKV, DO, p, stats, s_pad, nullptr, 0, stream, view);
+      case 2: return launch_bwd2<DD, false, false, 2, true>(QKV, DO, p, stats, s_pad, nullptr, 0, stream, view);
+      default: return launch_bwd2<DD, false, false, 1, true>(QKV, DO, p, stats, s_pad, nullptr, 0, stream, view);
+    }
+  };
+  if (int rc = D == 128 ? run(std::integral_constant<int, 128>()) : run(std::integral_constant<int, 64>())) return rc;
+  return attn_bwd_dq(QKV, DO, p, stats, s_pad, D, 1, stream, &view);
 }
 
 }  // extern "C"

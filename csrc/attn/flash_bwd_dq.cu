@@ -21,11 +21,13 @@
 // Warps 0-7: compute (0-3: key columns 0-63 of the tile, 4-7: columns 64-127; each warp covers 32
 // query rows = TMEM lanes), warp 8: TMA producer, warp 9: MMA issuer + TMEM owner.
 // TMEM: S0 [0,128) S1 [128,256) dP [256,384) dQ [384, 384+D).
+// PACKED (packed.cuh): sequences of different lengths in one stream of S tokens, each row with its own range of keys.
 // Replaces (with flash_bwd2.cu) the autograd of flash-attn 2 / SDPA used by the reference
 // (models/llama_simple.py:396-416).
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "attn_bwd_common.h"
+#include "packed.cuh"
 
 namespace zb {
 
@@ -40,12 +42,12 @@ struct AttnDqCfg {
   static constexpr int DP_COL = 256, DQ_COL = 384;
 };
 
-template <int D>
+template <int D, bool PACKED>
 __global__ void __launch_bounds__(320, 1)
 flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                     const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                     const __grid_constant__ CUtensorMap tmap_dq, const AttnBwdParams p, const float* stats, int s_pad,
-                    const int late) {
+                    const int late, const PackedView packed) {
   using Cfg = AttnDqCfg<D>;
   constexpr int BM = 128, BN = 128, NK = Cfg::NK, NV = Cfg::NV, DB = D / 64;
   constexpr int BLK = 128 * 128;  // bytes of one [128 rows x 64 cols] bf16 block
@@ -72,15 +74,16 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   const int n_qt = (p.S + BM - 1) / BM;
   // grid = (heads, query tiles, batch): x-fastest dispatch, the latest (heaviest under a causal mask)
   // query tile of every head first
-  const int qt = n_qt - 1 - int(blockIdx.y);
   const int head = blockIdx.x, batch = blockIdx.z;
   const int kv_head = head / (p.Hq / p.Hkv);
-  const int q0 = qt * BM;
+  int q0 = (n_qt - 1 - int(blockIdx.y)) * BM;
   const int n_kv = (p.S + BN - 1) / BN;
   int j_lo = 0, j_hi = n_kv;
   if (p.causal) j_hi = min(j_hi, (q0 + BM - 1) / BN + 1);
   if (p.window > 0) j_lo = max(0, (q0 - p.window + 1) / BN);
-  const int n = max(j_hi - j_lo, 0);
+  int n = max(j_hi - j_lo, 0);
+  [[maybe_unused]] int total = p.S;                 // PACKED: the end of the last sequence
+  [[maybe_unused]] int all_lo = 0, all_hi = 0;      // PACKED: keys that every row of the tile sees
   WaitCtx wctx{abort_flag, p.status};
 
   if (threadIdx.x == 0) {
@@ -113,6 +116,16 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   // 480 CTAs each (8 x 12 heads of 577 tokens) make 3.2 rounds on 148 SMs, so a quarter of its time most SMs idled.
   if (!late) chain_wait();
   chain_trigger();
+  if constexpr (PACKED) {
+    q0 = packed.order_tiles[blockIdx.y] * BM;
+    total = packed.total();
+    const int2 first = packed.bounds[q0], last = packed.bounds[q0 + BM - 1];
+    const KeyRange r = key_range(first, last, q0, p.causal, p.window);
+    j_lo = r.lo / BN;
+    n = r.hi > r.lo ? (r.hi + BN - 1) / BN - j_lo : 0;
+    all_lo = p.window > 0 ? max(last.x, q0 + BM - p.window) : last.x;
+    all_hi = p.causal ? min(first.y, q0 + 1) : first.y;
+  }
 
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
@@ -155,6 +168,8 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       auto k_of = [&](int i) { return smem_u32(sK + (i % NK) * Cfg::TILE_BYTES); };
       auto v_of = [&](int i) { return smem_u32(sV + (i % NV) * Cfg::TILE_BYTES); };
       auto issue_s = [&](int i) {    // S_i = Q K_i^T into S[i & 1]
+        // PACKED: what lies behind the last sequence (K, V, dO) meets weights of 0 in products, and 0 times a NaN is one
+        if constexpr (PACKED) clear_tail_rows<D>(k_of(i), total - (j_lo + i) * BN, lane);
         if (elected) {
           const uint32_t k_addr = k_of(i);
 #pragma unroll
@@ -168,6 +183,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         __syncwarp();
       };
       auto issue_dp = [&](int i) {   // dP_i = dO V_i^T
+        if constexpr (PACKED) clear_tail_rows<D>(v_of(i), total - (j_lo + i) * BN, lane);
         if (elected) {
           const uint32_t v_addr = v_of(i);
 #pragma unroll
@@ -186,6 +202,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       if (ok) ok = mbar_wait_warp(&v_full[0], 0, wctx, ST_TIMEOUT_FULL);
       if (ok) {
         tc_fence_after();
+        if constexpr (PACKED) clear_tail_rows<D>(do_addr, total - q0, lane);
         issue_s(0);
         issue_dp(0);
       }
@@ -234,12 +251,19 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       nl = st_row[row];
       nd = st_row[s_pad + row];
     }
+    [[maybe_unused]] int key_lo = 0, key_hi = 0;      // PACKED: keys this row sees
+    if constexpr (PACKED) {
+      const int2 b = packed.bounds[row];
+      key_lo = p.window > 0 ? max(b.x, row - p.window + 1) : b.x;
+      key_hi = p.causal ? min(row + 1, b.y) : b.y;
+    }
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const int kv0 = (j_lo + i) * BN;
       const uint32_t s_col = lane_addr + uint32_t((i & 1) * 128 + half * 64);
-      const bool need_mask = (p.causal && kv0 + BN - 1 > q0) || (p.window > 0 && kv0 < q0 + BM - p.window) ||
-                             (kv0 + BN > p.S) || (q0 + BM > p.S);
+      const bool need_mask = PACKED ? kv0 < all_lo || kv0 + BN > all_hi
+                                    : (p.causal && kv0 + BN - 1 > q0) || (p.window > 0 && kv0 < q0 + BM - p.window) ||
+                                          (kv0 + BN > p.S) || (q0 + BM > p.S);
       if (!__all_sync(0xffffffffu, mbar_wait(&s_full[i & 1], uint32_t(i >> 1) & 1, wctx, ST_TIMEOUT_TMEM_FULL))) { ok = false; break; }
       tc_fence_after();
       float pr[64];
@@ -261,8 +285,8 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         if (need_mask) {
           // keys of this half that this thread's query sees: columns [vis_lo, vis_lo + vis_n)
           const int col0 = kv0 + half * 64;
-          const int vis_lo = p.window > 0 ? max(row - p.window + 1 - col0, 0) : 0;
-          const int vis_hi = min((p.causal ? min(row + 1, p.S) : p.S) - col0, 64);
+          const int vis_lo = PACKED ? max(key_lo - col0, 0) : p.window > 0 ? max(row - p.window + 1 - col0, 0) : 0;
+          const int vis_hi = min((PACKED ? key_hi : p.causal ? min(row + 1, p.S) : p.S) - col0, 64);
           const uint32_t vis_n = row_ok ? uint32_t(max(vis_hi - vis_lo, 0)) : 0u;
 #pragma unroll
           for (int k = 0; k < 64; ++k) pr[k] = uint32_t(k - vis_lo) < vis_n ? pr[k] : 0.f;
@@ -355,9 +379,9 @@ static int make_head_tmap_dq(CUtensorMap* out, const __nv_bfloat16* base, int B,
   return make_tmap_nd_bf16(out, base, 4, dims, strides, box);
 }
 
-template <int D>
+template <int D, bool PACKED>
 static int launch_dq(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const AttnBwdParams& p, const float* stats,
-                     int s_pad, int late, cudaStream_t stream) {
+                     int s_pad, int late, cudaStream_t stream, const PackedView& packed) {
   using Cfg = AttnDqCfg<D>;
   const int width = (p.Hq + 2 * p.Hkv) * D;
   CUtensorMap tq, tk, tv, tdo, tdq;
@@ -367,14 +391,11 @@ static int launch_dq(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const A
   if ((rc = make_head_tmap_dq(&tv, qkv + size_t(p.Hq + p.Hkv) * D, p.B, p.S, p.Hkv, D, width))) return rc;
   if ((rc = make_head_tmap_dq(&tdo, d_o, p.B, p.S, p.Hq, D, p.Hq * D))) return rc;
   if ((rc = make_head_tmap_dq(&tdq, p.dqkv, p.B, p.S, p.Hq, D, width))) return rc;
-  auto kern = flash_bwd_dq_kernel<D>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
-    attr_set = true;
-  }
+  auto kern = flash_bwd_dq_kernel<D, PACKED>;
+  static SharedLimit limit;
+  ZB_CUDA_OK(limit.raise(kern, Cfg::SMEM_BYTES));
   dim3 grid(p.Hq, (p.S + 127) / 128, p.B);
-  ZB_CUDA_OK(launch_chained(kern, grid, 320, Cfg::SMEM_BYTES, stream, 0, tq, tk, tv, tdo, tdq, p, stats, s_pad, late));
+  ZB_CUDA_OK(launch_chained(kern, grid, 320, Cfg::SMEM_BYTES, stream, 0, tq, tk, tv, tdo, tdq, p, stats, s_pad, late, packed));
   return 0;
 }
 
@@ -382,9 +403,12 @@ static int launch_dq(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const A
 // kernel's statistics pass (lse in log2 units and delta per row, rows padded to s_pad).
 // late: the kernel in front in the stream is the key-tile kernel of the same call.
 int attn_bwd_dq(const __nv_bfloat16* qkv, const __nv_bfloat16* d_o, const AttnBwdParams& p, const float* stats, int s_pad,
-                int D, int late, cudaStream_t stream) {
-  if (D == 128) return launch_dq<128>(qkv, d_o, p, stats, s_pad, late, stream);
-  return launch_dq<64>(qkv, d_o, p, stats, s_pad, late, stream);
+                int D, int late, cudaStream_t stream, const PackedView* packed) {
+  if (packed != nullptr)
+    return D == 128 ? launch_dq<128, true>(qkv, d_o, p, stats, s_pad, late, stream, *packed)
+                    : launch_dq<64, true>(qkv, d_o, p, stats, s_pad, late, stream, *packed);
+  if (D == 128) return launch_dq<128, false>(qkv, d_o, p, stats, s_pad, late, stream, {});
+  return launch_dq<64, false>(qkv, d_o, p, stats, s_pad, late, stream, {});
 }
 
 }  // namespace zb

@@ -24,11 +24,16 @@
 // warpgroups can hold a 128-value score row each (setmaxnreg.inc).
 // TMEM: S_0 [0,128) S_1 [128,256) O_0 [256,256+D) O_1 [384,384+D).
 //
+// PACKED: sequences of different lengths lie one after another in one stream of S tokens (packed.cu).  Tiles stay on the
+// grid of 128 rows, so a tile holds the ends of several short sequences, and every row has its own range of keys: two
+// numbers a thread loads once.  The key tiles a CTA walks over go from the first row's sequence's begin to its last row.
+//
 // With TRACE the first `trace_ctas` CTAs record (clock64, code) pairs per warp at phase
 // boundaries into a global buffer; zorse_b200/profiler/attn_trace.py turns them into a
 // per-phase timeline.
 #include "../common/host.h"
 #include "../common/ptx.cuh"
+#include "packed.cuh"
 
 namespace zb {
 
@@ -42,6 +47,7 @@ struct AttnFwd4Params {
   int* status;
   unsigned long long* trace;  // [trace_ctas][10 warps][TRACE_EV] or nullptr
   int trace_ctas;
+  PackedView packed;          // PACKED: B = 1, S tokens in all
 };
 
 constexpr int FWD4_TRACE_EV = 256;
@@ -79,14 +85,14 @@ enum : int {
   TR_TMA_SLOT_FREE = 32, TR_TMA_ISSUED = 33,
 };
 
-template <int D, bool TRACE, int MODE>
+template <int D, bool TRACE, int MODE, bool PACKED>
 __global__ void __launch_bounds__(32 * FWD4_WARPS, 1)
 flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o,
                   const AttnFwd4Params p) {
   using Cfg = AttnFwd4Cfg<D>;
   constexpr int BM = 128, BN = 128, NSLOT = Cfg::NSLOT, DB = D / 64, BLK = 128 * 128;
-  constexpr bool PACKED = MODE >= 1;   // two-wide fp32 fma / add, three-input maximum
+  constexpr bool WIDE = MODE >= 1;     // two-wide fp32 fma / add, three-input maximum
   constexpr bool POLY = MODE >= 2;     // every fourth exponential on the fma pipe instead of MUFU
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -106,24 +112,40 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const int n_pairs = (p.S + 2 * BM - 1) / (2 * BM);
   // grid = (heads, query pairs, batch): CTAs are dispatched x-fastest, so every head's heaviest
   // (latest) pair starts first and the light ones fill the tail of the last wave
-  const int pair = n_pairs - 1 - int(blockIdx.y);
+  int pair = n_pairs - 1 - int(blockIdx.y);
   const int head = blockIdx.x, batch = blockIdx.z;
   const int kv_head = head / (p.Hq / p.Hkv);
   const int n_kv = (p.S + BN - 1) / BN;
-  int lo[2], hi[2];
+  int lo[2], hi[2], j_lo = 0, n_tiles = 0;
+  [[maybe_unused]] int total = p.S;               // PACKED: the end of the last sequence
+  [[maybe_unused]] int begin_of_last[2] = {0, 0};  // PACKED: where the sequence of a chain's last row begins
+  auto tile_ranges = [&] {
+    if constexpr (PACKED) {
+      pair = p.packed.order_pairs[blockIdx.y];
+      total = p.packed.total();
+    }
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int q0 = (2 * pair + c) * BM;
-    lo[c] = 0;
-    hi[c] = n_kv;
-    if (p.causal) hi[c] = min(hi[c], (q0 + BM - 1) / BN + 1);
-    if (p.window > 0) lo[c] = max(0, (q0 - p.window + 1) / BN);
-    if (q0 >= p.S) { lo[c] = 0; hi[c] = 0; }
-  }
-  const bool act0 = hi[0] > lo[0], act1 = hi[1] > lo[1];
-  const int j_lo = act1 ? (act0 ? min(lo[0], lo[1]) : lo[1]) : lo[0];
-  const int j_hi = max(hi[0], hi[1]);
-  const int n_tiles = max(j_hi - j_lo, 0);
+    for (int c = 0; c < 2; ++c) {
+      const int q0 = (2 * pair + c) * BM;
+      if constexpr (PACKED) {
+        const int2 first = p.packed.bounds[q0], last = p.packed.bounds[q0 + BM - 1];   // (padded to whole pairs)
+        const KeyRange r = key_range(first, last, q0, p.causal, p.window);
+        lo[c] = r.lo / BN;
+        hi[c] = r.hi > r.lo ? (r.hi + BN - 1) / BN : lo[c];
+        begin_of_last[c] = last.x;
+      } else {
+        lo[c] = 0;
+        hi[c] = n_kv;
+        if (p.causal) hi[c] = min(hi[c], (q0 + BM - 1) / BN + 1);
+        if (p.window > 0) lo[c] = max(0, (q0 - p.window + 1) / BN);
+        if (q0 >= p.S) { lo[c] = 0; hi[c] = 0; }
+      }
+    }
+    const bool act0 = hi[0] > lo[0], act1 = hi[1] > lo[1];
+    j_lo = act1 ? (act0 ? min(lo[0], lo[1]) : lo[1]) : lo[0];
+    n_tiles = max(max(act0 ? hi[0] : 0, act1 ? hi[1] : 0) - j_lo, 0);
+  };
+  if constexpr (!PACKED) tile_ranges();
   WaitCtx wctx{abort_flag, p.status};
 
   // ---- trace ----
@@ -164,6 +186,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const uint32_t tmem_base = *tmem_slot;
   chain_trigger();
   chain_wait();
+  if constexpr (PACKED) tile_ranges();
 
   if (warp >= 8) {
     setmaxnreg_dec<FWD4_OTHER_REGS>();
@@ -251,6 +274,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           tr(TR_MMA_V_READY);
           bool k_ready = false;
           const uint32_t v_addr = smem_u32(sR + vslot * Cfg::TILE_BYTES);
+          if constexpr (PACKED) clear_tail_rows<D>(v_addr, total - j * BN, lane);   // their weights are 0, but 0 times a NaN is one
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             if (!ok) break;
@@ -317,6 +341,16 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const int my_lo = c ? lo[1] : lo[0];
     const int my_tiles = max((c ? hi[1] : hi[0]) - my_lo, 0);
     const float scale = p.scale_log2;
+    [[maybe_unused]] int key_lo = 0, key_hi = 0;      // PACKED: keys this row sees
+    [[maybe_unused]] int all_lo = 0, all_hi = 0;      // and those that every row of the tile sees
+    if constexpr (PACKED) {
+      const int2 b = p.packed.bounds[row];
+      key_lo = p.window > 0 ? max(b.x, row - p.window + 1) : b.x;
+      key_hi = p.causal ? min(row + 1, b.y) : b.y;
+      const int last_begin = c ? begin_of_last[1] : begin_of_last[0];
+      all_lo = p.window > 0 ? max(last_begin, q0 + BM - p.window) : last_begin;
+      all_hi = min(p.packed.bounds[q0].y, p.causal ? q0 + 1 : p.S);
+    }
     float m_run = -INFINITY, l_run = 0.f;  // m_run in raw (unscaled) score units
     bool ok = true;
     for (int i = 0; i < my_tiles; ++i) {
@@ -332,12 +366,13 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       tmem_ld32(s_col + 96u, s3);
       tmem_wait_ld();
       tr(TR_S_LOADED);
-      const bool need_mask = (p.causal && kv0 + BN - 1 > q0) || (p.window > 0 && kv0 < q0 + BM - p.window) ||
-                             (kv0 + BN > p.S);
+      const bool need_mask = PACKED ? kv0 < all_lo || kv0 + BN > all_hi
+                                    : (p.causal && kv0 + BN - 1 > q0) || (p.window > 0 && kv0 < q0 + BM - p.window) ||
+                                          (kv0 + BN > p.S);
       if (need_mask) {
         // keys of the tile that this row sees: columns [vis_lo, vis_lo + vis_n)
-        const int vis_lo = p.window > 0 ? max(row - p.window + 1 - kv0, 0) : 0;
-        const uint32_t vis_n = uint32_t(max((p.causal ? min(row + 1, p.S) : p.S) - kv0 - vis_lo, 0));
+        const int vis_lo = PACKED ? max(key_lo - kv0, 0) : p.window > 0 ? max(row - p.window + 1 - kv0, 0) : 0;
+        const uint32_t vis_n = uint32_t(max((PACKED ? key_hi : p.causal ? min(row + 1, p.S) : p.S) - kv0 - vis_lo, 0));
         auto mask32 = [&](uint32_t (&r)[32], int base) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) r[k] = uint32_t(base + k - vis_lo) < vis_n ? r[k] : 0xff800000u;  // -inf
@@ -350,7 +385,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       float mx[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) mx[k] = -INFINITY;
-      if (PACKED) {
+      if (WIDE) {
         // three-input maximum: two new values per instruction, eight independent chains
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
@@ -407,7 +442,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           float x0, x1;
-          if (PACKED) {
+          if (WIDE) {
             ffma2(x0, x1, __uint_as_float(r[k]), __uint_as_float(r[k + 1]), scale, scale, neg_mc, neg_mc);
           } else {
             x0 = fmaf(__uint_as_float(r[k]), scale, neg_mc);
@@ -417,7 +452,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           const float e0 = exp2f(x0);
           const float e1 = (POLY && (k & 2)) ? exp2_poly3(x1) : exp2f(x1);
           const int a = ((k >> 1) & 3) * 2;
-          if (PACKED) {
+          if (WIDE) {
             fadd2(ls[a], ls[a + 1], ls[a], ls[a + 1], e0, e1);
           } else {
             ls[a] += e0;
@@ -507,7 +542,7 @@ static int make_head_tmap4(CUtensorMap* out, const __nv_bfloat16* base, int B, i
   return make_tmap_nd_bf16(out, base, 4, dims, strides, box);
 }
 
-template <int D, bool TRACE, int MODE>
+template <int D, bool TRACE, int MODE, bool PACKED = false>
 static int launch_fwd4(const __nv_bfloat16* qkv, int width, const AttnFwd4Params& p, cudaStream_t stream) {
   using Cfg = AttnFwd4Cfg<D>;
   CUtensorMap tq, tk, tv, to;
@@ -516,12 +551,9 @@ static int launch_fwd4(const __nv_bfloat16* qkv, int width, const AttnFwd4Params
   if ((rc = make_head_tmap4(&tq, qkv, p.B, p.S, p.Hq, D, width))) return rc;
   if ((rc = make_head_tmap4(&tk, qkv + size_t(p.Hq) * D, p.B, p.S, p.Hkv, D, width))) return rc;
   if ((rc = make_head_tmap4(&tv, qkv + size_t(p.Hq + p.Hkv) * D, p.B, p.S, p.Hkv, D, width))) return rc;
-  auto kern = flash_fwd4_kernel<D, TRACE, MODE>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    ZB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
-    attr_set = true;
-  }
+  auto kern = flash_fwd4_kernel<D, TRACE, MODE, PACKED>;
+  static SharedLimit limit;
+  ZB_CUDA_OK(limit.raise(kern, Cfg::SMEM_BYTES));
   dim3 grid(p.Hq, (p.S + 255) / 256, p.B);
   ZB_CUDA_OK(launch_chained(kern, grid, Cfg::THREADS, Cfg::SMEM_BYTES, stream, 0, tq, tk, tv, to, p));
   return 0;
@@ -541,7 +573,7 @@ extern "C" int zb_flash_fwd4(const void* qkv, void* out, float* lse, int B, int 
   using namespace zb;
   if (B <= 0 || S <= 0) return 0;
   if (Hkv <= 0 || Hq % Hkv != 0) ZB_FAIL(-1, "attention: Hq=%d not a multiple of Hkv=%d", Hq, Hkv);
-  AttnFwd4Params p;
+  AttnFwd4Params p = {};
   p.O = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   p.B = B; p.S = S; p.Hq = Hq; p.Hkv = Hkv;
@@ -570,4 +602,26 @@ extern "C" int zb_flash_fwd4(const void* qkv, void* out, float* lse, int B, int 
   if (D == 64) ZB_FWD4_DISPATCH(64);
 #undef ZB_FWD4_DISPATCH
   ZB_FAIL(-1, "attention: head dim %d unsupported (64 or 128)", D);
+}
+
+// Sequences of different lengths (packed.cu): qkv [T, (Hq + 2 Hkv) D], out [T, Hq D], lse [Hq, T]; tokens of no sequence get
+// zeros and -inf.  bounds, order_pairs: of zb_pack_sequences for T tokens.
+extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const void* bounds, const int* order_pairs, int T, int Hq,
+                                  int Hkv, int D, int causal, int window, float softmax_scale, int* status, cudaStream_t stream) {
+  using namespace zb;
+  if (T <= 0 || Hq <= 0) return 0;
+  if (int rc = packed_check(T, Hq, Hkv, D)) return rc;
+  AttnFwd4Params p = {};
+  p.O = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.B = 1; p.S = T; p.Hq = Hq; p.Hkv = Hkv;
+  p.window = window; p.causal = causal;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.ldo = Hq * D;
+  p.status = status;
+  p.packed = packed_view(bounds, T);
+  p.packed.order_pairs = order_pairs;
+  auto Q = static_cast<const __nv_bfloat16*>(qkv);
+  const int width = (Hq + 2 * Hkv) * D;
+  return D == 128 ? launch_fwd4<128, false, 1, true>(Q, width, p, stream) : launch_fwd4<64, false, 1, true>(Q, width, p, stream);
 }

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ref
+from . import packed, ref
 from .moments import decode
 
 _ACT_KINDS = {"gelu": 0, "gelu_new": 0, "gelu_tanh": 0, "relu": 1, "gelu_erf": 2}
@@ -134,6 +134,27 @@ class RefOps(_EpilogueOps, _LaterOps):
             out = ref.attention(q, B, S, Hq, Hkv, D, causal, window)
             (dq,) = torch.autograd.grad(out, q, do.float())
         return dq.to(qkv.dtype)
+
+    # ---- packed batches: sequences of different lengths, one after another -----------------
+    def pack_sequences(self, offsets, T):
+        """What the calls below need to know of sequences [offsets[i], offsets[i + 1]) in T tokens; once for all layers of a batch."""
+        return packed.pack(offsets, T)
+
+    def packed_attn_fwd(self, qkv, pk, Hq, Hkv, D, causal=True, window=0):
+        """Attention of every token over its own sequence: (out, lse [Hq, T])."""
+        return packed.attention(qkv, pk, Hq, Hkv, D, causal, window)
+
+    def packed_attn_bwd(self, do, qkv, o, lse, pk, Hq, Hkv, D, causal=True, window=0):
+        with torch.enable_grad():
+            q = qkv.detach().to(torch.promote_types(qkv.dtype, torch.float32)).requires_grad_(True)
+            out, _ = packed.attention(q, pk, Hq, Hkv, D, causal, window)
+            (dq,) = torch.autograd.grad(out, q, do.to(q.dtype))
+        return dq.to(qkv.dtype)
+
+    def rope_at_(self, buf, cs, positions, nheads, d, sections=None, backward=False):
+        """Rotation of heads [0, nheads) in place by rows `positions` of cs, with several axes each by its `sections` of the pairs."""
+        buf.copy_(packed.rope_at(buf, cs, positions, nheads, d, sections, backward))
+        return buf
 
     # ---- MLP activations --------------------------------------------------------
     def swiglu_fwd(self, gu):
@@ -319,6 +340,18 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
     def attn_bwd(self, do, qkv, o, lse, B, S, Hq, Hkv, D, causal=True, window=0):
         dqkv = self._attn_bwd(do, qkv, o, lse, B, S, Hq, Hkv, D, causal, window)
         return self.k.flash_bwd(do, qkv, o, lse, B, S, Hq, Hkv, D, causal, window) if dqkv is None else dqkv
+
+    def pack_sequences(self, offsets, T):
+        return self.k.pack_sequences(offsets, T)
+
+    def packed_attn_fwd(self, qkv, pk, Hq, Hkv, D, causal=True, window=0):
+        return self.k.packed_attn_fwd(qkv, pk, Hq, Hkv, D, causal, window)
+
+    def packed_attn_bwd(self, do, qkv, o, lse, pk, Hq, Hkv, D, causal=True, window=0):
+        return self.k.packed_attn_bwd(do, qkv, o, lse, pk, Hq, Hkv, D, causal, window)
+
+    def rope_at_(self, buf, cs, positions, nheads, d, sections=None, backward=False):
+        return self.k.rope_at_(buf, cs, positions, nheads, d, sections, backward)
 
     def swiglu_fwd(self, gu):
         y = self._swiglu_fwd(gu)

@@ -22,6 +22,7 @@ from typing import Optional
 import torch
 
 from .moments import BLOCK as MOMENT_BLOCK
+from .packed import MOST_AXES, MOST_TOKENS, PackedSequences, check_window
 
 _LIB_PATH = Path(__file__).resolve().parents[1] / "_C" / "libzorse_sm100.so"
 _lib = None
@@ -54,6 +55,8 @@ _SIGNATURES = {
     "zb_flash_fwd4": "pppiiiiiiifipipip", "zb_flash_bwd3": "ppppppiiiiiiifpipip",
     "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
     "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
+    "zb_pack_sequences": "piipppppp", "zb_packed_attn_fwd": "pppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
+    "zb_rope_at": "ppppiiiiilip",
     "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
 _CTYPES = {"p": c_void_p, "i": c_int, "l": c_long, "f": c_float}
@@ -754,6 +757,87 @@ def flash_bwd(do, qkv, o, lse, B: int, S: int, Hq: int, Hkv: int, D: int, causal
     global _launches
     _launches += 2  # delta + finish kernels
     return dqkv
+
+
+# --------------------------------------------------------------------------- packed sequences
+def pack_sequences(offsets, T: int) -> PackedSequences:
+    """What attention and rotation need to know of sequences that lie one after another in T tokens: sequence i has the tokens
+    [offsets[i], offsets[i + 1]).  offsets: int32 on the device, from 0 up, not falling; nothing waits for the GPU, so their values
+    are not checked (others than these give results of no meaning, within the batch)."""
+    _need(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and 1 <= offsets.numel() < 2 ** 31,
+          f"offsets {tuple(offsets.shape)}, {offsets.dtype}: expected int32 [sequences + 1]")
+    _on_current(offsets, "offsets")
+    _need(0 <= T <= MOST_TOKENS, f"{T} tokens: at most {MOST_TOKENS}")
+    dev, pairs, tiles = offsets.device, -(-T // 256), -(-T // 128)
+    bounds = torch.empty(pairs * 256, 2, dtype=torch.int32, device=dev)
+    rest = torch.empty(T + pairs + 2 * tiles, dtype=torch.int32, device=dev).split([T, pairs, tiles, tiles])
+    _check(lib().zb_pack_sequences(_a(offsets), offsets.numel() - 1, T, _a(bounds), *(_a(t) for t in rest), _stream()), "pack_sequences")
+    return PackedSequences(T, bounds, *rest)
+
+
+def _packed_operands(qkv, pk, Hq, Hkv, D, causal, window):
+    _bf16(qkv, "qkv")
+    _on_current(qkv, "qkv")
+    check_window(causal, window)
+    _need(Hq > 0 and Hkv > 0 and Hq % Hkv == 0 and D in (64, 128), f"{Hq} query heads, {Hkv} key heads of {D}: heads of 64 or 128 in whole groups")
+    _need(qkv.shape == (pk.tokens, (Hq + 2 * Hkv) * D) and qkv.is_contiguous(),
+          f"qkv {tuple(qkv.shape)}: expected contiguous rows of ({Hq} + 2 x {Hkv}) x {D}, one for each of {pk.tokens} tokens")
+    _need(pk.order_pairs is not None and pk.bounds.device == qkv.device, f"the packing is for another backend or device ({pk.bounds.device}, qkv on {qkv.device})")
+
+
+def packed_attn_fwd(qkv, pk: PackedSequences, Hq: int, Hkv: int, D: int, causal: bool = True, window: int = 0, scale: Optional[float] = None):
+    """Attention of every token over its own sequence: (out [T, Hq D], lse [Hq, T]).  Tokens of no sequence get zeros and -inf."""
+    _packed_operands(qkv, pk, Hq, Hkv, D, causal, window)
+    T = pk.tokens
+    out = torch.empty(T, Hq * D, dtype=qkv.dtype, device=qkv.device)
+    lse = torch.empty(Hq, T, dtype=torch.float32, device=qkv.device)
+    _check(lib().zb_packed_attn_fwd(_a(qkv), _a(out), _a(lse), _a(pk.bounds), _a(pk.order_pairs), T, Hq, Hkv, D, int(causal), _window(window, T),
+                                    1.0 / math.sqrt(D) if scale is None else scale, _a(status_word(qkv.device)), _stream()), "packed_attn_fwd")
+    return out, lse
+
+
+def packed_attn_bwd(do, qkv, o, lse, pk: PackedSequences, Hq: int, Hkv: int, D: int, causal: bool = True, window: int = 0,
+                    scale: Optional[float] = None):
+    """Gradient of the packed projection from the output's (o, lse: what the forward pass returned); zeros for tokens of no sequence."""
+    _packed_operands(qkv, pk, Hq, Hkv, D, causal, window)
+    _bf16(do, "do"); _bf16(o, "o")
+    T = pk.tokens
+    _need(do.shape == o.shape == (T, Hq * D) and do.is_contiguous() and o.is_contiguous() and do.device == o.device == qkv.device,
+          f"do {tuple(do.shape)}, o {tuple(o.shape)}: expected contiguous [{T}, {Hq * D}]")
+    _need(lse.shape == (Hq, T) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == qkv.device,
+          f"lse {tuple(lse.shape)}, {lse.dtype}: expected fp32 [{Hq}, {T}]")
+    stats = torch.empty(Hq * 2 * -(-T // 128) * 128, dtype=torch.float32, device=qkv.device)
+    dqkv = torch.empty_like(qkv)
+    _check(lib().zb_packed_attn_bwd(_a(do), _a(qkv), _a(o), _a(lse), _a(dqkv), _a(stats), _a(pk.bounds), _a(pk.order_tiles),
+                                    _a(pk.order_keys), T, Hq, Hkv, D, int(causal), _window(window, T),
+                                    1.0 / math.sqrt(D) if scale is None else scale, _a(status_word(qkv.device)), _stream()), "packed_attn_bwd")
+    global _launches
+    _launches += 2     # statistics, dQ
+    return dqkv
+
+
+def rope_at_(buf, cs, positions, nheads: int, d: int, sections=None, backward: bool = False):
+    """In-place rotation of heads [0, nheads) of buf [T, width] by given rows of the table cs [P, d] (`rope_table`): positions, int32
+    [axes, T] (or [T]); pair i of a head turns by its axis' row, the first sections[0] pairs by axis 0's and so on (None: one
+    axis for all).  Positions outside the table take its nearest row."""
+    _bf16(buf, "buf")
+    _on_current(buf, "buf")
+    sections = [d // 2] if sections is None else [int(x) for x in sections]
+    axes = len(sections)
+    _need(d > 0 and d % 2 == 0 and 1 <= axes <= MOST_AXES and min(sections) >= 0 and sum(sections) == d // 2,
+          f"sections {sections}: 1 to {MOST_AXES} that add up to {d // 2}, half of a head's columns")
+    _need(buf.dim() == 2 and buf.stride(1) == 1 and 0 <= nheads and nheads * d <= buf.shape[1] and (buf.shape[0] <= 1 or buf.stride(0) >= buf.shape[1])
+          and max(buf.shape) < 2 ** 31, f"buf {tuple(buf.shape)}, strides {buf.stride()}: expected rows of at least {nheads} heads of {d}")
+    T = buf.shape[0]
+    _need(positions.dtype == torch.int32 and positions.is_contiguous() and positions.device == buf.device
+          and (positions.shape == (axes, T) or (axes == 1 and positions.shape == (T,))),
+          f"positions {tuple(positions.shape)}, {positions.dtype}: expected int32 [{axes}, {T}] on {buf.device}")
+    _need(cs.dtype == torch.float32 and cs.dim() == 2 and cs.shape[1] == d and 0 < cs.shape[0] < 2 ** 31 and cs.is_contiguous() and cs.device == buf.device,
+          f"table {tuple(cs.shape)}, {cs.dtype}: expected fp32 [positions, {d}]")
+    pairs = (c_int * axes)(*sections)
+    _check(lib().zb_rope_at(_a(buf), _a(cs), _a(positions), ctypes.addressof(pairs), axes, T, cs.shape[0], nheads, d, buf.stride(0),
+                            int(backward), _stream()), "rope_at")
+    return buf
 
 
 # --------------------------------------------------------------------------- fused collectives
