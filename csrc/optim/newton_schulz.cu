@@ -1,0 +1,483 @@
+// Updates orthogonalised by Newton-Schulz products, over a list of matrices.
+//
+// U (n x m, n <= m; a matrix with more rows than columns is taken transposed) becomes X = U / ||U||_F and then, five times,
+//     A = X X^T,   B = b A + c A A,   X <- a X + B X
+// an odd polynomial of the singular values that drives them all towards 1 without an SVD.  Three products an iteration; A and A A
+// are symmetric, so only their tiles on and above the diagonal are formed and every other one is stored a second time, turned
+// over: 2 n^2 m + n^3 / 2 ... n^2 m + n^3 + 2 n^2 m floating-point operations instead of 4 n^2 m + 2 n^3.
+//
+// Every matrix of the list takes part in each launch: those of one shape lie one behind the other in the workspace behind one tensor
+// map, and the tiles of up to GROUPS shapes are dealt to persistent CTA pairs.  A model's matrices of 512 to 1024 columns have 3 to 10
+// tiles each, one by one a launch would leave most of the GPU idle.
+//
+// Operands are fp16, sums fp32 in tensor memory.  All values are bounded (singular values stay below 1.21), so the range of bf16 is
+// not needed and its eight bits would cost: relative error of X after five iterations 1.0e-2 with bf16 and 1.3e-3 with fp16 (512 x
+// 512 to 1024 x 1024, noise and few strong directions alike).  X is held times 2^round(log2(sqrt m)), so its entries are near 1 at the end,
+// A and B times 64, so that what the first iteration's small values round to stays far below what they add.
+//
+// Around the products: one pass over gradient and momentum with the sum of squares, one that scales, turns and rounds into the
+// workspace, and one that applies the result (momentum and scale come from fp32, sums of squares are held in 64 bits: no gradient is too
+// small or too large for them).
+#include "../common/host.h"
+#include "../common/ptx.cuh"
+#include "newton_schulz.cuh"
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+namespace zb {
+
+// --------------------------------------------------------------------------------------------- passes before and behind
+constexpr int NS_MATRICES = 64;      // of a launch of a pass
+constexpr int NS_PARTS = 256;        // sums of squares of one matrix, at most
+
+// What a caller hands over for each matrix.
+struct NsMatrix {
+  float* p;               // muon: fp32, rows x cols; else null
+  float* m;               // muon: momentum
+  const void* g;          // gradient (muon), or the matrix
+  __nv_bfloat16* out;     // muon: p's copy in bf16, or null; else the result
+  long rows, cols;
+  int g_f32, unused;
+};
+
+struct NsPassMatrix {
+  float* p;
+  float* m;
+  const void* g;
+  __nv_bfloat16* out;
+  __half* x;              // first the scaled matrix, at the end the result: [n, ld]
+  double* sums;           // [parts]
+  long ld;
+  int rows, cols, parts, tiles_c, first;   // first: of the blocks of a launch
+  int g_f32, wide;        // wide: rows start on 16 bytes in every type
+  float scale, step;      // X is held times scale; muon: what the result is multiplied with
+};
+struct NsPass {
+  NsPassMatrix t[NS_MATRICES];
+  int count;
+  float momentum, grad_scale, keep;
+  int nesterov, muon;
+};
+
+__device__ __forceinline__ int ns_find(const NsPass& a, int block) {
+  int lo = 0, hi = a.count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.t[mid].first <= block) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+__device__ __forceinline__ float4 ns_load4(const void* base, bool f32, size_t at) {
+  if (f32) {
+    const uint4 v = ld_v4(static_cast<const float*>(base) + at);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + at);
+  const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float ns_load1(const void* base, bool f32, size_t at) {
+  return f32 ? static_cast<const float*>(base)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
+}
+// The update from the scaled gradient and the new momentum.
+__device__ __forceinline__ float ns_update(const NsPass& a, float g, float m) { return a.nesterov ? fmaf(a.momentum, m, g) : m; }
+
+// Momentum (written back) and the sum of squares of the update; a block has an equal part of its matrix's elements.
+__global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ NsPass a) {
+  chain_trigger();
+  chain_wait();
+  const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
+  const int part = int(blockIdx.x) - t.first;
+  const size_t n = size_t(t.rows) * t.cols, each = ((n + t.parts - 1) / t.parts + 3) / 4 * 4;
+  const size_t lo = each * part, hi = lo + each < n ? lo + each : n;
+  double sum = 0.0;
+  auto one = [&](size_t i) {
+    float u = ns_load1(t.g, t.g_f32, i);
+    if (a.muon) {
+      const float g = u * a.grad_scale, m = fmaf(a.momentum, t.m[i], g);
+      t.m[i] = m;
+      u = ns_update(a, g, m);
+    }
+    sum += double(u) * double(u);
+  };
+  if (t.wide) {
+    constexpr int U = 4;     // loads in flight
+    const size_t whole = lo < hi ? lo + (hi - lo) / 4 * 4 : lo;
+    for (size_t i = lo + threadIdx.x * 4; i < whole; i += 256 * 4 * U) {
+      float4 g[U], m[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i + k * 1024 < whole) {
+          g[k] = ns_load4(t.g, t.g_f32, i + k * 1024);
+          if (a.muon) m[k] = ns_load4(t.m, true, i + k * 1024);
+        }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (i + k * 1024 < whole) {
+          float u[4] = {g[k].x, g[k].y, g[k].z, g[k].w};
+          if (a.muon) {
+            float w[4] = {m[k].x, m[k].y, m[k].z, m[k].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = u[j] * a.grad_scale;
+              w[j] = fmaf(a.momentum, w[j], x);
+              u[j] = ns_update(a, x, w[j]);
+            }
+            *reinterpret_cast<float4*>(t.m + i + k * 1024) = make_float4(w[0], w[1], w[2], w[3]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum += double(u[j]) * double(u[j]);
+        }
+    }
+    if (whole + threadIdx.x < hi) one(whole + threadIdx.x);
+  } else {
+    for (size_t i = lo + threadIdx.x; i < hi; i += 256) one(i);
+  }
+  __shared__ double part_sums[8];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+  if ((threadIdx.x & 31) == 0) part_sums[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += part_sums[i];
+    t.sums[part] = s;
+  }
+}
+
+// Tiles of 64 x 64: the update times scale / norm in fp16, turned over where the matrix has more rows than columns.
+__global__ void __launch_bounds__(256) ns_scale_kernel(const __grid_constant__ NsPass a) {
+  chain_trigger();
+  chain_wait();
+  const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
+  const int tile = int(blockIdx.x) - t.first, r0 = tile / t.tiles_c * 64, c0 = tile % t.tiles_c * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = c0 + tx * 4;
+  float u[4][4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + ty + 16 * k;
+    const size_t at = size_t(r) * t.cols + c;
+    if (r < t.rows && t.wide && c < t.cols) {
+      const float4 g = ns_load4(t.g, t.g_f32, at);
+      u[k][0] = g.x; u[k][1] = g.y; u[k][2] = g.z; u[k][3] = g.w;
+      if (a.muon) {
+        const float4 m = ns_load4(t.m, true, at);
+        const float w[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[k][j] = ns_update(a, u[k][j] * a.grad_scale, w[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u[k][j] = 0.f;
+        if (r < t.rows && c + j < t.cols) {
+          u[k][j] = ns_load1(t.g, t.g_f32, at + j);
+          if (a.muon) u[k][j] = ns_update(a, u[k][j] * a.grad_scale, t.m[at + j]);
+        }
+      }
+    }
+  }
+  __shared__ double sums[8];
+  double s = int(threadIdx.x) < t.parts ? t.sums[threadIdx.x] : 0.0;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += sums[i];
+  const double by = s == 0.0 ? 0.0 : double(t.scale) / sqrt(s);
+  __shared__ float tile_s[64][65];
+  const bool turned = t.rows > t.cols;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + ty + 16 * k;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[k][j] = float(double(u[k][j]) * by);
+    if (turned) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tile_s[ty + 16 * k][tx * 4 + j] = u[k][j];
+    } else if (r < t.rows && c < t.cols) {      // (rows of the workspace are padded to 8)
+      *reinterpret_cast<uint2*>(t.x + size_t(r) * t.ld + c) = make_uint2(pack_half2(u[k][0], u[k][1]), pack_half2(u[k][2], u[k][3]));
+    }
+  }
+  if (!turned) return;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int cc = c0 + ty + 16 * k, r = r0 + tx * 4;
+    if (cc < t.cols && r < t.rows)
+      *reinterpret_cast<uint2*>(t.x + size_t(cc) * t.ld + r) =
+          make_uint2(pack_half2(tile_s[tx * 4][ty + 16 * k], tile_s[tx * 4 + 1][ty + 16 * k]),
+                     pack_half2(tile_s[tx * 4 + 2][ty + 16 * k], tile_s[tx * 4 + 3][ty + 16 * k]));
+  }
+}
+
+// Tiles of 64 x 64: the result in bf16, or the step of the parameters.
+__global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ NsPass a) {
+  chain_trigger();
+  chain_wait();
+  const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
+  const int tile = int(blockIdx.x) - t.first, r0 = tile / t.tiles_c * 64, c0 = tile % t.tiles_c * 64;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = c0 + tx * 4;
+  const bool turned = t.rows > t.cols;
+  __shared__ float tile_s[64][65];
+  float4 old[4];
+  uint2 x[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + ty + 16 * k, xr = turned ? c0 + ty + 16 * k : r, xc = turned ? r0 + tx * 4 : c;
+    x[k] = make_uint2(0u, 0u);
+    if (xr < (turned ? t.cols : t.rows) && xc < (turned ? t.rows : t.cols)) x[k] = *reinterpret_cast<const uint2*>(t.x + size_t(xr) * t.ld + xc);
+    if (a.muon && t.wide && r < t.rows && c < t.cols) old[k] = ns_load4(t.p, true, size_t(r) * t.cols + c);
+  }
+  if (turned) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 lo = unpack_half2(x[k].x), hi = unpack_half2(x[k].y);
+      float* to = &tile_s[ty + 16 * k][tx * 4];
+      to[0] = lo.x; to[1] = lo.y; to[2] = hi.x; to[3] = hi.y;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int r = r0 + ty + 16 * k;
+    float v[4];
+    if (turned) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = tile_s[tx * 4 + j][ty + 16 * k];
+    } else {
+      const float2 lo = unpack_half2(x[k].x), hi = unpack_half2(x[k].y);
+      v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+    }
+    if (r >= t.rows) continue;
+    const size_t at = size_t(r) * t.cols + c;
+    const float w[4] = {old[k].x, old[k].y, old[k].z, old[k].w};
+    const bool four = t.wide && c < t.cols;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] *= t.step;
+      if (a.muon && c + j < t.cols) v[j] = fmaf(four ? w[j] : t.p[at + j], a.keep, -v[j]);
+    }
+    if (four) {
+      if (a.muon) *reinterpret_cast<float4*>(t.p + at) = make_float4(v[0], v[1], v[2], v[3]);
+      if (t.out != nullptr) *reinterpret_cast<uint2*>(t.out + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < t.cols) {
+          if (a.muon) t.p[at + j] = v[j];
+          if (t.out != nullptr) t.out[at + j] = __float2bfloat16(v[j]);
+        }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ the list
+struct NsShape {
+  long n, m;                       // short and long side
+  std::vector<int> members;        // of the list
+  size_t x[2], a, b;               // places in the workspace
+  long np() const { return (n + 7) / 8 * 8; }
+  long mp() const { return (m + 7) / 8 * 8; }
+};
+struct NsPlan {
+  std::vector<NsShape> shapes;     // the one with the longest products first: the last wave of a launch is then of short ones
+  std::vector<size_t> sums;        // of each matrix
+  std::vector<int> parts;
+  size_t bytes = 0;
+};
+
+static NsPlan ns_plan(const NsMatrix* t, int count) {
+  NsPlan plan;
+  auto take = [&](size_t n) {
+    const size_t at = plan.bytes;
+    plan.bytes += (n + 1023) / 1024 * 1024;
+    return at;
+  };
+  for (int i = 0; i < count; ++i) {
+    const long n = std::min(t[i].rows, t[i].cols), m = std::max(t[i].rows, t[i].cols);
+    auto s = std::find_if(plan.shapes.begin(), plan.shapes.end(), [&](const NsShape& x) { return x.n == n && x.m == m; });
+    if (s == plan.shapes.end()) s = plan.shapes.insert(s, NsShape{n, m, {}, {0, 0}, 0, 0});
+    s->members.push_back(i);
+  }
+  std::stable_sort(plan.shapes.begin(), plan.shapes.end(), [](const NsShape& a, const NsShape& b) { return a.m > b.m; });
+  for (NsShape& s : plan.shapes) {
+    const size_t k = s.members.size();
+    for (size_t& x : s.x) x = take(k * s.n * s.mp() * 2);
+    s.a = take(k * s.n * s.np() * 2);
+    s.b = take(k * s.n * s.np() * 2);
+  }
+  for (int i = 0; i < count; ++i) {
+    const long parts = (t[i].rows * t[i].cols + 4095) / 4096;
+    plan.parts.push_back(int(std::min<long>(parts, NS_PARTS)));
+    plan.sums.push_back(take(size_t(plan.parts.back()) * 8));
+  }
+  return plan;
+}
+
+// 3-D map of `count` matrices [rows, cols], ld elements a row (16-bit types are alike here); box: box_rows rows of 64 columns.
+static int ns_map(CUtensorMap* out, const void* base, long rows, long cols, long ld, long count, uint32_t box_rows) {
+  const uint64_t dims[3] = {uint64_t(cols), uint64_t(rows), uint64_t(count)};
+  const uint64_t strides[2] = {uint64_t(ld) * 2, uint64_t(rows) * ld * 2};
+  const uint32_t box[3] = {64, box_rows, 1};
+  return make_tmap_nd_bf16(out, base, 3, dims, strides, box);
+}
+
+static float ns_scale(long m) { return exp2f(float(std::min(13l, std::lround(0.5 * std::log2(double(m)))))); }
+
+template <int KIND>
+static int ns_product(const NsPlan& plan, char* ws, int from, float a, float b, float c, int* status, cudaStream_t stream, int* launches) {
+  for (size_t first = 0; first < plan.shapes.size(); first += NS_GROUPS) {
+    NsParams p = {};
+    p.status = status;
+    for (size_t i = first; i < std::min(first + NS_GROUPS, plan.shapes.size()); ++i) {
+      const NsShape& s = plan.shapes[i];
+      NsGroup& g = p.g[p.groups++];
+      const long k = long(s.members.size()), np = s.np(), mp = s.mp();
+      const float scale = ns_scale(s.m);
+      char *x = ws + s.x[from], *y = ws + s.x[1 - from], *ga = ws + s.a, *gb = ws + s.b;
+      int rc = 0;
+      if (KIND == NS_GRAM) {
+        rc = ns_map(&g.a, x, s.n, s.m, mp, k, 128) | ns_map(&g.c, ga, s.n, s.n, np, k, 32);
+        g.b = g.a;
+        g.x = g.c;
+        g.out = reinterpret_cast<__half*>(ga);
+        g.K = int(s.m);
+        g.alpha = NS_A_SCALE / (scale * scale);
+      } else if (KIND == NS_POLY) {
+        rc = ns_map(&g.a, ga, s.n, s.n, np, k, 128) | ns_map(&g.x, ga, s.n, s.n, np, k, 32) | ns_map(&g.c, gb, s.n, s.n, np, k, 32);
+        g.b = g.a;
+        g.out = reinterpret_cast<__half*>(gb);
+        g.K = int(s.n);
+        g.alpha = c / NS_A_SCALE;
+        g.beta = b;
+      } else {
+        rc = ns_map(&g.a, gb, s.n, s.n, np, k, 128) | ns_map(&g.b, x, s.n, s.m, mp, k, 64) | ns_map(&g.x, x, s.n, s.m, mp, k, 32) |
+             ns_map(&g.c, y, s.n, s.m, mp, k, 32);
+        g.K = int(s.n);
+        g.alpha = 1.f / NS_A_SCALE;
+        g.beta = a;
+      }
+      if (rc) return -5;
+      g.M = int(s.n);
+      g.N = int(KIND == NS_APPLY ? s.m : s.n);
+      g.ld = np;
+      g.step = s.n * np;
+      g.tiles_m = (g.M + NsCfg::BM - 1) / NsCfg::BM;
+      const long tn = (g.N + NsCfg::BN - 1) / NsCfg::BN;
+      const long tiles = KIND == NS_APPLY ? g.tiles_m * tn : long(g.tiles_m) * (g.tiles_m + 1) / 2;
+      if (p.items + tiles * k > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: matrices of %ld x %ld", s.n, s.m);
+      g.tiles = int(tiles);
+      g.first = p.items;
+      p.items += int(tiles * k);
+    }
+    if (int rc = ns_launch<KIND>(p, stream)) return rc;
+    ++*launches;
+  }
+  return 0;
+}
+
+// One of the passes over all matrices; PASS 0: sums, 1: scale, 2: apply.
+template <int PASS>
+static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, float lr, char* ws, int last, cudaStream_t stream, int* launches) {
+  NsPass a = common;
+  a.count = 0;
+  long blocks = 0;
+  auto flush = [&]() -> int {
+    if (a.count == 0) return 0;
+    if (blocks > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: %ld blocks", blocks);
+    const dim3 grid = dim3(unsigned(blocks));
+    if (PASS == 0) ZB_CUDA_OK(launch_pass(ns_sums_kernel, grid, 256, 0, stream, a));
+    else if (PASS == 1) ZB_CUDA_OK(launch_pass(ns_scale_kernel, grid, 256, 0, stream, a));
+    else ZB_CUDA_OK(launch_pass(ns_apply_kernel, grid, 256, 0, stream, a));
+    ++*launches;
+    a.count = 0;
+    blocks = 0;
+    return 0;
+  };
+  for (const NsShape& s : plan.shapes) {
+    const float scale = ns_scale(s.m);
+    for (size_t k = 0; k < s.members.size(); ++k) {
+      const int i = s.members[k];
+      NsPassMatrix& e = a.t[a.count++];
+      e.p = t[i].p;
+      e.m = t[i].m;
+      e.g = t[i].g;
+      e.out = t[i].out;
+      e.x = reinterpret_cast<__half*>(ws + s.x[PASS == 2 ? last : 0]) + k * s.n * s.mp();
+      e.sums = reinterpret_cast<double*>(ws + plan.sums[i]);
+      e.ld = s.mp();
+      e.rows = int(t[i].rows);
+      e.cols = int(t[i].cols);
+      e.parts = plan.parts[i];
+      e.tiles_c = (e.cols + 63) / 64;
+      e.first = int(blocks);
+      e.g_f32 = t[i].g_f32;
+      const uintptr_t f32 = reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.m) | (e.g_f32 ? reinterpret_cast<uintptr_t>(e.g) : 0);
+      const uintptr_t b16 = reinterpret_cast<uintptr_t>(e.out) | (e.g_f32 ? 0 : reinterpret_cast<uintptr_t>(e.g));
+      e.wide = e.cols % 4 == 0 && (f32 & 15) == 0 && (b16 & 7) == 0;
+      e.scale = scale;
+      e.step = (common.muon ? lr * 0.2f * sqrtf(float(s.m)) : 1.f) / scale;
+      blocks += PASS == 0 ? e.parts : long((e.rows + 63) / 64) * e.tiles_c;
+      if (a.count == NS_MATRICES)
+        if (int rc = flush()) return rc;
+    }
+  }
+  return flush();
+}
+
+static int ns_check(const NsMatrix* t, int count) {
+  for (int i = 0; i < count; ++i)
+    if (t[i].rows < 1 || t[i].cols < 1 || t[i].rows > 0x7fffffffL || t[i].cols > 0x7fffffffL)
+      ZB_FAIL(-1, "newton_schulz: matrix %d is %ld x %ld", i, t[i].rows, t[i].cols);
+  return 0;
+}
+
+}  // namespace zb
+
+extern "C" {
+
+// Bytes of workspace for a list (of zb_newton_schulz's table only rows and cols are looked at).
+int zb_newton_schulz_workspace(const void* table, int count, long* bytes) {
+  using namespace zb;
+  const NsMatrix* t = static_cast<const NsMatrix*>(table);
+  if (int rc = ns_check(t, count)) return rc;
+  *bytes = long(ns_plan(t, count).bytes);
+  return 0;
+}
+
+// table: `count` NsMatrix, none of them empty.  muon: p and m are stepped with lr, momentum (nesterov: the gradient looks ahead by it), the
+// gradient times grad_scale, and keep = 1 - lr weight_decay; else the orthogonalised matrices go to `out`.  a, b, c: coefficients.
+int zb_newton_schulz(const void* table, int count, int muon, float lr, float momentum, int nesterov, float keep, float grad_scale, int iterations,
+                     float a, float b, float c, void* workspace, long bytes, int* launches, int* status, cudaStream_t stream) {
+  using namespace zb;
+  const NsMatrix* t = static_cast<const NsMatrix*>(table);
+  *launches = 0;
+  if (count <= 0) return 0;
+  if (int rc = ns_check(t, count)) return rc;
+  const NsPlan plan = ns_plan(t, count);
+  if (bytes < long(plan.bytes) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    ZB_FAIL(-4, "newton_schulz: %ld bytes of workspace, %zu on a 16-byte boundary are needed", bytes, plan.bytes);
+  char* ws = static_cast<char*>(workspace);
+  NsPass pass = {};
+  pass.momentum = momentum;
+  pass.grad_scale = grad_scale;
+  pass.keep = keep;
+  pass.nesterov = nesterov;
+  pass.muon = muon;
+  int rc;
+  if ((rc = ns_pass<0>(plan, t, pass, lr, ws, 0, stream, launches))) return rc;
+  if ((rc = ns_pass<1>(plan, t, pass, lr, ws, 0, stream, launches))) return rc;
+  for (int i = 0; i < iterations; ++i) {
+    if ((rc = ns_product<NS_GRAM>(plan, ws, i & 1, a, b, c, status, stream, launches))) return rc;
+    if ((rc = ns_product<NS_POLY>(plan, ws, i & 1, a, b, c, status, stream, launches))) return rc;
+    if ((rc = ns_product<NS_APPLY>(plan, ws, i & 1, a, b, c, status, stream, launches))) return rc;
+  }
+  return ns_pass<2>(plan, t, pass, lr, ws, iterations & 1, stream, launches);
+}
+
+}  // extern "C"

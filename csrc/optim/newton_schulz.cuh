@@ -1,0 +1,315 @@
+// The products of the Newton-Schulz iterations (newton_schulz.cu): fp16 operands, fp32 sums, out = alpha (a b^T, or a b) + beta x, all
+// matrices of up to NS_GROUPS shapes in one launch.
+//
+// Persistent CTA pairs on tiles of 256 x 256, the form of the framework's bf16 product (csrc/gemm/gemm2_bf16.cu): one warp loads, one
+// issues, four take the accumulators out while the next tile is under way.
+#pragma once
+#include "../common/host.h"
+#include "../common/pair.cuh"
+#include "../common/ptx.cuh"
+#include <cuda_fp16.h>
+#include <algorithm>
+
+namespace zb {
+
+enum : int { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2 };
+constexpr int NS_GROUPS = 8;         // shapes of a launch
+constexpr float NS_A_SCALE = 64.f;   // A and B are held times this
+
+struct NsCfg {
+  static constexpr int BM = 256, BN = 256, BK = 64, HALF_N = 128;
+  static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = HALF_N * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 6, BOX_BYTES = 32 * 128, BOXES = 2;   // epilogue boxes a warp: 32 rows of 64 columns
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES + 4 * BOXES * BOX_BYTES;
+  static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 256;
+};
+
+// Matrices of one shape.  out = alpha (a b^T, or a b) + beta x
+struct alignas(64) NsGroup {
+  CUtensorMap a, b, x, c;
+  __half* out;            // of c, for the tiles that are stored turned over
+  long ld, step;          // elements from row to row and from matrix to matrix of `out`
+  int M, N, K, tiles_m, tiles;
+  int first;              // its first item
+  float alpha, beta;
+};
+struct NsParams {
+  NsGroup g[NS_GROUPS];
+  int groups, items;
+  int* status;
+};
+
+__host__ __device__ constexpr uint32_t umma_idesc_f16(int M, int N, bool a_mn_major, bool b_mn_major) {
+  return umma_idesc_bf16(M, N, a_mn_major, b_mn_major) & ~((7u << 7) | (7u << 10));   // operand types 0: fp16
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+template <int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schulz_kernel(const __grid_constant__ NsParams p) {
+  using Cfg = NsCfg;
+  constexpr bool SYM = KIND != NS_APPLY, ADD = KIND != NS_GRAM;
+  constexpr int BK = Cfg::BK, BN = Cfg::BN, STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* boxes = smem + STAGES * Cfg::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::RING_BYTES);   // the leader's are in use
+  uint64_t* empty = full + STAGES;            // each CTA waits on its own
+  uint64_t* tmem_full = empty + STAGES;       // [2], each CTA waits on its own
+  uint64_t* tmem_empty = tmem_full + 2;       // [2], the leader's, one arrival per epilogue warp of both CTAs
+  uint64_t* x_full = tmem_empty + 2;          // [4 warps][BOXES]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 4 * Cfg::BOXES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank();
+  const bool leader = cta == 0;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  WaitCtx wctx{abort_flag, p.status};
+
+  // Item -> shape, matrix, tile.  Symmetric: the tiles tn >= tm, row by row; else column by column, so that pairs at work
+  // together read few columns of the wide operand.
+  struct Item { int g, matrix, tm, tn; };
+  auto item_at = [&](int item) {
+    Item it;
+    it.g = 0;
+    while (it.g + 1 < p.groups && item >= p.g[it.g + 1].first) ++it.g;
+    const NsGroup& g = p.g[it.g];
+    int r = item - g.first;
+    it.matrix = r / g.tiles;
+    r -= it.matrix * g.tiles;
+    if (SYM) {
+      it.tm = 0;
+      for (int n = g.tiles_m; r >= n; --n) { r -= n; ++it.tm; }
+      it.tn = it.tm + r;
+    } else {
+      it.tn = r / g.tiles_m;
+      it.tm = r - it.tn * g.tiles_m;
+    }
+    return it;
+  };
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tmem_full[i], 1);
+      mbar_init(&tmem_empty[i], 8);
+    }
+    for (int i = 0; i < 4 * Cfg::BOXES; ++i) mbar_init(&x_full[i], 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  chain_wait();
+  chain_trigger();
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer (both CTAs) ------------------------------
+    const bool elected = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int item = pair; item < p.items && ok; item += num_pairs) {
+      const Item it = item_at(item);
+      const NsGroup& g = p.g[it.g];
+      const int m0 = it.tm * Cfg::BM + int(cta) * 128, n0 = it.tn * BN + int(cta) * Cfg::HALF_N;
+      if (!zb_in_bounds(it.tm * Cfg::BM < g.M && it.tn * BN < g.N, p.status, 1)) break;
+      const int num_kb = (g.K + BK - 1) / BK;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, wctx, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        uint8_t* sa = smem + stage * Cfg::STAGE_BYTES;
+        uint8_t* sb = sa + Cfg::A_BYTES;
+        if (elected) {
+          if (leader) mbar_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
+          tma_load_3d_pair(sa, &g.a, &full[stage], kb * BK, m0, it.matrix);
+          if (SYM) {
+            tma_load_3d_pair(sb, &g.b, &full[stage], kb * BK, n0, it.matrix);
+          } else {
+            tma_load_3d_pair(sb, &g.b, &full[stage], n0, kb * BK, it.matrix);
+            tma_load_3d_pair(sb + BK * 128, &g.b, &full[stage], n0 + 64, kb * BK, it.matrix);
+          }
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    // the leader's commits arrive on the barriers of both CTAs: none may be on its way to a CTA that has left
+    for (int i = 0; i < STAGES && ok; ++i) {
+      ok = mbar_wait_warp(&empty[stage], phase ^ 1, wctx, ST_TIMEOUT_EMPTY);
+      if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer (leader CTA only) ------------------------------
+    if (leader) {
+      constexpr uint32_t idesc = umma_idesc_f16(256, BN, false, !SYM);
+      const bool elected = elect_one();
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int item = pair; item < p.items && ok; item += num_pairs, ++local) {
+        const int num_kb = (p.g[item_at(item).g].K + BK - 1) / BK;
+        const int buf = local & 1;
+        ok = mbar_wait_warp(&tmem_empty[buf], (uint32_t(local >> 1) & 1) ^ 1, wctx, ST_TIMEOUT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + uint32_t(buf * BN);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait_warp(&full[stage], phase, wctx, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * Cfg::STAGE_BYTES), sb = sa + Cfg::A_BYTES;
+          if (elected) {
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk)
+              umma_f16_ss_pair(d_tmem, umma_desc_kmajor(sa + kk * 32),
+                               SYM ? umma_desc_kmajor(sb + kk * 32) : umma_desc_mnmajor(sb + kk * 16 * 128, BK * 128), idesc,
+                               kb != 0 || kk != 0 ? 1u : 0u);
+            umma_commit_pair(&empty[stage]);
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (ok && elected) umma_commit_pair(&tmem_full[buf]);
+        __syncwarp();
+      }
+      // arrivals of the second CTA's epilogue warps: those of two more tiles have landed before this CTA leaves
+      for (int i = 0; i < 2 && ok; ++i, ++local)
+        ok = mbar_wait_warp(&tmem_empty[local & 1], (uint32_t(local >> 1) & 1) ^ 1, wctx, ST_TIMEOUT_TMEM_EMPTY);
+    }
+  } else {
+    // ------------------------------ epilogue (own 128 rows) ------------------------------
+    const int q = warp & 3;
+    uint8_t* my_boxes = boxes + q * Cfg::BOXES * Cfg::BOX_BYTES;
+    uint64_t* my_full = x_full + q * Cfg::BOXES;
+    uint32_t count = 0;      // boxes of this warp so far: slot and barrier phase of the next one
+    int local = 0;
+    for (int item = pair; item < p.items; item += num_pairs, ++local) {
+      const Item it = item_at(item);
+      const NsGroup& g = p.g[it.g];
+      const int row0 = it.tm * Cfg::BM + int(cta) * 128 + q * 32, n0 = it.tn * BN;
+      const int n_boxes = row0 < g.M ? min(BN / 64, (g.N - n0 + 63) / 64) : 0;
+      const int buf = local & 1;
+      const float alpha = g.alpha, beta = g.beta;
+      auto box_of = [&](uint32_t k) { return my_boxes + (k & 1) * Cfg::BOX_BYTES; };
+      auto load_box = [&](int i) {      // lane 0
+        const uint32_t k = count + uint32_t(i);
+        mbar_expect_tx(&my_full[k & 1], Cfg::BOX_BYTES);
+        tma_load_3d(box_of(k), &g.x, &my_full[k & 1], n0 + i * 64, row0, it.matrix);
+      };
+      if (ADD && lane == 0) {
+        bulk_wait_read<0>();
+        for (int i = 0; i < Cfg::BOXES && i < n_boxes; ++i) load_box(i);
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], uint32_t(local >> 1) & 1, wctx, ST_TIMEOUT_TMEM_FULL))) break;
+      tc_fence_after();
+      auto release_tmem = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(&tmem_empty[buf], 0);
+      };
+      const bool turned = SYM && it.tm != it.tn;
+      bool ok = true;
+      if (n_boxes == 0) release_tmem();
+#pragma unroll 1
+      for (int i = 0; i < n_boxes; ++i) {
+        const uint32_t k = count + uint32_t(i);
+        const int col0 = n0 + i * 64;
+        const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + i * 64);
+        uint32_t r[32], s[32];
+        tmem_ld32(t_addr, r);
+        tmem_ld32(t_addr + 32u, s);
+        if (lane == 0) {
+          if (!ADD) {
+            bulk_wait_read<Cfg::BOXES - 1>();
+          } else if (i > 0 && i - 1 + Cfg::BOXES < n_boxes) {
+            bulk_wait_read<0>();
+            load_box(i - 1 + Cfg::BOXES);
+          }
+        }
+        tmem_wait_ld();
+        if (i == n_boxes - 1) release_tmem();
+        else __syncwarp();
+        const uint32_t row_at = smem_u32(box_of(k)) + uint32_t(lane) * 128;
+        if (ADD) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&my_full[k & 1], (k >> 1) & 1, wctx, ST_TIMEOUT_FULL));
+          if (!ok) break;
+        }
+        uint32_t o[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t at = row_at + uint32_t((j ^ (lane & 7)) << 4);
+          uint32_t x[4] = {0u, 0u, 0u, 0u};
+          if (ADD) {
+            const uint4 v = ld_shared_v4(at);
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int e = (j & 3) * 8 + 2 * u;
+            const float lo = __uint_as_float(j < 4 ? r[e] : s[e]) * alpha, hi = __uint_as_float(j < 4 ? r[e + 1] : s[e + 1]) * alpha;
+            const float2 add = ADD ? unpack_half2(x[u]) : make_float2(0.f, 0.f);
+            o[j * 4 + u] = ADD ? pack_half2(fmaf(beta, add.x, lo), fmaf(beta, add.y, hi)) : pack_half2(lo, hi);
+          }
+          st_shared_v4(at, o[j * 4], o[j * 4 + 1], o[j * 4 + 2], o[j * 4 + 3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.c, box_of(k), col0, row0, it.matrix);
+          bulk_commit();
+        }
+        if (turned) {
+          // Two lanes trade halves, so that each has two rows of one column: 64 bytes of a row of the turned tile a store.  (For an odd
+          // M the last pair reaches one element into the row's padding.)
+          const int row = row0 + (lane & ~1);
+          __half* to = g.out + size_t(it.matrix) * g.step + size_t(col0 + (lane & 1)) * g.ld + row;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, o[j], 1);
+            const uint32_t v = lane & 1 ? __byte_perm(other, o[j], 0x7632) : __byte_perm(o[j], other, 0x5410);
+            if (row < g.M && col0 + 2 * j + (lane & 1) < g.N) *reinterpret_cast<uint32_t*>(to + size_t(2 * j) * g.ld) = v;
+          }
+        }
+      }
+      count += uint32_t(n_boxes);
+      if (!ok) break;
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) {
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // (what was sent to the other CTA's barriers has been waited for)
+  if (warp >= 2 && lane == 0) bulk_wait_read<0>();
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+template <int KIND>
+inline int ns_launch(const NsParams& p, cudaStream_t stream) {
+  static SharedLimit limit;
+  ZB_CUDA_OK(limit.raise(newton_schulz_kernel<KIND>, NsCfg::SMEM_BYTES));
+  const int pairs = std::min(num_sms() / 2, p.items);
+  ZB_CUDA_OK(launch_chained(newton_schulz_kernel<KIND>, dim3(2 * pairs), 192, NsCfg::SMEM_BYTES, stream, 0, p));
+  return 0;
+}
+
+}  // namespace zb

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import torch
 
-from . import packed, ref
+from . import muon, packed, ref
 from .moments import decode
 
 _ACT_KINDS = {"gelu": 0, "gelu_new": 0, "gelu_tanh": 0, "relu": 1, "gelu_erf": 2}
@@ -227,6 +227,18 @@ class RefOps(_EpilogueOps, _LaterOps):
     def moment_values(self, moments, dtype=torch.float32):
         return tuple(t.to(dtype) for t in decode(moments))
 
+    def orthogonalize(self, mats, iterations=5):
+        """The matrices with their singular values driven to about 1 by Newton-Schulz products (a list; in bf16 where they are computed by the kernels)."""
+        return [muon.orthogonalize(u, iterations) for u in mats]
+
+    def muon_step(self, p, m, g, p16, *, lr, momentum=0.95, weight_decay=0.0, nesterov=True, iterations=5, grad_scale=1.0):
+        """Muon over lists of weight matrices and their momenta."""
+        for x, mom, d, y in zip(p, m, g, p16):
+            muon.muon_step(x, mom, d, lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, iterations=iterations,
+                           grad_scale=grad_scale)
+            if y is not None:
+                y.copy_(x)
+
 
 def _decline(*args):
     """Stands for a native call that is switched off: as if it had declined its arguments."""
@@ -408,6 +420,12 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
 
     def moment_values(self, moments, dtype=torch.float32):
         return self.k.moment_values(moments, dtype)
+
+    def orthogonalize(self, mats, iterations=5):
+        return self.k.orthogonalize(mats, iterations)
+
+    def muon_step(self, p, m, g, p16, **kw):
+        self.k.muon_step(p, m, g, p16, **kw)
 
 
 _cache: dict[str, object] = {}

@@ -22,6 +22,7 @@ from typing import Optional
 import torch
 
 from .moments import BLOCK as MOMENT_BLOCK
+from .muon import COEFFICIENTS as NEWTON_SCHULZ
 from .packed import MOST_AXES, MOST_TOKENS, PackedSequences, check_window
 
 _LIB_PATH = Path(__file__).resolve().parents[1] / "_C" / "libzorse_sm100.so"
@@ -56,7 +57,7 @@ _SIGNATURES = {
     "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
     "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
     "zb_pack_sequences": "piipppppp", "zb_packed_attn_fwd": "pppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
-    "zb_rope_at": "ppppiiiiilip",
+    "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pip", "zb_newton_schulz": "piiffiffifffplppp",
     "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
 _CTYPES = {"p": c_void_p, "i": c_int, "l": c_long, "f": c_float}
@@ -612,6 +613,89 @@ def moment_values(moments, dtype=torch.float32):
     _check(lib().zb_moment_values(_a(m), _a(mb), _a(v), _a(vb), _a(out[0]), _a(out[1]), n, int(dtype == torch.float32), _stream()),
            "moment_values")
     return out
+
+
+# Matrices of a list are taken together as far as their workspace (8 bytes an element, 4 a pair of rows of the short side) stays below this:
+# enough tiles for many waves.
+NEWTON_SCHULZ_BYTES = 1 << 30
+
+
+def _newton_schulz(table, muon: bool, iterations: int, dev, lr=0.0, momentum=0.0, nesterov=False, keep=1.0, grad_scale=1.0) -> None:
+    """table: (p, m, g, out, rows, cols, g in fp32) of matrices that have elements."""
+    _need(isinstance(iterations, int) and 1 <= iterations <= 100, f"{iterations} iterations: 1 to 100")
+    chunks, room = [], 0
+    for t in table:
+        n, k = min(t[4:6]), max(t[4:6])
+        size = 4 * n * (k + 8) + 4 * n * (n + 8) + 8192
+        if not chunks or size > room:
+            chunks.append([])
+            room = NEWTON_SCHULZ_BYTES
+        chunks[-1].append(t)
+        room -= size
+    packed = [struct.pack("4Q2q2i" * len(c), *(x for t in c for x in (*t, 0))) for c in chunks]
+    L, launches = lib(), c_int(0)
+    sizes = [_workspace_size(L.zb_newton_schulz_workspace, data, len(c)) for data, c in zip(packed, chunks)]
+    if not sizes:
+        return
+    ws = torch.empty(max(sizes), dtype=torch.uint8, device=dev)
+    global _launches
+    for data, c in zip(packed, chunks):
+        _check(L.zb_newton_schulz(data, len(c), int(muon), lr, momentum, int(nesterov), keep, grad_scale, iterations, *NEWTON_SCHULZ, _a(ws),
+                                  ws.numel(), ctypes.addressof(launches), _a(status_word(dev)), _stream()), "newton_schulz")
+        _launches += launches.value - 1
+
+
+def _matrix(t, name: str, dtypes, dev, shape=None) -> None:
+    _need(t.dim() == 2 and t.is_contiguous() and t.dtype in dtypes and t.device == dev and (shape is None or t.shape == shape) and max(t.shape) < 2 ** 31,
+          f"{name} {tuple(t.shape)}, {t.dtype} on {t.device}: expected a contiguous matrix{'' if shape is None else f' {tuple(shape)}'} on {dev} "
+          f"of {' or '.join(str(d) for d in dtypes)}")
+
+
+def orthogonalize(mats, iterations: int = 5) -> list:
+    """Newton-Schulz products on a list of matrices (fp32 or bf16, each): what `ops/muon.py` has the formula of, in bf16."""
+    out = []
+    if len(mats) == 0:
+        return out
+    dev, table = mats[0].device, []
+    _on_current(mats[0], "mats")
+    for i, u in enumerate(mats):
+        _matrix(u, f"mats[{i}]", (torch.float32, torch.bfloat16), dev)
+        out.append(torch.empty(u.shape, dtype=torch.bfloat16, device=dev))
+        if u.numel():
+            table.append((0, 0, u.data_ptr(), out[-1].data_ptr(), *u.shape, int(u.dtype == torch.float32)))
+    _newton_schulz(table, False, iterations, dev)
+    return out
+
+
+def muon_step(p, m, g, p16, *, lr: float, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True, iterations: int = 5,
+              grad_scale: float = 1.0) -> None:
+    """Muon over lists of weight matrices: p and momentum m (fp32), gradients g (fp32 or bf16, scaled by grad_scale first), p16: the copies in
+    bf16 to refresh, or None for a matrix that has none."""
+    n = len(p)
+    _need(len(m) == n and len(g) == n and len(p16) == n, f"lists of {n}, {len(m)}, {len(g)} and {len(p16)} matrices")
+    _need(0 <= momentum < 1, f"momentum {momentum} is not in [0, 1)")
+    if n == 0:
+        return
+    dev = p[0].device
+    _on_current(p[0], "p")
+    table, written, read = [], [], []
+    for i, (x, mom, d, y) in enumerate(zip(p, m, g, p16)):
+        _matrix(x, f"p[{i}]", (torch.float32,), dev)
+        _matrix(mom, f"m[{i}]", (torch.float32,), dev, x.shape)
+        _matrix(d, f"g[{i}]", (torch.float32, torch.bfloat16), dev, x.shape)
+        if y is not None:
+            _matrix(y, f"p16[{i}]", (torch.bfloat16,), dev, x.shape)
+        if x.numel() == 0:
+            continue
+        written += [(*_stretch(t), i) for t in (x, mom, y) if t is not None]
+        read.append((*_stretch(d), i))
+        table.append((x.data_ptr(), mom.data_ptr(), d.data_ptr(), _a(y), *x.shape, int(d.dtype == torch.float32)))
+    written.sort()
+    _need(all(a[1] <= b[0] for a, b in zip(written, written[1:])), "matrices that the step writes overlap (one is in the list twice?)")
+    for lo, hi, i in read:       # (read by two passes, with the momentum's writes in between)
+        at = bisect.bisect_left(written, (lo + 1,)) - 1
+        _need((at < 0 or written[at][1] <= lo) and (at + 1 == len(written) or written[at + 1][0] >= hi), f"g[{i}] overlaps a matrix that the step writes")
+    _newton_schulz(table, True, iterations, dev, lr, momentum, nesterov, 1 - lr * weight_decay, grad_scale)
 
 
 # --------------------------------------------------------------------------- attention
