@@ -83,9 +83,10 @@ inline int make_tmap_2d_out(CUtensorMap* out, const void* base, uint64_t rows, u
   return 0;
 }
 
-// General N-d bf16 tensor map (innermost dimension first), 128-byte swizzle.
+// General N-d tensor map of a 16-bit type (innermost dimension first), 128-byte swizzle unless named.
 inline int make_tmap_nd_bf16(CUtensorMap* out, const void* base, int rank, const uint64_t* dims,
-                             const uint64_t* strides_bytes /* rank-1 */, const uint32_t* box) {
+                             const uint64_t* strides_bytes /* rank-1 */, const uint32_t* box,
+                             CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) ZB_FAIL(-3, "cuTensorMapEncodeTiled entry point not available");
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) ZB_FAIL(-4, "TMA base not 16-byte aligned");
@@ -102,7 +103,7 @@ inline int make_tmap_nd_bf16(CUtensorMap* out, const void* base, int rank, const
     }
   }
   CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, e,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) ZB_FAIL(-5, "cuTensorMapEncodeTiled failed with %d", int(r));
   return 0;

@@ -6,12 +6,12 @@
 // are symmetric, so only their tiles on and above the diagonal are formed and every other one is stored a second time, turned
 // over: 2 n^2 m + n^3 / 2 ... n^2 m + n^3 + 2 n^2 m floating-point operations instead of 4 n^2 m + 2 n^3.
 //
-// Every matrix of the list takes part in each launch: those of one shape lie one behind the other in the workspace behind one tensor
+// Every matrix of the list takes part in each launch: those of one shape lie one behind the other in the workspace under one tensor
 // map, and the tiles of up to GROUPS shapes are dealt to persistent CTA pairs.  A model's matrices of 512 to 1024 columns have 3 to 10
 // tiles each, one by one a launch would leave most of the GPU idle.
 //
 // Operands are fp16, sums fp32 in tensor memory.  All values are bounded (singular values stay below 1.21), so the range of bf16 is
-// not needed and its eight bits would cost: relative error of X after five iterations 1.0e-2 with bf16 and 1.3e-3 with fp16 (512 x
+// not needed and its eight bits would cost: relative error of X after five iterations 1.0e-2 with bf16 and 1.0e-3 with fp16 (512 x
 // 512 to 1024 x 1024, noise and few strong directions alike).  X is held times 2^round(log2(sqrt m)), so its entries are near 1 at the end,
 // A and B times 64, so that what the first iteration's small values round to stays far below what they add.
 //
@@ -26,6 +26,8 @@
 #include <vector>
 
 namespace zb {
+
+constexpr float NS_A_SCALE = 64.f;   // what is n x n is held times this
 
 // --------------------------------------------------------------------------------------------- passes before and behind
 constexpr int NS_MATRICES = 64;      // of a launch of a pass
@@ -148,12 +150,16 @@ __global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ Ns
 }
 
 // Tiles of 64 x 64: the update times scale / norm in fp16, turned over where the matrix has more rows than columns.
-__global__ void __launch_bounds__(256) ns_scale_kernel(const __grid_constant__ NsPass a) {
+__global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant__ NsPass a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
   const int tile = int(blockIdx.x) - t.first, r0 = tile / t.tiles_c * 64, c0 = tile % t.tiles_c * 64;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = c0 + tx * 4;
+  double s = 0.0;      // every warp adds the parts up for itself
+#pragma unroll
+  for (int i = 0; i < NS_PARTS; i += 32)
+    if (i + int(threadIdx.x & 31) < t.parts) s += t.sums[i + (threadIdx.x & 31)];
   float u[4][4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -179,23 +185,20 @@ __global__ void __launch_bounds__(256) ns_scale_kernel(const __grid_constant__ N
       }
     }
   }
-  __shared__ double sums[8];
-  double s = int(threadIdx.x) < t.parts ? t.sums[threadIdx.x] : 0.0;
+  // scale / norm as a power of two and the rest, either of which fp32 holds for any norm; NaN and infinite norms give NaN
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = 0.0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s += sums[i];
+  int e = 0;
   const double by = s == 0.0 ? 0.0 : double(t.scale) / sqrt(s);
+  const float low = float(frexp(by, &e) * 2.0);
+  const float half = exp2f(float((e - 1) / 2)), rest = exp2f(float(e - 1 - (e - 1) / 2)) * low;
   __shared__ float tile_s[64][65];
   const bool turned = t.rows > t.cols;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int r = r0 + ty + 16 * k;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[k][j] = float(double(u[k][j]) * by);
+    for (int j = 0; j < 4; ++j) u[k][j] = u[k][j] * half * rest;
     if (turned) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) tile_s[ty + 16 * k][tx * 4 + j] = u[k][j];
@@ -277,15 +280,17 @@ __global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ N
 }
 
 // ------------------------------------------------------------------------------------------------------------ the list
+enum : int { NS_X0 = 0, NS_X1 = 1, NS_A = 2, NS_B = 3, NS_BUFFERS = 4 };   // X in turns, and what is n x n
+
 struct NsShape {
   long n, m;                       // short and long side
   std::vector<int> members;        // of the list
-  size_t x[2], a, b;               // places in the workspace
-  long np() const { return (n + 7) / 8 * 8; }
-  long mp() const { return (m + 7) / 8 * 8; }
+  size_t at[NS_BUFFERS];           // places in the workspace
+  long ld(int buffer) const { return ((buffer < NS_A ? m : n) + 7) / 8 * 8; }
+  long cols(int buffer) const { return buffer < NS_A ? m : n; }
 };
 struct NsPlan {
-  std::vector<NsShape> shapes;     // the one with the longest products first: the last wave of a launch is then of short ones
+  std::vector<NsShape> shapes;     // long sides first
   std::vector<size_t> sums;        // of each matrix
   std::vector<int> parts;
   size_t bytes = 0;
@@ -301,16 +306,12 @@ static NsPlan ns_plan(const NsMatrix* t, int count) {
   for (int i = 0; i < count; ++i) {
     const long n = std::min(t[i].rows, t[i].cols), m = std::max(t[i].rows, t[i].cols);
     auto s = std::find_if(plan.shapes.begin(), plan.shapes.end(), [&](const NsShape& x) { return x.n == n && x.m == m; });
-    if (s == plan.shapes.end()) s = plan.shapes.insert(s, NsShape{n, m, {}, {0, 0}, 0, 0});
+    if (s == plan.shapes.end()) s = plan.shapes.insert(s, NsShape{n, m, {}, {}});
     s->members.push_back(i);
   }
   std::stable_sort(plan.shapes.begin(), plan.shapes.end(), [](const NsShape& a, const NsShape& b) { return a.m > b.m; });
-  for (NsShape& s : plan.shapes) {
-    const size_t k = s.members.size();
-    for (size_t& x : s.x) x = take(k * s.n * s.mp() * 2);
-    s.a = take(k * s.n * s.np() * 2);
-    s.b = take(k * s.n * s.np() * 2);
-  }
+  for (NsShape& s : plan.shapes)
+    for (int i = 0; i < NS_BUFFERS; ++i) s.at[i] = take(s.members.size() * s.n * s.ld(i) * 2);
   for (int i = 0; i < count; ++i) {
     const long parts = (t[i].rows * t[i].cols + 4095) / 4096;
     plan.parts.push_back(int(std::min<long>(parts, NS_PARTS)));
@@ -319,71 +320,95 @@ static NsPlan ns_plan(const NsMatrix* t, int count) {
   return plan;
 }
 
-// 3-D map of `count` matrices [rows, cols], ld elements a row (16-bit types are alike here); box: box_rows rows of 64 columns.
-static int ns_map(CUtensorMap* out, const void* base, long rows, long cols, long ld, long count, uint32_t box_rows) {
-  const uint64_t dims[3] = {uint64_t(cols), uint64_t(rows), uint64_t(count)};
-  const uint64_t strides[2] = {uint64_t(ld) * 2, uint64_t(rows) * ld * 2};
-  const uint32_t box[3] = {64, box_rows, 1};
-  return make_tmap_nd_bf16(out, base, 3, dims, strides, box);
-}
-
 static float ns_scale(long m) { return exp2f(float(std::min(13l, std::lround(0.5 * std::log2(double(m)))))); }
 
-template <int KIND>
-static int ns_product(const NsPlan& plan, char* ws, int from, float a, float b, float c, int* status, cudaStream_t stream, int* launches) {
-  for (size_t first = 0; first < plan.shapes.size(); first += NS_GROUPS) {
-    NsParams p = {};
-    p.status = status;
-    for (size_t i = first; i < std::min(first + NS_GROUPS, plan.shapes.size()); ++i) {
-      const NsShape& s = plan.shapes[i];
-      NsGroup& g = p.g[p.groups++];
-      const long k = long(s.members.size()), np = s.np(), mp = s.mp();
-      const float scale = ns_scale(s.m);
-      char *x = ws + s.x[from], *y = ws + s.x[1 - from], *ga = ws + s.a, *gb = ws + s.b;
-      int rc = 0;
-      if (KIND == NS_GRAM) {
-        rc = ns_map(&g.a, x, s.n, s.m, mp, k, 128) | ns_map(&g.c, ga, s.n, s.n, np, k, 32);
-        g.b = g.a;
-        g.x = g.c;
-        g.out = reinterpret_cast<__half*>(ga);
-        g.K = int(s.m);
-        g.alpha = NS_A_SCALE / (scale * scale);
-      } else if (KIND == NS_POLY) {
-        rc = ns_map(&g.a, ga, s.n, s.n, np, k, 128) | ns_map(&g.x, ga, s.n, s.n, np, k, 32) | ns_map(&g.c, gb, s.n, s.n, np, k, 32);
-        g.b = g.a;
-        g.out = reinterpret_cast<__half*>(gb);
-        g.K = int(s.n);
-        g.alpha = c / NS_A_SCALE;
-        g.beta = b;
-      } else {
-        rc = ns_map(&g.a, gb, s.n, s.n, np, k, 128) | ns_map(&g.b, x, s.n, s.m, mp, k, 64) | ns_map(&g.x, x, s.n, s.m, mp, k, 32) |
-             ns_map(&g.c, y, s.n, s.m, mp, k, 32);
-        g.K = int(s.n);
-        g.alpha = 1.f / NS_A_SCALE;
-        g.beta = a;
-      }
-      if (rc) return -5;
-      g.M = int(s.n);
-      g.N = int(KIND == NS_APPLY ? s.m : s.n);
-      g.ld = np;
-      g.step = s.n * np;
-      g.tiles_m = (g.M + NsCfg::BM - 1) / NsCfg::BM;
-      const long tn = (g.N + NsCfg::BN - 1) / NsCfg::BN;
-      const long tiles = KIND == NS_APPLY ? g.tiles_m * tn : long(g.tiles_m) * (g.tiles_m + 1) / 2;
-      if (p.items + tiles * k > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: matrices of %ld x %ld", s.n, s.m);
-      g.tiles = int(tiles);
-      g.first = p.items;
-      p.items += int(tiles * k);
+// out = alpha P P^T + beta R + diag I (symmetric), or alpha P X + beta R; numbers of buffers, add < 0: no R.
+struct NsStep {
+  bool symmetric;
+  int p, q, add, out;
+  float alpha, beta, diag;
+};
+// Launch by launch.  B goes with 2 I added and X with a - 2: once singular values are near 1, B is nearly -2.7 I, most of which a takes
+// away again, rounding errors excepted.  (1.43e-3 -> 0.95e-3 for 512 x 1376 noise, 1.64e-3 -> 0.69e-3 for 8 x 600, never more.)  (Two iterations of long matrices taken as one, X2 = q(A1) q(A) X0 with A1 = q(A) A q(A), save 3 n^2 m - 3 n^3 operations,
+// but q(A1) q(A) is 11.9 I less as much along a direction that holds most of a matrix: 1.4e-2 of a matrix of ones instead of 1e-4.)
+static std::vector<NsStep> ns_program(int iterations, float a, float b, float c) {
+  std::vector<NsStep> steps;
+  for (int i = 0, x = NS_X0; i < iterations; ++i, x = 1 - x) {
+    steps.push_back({true, x, x, -1, NS_A, 1.f, 0.f, 0.f});
+    steps.push_back({true, NS_A, NS_A, NS_A, NS_B, c, b, 2.f});
+    steps.push_back({false, NS_B, x, x, 1 - x, 1.f, a - 2.f, 0.f});
+  }
+  return steps;
+}
+
+// The maps of a shape's buffers, made when first asked for: boxes of `rows` rows of 64 columns, or (rows 0) of 64 rows of 32.
+struct NsMaps {
+  CUtensorMap map[NS_BUFFERS][4];
+  bool made[NS_BUFFERS][4] = {};
+  int get(CUtensorMap* out, const NsShape& s, char* ws, int buffer, uint32_t rows) {
+    const int i = rows == 128 ? 0 : rows == 64 ? 1 : rows == 32 ? 2 : 3;
+    if (!made[buffer][i]) {
+      const uint64_t dims[3] = {uint64_t(s.cols(buffer)), uint64_t(s.n), s.members.size()};
+      const uint64_t strides[2] = {uint64_t(s.ld(buffer)) * 2, uint64_t(s.n * s.ld(buffer)) * 2};
+      const uint32_t box[3] = {rows ? 64u : 32u, rows ? rows : 64u, 1};
+      if (int rc = make_tmap_nd_bf16(&map[buffer][i], ws + s.at[buffer], 3, dims, strides, box,
+                                     rows ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE))
+        return rc;
+      made[buffer][i] = true;
     }
-    if (int rc = ns_launch<KIND>(p, stream)) return rc;
-    ++*launches;
+    *out = map[buffer][i];
+    return 0;
+  }
+};
+
+static int ns_products(const NsPlan& plan, char* ws, const std::vector<NsStep>& program, int* status, cudaStream_t stream, int* launches) {
+  std::vector<NsMaps> maps(plan.shapes.size());
+  std::vector<size_t> order(plan.shapes.size());
+  for (const NsStep& e : program) {
+    for (size_t i = 0; i < order.size(); ++i) order[i] = i;
+    // the longest reductions first: the last wave of a launch is then of short ones
+    std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return plan.shapes[i].cols(e.p) > plan.shapes[j].cols(e.p); });
+    for (size_t first = 0; first < order.size(); first += NS_GROUPS) {
+      NsParams p;
+      p.status = status;
+      p.groups = p.items = 0;
+      for (size_t k = first; k < std::min(first + NS_GROUPS, order.size()); ++k) {
+        const NsShape& s = plan.shapes[order[k]];
+        NsMaps& m = maps[order[k]];
+        NsGroup& g = p.g[p.groups++];
+        int rc = m.get(&g.a, s, ws, e.p, 128);
+        if (!rc) rc = m.get(&g.b, s, ws, e.q, e.symmetric ? 128 : 64);
+        if (!rc) rc = m.get(&g.c, s, ws, e.out, 32);
+        if (!rc) rc = m.get(&g.x, s, ws, e.add >= 0 ? e.add : e.out, 32);
+        if (!rc && e.symmetric) rc = m.get(&g.t, s, ws, e.out, 0);
+        if (rc) return rc;
+        const float scale = ns_scale(s.m);
+        g.symmetric = e.symmetric;
+        g.M = int(s.n);
+        g.N = int(s.cols(e.out));
+        g.K = int(s.cols(e.p));
+        g.alpha = e.alpha * (e.p < NS_A ? NS_A_SCALE / (scale * scale) : 1.f / NS_A_SCALE);
+        g.beta = e.beta;
+        g.diag = e.diag * NS_A_SCALE;
+        g.tiles_m = (g.M + NsCfg::BM - 1) / NsCfg::BM;
+        const long columns = (g.N + NsCfg::BN - 1) / NsCfg::BN, count = long(s.members.size());
+        const long tiles = e.symmetric ? long(g.tiles_m) * (g.tiles_m + 1) / 2 : g.tiles_m * columns;
+        if (p.items + tiles * count > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: %ld matrices of %ld x %ld", count, s.n, s.m);
+        g.tiles = int(tiles);
+        g.first = p.items;
+        p.items += int(tiles * count);
+      }
+      p.stages = p.g[0].K >= NsCfg::LONG_K ? 6 : 5;
+      if (int rc = ns_launch(p, stream)) return rc;
+      ++*launches;
+    }
   }
   return 0;
 }
 
 // One of the passes over all matrices; PASS 0: sums, 1: scale, 2: apply.
 template <int PASS>
-static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, float lr, char* ws, int last, cudaStream_t stream, int* launches) {
+static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, float lr, char* ws, int x, cudaStream_t stream, int* launches) {
   NsPass a = common;
   a.count = 0;
   long blocks = 0;
@@ -408,9 +433,9 @@ static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, 
       e.m = t[i].m;
       e.g = t[i].g;
       e.out = t[i].out;
-      e.x = reinterpret_cast<__half*>(ws + s.x[PASS == 2 ? last : 0]) + k * s.n * s.mp();
+      e.x = reinterpret_cast<__half*>(ws + s.at[x]) + k * s.n * s.ld(NS_X0);
       e.sums = reinterpret_cast<double*>(ws + plan.sums[i]);
-      e.ld = s.mp();
+      e.ld = s.ld(NS_X0);
       e.rows = int(t[i].rows);
       e.cols = int(t[i].cols);
       e.parts = plan.parts[i];
@@ -469,15 +494,10 @@ int zb_newton_schulz(const void* table, int count, int muon, float lr, float mom
   pass.keep = keep;
   pass.nesterov = nesterov;
   pass.muon = muon;
-  int rc;
-  if ((rc = ns_pass<0>(plan, t, pass, lr, ws, 0, stream, launches))) return rc;
-  if ((rc = ns_pass<1>(plan, t, pass, lr, ws, 0, stream, launches))) return rc;
-  for (int i = 0; i < iterations; ++i) {
-    if ((rc = ns_product<NS_GRAM>(plan, ws, i & 1, a, b, c, status, stream, launches))) return rc;
-    if ((rc = ns_product<NS_POLY>(plan, ws, i & 1, a, b, c, status, stream, launches))) return rc;
-    if ((rc = ns_product<NS_APPLY>(plan, ws, i & 1, a, b, c, status, stream, launches))) return rc;
-  }
-  return ns_pass<2>(plan, t, pass, lr, ws, iterations & 1, stream, launches);
+  int rc = ns_pass<0>(plan, t, pass, lr, ws, NS_X0, stream, launches);
+  if (!rc) rc = ns_pass<1>(plan, t, pass, lr, ws, NS_X0, stream, launches);
+  if (!rc) rc = ns_products(plan, ws, ns_program(iterations, a, b, c), status, stream, launches);
+  return rc ? rc : ns_pass<2>(plan, t, pass, lr, ws, iterations & 1 ? NS_X1 : NS_X0, stream, launches);
 }
 
 }  // extern "C"

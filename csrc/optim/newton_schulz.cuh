@@ -1,8 +1,14 @@
-// The products of the Newton-Schulz iterations (newton_schulz.cu): fp16 operands, fp32 sums, out = alpha (a b^T, or a b) + beta x, all
-// matrices of up to NS_GROUPS shapes in one launch.
+// The products of the Newton-Schulz iterations (newton_schulz.cu): fp16 operands, fp32 sums, all matrices of up to NS_GROUPS shapes in one
+// launch.  Two forms, by shape:
+//     symmetric   out = alpha P P^T + beta R + diag I
+//     plain       out = alpha P X + beta R            P symmetric, X [n, m]
+// Of a symmetric result only the tiles on and above the diagonal are formed; the others are stored as well, turned over.
 //
 // Persistent CTA pairs on tiles of 256 x 256, the form of the framework's bf16 product (csrc/gemm/gemm2_bf16.cu): one warp loads, one
-// issues, four take the accumulators out while the next tile is under way.
+// issues, eight take the accumulators out while the next tile is under way, in boxes of 32 rows and 64 columns through shared memory.  A warp has
+// at most two boxes of a tile, so what is added to them (R) is asked for before the accumulators are complete.  With four warps,
+// boxes loaded two at a time and the turned tiles stored from registers a tile took 14 us (26 thousand clocks) to leave, more than the
+// 8 thousand of a reduction of 1024.
 #pragma once
 #include "../common/host.h"
 #include "../common/pair.cuh"
@@ -12,30 +18,34 @@
 
 namespace zb {
 
-enum : int { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2 };
 constexpr int NS_GROUPS = 8;         // shapes of a launch
-constexpr float NS_A_SCALE = 64.f;   // A and B are held times this
 
 struct NsCfg {
   static constexpr int BM = 256, BN = 256, BK = 64, HALF_N = 128;
   static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = HALF_N * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 6, BOX_BYTES = 32 * 128, BOXES = 2;   // epilogue boxes a warp: 32 rows of 64 columns
-  static constexpr int RING_BYTES = STAGES * STAGE_BYTES + 4 * BOXES * BOX_BYTES;
-  static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 256;
+  // Shared memory is split at launch: a second box for each epilogue warp, or a sixth stage for long reductions, under which the
+  // epilogue has time.
+  static constexpr int EP_WARPS = 8, BOX_BYTES = 32 * 128, MAX_STAGES = 6;
+  static constexpr int RING_BYTES = MAX_STAGES * STAGE_BYTES + EP_WARPS * BOX_BYTES;
+  static constexpr int LONG_K = 2048;
+  static_assert(STAGE_BYTES == EP_WARPS * BOX_BYTES, "a stage makes room for a box a warp");
+  static constexpr int SMEM_BYTES = RING_BYTES + 1024 + 512;
+  static constexpr int THREADS = 64 + 32 * EP_WARPS;
 };
 
-// Matrices of one shape.  out = alpha (a b^T, or a b) + beta x
+// Matrices of one shape.
 struct alignas(64) NsGroup {
-  CUtensorMap a, b, x, c;
-  __half* out;            // of c, for the tiles that are stored turned over
-  long ld, step;          // elements from row to row and from matrix to matrix of `out`
+  CUtensorMap a, b;       // operands: boxes of 128 rows (plain: b's of 64 rows of the reduction)
+  CUtensorMap x, c, t;    // R, the result, and the result in boxes of 64 rows and 32 columns for turned tiles
   int M, N, K, tiles_m, tiles;
+  int symmetric;
   int first;              // its first item
-  float alpha, beta;
+  float alpha, beta, diag;
 };
 struct NsParams {
   NsGroup g[NS_GROUPS];
   int groups, items;
+  int stages;             // 6 with one box a warp, 5 with two
   int* status;
 };
 
@@ -48,20 +58,19 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-template <int KIND>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schulz_kernel(const __grid_constant__ NsParams p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) newton_schulz_kernel(const __grid_constant__ NsParams p) {
   using Cfg = NsCfg;
-  constexpr bool SYM = KIND != NS_APPLY, ADD = KIND != NS_GRAM;
-  constexpr int BK = Cfg::BK, BN = Cfg::BN, STAGES = Cfg::STAGES;
+  constexpr int BK = Cfg::BK, BN = Cfg::BN, EP_WARPS = Cfg::EP_WARPS;
+  const int STAGES = p.stages, BOXES = Cfg::MAX_STAGES + 1 - STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* boxes = smem + STAGES * Cfg::STAGE_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::RING_BYTES);   // the leader's are in use
-  uint64_t* empty = full + STAGES;            // each CTA waits on its own
-  uint64_t* tmem_full = empty + STAGES;       // [2], each CTA waits on its own
+  uint64_t* empty = full + Cfg::MAX_STAGES;   // each CTA waits on its own
+  uint64_t* tmem_full = empty + Cfg::MAX_STAGES;   // [2], each CTA waits on its own
   uint64_t* tmem_empty = tmem_full + 2;       // [2], the leader's, one arrival per epilogue warp of both CTAs
-  uint64_t* x_full = tmem_empty + 2;          // [4 warps][BOXES]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 4 * Cfg::BOXES);
+  uint64_t* x_full = tmem_empty + 2;          // [EP_WARPS][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + EP_WARPS * 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -81,7 +90,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
     int r = item - g.first;
     it.matrix = r / g.tiles;
     r -= it.matrix * g.tiles;
-    if (SYM) {
+    if (g.symmetric) {
       it.tm = 0;
       for (int n = g.tiles_m; r >= n; --n) { r -= n; ++it.tm; }
       it.tn = it.tm + r;
@@ -100,9 +109,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tmem_full[i], 1);
-      mbar_init(&tmem_empty[i], 8);
+      mbar_init(&tmem_empty[i], 2 * EP_WARPS);
     }
-    for (int i = 0; i < 4 * Cfg::BOXES; ++i) mbar_init(&x_full[i], 1);
+    for (int i = 0; i < EP_WARPS * 2; ++i) mbar_init(&x_full[i], 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -125,6 +134,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
     for (int item = pair; item < p.items && ok; item += num_pairs) {
       const Item it = item_at(item);
       const NsGroup& g = p.g[it.g];
+      const bool sym = g.symmetric != 0;
       const int m0 = it.tm * Cfg::BM + int(cta) * 128, n0 = it.tn * BN + int(cta) * Cfg::HALF_N;
       if (!zb_in_bounds(it.tm * Cfg::BM < g.M && it.tn * BN < g.N, p.status, 1)) break;
       const int num_kb = (g.K + BK - 1) / BK;
@@ -135,7 +145,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
         if (elected) {
           if (leader) mbar_expect_tx(&full[stage], 2 * Cfg::STAGE_BYTES);
           tma_load_3d_pair(sa, &g.a, &full[stage], kb * BK, m0, it.matrix);
-          if (SYM) {
+          if (sym) {
             tma_load_3d_pair(sb, &g.b, &full[stage], kb * BK, n0, it.matrix);
           } else {
             tma_load_3d_pair(sb, &g.b, &full[stage], n0, kb * BK, it.matrix);
@@ -154,13 +164,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
   } else if (warp == 1) {
     // ------------------------------ MMA issuer (leader CTA only) ------------------------------
     if (leader) {
-      constexpr uint32_t idesc = umma_idesc_f16(256, BN, false, !SYM);
       const bool elected = elect_one();
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int item = pair; item < p.items && ok; item += num_pairs, ++local) {
-        const int num_kb = (p.g[item_at(item).g].K + BK - 1) / BK;
+        const NsGroup& g = p.g[item_at(item).g];
+        const int num_kb = (g.K + BK - 1) / BK;
+        // b: rows of the tile with the reduction inside a row, or rows of the reduction (16 of them a product, 128 bytes apart, and
+        // 64-column blocks behind one another)
+        const bool sym = g.symmetric != 0;
+        const uint32_t idesc = sym ? umma_idesc_f16(256, BN, false, false) : umma_idesc_f16(256, BN, false, true);
+        const uint32_t b_step = sym ? 32u : 16u * 128u, b_lbo = sym ? 16u : uint32_t(BK * 128);
         const int buf = local & 1;
         ok = mbar_wait_warp(&tmem_empty[buf], (uint32_t(local >> 1) & 1) ^ 1, wctx, ST_TIMEOUT_TMEM_EMPTY);
         if (!ok) break;
@@ -173,8 +188,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
           if (elected) {
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk)
-              umma_f16_ss_pair(d_tmem, umma_desc_kmajor(sa + kk * 32),
-                               SYM ? umma_desc_kmajor(sb + kk * 32) : umma_desc_mnmajor(sb + kk * 16 * 128, BK * 128), idesc,
+              umma_f16_ss_pair(d_tmem, umma_desc_kmajor(sa + kk * 32), umma_desc_sw128(sb + kk * b_step, b_lbo, 1024), idesc,
                                kb != 0 || kk != 0 ? 1u : 0u);
             umma_commit_pair(&empty[stage]);
           }
@@ -190,27 +204,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
     }
   } else {
     // ------------------------------ epilogue (own 128 rows) ------------------------------
-    const int q = warp & 3;
-    uint8_t* my_boxes = boxes + q * Cfg::BOXES * Cfg::BOX_BYTES;
-    uint64_t* my_full = x_full + q * Cfg::BOXES;
-    uint32_t count = 0;      // boxes of this warp so far: slot and barrier phase of the next one
+    const int q = warp & 3, h = (warp - 2) >> 2;     // which 32 rows; boxes h and h + 2 of a tile
+    uint8_t* my_boxes = boxes + (warp - 2) * BOXES * Cfg::BOX_BYTES;
+    uint64_t* my_full = x_full + (warp - 2) * 2;
+    uint32_t phases = 0;     // bit u: phase of my_full[u]
     int local = 0;
     for (int item = pair; item < p.items; item += num_pairs, ++local) {
       const Item it = item_at(item);
       const NsGroup& g = p.g[it.g];
       const int row0 = it.tm * Cfg::BM + int(cta) * 128 + q * 32, n0 = it.tn * BN;
       const int n_boxes = row0 < g.M ? min(BN / 64, (g.N - n0 + 63) / 64) : 0;
+      const int mine = (n_boxes - h + 1) >> 1;
       const int buf = local & 1;
-      const float alpha = g.alpha, beta = g.beta;
-      auto box_of = [&](uint32_t k) { return my_boxes + (k & 1) * Cfg::BOX_BYTES; };
-      auto load_box = [&](int i) {      // lane 0
-        const uint32_t k = count + uint32_t(i);
-        mbar_expect_tx(&my_full[k & 1], Cfg::BOX_BYTES);
-        tma_load_3d(box_of(k), &g.x, &my_full[k & 1], n0 + i * 64, row0, it.matrix);
+      const float alpha = g.alpha, beta = g.beta, diag = g.diag;
+      const bool add = beta != 0.f, turned = g.symmetric && it.tm != it.tn;
+      auto load_box = [&](int u) {   // lane 0; every store from its place has left
+        mbar_expect_tx(&my_full[u], Cfg::BOX_BYTES);
+        tma_load_3d(my_boxes + (u & (BOXES - 1)) * Cfg::BOX_BYTES, &g.x, &my_full[u], n0 + (h + 2 * u) * 64, row0, it.matrix);
       };
-      if (ADD && lane == 0) {
-        bulk_wait_read<0>();
-        for (int i = 0; i < Cfg::BOXES && i < n_boxes; ++i) load_box(i);
+      if (lane == 0) {
+        bulk_wait_read<0>();      // (of boxes stored a main loop ago)
+        if (add)
+          for (int u = 0; u < min(mine, BOXES); ++u) load_box(u);
       }
       if (!__all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], uint32_t(local >> 1) & 1, wctx, ST_TIMEOUT_TMEM_FULL))) break;
       tc_fence_after();
@@ -219,71 +234,84 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(&tmem_empty[buf], 0);
       };
-      const bool turned = SYM && it.tm != it.tn;
       bool ok = true;
-      if (n_boxes == 0) release_tmem();
+      if (mine <= 0) release_tmem();
 #pragma unroll 1
-      for (int i = 0; i < n_boxes; ++i) {
-        const uint32_t k = count + uint32_t(i);
-        const int col0 = n0 + i * 64;
-        const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + i * 64);
+      for (int u = 0; u < mine; ++u) {
+        const int col0 = n0 + (h + 2 * u) * 64;
+        const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + (h + 2 * u) * 64);
         uint32_t r[32], s[32];
         tmem_ld32(t_addr, r);
         tmem_ld32(t_addr + 32u, s);
-        if (lane == 0) {
-          if (!ADD) {
-            bulk_wait_read<Cfg::BOXES - 1>();
-          } else if (i > 0 && i - 1 + Cfg::BOXES < n_boxes) {
-            bulk_wait_read<0>();
-            load_box(i - 1 + Cfg::BOXES);
-          }
+        if (BOXES == 1 && u == 1 && lane == 0) {
+          bulk_wait_read<0>();
+          if (add) load_box(1);
         }
         tmem_wait_ld();
-        if (i == n_boxes - 1) release_tmem();
+        if (u == mine - 1) release_tmem();
         else __syncwarp();
-        const uint32_t row_at = smem_u32(box_of(k)) + uint32_t(lane) * 128;
-        if (ADD) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&my_full[k & 1], (k >> 1) & 1, wctx, ST_TIMEOUT_FULL));
+        uint8_t* box = my_boxes + (u & (BOXES - 1)) * Cfg::BOX_BYTES;
+        const uint32_t row_at = smem_u32(box) + uint32_t(lane) * 128;
+        if (add) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&my_full[u], (phases >> u) & 1, wctx, ST_TIMEOUT_FULL));
           if (!ok) break;
+          phases ^= 1u << u;
         }
+        // the one column of this box that lies on the diagonal in this thread's row
+        const int diag_at = it.tm == it.tn && (row0 & ~63) == col0 ? (row0 & 32) + lane : -1;
         uint32_t o[32];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t at = row_at + uint32_t((j ^ (lane & 7)) << 4);
           uint32_t x[4] = {0u, 0u, 0u, 0u};
-          if (ADD) {
+          if (add) {
             const uint4 v = ld_shared_v4(at);
             x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int e = (j & 3) * 8 + 2 * u;
-            const float lo = __uint_as_float(j < 4 ? r[e] : s[e]) * alpha, hi = __uint_as_float(j < 4 ? r[e + 1] : s[e + 1]) * alpha;
-            const float2 add = ADD ? unpack_half2(x[u]) : make_float2(0.f, 0.f);
-            o[j * 4 + u] = ADD ? pack_half2(fmaf(beta, add.x, lo), fmaf(beta, add.y, hi)) : pack_half2(lo, hi);
+          for (int w = 0; w < 4; ++w) {
+            const int e = (j & 3) * 8 + 2 * w;
+            float lo = __uint_as_float(j < 4 ? r[e] : s[e]) * alpha, hi = __uint_as_float(j < 4 ? r[e + 1] : s[e + 1]) * alpha;
+            const float2 more = unpack_half2(x[w]);
+            lo = fmaf(beta, more.x, lo);
+            hi = fmaf(beta, more.y, hi);
+            if (diag_at >= 0) {
+              lo += diag_at == j * 8 + 2 * w ? diag : 0.f;
+              hi += diag_at == j * 8 + 2 * w + 1 ? diag : 0.f;
+            }
+            o[j * 4 + w] = pack_half2(lo, hi);
           }
           st_shared_v4(at, o[j * 4], o[j * 4 + 1], o[j * 4 + 2], o[j * 4 + 3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.c, box_of(k), col0, row0, it.matrix);
+          if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.c, box, col0, row0, it.matrix);
           bulk_commit();
+          // turned boxes leave from the first place: what it holds (this box, or the turned one before it) has been read by then
+          if (turned) {
+            if (u == 0 || BOXES == 1) bulk_wait_read<0>();
+            else bulk_wait_read<1>();
+          }
         }
         if (turned) {
-          // Two lanes trade halves, so that each has two rows of one column: 64 bytes of a row of the turned tile a store.  (For an odd
-          // M the last pair reaches one element into the row's padding.)
-          const int row = row0 + (lane & ~1);
-          __half* to = g.out + size_t(it.matrix) * g.step + size_t(col0 + (lane & 1)) * g.ld + row;
+          // Two lanes trade halves, so that each has two rows of one column: 64 rows of 32 of the turned box, 128 bytes a store.
+          __syncwarp();
+          const uint32_t to = smem_u32(my_boxes) + uint32_t(lane & 1) * 64 + uint32_t(lane >> 1) * 4;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             const uint32_t other = __shfl_xor_sync(0xffffffffu, o[j], 1);
             const uint32_t v = lane & 1 ? __byte_perm(other, o[j], 0x7632) : __byte_perm(o[j], other, 0x5410);
-            if (row < g.M && col0 + 2 * j + (lane & 1) < g.N) *reinterpret_cast<uint32_t*>(to + size_t(2 * j) * g.ld) = v;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + uint32_t(j * 128)), "r"(v) : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.t, my_boxes, row0, col0, it.matrix);
+            bulk_commit();
           }
         }
       }
-      count += uint32_t(n_boxes);
       if (!ok) break;
     }
   }
@@ -303,12 +331,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) newton_schul
   }
 }
 
-template <int KIND>
 inline int ns_launch(const NsParams& p, cudaStream_t stream) {
   static SharedLimit limit;
-  ZB_CUDA_OK(limit.raise(newton_schulz_kernel<KIND>, NsCfg::SMEM_BYTES));
+  ZB_CUDA_OK(limit.raise(newton_schulz_kernel, NsCfg::SMEM_BYTES));
   const int pairs = std::min(num_sms() / 2, p.items);
-  ZB_CUDA_OK(launch_chained(newton_schulz_kernel<KIND>, dim3(2 * pairs), 192, NsCfg::SMEM_BYTES, stream, 0, p));
+  ZB_CUDA_OK(launch_chained(newton_schulz_kernel, dim3(2 * pairs), NsCfg::THREADS, NsCfg::SMEM_BYTES, stream, 0, p));
   return 0;
 }
 

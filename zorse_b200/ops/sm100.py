@@ -615,7 +615,7 @@ def moment_values(moments, dtype=torch.float32):
     return out
 
 
-# Matrices of a list are taken together as far as their workspace (8 bytes an element, 4 a pair of rows of the short side) stays below this:
+# Matrices of a list are taken together as far as their workspace (4 bytes an element, 4 a pair of rows of the short side) stays below this:
 # enough tiles for many waves.
 NEWTON_SCHULZ_BYTES = 1 << 30
 
@@ -645,10 +645,13 @@ def _newton_schulz(table, muon: bool, iterations: int, dev, lr=0.0, momentum=0.0
         _launches += launches.value - 1
 
 
-def _matrix(t, name: str, dtypes, dev, shape=None) -> None:
-    _need(t.dim() == 2 and t.is_contiguous() and t.dtype in dtypes and t.device == dev and (shape is None or t.shape == shape) and max(t.shape) < 2 ** 31,
-          f"{name} {tuple(t.shape)}, {t.dtype} on {t.device}: expected a contiguous matrix{'' if shape is None else f' {tuple(shape)}'} on {dev} "
-          f"of {' or '.join(str(d) for d in dtypes)}")
+def _matrix(t, name: str, i: int, dtypes, dev, shape=None) -> None:
+    if t.dim() != 2 or not t.is_contiguous() or t.dtype not in dtypes or t.device != dev or (shape is not None and t.shape != shape) or t.numel() >= 2 ** 40:
+        raise ValueError(f"{name}[{i}] {tuple(t.shape)}, {t.dtype} on {t.device}: expected a contiguous matrix{'' if shape is None else f' {tuple(shape)}'} "
+                         f"on {dev} of {' or '.join(str(d) for d in dtypes)}")
+
+
+_FP32, _BF16, _EITHER = (torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)
 
 
 def orthogonalize(mats, iterations: int = 5) -> list:
@@ -659,7 +662,7 @@ def orthogonalize(mats, iterations: int = 5) -> list:
     dev, table = mats[0].device, []
     _on_current(mats[0], "mats")
     for i, u in enumerate(mats):
-        _matrix(u, f"mats[{i}]", (torch.float32, torch.bfloat16), dev)
+        _matrix(u, "mats", i, _EITHER, dev)
         out.append(torch.empty(u.shape, dtype=torch.bfloat16, device=dev))
         if u.numel():
             table.append((0, 0, u.data_ptr(), out[-1].data_ptr(), *u.shape, int(u.dtype == torch.float32)))
@@ -680,21 +683,27 @@ def muon_step(p, m, g, p16, *, lr: float, momentum: float = 0.95, weight_decay: 
     _on_current(p[0], "p")
     table, written, read = [], [], []
     for i, (x, mom, d, y) in enumerate(zip(p, m, g, p16)):
-        _matrix(x, f"p[{i}]", (torch.float32,), dev)
-        _matrix(mom, f"m[{i}]", (torch.float32,), dev, x.shape)
-        _matrix(d, f"g[{i}]", (torch.float32, torch.bfloat16), dev, x.shape)
+        shape = x.shape
+        _matrix(x, "p", i, _FP32, dev)
+        _matrix(mom, "m", i, _FP32, dev, shape)
+        _matrix(d, "g", i, _EITHER, dev, shape)
         if y is not None:
-            _matrix(y, f"p16[{i}]", (torch.bfloat16,), dev, x.shape)
-        if x.numel() == 0:
+            _matrix(y, "p16", i, _BF16, dev, shape)
+        size, f32 = x.numel(), d.dtype == torch.float32
+        if size == 0:
             continue
-        written += [(*_stretch(t), i) for t in (x, mom, y) if t is not None]
-        read.append((*_stretch(d), i))
-        table.append((x.data_ptr(), mom.data_ptr(), d.data_ptr(), _a(y), *x.shape, int(d.dtype == torch.float32)))
+        at = x.data_ptr(), mom.data_ptr(), d.data_ptr(), _a(y)
+        written += [(at[0], at[0] + 4 * size), (at[1], at[1] + 4 * size)]
+        if y is not None:
+            written.append((at[3], at[3] + 2 * size))
+        read.append((at[2], at[2] + (4 if f32 else 2) * size, i))
+        table.append((*at, *shape, int(f32)))
     written.sort()
     _need(all(a[1] <= b[0] for a, b in zip(written, written[1:])), "matrices that the step writes overlap (one is in the list twice?)")
     for lo, hi, i in read:       # (read by two passes, with the momentum's writes in between)
         at = bisect.bisect_left(written, (lo + 1,)) - 1
-        _need((at < 0 or written[at][1] <= lo) and (at + 1 == len(written) or written[at + 1][0] >= hi), f"g[{i}] overlaps a matrix that the step writes")
+        if (at >= 0 and written[at][1] > lo) or (at + 1 < len(written) and written[at + 1][0] < hi):
+            raise ValueError(f"g[{i}] overlaps a matrix that the step writes")
     _newton_schulz(table, True, iterations, dev, lr, momentum, nesterov, 1 - lr * weight_decay, grad_scale)
 
 
