@@ -66,6 +66,13 @@ struct Entry {
   int (*embedding_by_token_workspace)(int, int, long*);
   int (*embedding_by_token)(const long*, const void*, void*, void*, void*, int, int, int, int, int, float, int, cudaStream_t);
   int (*adamw_list)(const void*, int, int, float, float, float, float, float, float, float, cudaStream_t);
+  int (*packed_attn_fwd)(const void*, void*, float*, const void*, const int*, int, int, int, int, int, int, float, int*, cudaStream_t);
+  int (*packed_attn_bwd)(const void*, const void*, const void*, const float*, void*, float*, const void*, const int*, const int*, int, int,
+                         int, int, int, int, float, int*, cudaStream_t);
+  int (*rope_at)(void*, const float*, const int*, const int*, int, int, int, int, int, long, int, cudaStream_t);
+  int (*newton_schulz_workspace)(const void*, int, long, long*);
+  int (*newton_schulz)(const void*, int, int, float, float, int, float, float, int, float, float, float, long, void*, long, int*, int*,
+                       cudaStream_t);
   const char* (*last_error)();
 };
 Entry lib;
@@ -950,6 +957,210 @@ PyObject* adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// What forward and backward pass over packed sequences have in common.
+struct Packed {
+  const Tensor *qkv, *bounds;
+  int64_t T, Hq, Hkv, D, window;
+  bool causal;
+  bool take(PyObject* const* rest) {   // T, Hq, Hkv, D, causal, window
+    if (!int_arg(rest[0], T) || !int_arg(rest[1], Hq) || !int_arg(rest[2], Hkv) || !int_arg(rest[3], D) || !int_arg(rest[5], window)) return false;
+    causal = truth(rest[4]);
+    if (!fits(T) || !fits(Hq) || !fits(Hkv) || Hq % Hkv != 0 || (D != 64 && D != 128) || window < 0 || (window > 0 && !causal)) return false;
+    if (window >= T) window = 0;
+    return dense(qkv, BF16) && qkv->dim() == 2 && qkv->size(0) == T && qkv->size(1) == (Hq + 2 * Hkv) * D && fits(qkv->size(1)) &&
+           status_of(*qkv) != nullptr && dense(bounds, at::kInt) && bounds->numel() == (T + 255) / 256 * 512 && on(bounds, *qkv);
+  }
+  bool order(const Tensor* t, int64_t n) const { return dense(t, at::kInt) && t->numel() == n && on(t, *qkv); }
+};
+// packed_attn_fwd(qkv, bounds, order_pairs, T, Hq, Hkv, D, causal, window) -> (out, lse)
+PyObject* packed_attn_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(9)
+  Packed a = {tensor_of(args[0]), tensor_of(args[1])};
+  const Tensor* pairs = tensor_of(args[2]);
+  if (!a.take(args + 3) || !a.order(pairs, (a.T + 255) / 256)) Py_RETURN_NONE;
+  Tensor out = fresh({a.T, a.Hq * a.D}, *a.qkv, BF16), lse = fresh({a.Hq, a.T}, *a.qkv, F32);
+  const float scale = float(1.0 / std::sqrt(double(a.D)));
+  int* status = status_of(*a.qkv);
+  const cudaStream_t s = stream();
+  if (!launch("packed_attn_fwd", 1, [&] {
+        return lib.packed_attn_fwd(ptr(a.qkv), out.data_ptr(), static_cast<float*>(lse.data_ptr()), ptr(a.bounds),
+                                   static_cast<const int*>(ptr(pairs)), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window),
+                                   scale, status, s);
+      }))
+    return nullptr;
+  PyObject* r = PyTuple_New(2);
+  if (r == nullptr) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(lse)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+// packed_attn_bwd(do, qkv, o, lse, bounds, order_tiles, order_keys, T, Hq, Hkv, D, causal, window) -> dqkv
+PyObject* packed_attn_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(13)
+  Packed a = {tensor_of(args[1]), tensor_of(args[4])};
+  const Tensor *d_o = tensor_of(args[0]), *o = tensor_of(args[2]), *lse = tensor_of(args[3]), *tiles = tensor_of(args[5]), *keys = tensor_of(args[6]);
+  if (!a.take(args + 7) || !a.order(tiles, (a.T + 127) / 128) || !a.order(keys, (a.T + 127) / 128)) Py_RETURN_NONE;
+  for (const Tensor* t : {d_o, o})
+    if (!dense(t, BF16) || t->dim() != 2 || t->size(0) != a.T || t->size(1) != a.Hq * a.D || !on(t, *a.qkv)) Py_RETURN_NONE;
+  if (!dense(lse, F32) || lse->dim() != 2 || lse->size(0) != a.Hq || lse->size(1) != a.T || !on(lse, *a.qkv)) Py_RETURN_NONE;
+  Tensor dqkv = fresh(a.qkv->sizes(), *a.qkv, BF16);
+  const Tensor stats = fresh({a.Hq * 2 * ((a.T + 127) / 128 * 128)}, *a.qkv, F32);
+  const float scale = float(1.0 / std::sqrt(double(a.D)));
+  int* status = status_of(*a.qkv);
+  const cudaStream_t s = stream();
+  if (!launch("packed_attn_bwd", 3, [&] {
+        return lib.packed_attn_bwd(ptr(d_o), ptr(a.qkv), ptr(o), static_cast<const float*>(ptr(lse)), dqkv.data_ptr(),
+                                   static_cast<float*>(stats.data_ptr()), ptr(a.bounds), static_cast<const int*>(ptr(tiles)),
+                                   static_cast<const int*>(ptr(keys)), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window), scale,
+                                   status, s);
+      }))
+    return nullptr;
+  return THPVariable_Wrap(std::move(dqkv));
+  END_HANDLE_TH_ERRORS
+}
+// rope_at(buf, cs, positions, heads, d, sections | None, backward) -> True
+PyObject* rope_at(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(7)
+  const Tensor *buf = tensor_of(args[0]), *cs = tensor_of(args[1]), *positions = tensor_of(args[2]);
+  int64_t heads, d, sum = 0;
+  if (!int_arg(args[3], heads) || !int_arg(args[4], d) || !fits(heads) || !fits(d) || d % 2 != 0) Py_RETURN_NONE;
+  int sections[4] = {int(d / 2), 0, 0, 0}, axes = 1;
+  if (args[5] != Py_None) {
+    if (!PyList_Check(args[5]) || PyList_GET_SIZE(args[5]) < 1 || PyList_GET_SIZE(args[5]) > 4) Py_RETURN_NONE;
+    axes = int(PyList_GET_SIZE(args[5]));
+    for (int i = 0; i < axes; ++i) {
+      int64_t n;
+      if (!int_arg(PyList_GET_ITEM(args[5], i), n) || n < 0 || n > d / 2) Py_RETURN_NONE;
+      sections[i] = int(n);
+    }
+  }
+  for (int i = 0; i < axes; ++i) sum += sections[i];
+  if (sum != d / 2 || !matrix(buf, BF16) || !here(*buf) || !fits(buf->size(0)) || !fits(buf->size(1)) || heads * d > buf->size(1) ||
+      (buf->size(0) > 1 && buf->stride(0) < buf->size(1)))
+    Py_RETURN_NONE;
+  const int64_t T = buf->size(0);
+  if (!dense(positions, at::kInt) || positions->numel() != axes * T || positions->dim() < 1 || positions->dim() > 2 || positions->size(-1) != T || !on(positions, *buf) ||
+      !dense(cs, F32) || cs->dim() != 2 || cs->size(1) != d || !fits(cs->size(0)) || !on(cs, *buf))
+    Py_RETURN_NONE;
+  const bool backward = truth(args[6]);
+  const cudaStream_t s = stream();
+  if (!launch("rope_at", 1, [&] {
+        return lib.rope_at(ptr(buf), static_cast<const float*>(ptr(cs)), static_cast<const int*>(ptr(positions)), sections, axes, int(T),
+                           int(cs->size(0)), int(heads), int(d), buf->stride(0), backward, s);
+      }))
+    return nullptr;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// A matrix as zb_newton_schulz reads it.
+struct NsMatrix {
+  void *p, *m, *g, *out;
+  long rows, cols;
+  int g_f32, unused;
+};
+bool any_matrix(const Tensor* t, const Tensor& like) {   // contiguous, of a type that the products take
+  return gradient(t) && t->dim() == 2 && on(t, like) && t->size(0) <= INT32_MAX && t->size(1) <= INT32_MAX;
+}
+// 1: done, 0: not for here, -1: error set
+int newton_schulz(c10::SmallVectorImpl<NsMatrix>& table, const Tensor& like, bool muon, const double (&h)[4], bool nesterov, int64_t iterations,
+                  const double (&abc)[3], int64_t limit) {   // h: lr, momentum, keep, grad_scale
+  int* status = status_of(like);
+  if (status == nullptr || iterations < 1 || iterations > 100) return 0;
+  long bytes = 0;
+  if (lib.newton_schulz_workspace(table.data(), int(table.size()), limit, &bytes) != 0) return 0;
+  const Tensor ws = fresh({bytes}, like, at::kByte);
+  const cudaStream_t s = stream();
+  int n = 0;
+  if (!launch("newton_schulz", 0, [&] {
+        return lib.newton_schulz(table.data(), int(table.size()), muon, float(h[0]), float(h[1]), nesterov, float(h[2]), float(h[3]),
+                                 int(iterations), float(abc[0]), float(abc[1]), float(abc[2]), limit, ws.data_ptr(), bytes, &n, status, s);
+      }))
+    return -1;
+  launches += n;
+  return 1;
+}
+// orthogonalize(mats, iterations, (a, b, c), limit) -> the results
+PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(4)
+  const Py_ssize_t n = PyList_Check(args[0]) ? PyList_GET_SIZE(args[0]) : 0;
+  int64_t iterations, limit;
+  double abc[3];
+  if (n == 0 || !int_arg(args[1], iterations) || !int_arg(args[3], limit) || !PyTuple_Check(args[2]) || PyTuple_GET_SIZE(args[2]) != 3) Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i)
+    if (!float_arg(PyTuple_GET_ITEM(args[2], i), abc[i])) Py_RETURN_NONE;
+  const Tensor* first = tensor_of(PyList_GET_ITEM(args[0], 0));
+  if (!gradient(first) || !here(*first)) Py_RETURN_NONE;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const Tensor* u = tensor_of(PyList_GET_ITEM(args[0], i));
+    if (!any_matrix(u, *first) || u->numel() == 0) Py_RETURN_NONE;
+  }
+  c10::SmallVector<NsMatrix, 32> table;
+  c10::SmallVector<Tensor, 32> out;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const Tensor* u = tensor_of(PyList_GET_ITEM(args[0], i));
+    out.push_back(fresh(u->sizes(), *first, BF16));
+    table.push_back({nullptr, nullptr, ptr(u), out.back().data_ptr(), long(u->size(0)), long(u->size(1)), u->scalar_type() == F32, 0});
+  }
+  const int done = newton_schulz(table, *first, false, {0.0, 0.0, 1.0, 1.0}, false, iterations, abc, limit);
+  if (done < 0) return nullptr;
+  if (done == 0) Py_RETURN_NONE;
+  PyObject* list = PyList_New(n);
+  if (list == nullptr) return nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) PyList_SET_ITEM(list, i, THPVariable_Wrap(std::move(out[i])));
+  return list;
+  END_HANDLE_TH_ERRORS
+}
+// muon_step(p, m, g, p16, lr, momentum, weight_decay, nesterov, iterations, grad_scale, (a, b, c), limit) -> True; lists
+PyObject* muon_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  ZB_ARGS(12)
+  const Py_ssize_t n = PyList_Check(args[0]) ? PyList_GET_SIZE(args[0]) : 0;
+  auto list = [&](PyObject* o) { return PyList_Check(o) && PyList_GET_SIZE(o) == n; };
+  double lr, momentum, decay, grad_scale, abc[3];
+  int64_t iterations, limit;
+  if (n == 0 || !list(args[1]) || !list(args[2]) || !list(args[3]) || !float_arg(args[4], lr) || !float_arg(args[5], momentum) ||
+      !float_arg(args[6], decay) || !int_arg(args[8], iterations) || !float_arg(args[9], grad_scale) || !PyTuple_Check(args[10]) ||
+      PyTuple_GET_SIZE(args[10]) != 3 || !int_arg(args[11], limit) || !(momentum >= 0 && momentum < 1))
+    Py_RETURN_NONE;
+  for (int i = 0; i < 3; ++i)
+    if (!float_arg(PyTuple_GET_ITEM(args[10], i), abc[i])) Py_RETURN_NONE;
+  const Tensor* first = tensor_of(PyList_GET_ITEM(args[0], 0));
+  if (!dense(first, F32) || !here(*first)) Py_RETURN_NONE;
+  c10::SmallVector<NsMatrix, 32> table;
+  c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 96> written;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const Tensor *p = tensor_of(PyList_GET_ITEM(args[0], i)), *m = tensor_of(PyList_GET_ITEM(args[1], i)), *g = tensor_of(PyList_GET_ITEM(args[2], i)), *p16;
+    if (!optional_tensor(PyList_GET_ITEM(args[3], i), p16) || !any_matrix(p, *first) || !any_matrix(m, *first) || !any_matrix(g, *first) ||
+        p->scalar_type() != F32 || m->scalar_type() != F32 || m->sizes() != p->sizes() || g->sizes() != p->sizes() ||
+        (p16 != nullptr && (!any_matrix(p16, *first) || p16->scalar_type() != BF16 || p16->sizes() != p->sizes())))
+      Py_RETURN_NONE;
+    if (p->numel() == 0) continue;
+    table.push_back({ptr(p), ptr(m), ptr(g), ptr(p16), long(p->size(0)), long(p->size(1)), g->scalar_type() == F32, 0});
+    for (const Tensor* t : {p, m, p16})
+      if (t != nullptr) written.push_back({reinterpret_cast<uintptr_t>(t->data_ptr()), reinterpret_cast<uintptr_t>(t->data_ptr()) + t->nbytes()});
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second) Py_RETURN_NONE;
+  for (const NsMatrix& t : table) {   // no gradient may lie in what is written
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(t.g), hi = lo + uintptr_t(t.rows) * uintptr_t(t.cols) * (t.g_f32 ? 4 : 2);
+    auto next = std::upper_bound(written.begin(), written.end(), lo, [](uintptr_t x, const auto& w) { return x < w.first; });
+    if ((next != written.end() && next->first < hi) || (next != written.begin() && (next - 1)->second > lo)) Py_RETURN_NONE;
+  }
+  if (table.empty()) Py_RETURN_NONE;
+  const int done = newton_schulz(table, *first, true, {lr, momentum, 1 - lr * decay, grad_scale}, truth(args[7]), iterations, abc, limit);
+  if (done < 0) return nullptr;
+  if (done == 0) Py_RETURN_NONE;
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // init(addresses of the entry points in Entry's order, KernelError)
 PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ZB_ARGS(2)
@@ -987,7 +1198,8 @@ PyMethodDef methods[] = {ZB_FN(init), ZB_FN(set_status), ZB_FN(launch_count), ZB
                          ZB_FN(norm_fwd), ZB_FN(norm_bwd), ZB_FN(finish), ZB_FN(rope), ZB_FN(swiglu_fwd),
                          ZB_FN(swiglu_bwd), ZB_FN(act_fwd), ZB_FN(act_bwd), ZB_FN(attn_fwd), ZB_FN(attn_bwd),
                          ZB_FN(qk_norm_rope_fwd), ZB_FN(qk_norm_rope_bwd), ZB_FN(embedding_scaled), ZB_FN(embedding_by_token),
-                         ZB_FN(adamw_step),
+                         ZB_FN(adamw_step), ZB_FN(packed_attn_fwd), ZB_FN(packed_attn_bwd), ZB_FN(rope_at), ZB_FN(orthogonalize),
+                         ZB_FN(muon_step),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "zorse_fastops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

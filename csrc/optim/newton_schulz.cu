@@ -30,7 +30,7 @@ namespace zb {
 constexpr float NS_A_SCALE = 64.f;   // what is n x n is held times this
 
 // --------------------------------------------------------------------------------------------- passes before and behind
-constexpr int NS_MATRICES = 64;      // of a launch of a pass
+constexpr int NS_MATRICES = 64;      // of a launch of a pass; 12 where there are no more
 constexpr int NS_PARTS = 256;        // sums of squares of one matrix, at most
 
 // What a caller hands over for each matrix.
@@ -55,14 +55,16 @@ struct NsPassMatrix {
   int g_f32, wide;        // wide: rows start on 16 bytes in every type
   float scale, step;      // X is held times scale; muon: what the result is multiplied with
 };
+template <int MATRICES>
 struct NsPass {
-  NsPassMatrix t[NS_MATRICES];
+  NsPassMatrix t[MATRICES];
   int count;
   float momentum, grad_scale, keep;
   int nesterov, muon;
 };
 
-__device__ __forceinline__ int ns_find(const NsPass& a, int block) {
+template <int N>
+__device__ __forceinline__ int ns_find(const NsPass<N>& a, int block) {
   int lo = 0, hi = a.count;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -83,10 +85,12 @@ __device__ __forceinline__ float ns_load1(const void* base, bool f32, size_t at)
   return f32 ? static_cast<const float*>(base)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
 }
 // The update from the scaled gradient and the new momentum.
-__device__ __forceinline__ float ns_update(const NsPass& a, float g, float m) { return a.nesterov ? fmaf(a.momentum, m, g) : m; }
+template <int N>
+__device__ __forceinline__ float ns_update(const NsPass<N>& a, float g, float m) { return a.nesterov ? fmaf(a.momentum, m, g) : m; }
 
 // Momentum (written back) and the sum of squares of the update; a block has an equal part of its matrix's elements.
-__global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ NsPass a) {
+template <int N>
+__global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ NsPass<N> a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
@@ -150,7 +154,8 @@ __global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ Ns
 }
 
 // Tiles of 64 x 64: the update times scale / norm in fp16, turned over where the matrix has more rows than columns.
-__global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant__ NsPass a) {
+template <int N>
+__global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant__ NsPass<N> a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
@@ -219,7 +224,8 @@ __global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant_
 }
 
 // Tiles of 64 x 64: the result in bf16, or the step of the parameters.
-__global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ NsPass a) {
+template <int N>
+__global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ NsPass<N> a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
@@ -369,7 +375,7 @@ static int ns_products(const NsPlan& plan, char* ws, const std::vector<NsStep>& 
     // the longest reductions first: the last wave of a launch is then of short ones
     std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return plan.shapes[i].cols(e.p) > plan.shapes[j].cols(e.p); });
     for (size_t first = 0; first < order.size(); first += NS_GROUPS) {
-      NsParams p;
+      NsParams<NS_GROUPS> p;
       p.status = status;
       p.groups = p.items = 0;
       for (size_t k = first; k < std::min(first + NS_GROUPS, order.size()); ++k) {
@@ -406,19 +412,33 @@ static int ns_products(const NsPlan& plan, char* ws, const std::vector<NsStep>& 
   return 0;
 }
 
+template <int PASS, int N>
+static int ns_pass_launch(const NsPass<NS_MATRICES>& all, unsigned blocks, cudaStream_t stream) {
+  NsPass<N> a;
+  std::copy(all.t, all.t + all.count, a.t);
+  a.count = all.count;
+  a.momentum = all.momentum;
+  a.grad_scale = all.grad_scale;
+  a.keep = all.keep;
+  a.nesterov = all.nesterov;
+  a.muon = all.muon;
+  if (PASS == 0) ZB_CUDA_OK(launch_pass(ns_sums_kernel<N>, dim3(blocks), 256, 0, stream, a));
+  else if (PASS == 1) ZB_CUDA_OK(launch_pass(ns_scale_kernel<N>, dim3(blocks), 256, 0, stream, a));
+  else ZB_CUDA_OK(launch_pass(ns_apply_kernel<N>, dim3(blocks), 256, 0, stream, a));
+  return 0;
+}
+
 // One of the passes over all matrices; PASS 0: sums, 1: scale, 2: apply.
 template <int PASS>
-static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, float lr, char* ws, int x, cudaStream_t stream, int* launches) {
-  NsPass a = common;
+static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRICES>& common, float lr, char* ws, int x, cudaStream_t stream, int* launches) {
+  NsPass<NS_MATRICES> a = common;
   a.count = 0;
   long blocks = 0;
   auto flush = [&]() -> int {
     if (a.count == 0) return 0;
     if (blocks > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: %ld blocks", blocks);
-    const dim3 grid = dim3(unsigned(blocks));
-    if (PASS == 0) ZB_CUDA_OK(launch_pass(ns_sums_kernel, grid, 256, 0, stream, a));
-    else if (PASS == 1) ZB_CUDA_OK(launch_pass(ns_scale_kernel, grid, 256, 0, stream, a));
-    else ZB_CUDA_OK(launch_pass(ns_apply_kernel, grid, 256, 0, stream, a));
+    const int rc = a.count <= 12 ? ns_pass_launch<PASS, 12>(a, unsigned(blocks), stream) : ns_pass_launch<PASS, NS_MATRICES>(a, unsigned(blocks), stream);
+    if (rc) return rc;
     ++*launches;
     a.count = 0;
     blocks = 0;
@@ -462,42 +482,64 @@ static int ns_check(const NsMatrix* t, int count) {
   return 0;
 }
 
+// How many of the list's first matrices are taken together.
+static int ns_together(const NsMatrix* t, int count, long limit) {
+  double room = double(limit);
+  for (int i = 0; i < count; ++i) {
+    const double n = double(std::min(t[i].rows, t[i].cols)), m = double(std::max(t[i].rows, t[i].cols));
+    room -= 4 * n * (m + 8) + 4 * n * (n + 8) + 8192;
+    if (room < 0) return std::max(i, 1);
+  }
+  return count;
+}
+
 }  // namespace zb
 
 extern "C" {
 
-// Bytes of workspace for a list (of zb_newton_schulz's table only rows and cols are looked at).
-int zb_newton_schulz_workspace(const void* table, int count, long* bytes) {
+// Bytes of workspace for a list (of zb_newton_schulz's table only rows and cols are looked at).  Its matrices are taken together as far as their
+// workspace stays below `limit`, or one by one.
+int zb_newton_schulz_workspace(const void* table, int count, long limit, long* bytes) {
   using namespace zb;
   const NsMatrix* t = static_cast<const NsMatrix*>(table);
   if (int rc = ns_check(t, count)) return rc;
-  *bytes = long(ns_plan(t, count).bytes);
+  *bytes = 0;
+  for (int i = 0, n; i < count; i += n) {
+    n = ns_together(t + i, count - i, limit);
+    *bytes = std::max(*bytes, long(ns_plan(t + i, n).bytes));
+  }
   return 0;
 }
 
 // table: `count` NsMatrix, none of them empty.  muon: p and m are stepped with lr, momentum (nesterov: the gradient looks ahead by it), the
 // gradient times grad_scale, and keep = 1 - lr weight_decay; else the orthogonalised matrices go to `out`.  a, b, c: coefficients.
 int zb_newton_schulz(const void* table, int count, int muon, float lr, float momentum, int nesterov, float keep, float grad_scale, int iterations,
-                     float a, float b, float c, void* workspace, long bytes, int* launches, int* status, cudaStream_t stream) {
+                     float a, float b, float c, long limit, void* workspace, long bytes, int* launches, int* status, cudaStream_t stream) {
   using namespace zb;
   const NsMatrix* t = static_cast<const NsMatrix*>(table);
   *launches = 0;
   if (count <= 0) return 0;
   if (int rc = ns_check(t, count)) return rc;
-  const NsPlan plan = ns_plan(t, count);
-  if (bytes < long(plan.bytes) || (reinterpret_cast<uintptr_t>(workspace) & 15))
-    ZB_FAIL(-4, "newton_schulz: %ld bytes of workspace, %zu on a 16-byte boundary are needed", bytes, plan.bytes);
-  char* ws = static_cast<char*>(workspace);
-  NsPass pass = {};
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) ZB_FAIL(-4, "newton_schulz: the workspace is not on a 16-byte boundary");
+  NsPass<NS_MATRICES> pass = {};
   pass.momentum = momentum;
   pass.grad_scale = grad_scale;
   pass.keep = keep;
   pass.nesterov = nesterov;
   pass.muon = muon;
-  int rc = ns_pass<0>(plan, t, pass, lr, ws, NS_X0, stream, launches);
-  if (!rc) rc = ns_pass<1>(plan, t, pass, lr, ws, NS_X0, stream, launches);
-  if (!rc) rc = ns_products(plan, ws, ns_program(iterations, a, b, c), status, stream, launches);
-  return rc ? rc : ns_pass<2>(plan, t, pass, lr, ws, iterations & 1 ? NS_X1 : NS_X0, stream, launches);
+  char* ws = static_cast<char*>(workspace);
+  const std::vector<NsStep> program = ns_program(iterations, a, b, c);
+  for (int i = 0, n; i < count; i += n) {
+    n = ns_together(t + i, count - i, limit);
+    const NsPlan plan = ns_plan(t + i, n);
+    if (bytes < long(plan.bytes)) ZB_FAIL(-4, "newton_schulz: %ld bytes of workspace, %zu are needed", bytes, plan.bytes);
+    int rc = ns_pass<0>(plan, t + i, pass, lr, ws, NS_X0, stream, launches);
+    if (!rc) rc = ns_pass<1>(plan, t + i, pass, lr, ws, NS_X0, stream, launches);
+    if (!rc) rc = ns_products(plan, ws, program, status, stream, launches);
+    if (!rc) rc = ns_pass<2>(plan, t + i, pass, lr, ws, iterations & 1 ? NS_X1 : NS_X0, stream, launches);
+    if (rc) return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"

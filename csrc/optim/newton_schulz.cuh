@@ -42,8 +42,9 @@ struct alignas(64) NsGroup {
   int first;              // its first item
   float alpha, beta, diag;
 };
+template <int GROUPS>      // (a launch with few shapes has few parameters to send: 2 of 8 shapes' 5.6 KB)
 struct NsParams {
-  NsGroup g[NS_GROUPS];
+  NsGroup g[GROUPS];
   int groups, items;
   int stages;             // 6 with one box a warp, 5 with two
   int* status;
@@ -58,7 +59,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) newton_schulz_kernel(const __grid_constant__ NsParams p) {
+template <int GROUPS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) newton_schulz_kernel(const __grid_constant__ NsParams<GROUPS> p) {
   using Cfg = NsCfg;
   constexpr int BK = Cfg::BK, BN = Cfg::BN, EP_WARPS = Cfg::EP_WARPS;
   const int STAGES = p.stages, BOXES = Cfg::MAX_STAGES + 1 - STAGES;
@@ -331,12 +333,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) n
   }
 }
 
-inline int ns_launch(const NsParams& p, cudaStream_t stream) {
+template <int GROUPS>
+inline int ns_launch_few(const NsParams<NS_GROUPS>& all, cudaStream_t stream) {
+  NsParams<GROUPS> p;
+  std::copy(all.g, all.g + all.groups, p.g);
+  p.groups = all.groups;
+  p.items = all.items;
+  p.stages = all.stages;
+  p.status = all.status;
   static SharedLimit limit;
-  ZB_CUDA_OK(limit.raise(newton_schulz_kernel, NsCfg::SMEM_BYTES));
+  ZB_CUDA_OK(limit.raise(newton_schulz_kernel<GROUPS>, NsCfg::SMEM_BYTES));
   const int pairs = std::min(num_sms() / 2, p.items);
-  ZB_CUDA_OK(launch_chained(newton_schulz_kernel, dim3(2 * pairs), NsCfg::THREADS, NsCfg::SMEM_BYTES, stream, 0, p));
+  ZB_CUDA_OK(launch_chained(newton_schulz_kernel<GROUPS>, dim3(2 * pairs), NsCfg::THREADS, NsCfg::SMEM_BYTES, stream, 0, p));
   return 0;
+}
+inline int ns_launch(const NsParams<NS_GROUPS>& p, cudaStream_t stream) {
+  return p.groups <= 2 ? ns_launch_few<2>(p, stream) : ns_launch_few<NS_GROUPS>(p, stream);
 }
 
 }  // namespace zb

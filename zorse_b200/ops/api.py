@@ -272,7 +272,8 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
         self._attn_fwd = fast.attn_fwd if default and sm100.ATTN_FWD_VERSION == 0 else _decline
         self._attn_bwd = fast.attn_bwd if default and sm100.ATTN_BWD_VERSION == 0 else _decline
         for name in ("rope", "swiglu_fwd", "swiglu_bwd", "act_fwd", "act_bwd", "qk_norm_rope_fwd", "qk_norm_rope_bwd",
-                     "embedding_scaled", "embedding_by_token", "adamw_step"):
+                     "embedding_scaled", "embedding_by_token", "adamw_step", "packed_attn_fwd", "packed_attn_bwd", "rope_at",
+                     "orthogonalize", "muon_step"):
             setattr(self, "_" + name, getattr(fast, name) if default else _decline)
 
     def linear_fwd(self, x, w, bias=None, addend=None):
@@ -357,13 +358,17 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
         return self.k.pack_sequences(offsets, T)
 
     def packed_attn_fwd(self, qkv, pk, Hq, Hkv, D, causal=True, window=0):
-        return self.k.packed_attn_fwd(qkv, pk, Hq, Hkv, D, causal, window)
+        r = self._packed_attn_fwd(qkv, pk.bounds, pk.order_pairs, pk.tokens, Hq, Hkv, D, causal, window)
+        return self.k.packed_attn_fwd(qkv, pk, Hq, Hkv, D, causal, window) if r is None else r
 
     def packed_attn_bwd(self, do, qkv, o, lse, pk, Hq, Hkv, D, causal=True, window=0):
-        return self.k.packed_attn_bwd(do, qkv, o, lse, pk, Hq, Hkv, D, causal, window)
+        dqkv = self._packed_attn_bwd(do, qkv, o, lse, pk.bounds, pk.order_tiles, pk.order_keys, pk.tokens, Hq, Hkv, D, causal, window)
+        return self.k.packed_attn_bwd(do, qkv, o, lse, pk, Hq, Hkv, D, causal, window) if dqkv is None else dqkv
 
     def rope_at_(self, buf, cs, positions, nheads, d, sections=None, backward=False):
-        return self.k.rope_at_(buf, cs, positions, nheads, d, sections, backward)
+        if self._rope_at(buf, cs, positions, nheads, d, sections, backward) is None:
+            self.k.rope_at_(buf, cs, positions, nheads, d, sections, backward)
+        return buf
 
     def swiglu_fwd(self, gu):
         y = self._swiglu_fwd(gu)
@@ -422,10 +427,15 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
         return self.k.moment_values(moments, dtype)
 
     def orthogonalize(self, mats, iterations=5):
-        return self.k.orthogonalize(mats, iterations)
+        k = self.k
+        r = self._orthogonalize(mats, iterations, k.NEWTON_SCHULZ, k.NEWTON_SCHULZ_BYTES)
+        return k.orthogonalize(mats, iterations) if r is None else r
 
-    def muon_step(self, p, m, g, p16, **kw):
-        self.k.muon_step(p, m, g, p16, **kw)
+    def muon_step(self, p, m, g, p16, *, lr, momentum=0.95, weight_decay=0.0, nesterov=True, iterations=5, grad_scale=1.0):
+        k = self.k
+        if self._muon_step(p, m, g, p16, lr, momentum, weight_decay, nesterov, iterations, grad_scale, k.NEWTON_SCHULZ, k.NEWTON_SCHULZ_BYTES) is None:
+            k.muon_step(p, m, g, p16, lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, iterations=iterations,
+                        grad_scale=grad_scale)
 
 
 _cache: dict[str, object] = {}

@@ -57,7 +57,7 @@ _SIGNATURES = {
     "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
     "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
     "zb_pack_sequences": "piipppppp", "zb_packed_attn_fwd": "pppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
-    "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pip", "zb_newton_schulz": "piiffiffifffplppp",
+    "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pilp", "zb_newton_schulz": "piiffiffiffflplppp",
     "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
 _CTYPES = {"p": c_void_p, "i": c_int, "l": c_long, "f": c_float}
@@ -104,7 +104,8 @@ _FAST_ENTRIES = ("zb_gemm_bf16", "zb_gemm2_bf16", "zb_gemm2_split_bf16", "zb_gem
                  "zb_flash_fwd4", "zb_flash_bwd3", "zb_flash_bwd2_stats_floats", "zb_gemm2_act_fwd",
                  "zb_gemm2_act_bwd", "zb_gemm2_rope_fwd", "zb_column_sums", "zb_qk_norm_rope_fwd", "zb_qk_norm_rope_workspace",
                  "zb_qk_norm_rope_bwd", "zb_embedding_scaled", "zb_embedding_by_token_workspace", "zb_embedding_by_token",
-                 "zb_adamw_list", "zb_last_error")   # the order of its `Entry`
+                 "zb_adamw_list", "zb_packed_attn_fwd", "zb_packed_attn_bwd", "zb_rope_at", "zb_newton_schulz_workspace", "zb_newton_schulz",
+                 "zb_last_error")   # the order of its `Entry`
 
 
 def _load_fast() -> None:
@@ -623,26 +624,15 @@ NEWTON_SCHULZ_BYTES = 1 << 30
 def _newton_schulz(table, muon: bool, iterations: int, dev, lr=0.0, momentum=0.0, nesterov=False, keep=1.0, grad_scale=1.0) -> None:
     """table: (p, m, g, out, rows, cols, g in fp32) of matrices that have elements."""
     _need(isinstance(iterations, int) and 1 <= iterations <= 100, f"{iterations} iterations: 1 to 100")
-    chunks, room = [], 0
-    for t in table:
-        n, k = min(t[4:6]), max(t[4:6])
-        size = 4 * n * (k + 8) + 4 * n * (n + 8) + 8192
-        if not chunks or size > room:
-            chunks.append([])
-            room = NEWTON_SCHULZ_BYTES
-        chunks[-1].append(t)
-        room -= size
-    packed = [struct.pack("4Q2q2i" * len(c), *(x for t in c for x in (*t, 0))) for c in chunks]
-    L, launches = lib(), c_int(0)
-    sizes = [_workspace_size(L.zb_newton_schulz_workspace, data, len(c)) for data, c in zip(packed, chunks)]
-    if not sizes:
+    if not table:
         return
-    ws = torch.empty(max(sizes), dtype=torch.uint8, device=dev)
+    packed = struct.pack("4Q2q2i" * len(table), *(x for t in table for x in (*t, 0)))
+    L, launches, limit = lib(), c_int(0), NEWTON_SCHULZ_BYTES
+    ws = torch.empty(_workspace_size(L.zb_newton_schulz_workspace, packed, len(table), limit), dtype=torch.uint8, device=dev)
+    _check(L.zb_newton_schulz(packed, len(table), int(muon), lr, momentum, int(nesterov), keep, grad_scale, iterations, *NEWTON_SCHULZ, limit,
+                              _a(ws), ws.numel(), ctypes.addressof(launches), _a(status_word(dev)), _stream()), "newton_schulz")
     global _launches
-    for data, c in zip(packed, chunks):
-        _check(L.zb_newton_schulz(data, len(c), int(muon), lr, momentum, int(nesterov), keep, grad_scale, iterations, *NEWTON_SCHULZ, _a(ws),
-                                  ws.numel(), ctypes.addressof(launches), _a(status_word(dev)), _stream()), "newton_schulz")
-        _launches += launches.value - 1
+    _launches += launches.value - 1
 
 
 def _matrix(t, name: str, i: int, dtypes, dev, shape=None) -> None:
