@@ -147,6 +147,14 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   };
 
+  const bool early = PACKED && later_wave();
+  [[maybe_unused]] PackedTile mine = {};
+  if constexpr (PACKED) {
+    if (early) {
+      chain_wait();
+      mine = load_packed(packed.tiles + blockIdx.y);
+    }
+  }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     mbar_init(k_full, 1);
@@ -173,19 +181,19 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (!DQ) {
-    chain_wait();
+    if (!early) chain_wait();
     chain_trigger();   // behind the wait: the dQ kernel starts on this, under the last CTAs here (chain_late in ptx.cuh)
   }
   if constexpr (PACKED) {
-    kv0 = packed.order_keys[blockIdx.y] * BN;
-    total = packed.total();
-    const int2 first = packed.bounds[kv0], last = packed.bounds[kv0 + BN - 1];
-    const KeyRange r = query_range(first, last, kv0, p.causal, p.window);
+    if (!early) mine = load_packed(packed.tiles + blockIdx.y);
+    kv0 = mine.tile * BN;
+    total = mine.total;
+    const KeyRange r = query_range(mine.first, mine.last, kv0, p.causal, p.window);
     i_lo = r.lo / BM;
     i_hi = r.hi > r.lo ? (r.hi + BM - 1) / BM : i_lo;
     n_iters = (i_hi - i_lo) * rep;
-    all_lo = p.causal ? kv0 + BN - 1 : last.x;
-    all_hi = p.window > 0 ? min(first.y, kv0 + p.window) : first.y;
+    all_lo = p.causal ? kv0 + BN - 1 : mine.last.x;
+    all_hi = p.window > 0 ? min(mine.first.y, kv0 + p.window) : mine.first.y;
   }
 
   if (warp == 8) {
@@ -975,7 +983,7 @@ int zb_flash_bwd3(const void* d_o, const void* qkv, const void* o, const float* 
 // The same three kernels for sequences of different lengths (packed.cu): d_o, o [T, Hq D], qkv and dqkv [T, (Hq + 2 Hkv) D], lse
 // [Hq, T].  The gradient of tokens of no sequence is 0, whatever they hold.  Scratch: stats fp32 [Hq * 2 * T rounded up to 128].
 int zb_packed_attn_bwd(const void* d_o, const void* qkv, const void* o, const float* lse, void* dqkv, float* stats, const void* bounds,
-                       const int* order_tiles, const int* order_keys, int T, int Hq, int Hkv, int D, int causal, int window,
+                       const void* order_tiles, const void* order_keys, int T, int Hq, int Hkv, int D, int causal, int window,
                        float softmax_scale, int* status, cudaStream_t stream) {
   using namespace zb;
   if (T <= 0 || Hq <= 0) return 0;
@@ -984,9 +992,9 @@ int zb_packed_attn_bwd(const void* d_o, const void* qkv, const void* o, const fl
   auto O = static_cast<const __nv_bfloat16*>(o);
   auto QKV = static_cast<const __nv_bfloat16*>(qkv);
   const int s_pad = (T + 127) / 128 * 128;
-  PackedView view = packed_view(bounds, T);
-  view.order_tiles = order_tiles;
-  view.order_keys = order_keys;
+  PackedView view = {};
+  view.bounds = static_cast<const int2*>(bounds);
+  view.tiles = static_cast<const PackedTile*>(order_keys);
   if (int rc = launch_stats(O, DO, lse, stats, 1, T, Hq, D, s_pad, stream, view.bounds)) return rc;
   AttnBwdParams p;
   p.lse = lse; p.delta = nullptr; p.dq_acc = nullptr;
@@ -1005,6 +1013,7 @@ int zb_packed_attn_bwd(const void* d_o, const void* qkv, const void* o, const fl
     }
   };
   if (int rc = D == 128 ? run(std::integral_constant<int, 128>()) : run(std::integral_constant<int, 64>())) return rc;
+  view.tiles = static_cast<const PackedTile*>(order_tiles);
   return attn_bwd_dq(QKV, DO, p, stats, s_pad, D, 1, stream, &view);
 }
 

@@ -86,6 +86,8 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   [[maybe_unused]] int all_lo = 0, all_hi = 0;      // PACKED: keys that every row of the tile sees
   WaitCtx wctx{abort_flag, p.status};
 
+  [[maybe_unused]] PackedTile mine = {};
+  if constexpr (PACKED) mine = load_packed(packed.tiles + blockIdx.y);   // (always late: the plan is older than the kernel before)
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     mbar_init(qdo_full, 1);
@@ -117,14 +119,13 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
   if (!late) chain_wait();
   chain_trigger();
   if constexpr (PACKED) {
-    q0 = packed.order_tiles[blockIdx.y] * BM;
-    total = packed.total();
-    const int2 first = packed.bounds[q0], last = packed.bounds[q0 + BM - 1];
-    const KeyRange r = key_range(first, last, q0, p.causal, p.window);
+    q0 = mine.tile * BM;
+    total = mine.total;
+    const KeyRange r = key_range(mine.first, mine.last, q0, p.causal, p.window);
     j_lo = r.lo / BN;
     n = r.hi > r.lo ? (r.hi + BN - 1) / BN - j_lo : 0;
-    all_lo = p.window > 0 ? max(last.x, q0 + BM - p.window) : last.x;
-    all_hi = p.causal ? min(first.y, q0 + 1) : first.y;
+    all_lo = p.window > 0 ? max(mine.last.x, q0 + BM - p.window) : mine.last.x;
+    all_hi = p.causal ? min(mine.first.y, q0 + 1) : mine.first.y;
   }
 
   if (warp == 8) {

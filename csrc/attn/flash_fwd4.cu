@@ -118,21 +118,19 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   const int n_kv = (p.S + BN - 1) / BN;
   int lo[2], hi[2], j_lo = 0, n_tiles = 0;
   [[maybe_unused]] int total = p.S;               // PACKED: the end of the last sequence
-  [[maybe_unused]] int begin_of_last[2] = {0, 0};  // PACKED: where the sequence of a chain's last row begins
+  [[maybe_unused]] PackedPair mine = {};
   auto tile_ranges = [&] {
     if constexpr (PACKED) {
-      pair = p.packed.order_pairs[blockIdx.y];
-      total = p.packed.total();
+      pair = mine.pair;
+      total = mine.total;
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int q0 = (2 * pair + c) * BM;
       if constexpr (PACKED) {
-        const int2 first = p.packed.bounds[q0], last = p.packed.bounds[q0 + BM - 1];   // (padded to whole pairs)
-        const KeyRange r = key_range(first, last, q0, p.causal, p.window);
+        const KeyRange r = key_range(mine.first[c], mine.last[c], q0, p.causal, p.window);
         lo[c] = r.lo / BN;
         hi[c] = r.hi > r.lo ? (r.hi + BN - 1) / BN : lo[c];
-        begin_of_last[c] = last.x;
       } else {
         lo[c] = 0;
         hi[c] = n_kv;
@@ -145,7 +143,15 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     j_lo = act1 ? (act0 ? min(lo[0], lo[1]) : lo[1]) : lo[0];
     n_tiles = max(max(act0 ? hi[0] : 0, act1 ? hi[1] : 0) - j_lo, 0);
   };
-  if constexpr (!PACKED) tile_ranges();
+  const bool early = PACKED && later_wave();
+  if constexpr (PACKED) {
+    if (early) {
+      chain_wait();
+      mine = load_packed(p.packed.pairs + blockIdx.y);
+    }
+  } else {
+    tile_ranges();
+  }
   WaitCtx wctx{abort_flag, p.status};
 
   // ---- trace ----
@@ -185,8 +191,11 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   chain_trigger();
-  chain_wait();
-  if constexpr (PACKED) tile_ranges();
+  if (!early) chain_wait();
+  if constexpr (PACKED) {
+    if (!early) mine = load_packed(p.packed.pairs + blockIdx.y);
+    tile_ranges();
+  }
 
   if (warp >= 8) {
     setmaxnreg_dec<FWD4_OTHER_REGS>();
@@ -347,9 +356,9 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       const int2 b = p.packed.bounds[row];
       key_lo = p.window > 0 ? max(b.x, row - p.window + 1) : b.x;
       key_hi = p.causal ? min(row + 1, b.y) : b.y;
-      const int last_begin = c ? begin_of_last[1] : begin_of_last[0];
+      const int last_begin = c ? mine.last[1].x : mine.last[0].x, first_end = c ? mine.first[1].y : mine.first[0].y;
       all_lo = p.window > 0 ? max(last_begin, q0 + BM - p.window) : last_begin;
-      all_hi = min(p.packed.bounds[q0].y, p.causal ? q0 + 1 : p.S);
+      all_hi = min(first_end, p.causal ? q0 + 1 : p.S);
     }
     float m_run = -INFINITY, l_run = 0.f;  // m_run in raw (unscaled) score units
     bool ok = true;
@@ -606,7 +615,7 @@ extern "C" int zb_flash_fwd4(const void* qkv, void* out, float* lse, int B, int 
 
 // Sequences of different lengths (packed.cu): qkv [T, (Hq + 2 Hkv) D], out [T, Hq D], lse [Hq, T]; tokens of no sequence get
 // zeros and -inf.  bounds, order_pairs: of zb_pack_sequences for T tokens.
-extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const void* bounds, const int* order_pairs, int T, int Hq,
+extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const void* bounds, const void* order_pairs, int T, int Hq,
                                   int Hkv, int D, int causal, int window, float softmax_scale, int* status, cudaStream_t stream) {
   using namespace zb;
   if (T <= 0 || Hq <= 0) return 0;
@@ -619,8 +628,8 @@ extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const 
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.ldo = Hq * D;
   p.status = status;
-  p.packed = packed_view(bounds, T);
-  p.packed.order_pairs = order_pairs;
+  p.packed.bounds = static_cast<const int2*>(bounds);
+  p.packed.pairs = static_cast<const PackedPair*>(order_pairs);
   auto Q = static_cast<const __nv_bfloat16*>(qkv);
   const int width = (Hq + 2 * Hkv) * D;
   return D == 128 ? launch_fwd4<128, false, 1, true>(Q, width, p, stream) : launch_fwd4<64, false, 1, true>(Q, width, p, stream);

@@ -66,8 +66,8 @@ struct Entry {
   int (*embedding_by_token_workspace)(int, int, long*);
   int (*embedding_by_token)(const long*, const void*, void*, void*, void*, int, int, int, int, int, float, int, cudaStream_t);
   int (*adamw_list)(const void*, int, int, float, float, float, float, float, float, float, cudaStream_t);
-  int (*packed_attn_fwd)(const void*, void*, float*, const void*, const int*, int, int, int, int, int, int, float, int*, cudaStream_t);
-  int (*packed_attn_bwd)(const void*, const void*, const void*, const float*, void*, float*, const void*, const int*, const int*, int, int,
+  int (*packed_attn_fwd)(const void*, void*, float*, const void*, const void*, int, int, int, int, int, int, float, int*, cudaStream_t);
+  int (*packed_attn_bwd)(const void*, const void*, const void*, const float*, void*, float*, const void*, const void*, const void*, int, int,
                          int, int, int, int, float, int*, cudaStream_t);
   int (*rope_at)(void*, const float*, const int*, const int*, int, int, int, int, int, long, int, cudaStream_t);
   int (*newton_schulz_workspace)(const void*, int, long, long*);
@@ -978,14 +978,14 @@ PyObject* packed_attn_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ZB_ARGS(9)
   Packed a = {tensor_of(args[0]), tensor_of(args[1])};
   const Tensor* pairs = tensor_of(args[2]);
-  if (!a.take(args + 3) || !a.order(pairs, (a.T + 255) / 256)) Py_RETURN_NONE;
+  if (!a.take(args + 3) || !a.order(pairs, (a.T + 255) / 256 * 12)) Py_RETURN_NONE;
   Tensor out = fresh({a.T, a.Hq * a.D}, *a.qkv, BF16), lse = fresh({a.Hq, a.T}, *a.qkv, F32);
   const float scale = float(1.0 / std::sqrt(double(a.D)));
   int* status = status_of(*a.qkv);
   const cudaStream_t s = stream();
   if (!launch("packed_attn_fwd", 1, [&] {
         return lib.packed_attn_fwd(ptr(a.qkv), out.data_ptr(), static_cast<float*>(lse.data_ptr()), ptr(a.bounds),
-                                   static_cast<const int*>(ptr(pairs)), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window),
+                                   ptr(pairs), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window),
                                    scale, status, s);
       }))
     return nullptr;
@@ -1002,7 +1002,7 @@ PyObject* packed_attn_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ZB_ARGS(13)
   Packed a = {tensor_of(args[1]), tensor_of(args[4])};
   const Tensor *d_o = tensor_of(args[0]), *o = tensor_of(args[2]), *lse = tensor_of(args[3]), *tiles = tensor_of(args[5]), *keys = tensor_of(args[6]);
-  if (!a.take(args + 7) || !a.order(tiles, (a.T + 127) / 128) || !a.order(keys, (a.T + 127) / 128)) Py_RETURN_NONE;
+  if (!a.take(args + 7) || !a.order(tiles, (a.T + 127) / 128 * 8) || !a.order(keys, (a.T + 127) / 128 * 8)) Py_RETURN_NONE;
   for (const Tensor* t : {d_o, o})
     if (!dense(t, BF16) || t->dim() != 2 || t->size(0) != a.T || t->size(1) != a.Hq * a.D || !on(t, *a.qkv)) Py_RETURN_NONE;
   if (!dense(lse, F32) || lse->dim() != 2 || lse->size(0) != a.Hq || lse->size(1) != a.T || !on(lse, *a.qkv)) Py_RETURN_NONE;
@@ -1013,8 +1013,7 @@ PyObject* packed_attn_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const cudaStream_t s = stream();
   if (!launch("packed_attn_bwd", 3, [&] {
         return lib.packed_attn_bwd(ptr(d_o), ptr(a.qkv), ptr(o), static_cast<const float*>(ptr(lse)), dqkv.data_ptr(),
-                                   static_cast<float*>(stats.data_ptr()), ptr(a.bounds), static_cast<const int*>(ptr(tiles)),
-                                   static_cast<const int*>(ptr(keys)), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window), scale,
+                                   static_cast<float*>(stats.data_ptr()), ptr(a.bounds), ptr(tiles), ptr(keys), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window), scale,
                                    status, s);
       }))
     return nullptr;

@@ -200,12 +200,18 @@ def test_bounds_and_orders(ops, case):
     pk, want = ops.pack_sequences(_offsets(lengths).cuda(), T), packed.pack(_offsets(lengths), T)
     assert torch.equal(pk.bounds.cpu(), want.bounds) and torch.equal(pk.positions.cpu(), want.positions)
     b, total = want.bounds, sum(lengths)
-    pairs, tiles = -(-T // 256), -(-T // 128)
-    works = ([min(T, 256 * (i + 1)) - int(b[256 * i, 0]) for i in range(pairs)], [min(T, 128 * (i + 1)) - int(b[128 * i, 0]) for i in range(tiles)],
-             [max(int(b[max(min(T, 128 * (i + 1), total) - 1, 0), 1]) - 128 * i, 0) for i in range(tiles)])
-    for order, work in zip((pk.order_pairs, pk.order_tiles, pk.order_keys), works):
-        work = [max(w, 0) for w in work]
-        assert order.tolist() == sorted(range(len(work)), key=lambda i: (-work[i], i))
+
+    def of(row):       # the longest sequence first, then as they lie
+        lo, hi = b[row].tolist()
+        return lo - hi, lo
+
+    for records, rows, keys in ((pk.order_pairs, 256, False), (pk.order_tiles, 128, False), (pk.order_keys, 128, True)):
+        count = -(-T // rows)
+        order = sorted(range(count), key=lambda i: (*of(max(min(rows * (i + 1), total) - 1, rows * i)), i) if keys else (*of(rows * i), -i))
+        halves = [torch.tensor(order) * rows + h for h in range(0, rows, 128)]
+        ends = [b[h] for h in halves] + [b[h + 127] for h in halves]           # bounds of the first rows, of the last ones; tile, total
+        all_of_it = torch.cat([*ends, torch.tensor(order)[:, None], torch.full((count, 1), total)], 1)
+        assert torch.equal(records[:, :all_of_it.shape[1]].cpu(), all_of_it.to(torch.int32))
 
 
 @pytest.mark.gpu
@@ -285,8 +291,8 @@ def test_offsets_that_do_not_rise_stay_inside(ops):
     for wrong in ([0, 600, 100, 5000], [-50, 300, 2 ** 31 - 1], [500, 400, 300, 0], [2 ** 31 - 1, -(2 ** 31)], [0, 700, 0, 700]):
         pk = ops.pack_sequences(torch.tensor(wrong, dtype=torch.int32, device="cuda"), T)
         assert ((pk.bounds >= 0) & (pk.bounds <= T)).all()
-        for order, n in ((pk.order_pairs, 3), (pk.order_tiles, 6), (pk.order_keys, 6)):
-            assert sorted(order.tolist()) == list(range(n))
+        for order, n, at in ((pk.order_pairs, 3, 8), (pk.order_tiles, 6, 4), (pk.order_keys, 6, 4)):
+            assert sorted(order[:, at].tolist()) == list(range(n))
         out, lse = ops.packed_attn_fwd(qkv, pk, Hq, Hkv, D)
         ops.packed_attn_bwd(do, qkv, out, lse, pk, Hq, Hkv, D)
         ops.k.check_status()

@@ -45,7 +45,7 @@ def main(argv=None) -> int:
         activation_offload=True if args.offload_activations_to_host else None, lr=args.lr, seed=args.seed,
         backend=args.backend, pipeline_log=plog, shift_labels=args.shift_labels, defer_wgrad=args.defer_wgrad,
         defer_tail_wgrad=args.defer_tail_wgrad, prepost_recv=args.prepost_recv,
-        optimizer=args.optimizer, weight_decay=args.weight_decay, moment_bits=args.moment_bits,
+        optimizer=args.optimizer, weight_decay=args.weight_decay, moment_bits=args.moment_bits, documents=args.documents,
         model_overrides=model_overrides(args),
         p2p_timeout_s=args.p2p_timeout or None,
         p2p_fault_hooks=bool(args.inject_fault) and (":drop" in args.inject_fault or ":delay=" in args.inject_fault))
@@ -134,6 +134,7 @@ def main(argv=None) -> int:
         watchdog.start()
     batch = tr.synthetic_batch()
     inputs, targets, _ = tr.to_device(batch)
+    packed = tr.pack(batch)
     cuda = tr.device.type == "cuda"
     if args.replay_check:
         from ..utils.replay import replay_check
@@ -213,7 +214,7 @@ def main(argv=None) -> int:
             b = torch.cuda.Event(enable_timing=True)
             a.record()
         ti = time.perf_counter()
-        loss = tr.train_step(inputs, targets)
+        loss = tr.train_step(inputs, targets, packed)
         if cuda:
             b.record()
             torch.cuda.synchronize()

@@ -68,8 +68,11 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--no_recompute", action="store_true", help="keep activations instead of recomputing layers")
     p.add_argument("--offload_activations_to_host", action="store_true")
     p.add_argument("--lr", type=float, default=1e-3)
-    p.add_argument("--optimizer", default="adam", choices=["adam", "adamw"],
-                   help="adam: weight decay through the gradient; adamw: decoupled weight decay, all units in one launch")
+    p.add_argument("--optimizer", default="adam", choices=["adam", "adamw", "muon"],
+                   help="adam: weight decay through the gradient; adamw: decoupled weight decay, all units in one launch; muon: the blocks' weight "
+                        "matrices orthogonalised, the rest adamw (shard groups of one rank)")
+    p.add_argument("--documents", type=int, default=0, metavar="TOKENS",
+                   help="synthetic microbatches packed of documents of about this many tokens, each of which attends to itself alone")
     p.add_argument("--weight_decay", type=float, default=0.0)
     p.add_argument("--moment_bits", type=int, default=32, choices=[8, 32],
                    help="adamw: 8 holds both moments in two bytes a parameter instead of eight")

@@ -71,12 +71,16 @@ class AdamConfig:
     weight_decay: float = 0.0
     decoupled: bool = False    # AdamW: the decay acts on the parameters and not through the gradient
     moment_bits: int = 32      # 8 (with `decoupled`): both moments in two bytes a parameter (ops/moments.py) instead of eight
+    muon: bool = False         # (with `decoupled`) the blocks' matrices (`Layer.matrices`) step with Muon (ops/muon.py), the rest with AdamW
+    momentum: float = 0.95     # of Muon
 
     def __post_init__(self):
         if self.moment_bits not in (8, 32):
             raise ValueError(f"moment_bits is 8 or 32, not {self.moment_bits}")
         if self.moment_bits == 8 and not self.decoupled:
             raise ValueError("moments in 8 bits are for AdamW (decoupled weight decay)")
+        if self.muon and (not self.decoupled or self.moment_bits != 32):
+            raise ValueError("Muon goes with decoupled weight decay and moments in 32 bits")
 
 
 @dataclass
@@ -231,6 +235,14 @@ class ZeroUnit:
         self.master = full32[lo:hi].clone()
         del full32
         self.m = self.v = self.moments = None
+        # Muon: the matrices, and the ranges of everything else.  A matrix has a momentum (in m) but no second moment, so v holds the rest's alone
+        self.matrices = layer.matrices() if cfg.adam.muon else []
+        self.rest = [(0, self.shard_n)]
+        if cfg.adam.muon and (self.R > 1 or self.tp_group is not None):
+            raise ValueError("Muon orthogonalises whole matrices: shard groups of one rank, without tensor parallelism")
+        if self.matrices:
+            ends = [0] + [(o + r * c + ALIGN - 1) // ALIGN * ALIGN for o, r, c in self.matrices]
+            self.rest = [(a, b) for a, b in zip(ends, [o for o, _, _ in self.matrices] + [self.shard_n]) if a < b]
         if cfg.adam.moment_bits == 8:
             if self.tp_group is not None:
                 # the blocks of values with one base hold neighbours that differ from slice to slice, so what the slices hold
@@ -239,7 +251,7 @@ class ZeroUnit:
             self.moments = Moments8.zeros(self.shard_n, device)
         else:
             self.m = torch.zeros_like(self.master)
-            self.v = torch.zeros_like(self.master)
+            self.v = torch.zeros(sum(b - a for a, b in self.rest), dtype=torch.float32, device=device)
         self.p_shard = self.master.to(cfg.compute_dtype)
         self.grad_shard: Optional[torch.Tensor] = None  # reduced gradients awaiting optimizer_step
         # ---- transient state -------------------------------------------------------
@@ -556,7 +568,15 @@ class ZeroUnit:
     def state_tensors(self) -> dict[str, torch.Tensor]:
         mine = self.master if self.master is not None else self.host_master
         m, v = (self.m, self.v) if self.moments is None else self.ops.moment_values(self.moments)
+        if self.matrices:
+            v, held = torch.zeros_like(self.m), v
+            for (a, b), part in zip(self.rest, self._of_rest(held)):
+                v[a:b] = part
         return {"master": mine, "m": m, "v": v}
+
+    def _of_rest(self, v: torch.Tensor):
+        """What `v` holds one behind the other for the ranges of `rest`."""
+        return v.split([b - a for a, b in self.rest])
 
     def load_state(self, master: torch.Tensor, m: torch.Tensor, v: torch.Tensor, step: int) -> None:
         self._drop_master()
@@ -568,7 +588,8 @@ class ZeroUnit:
             self.p_shard.copy_(self.master.to(self.cfg.compute_dtype))
         if self.moments is None:
             self.m.copy_(m)
-            self.v.copy_(v)
+            for (a, b), part in zip(self.rest, self._of_rest(self.v)):
+                part.copy_(v[a:b])
         else:
             self.moments.load(m.to(self.device), v.to(self.device))
         self.step_count = step
@@ -576,9 +597,25 @@ class ZeroUnit:
 
 
 def adamw_step(units: list[ZeroUnit], masters: list, grads: list, copies: list, grad_scale: float) -> None:
-    """AdamW on the shards of several units in one launch; their step counts have been raised."""
+    """AdamW on the shards of several units in one launch; their step counts have been raised.  With Muon: on what is no matrix, and
+    Muon on all matrices together."""
     cfg = units[0].cfg
     a, seeds = cfg.adam, None
+    if a.muon:
+        lists = [[], [], [], []]
+        rest = [[], [], [], [], []]
+        for u, p, g, p16 in zip(units, masters, grads, copies):
+            for o, r, c in u.matrices:
+                for out, t in zip(lists, (p, u.m, g, p16)):
+                    out.append(t[o:o + r * c].view(r, c))
+            for (lo, hi), v in zip(u.rest, u._of_rest(u.v)):
+                for out, t in zip(rest, (p[lo:hi], (u.m[lo:hi], v), g[lo:hi], p16[lo:hi], u.step_count)):
+                    out.append(t)
+        if lists[0]:
+            units[0].ops.muon_step(*lists, lr=a.lr, momentum=a.momentum, weight_decay=a.weight_decay, grad_scale=grad_scale)
+        units[0].ops.adamw_step(*rest[:4], lr=a.lr, beta1=a.beta1, beta2=a.beta2, eps=a.eps, weight_decay=a.weight_decay, step=rest[4],
+                                grad_scale=grad_scale)
+        return
     if a.moment_bits == 8:
         # replicas of a shard (hybrid shard) round alike: their seeds are those of the shard
         seeds = [dither_seed(cfg.seed, u.gid, u.lo, u.step_count) for u in units]
@@ -605,7 +642,7 @@ class StageEngine:
             from .fused import FusedZeroUnit
 
             if cfg.adam.decoupled:
-                raise ValueError("the fused reduce-scatter kernel applies Adam: AdamW needs collectives=\"library\"")
+                raise ValueError("the fused reduce-scatter kernel applies Adam: AdamW and Muon need collectives=\"library\"")
             cls = FusedZeroUnit
         self.units = [cls(ly, gid, device=device, cfg=cfg, ops=ops, shard=shard, replicate=replicate, rank=rank,
                           streams=self.streams, zero_level=zero_level, counters=self.counters, meta_init=meta_init,

@@ -9,7 +9,8 @@ caller-provided dict, so a schedule chooses between keeping activations and reco
 
 All math goes through an ops backend (`ops/api.py`): `sm100` kernels or the PyTorch
 oracle.  Tensors are `[tokens, features]`; `ctx["B"]`, `ctx["S"]` give the microbatch
-geometry.
+geometry.  `ctx["packed"]` (`ops/packed.py`): its B S tokens are one stream of sequences of different lengths, each of which
+attends to itself alone and counts its positions from 0.
 """
 from __future__ import annotations
 
@@ -102,6 +103,11 @@ class Layer:
     def backward(self, dy, ctx: dict, ops, saved: dict):
         raise NotImplementedError
 
+    def matrices(self) -> list[tuple[int, int, int]]:
+        """(offset in the flat buffer, rows, columns) of the weights that Muon orthogonalises, each a map of its own: what is stored as one
+        (queries, keys and values; gate and up) apart.  Everything else is AdamW's."""
+        return []
+
     def flops_per_token(self, S: int) -> float:
         return 2.0 * self.num_params()
 
@@ -161,6 +167,16 @@ class TransformerBlock(Layer):
             sp.append(ParamSpec("down_b", (H,), "zeros"))
         return sp
 
+    def matrices(self):
+        lay, out = self.layout()[0], []
+        for name, parts in (("qkv_w", [self.Hq * self.D, self.Hkv * self.D, self.Hkv * self.D]), ("o_w", [self.H]),
+                            ("up_w", [self.F] * (2 if self.act == "swiglu" else 1)), ("down_w", [self.H])):
+            at, (_, cols) = lay[name]
+            for rows in parts:
+                out.append((at, rows, cols))
+                at += rows * cols
+        return out
+
     def _rope(self, ops, S, device):
         if self.rope_theta is None:
             return None
@@ -182,9 +198,12 @@ class TransformerBlock(Layer):
 
     # ---- sub-blocks ---------------------------------------------------------------
     def _attn_fwd(self, xin, resid, ctx, ops, sv):
-        p, B, S = self.p, ctx["B"], ctx["S"]
+        p, B, S, packed = self.p, ctx["B"], ctx["S"], ctx.get("packed")
         ag = self.__dict__.pop("_ag", None)  # left by a fused ZeRO unit: gather the unit inside this GEMM
-        cs = self._rope(ops, S, xin.device)
+        turns = None                         # packed: positions are the sequences' own, so the rotation is a pass by them
+        cs = self._rope(ops, S if packed is None else packed.tokens, xin.device)
+        if packed is not None:
+            cs, turns = None, cs
         if ag is not None:
             qkv = ops.linear_fwd_gather(xin, "qkv_w", ag, p.get("qkv_b"))
             if cs is not None and not self.qk_norm:
@@ -195,7 +214,12 @@ class TransformerBlock(Layer):
             qkv = ops.linear_fwd(xin, p["qkv_w"], p.get("qkv_b"))
         if self.qk_norm:
             qkv = self._head_norm_fwd(qkv, cs, S, ops, sv)
-        att, lse = ops.attn_fwd(qkv, B, S, self.Hq, self.Hkv, self.D, self.causal, self.window)
+        if packed is None:
+            att, lse = ops.attn_fwd(qkv, B, S, self.Hq, self.Hkv, self.D, self.causal, self.window)
+        else:
+            if turns is not None:
+                ops.rope_at_(qkv, turns, packed.positions, self.Hq + self.Hkv, self.D)
+            att, lse = ops.packed_attn_fwd(qkv, packed, self.Hq, self.Hkv, self.D, self.causal, self.window)
         out = ops.linear_fwd(att, p["o_w"], p.get("o_b"), addend=resid)
         if sv is not None:
             sv.update(qkv=qkv, att=att, lse=lse)
@@ -203,12 +227,18 @@ class TransformerBlock(Layer):
 
     def _attn_bwd(self, dout, xin, ctx, ops, sv, dres, later):
         """dout: grad of the o-projection output; returns grad wrt xin (+ dres)."""
-        p, g, B, S = self.p, self.g, ctx["B"], ctx["S"]
+        p, g, B, S, packed = self.p, self.g, ctx["B"], ctx["S"], ctx.get("packed")
         datt = ops.linear_dgrad(dout, p["o_w"])
         ops.linear_wgrad(dout, sv["att"], g["o_w"], g.get("o_b"), later=later)
-        dqkv = ops.attn_bwd(datt, sv["qkv"], sv["att"], sv["lse"], B, S, self.Hq, self.Hkv, self.D, self.causal,
-                            self.window)
-        cs = self._rope(ops, S, dout.device)
+        if packed is None:
+            dqkv = ops.attn_bwd(datt, sv["qkv"], sv["att"], sv["lse"], B, S, self.Hq, self.Hkv, self.D, self.causal,
+                                self.window)
+            cs = self._rope(ops, S, dout.device)
+        else:
+            dqkv = ops.packed_attn_bwd(datt, sv["qkv"], sv["att"], sv["lse"], packed, self.Hq, self.Hkv, self.D, self.causal, self.window)
+            cs, turns = None, self._rope(ops, packed.tokens, dout.device)
+            if turns is not None:
+                ops.rope_at_(dqkv, turns, packed.positions, self.Hq + self.Hkv, self.D, backward=True)
         if self.qk_norm:
             self._head_norm_bwd(dqkv, cs, S, ops, sv)
         elif cs is not None:
@@ -295,9 +325,17 @@ class EmbeddingLayer(Layer):
             sp += [ParamSpec("norm_w", (self.H,), "ones"), ParamSpec("norm_b", (self.H,), "zeros")]
         return sp
 
+    def _places(self, ctx):
+        """Rows of the learned positions in a packed batch: looked up like tokens.  None: position t mod S, or there are none."""
+        packed = ctx.get("packed")
+        return None if packed is None or not self.max_pos else packed.positions.long() + self.pos_offset
+
     def forward(self, ids, ctx, ops, saved=None):
-        S = ctx["S"]
-        e = ops.embedding_fwd(ids.reshape(-1), self.p["tok"], self.p.get("pos"), S, self.pos_offset, scale=self.scale)
+        S, places = ctx["S"], self._places(ctx)
+        if places is None:
+            e = ops.embedding_fwd(ids.reshape(-1), self.p["tok"], self.p.get("pos"), S, self.pos_offset, scale=self.scale)
+        else:
+            e = ops.embedding_fwd(ids.reshape(-1), self.p["tok"], scale=self.scale) + ops.embedding_fwd(places, self.p["pos"])
         if self.post_norm:
             y, st = ops.norm_fwd(e, self.p["norm_w"], self.p["norm_b"], self.eps, True)
             if saved is not None:
@@ -310,8 +348,11 @@ class EmbeddingLayer(Layer):
     def backward(self, dy, ctx, ops, saved):
         if self.post_norm:
             dy = ops.norm_bwd(dy, saved["e"], self.p["norm_w"], saved["st"], None, self.g["norm_w"], self.g["norm_b"], True)
-        ops.embedding_bwd(saved["ids"].reshape(-1), dy, self.g["tok"], self.g.get("pos"), ctx["S"], self.pos_offset,
+        places = self._places(ctx)
+        ops.embedding_bwd(saved["ids"].reshape(-1), dy, self.g["tok"], self.g.get("pos") if places is None else None, ctx["S"], self.pos_offset,
                           scale=self.scale, by_token=self.by_token)
+        if places is not None:      # (each position has a row from every sequence that reaches it)
+            ops.embedding_bwd(places, dy, self.g["pos"], by_token=True)
         return None
 
     def flops_per_token(self, S):

@@ -16,7 +16,7 @@ MOST_AXES = 4
 
 class PackedSequences(NamedTuple):
     """tokens: T.  bounds [T rounded up to 256, 2]: begin and end of each token's sequence.  positions [T]: places within the sequences
-    (0 for tokens of none).  The orders, of the kernels alone: tiles with the most work first."""
+    (0 for tokens of none).  The orders, of the kernels alone: a record for each tile, long sequences first."""
     tokens: int
     bounds: torch.Tensor
     positions: torch.Tensor

@@ -853,9 +853,10 @@ def pack_sequences(offsets, T: int) -> PackedSequences:
     _need(0 <= T <= MOST_TOKENS, f"{T} tokens: at most {MOST_TOKENS}")
     dev, pairs, tiles = offsets.device, -(-T // 256), -(-T // 128)
     bounds = torch.empty(pairs * 256, 2, dtype=torch.int32, device=dev)
-    rest = torch.empty(T + pairs + 2 * tiles, dtype=torch.int32, device=dev).split([T, pairs, tiles, tiles])
-    _check(lib().zb_pack_sequences(_a(offsets), offsets.numel() - 1, T, _a(bounds), *(_a(t) for t in rest), _stream()), "pack_sequences")
-    return PackedSequences(T, bounds, *rest)
+    rest = torch.empty(12 * pairs + 16 * tiles + T, dtype=torch.int32, device=dev).split([12 * pairs, 8 * tiles, 8 * tiles, T])
+    orders = rest[0].view(pairs, 12), rest[1].view(tiles, 8), rest[2].view(tiles, 8)
+    _check(lib().zb_pack_sequences(_a(offsets), offsets.numel() - 1, T, _a(bounds), _a(rest[3]), *(_a(t) for t in orders), _stream()), "pack_sequences")
+    return PackedSequences(T, bounds, rest[3], *orders)
 
 
 def _packed_operands(qkv, pk, Hq, Hkv, D, causal, window):

@@ -185,6 +185,7 @@ class PipelineStage:
         self.wgrad_tail = DeferredWgrad(ops)  # weight gradients held back until the stage's last backward is done
         self.stash = ActivationStash(device, activation_offload, streams.copy)
         self.saved: dict = {}
+        self.packed: dict = {}               # global microbatch -> the sequences it is packed of (`Trainer.train_step`)
         self.loss_sum: Optional[torch.Tensor] = None
         # gradient scale: true mean over every token of the global batch, or the reference's
         # arithmetic (per-microbatch mean, summed over local microbatches, averaged over DP ranks)
@@ -199,6 +200,9 @@ class PipelineStage:
         c = {"B": self.B, "S": self.S, "loss_scale": self.loss_scale}
         if self.tp is not None:
             c["tp"] = self.tp
+        packed = self.packed.get(self.microbatches[mbl])
+        if packed is not None:
+            c["packed"] = packed
         if targets is not None:
             c["targets"] = targets
         return c

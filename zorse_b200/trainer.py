@@ -41,7 +41,7 @@ class TrainerOptions:
     activation_recompute: Optional[bool] = None
     activation_offload: Optional[bool] = None
     lr: float = 1e-3
-    optimizer: str = "adam"                # "adam" (decay through the gradient) | "adamw" (decoupled decay)
+    optimizer: str = "adam"                # "adam" (decay through the gradient) | "adamw" (decoupled decay) | "muon" (blocks' matrices; else adamw)
     weight_decay: float = 0.0
     moment_bits: int = 32                  # adamw: 8 keeps both moments in two bytes a parameter instead of eight
     seed: int = 0
@@ -54,14 +54,15 @@ class TrainerOptions:
     p2p_fault_hooks: bool = False          # wrap the transport so that tests can drop or delay messages (host side)
     prepost_recv: bool = False             # 1F1B: post the next operation's receive ahead (per-boundary p2p groups)
     shift_labels: bool = False             # synthetic targets = next token of the inputs (last position ignored)
+    documents: int = 0                     # synthetic microbatches packed of documents of about this many tokens (0: equal sequences)
 
 
 class Trainer:
     def __init__(self, cfg: PipelineConfig, opt: TrainerOptions):
         if opt.offload_model_params and not opt.optimizer_in_backward:
             raise ValueError("--offload_model_params requires --optimizer_in_backwards")
-        if opt.optimizer not in ("adam", "adamw"):
-            raise ValueError(f"optimizer is adam or adamw, not {opt.optimizer!r}")
+        if opt.optimizer not in ("adam", "adamw", "muon"):
+            raise ValueError(f"optimizer is adam, adamw or muon, not {opt.optimizer!r}")
         if opt.collectives == "fused":
             opt.optimizer_in_backward = True  # the fused reduce-scatter kernel applies Adam itself
         self.cfg, self.opt = cfg, opt
@@ -78,8 +79,8 @@ class Trainer:
             compute_dtype=compute, reduce_dtype=dtype_from_str(cfg.reduce_dtype),
             optimizer_in_backward=opt.optimizer_in_backward, offload_params=opt.offload_model_params,
             collectives=opt.collectives, grad_divide_by_group=cfg.grad_norm_compat == "reference",
-            adam=AdamConfig(lr=opt.lr, weight_decay=opt.weight_decay, decoupled=opt.optimizer == "adamw",
-                            moment_bits=opt.moment_bits), seed=opt.seed)
+            adam=AdamConfig(lr=opt.lr, weight_decay=opt.weight_decay, decoupled=opt.optimizer != "adam",
+                            muon=opt.optimizer == "muon", moment_bits=opt.moment_bits), seed=opt.seed)
         self.streams = Streams(self.device)
         # tensor parallelism: the config numbers lanes of tp processes; everything that follows the plan
         # (stages, microbatches, p2p peers) uses the lane number, the groups use process ranks
@@ -143,6 +144,11 @@ class Trainer:
         g = torch.Generator().manual_seed(cfg_seed(self.opt.seed if seed is None else seed))
         M, B, S = cfg.num_microbatches, cfg.microbatch_size, cfg.sequence_length
         spec = self.spec
+        if self.opt.documents:
+            from .utils.data import random_documents
+
+            batch = random_documents(M, B, S, cfg.vocab_size, self.opt.documents, g)
+            return {k: t.pin_memory() for k, t in batch.items()} if pin and self.device.type == "cuda" else batch
         if spec.family == "vit":
             x = torch.randn(M, B, 3, spec.image, spec.image, generator=g)
             y = torch.randint(0, spec.classes, (M, B), generator=g)
@@ -177,10 +183,32 @@ class Trainer:
             nbytes += t.numel() * t.element_size()
         return inputs, targets, nbytes
 
+    def pack(self, batch: dict) -> Optional[dict]:
+        """What the layers need to know of a batch with "offsets" [M, n + 1] (int32 on the host): microbatch g is one stream of its B S tokens,
+        in which sequence i has the tokens [offsets[g, i], offsets[g, i + 1]) (rows are filled up with their last value; tokens behind
+        it are padding, whose targets the batch ignores).  On every stage, as all of them attend."""
+        offsets = batch.get("offsets")
+        if offsets is None:
+            return None
+        T = self.cfg.microbatch_size * self.cfg.sequence_length
+        if self.spec.family == "vit" or self.spec.pool or self.cfg.tensor_parallel_size > 1:
+            raise ValueError("packed sequences are for token models that predict at every position, without tensor parallelism")
+        if offsets.dtype != torch.int32 or offsets.dim() != 2 or offsets.device.type != "cpu" or offsets.shape[0] != self.cfg.num_microbatches or offsets.shape[1] < 1:
+            raise ValueError(f"offsets {tuple(offsets.shape)}, {offsets.dtype}: expected int32 [{self.cfg.num_microbatches}, sequences + 1] on the host")
+        if bool((offsets[:, 0] != 0).any()) or bool((offsets[:, 1:] < offsets[:, :-1]).any()) or bool((offsets[:, -1] > T).any()):
+            raise ValueError(f"offsets rise from 0 to at most {T} tokens")
+        if self.spec.max_positions and offsets.shape[1] > 1 and int((offsets[:, 1:] - offsets[:, :-1]).max()) > max(self.spec.max_positions, self.cfg.sequence_length):
+            raise ValueError(f"a sequence is longer than the {self.spec.max_positions} learned positions")
+        mine = sorted({g for st in self.stages for g in st.microbatches})
+        rows = offsets.to(self.device, non_blocking=True)
+        return {g: self.ops.pack_sequences(rows[g], T) for g in mine}
+
     # ------------------------------------------------------------------ steps
-    def train_step(self, inputs: dict, targets: dict):
-        """One optimizer step on device-resident microbatches. Returns this rank's share of
+    def train_step(self, inputs: dict, targets: dict, packed: Optional[dict] = None):
+        """One optimizer step on device-resident microbatches (`packed`: of `pack`). Returns this rank's share of
         the mean loss as a device scalar (None on ranks without the last stage)."""
+        for st in self.stages:
+            st.packed = packed or {}
         loss = self.schedule.step(self.step_idx, inputs, targets)
         self.step_idx += 1
         if canary.enabled():
@@ -194,7 +222,7 @@ class Trainer:
         nothing here, raises at its next call."""
         self._raise_kernel_status()
         inputs, targets, _ = self.to_device(batch)
-        loss = self.train_step(inputs, targets)
+        loss = self.train_step(inputs, targets, self.pack(batch))
         if self._status_host is not None:     # rides ahead of the loss on the same stream: one wait for both
             self._status_host.copy_(self.ops.k.status_word(self.device), non_blocking=True)
         if loss is None:

@@ -1,6 +1,8 @@
 """Synthetic data helpers (reference utils/data_loader.py:7-144, utils/loss_funcs.py)."""
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -97,6 +99,39 @@ def shift_labels(tokens: torch.Tensor, ignore_index: int = -100) -> torch.Tensor
     y = torch.full_like(tokens, ignore_index)
     y[..., :-1] = tokens[..., 1:]
     return y
+
+
+def pack_documents(documents, microbatches: int, B: int, S: int, ignore_index: int = -100, pad: int = 0) -> dict:
+    """A batch for `Trainer.train_step_from_host` from token documents (1-D int64 tensors) of any lengths: inputs and targets [M, B, S] and
+    "offsets" [M, n + 1].  Documents lie one after another in each microbatch's B S tokens; one that does not fit goes on in the next
+    microbatch as a sequence of its own.  Targets are the document's next tokens; the last token of each part and what is left
+    over are ignored.  Documents that no microbatch has room for are left out."""
+    T = B * S
+    x, y = torch.full((microbatches, T), pad, dtype=torch.int64), torch.full((microbatches, T), ignore_index, dtype=torch.int64)
+    ends = [[0] for _ in range(microbatches)]
+    m = 0
+    for doc in documents:
+        while doc.numel() and m < microbatches:
+            at = ends[m][-1]
+            n = min(doc.numel(), T - at)
+            x[m, at:at + n] = doc[:n]
+            y[m, at:at + n - 1] = doc[1:n]
+            ends[m].append(at + n)
+            doc = doc[n:]
+            m += at + n == T
+    width = max(len(e) for e in ends)
+    offsets = torch.tensor([e + [e[-1]] * (width - len(e)) for e in ends], dtype=torch.int32)
+    return {"inputs": x.view(microbatches, B, S), "targets": y.view(microbatches, B, S), "offsets": offsets}
+
+
+def random_documents(microbatches: int, B: int, S: int, vocab_size: int, mean: int, generator: torch.Generator) -> dict:
+    """A packed batch of random documents whose lengths spread about `mean` (log-normal), at most S tokens each."""
+    left, docs = microbatches * B * S, []
+    while left > 0:
+        n = int(mean * math.exp(0.8 * float(torch.randn((), generator=generator)) - 0.32))
+        docs.append(torch.randint(0, vocab_size, (min(max(n, 1), S, left),), generator=generator))
+        left -= docs[-1].numel()
+    return pack_documents(docs, microbatches, B, S)
 
 
 class LMLoss(torch.nn.Module):
