@@ -222,7 +222,8 @@ class Trainer:
         nothing here, raises at its next call."""
         self._raise_kernel_status()
         inputs, targets, _ = self.to_device(batch)
-        loss = self.train_step(inputs, targets, self.pack(batch))
+        packed = self.pack(batch)
+        loss = self.train_step(inputs, targets) if packed is None else self.train_step(inputs, targets, packed)
         if self._status_host is not None:     # rides ahead of the loss on the same stream: one wait for both
             self._status_host.copy_(self.ops.k.status_word(self.device), non_blocking=True)
         if loss is None:
