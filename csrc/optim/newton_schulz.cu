@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant_
     if (turned) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) tile_s[ty + 16 * k][tx * 4 + j] = u[k][j];
-    } else if (r < t.rows && c < t.cols) {      // (rows of the workspace are padded to 8)
+    } else if (r < t.rows && c < t.cols) {      // (rows of the workspace are padded to 64)
       *reinterpret_cast<uint2*>(t.x + size_t(r) * t.ld + c) = make_uint2(pack_half2(u[k][0], u[k][1]), pack_half2(u[k][2], u[k][3]));
     }
   }
@@ -292,7 +292,9 @@ struct NsShape {
   long n, m;                       // short and long side
   std::vector<int> members;        // of the list
   size_t at[NS_BUFFERS];           // places in the workspace
-  long ld(int buffer) const { return ((buffer < NS_A ? m : n) + 7) / 8 * 8; }
+  // Rows start on 128-byte lines, so that a row of a box is one line and not parts of two: lists of 3 x 1000 x 333 and 4097 x 641 and the
+  // like 310 -> 265 us.
+  long ld(int buffer) const { return ((buffer < NS_A ? m : n) + 63) / 64 * 64; }
   long cols(int buffer) const { return buffer < NS_A ? m : n; }
 };
 struct NsPlan {
@@ -487,7 +489,7 @@ static int ns_together(const NsMatrix* t, int count, long limit) {
   double room = double(limit);
   for (int i = 0; i < count; ++i) {
     const double n = double(std::min(t[i].rows, t[i].cols)), m = double(std::max(t[i].rows, t[i].cols));
-    room -= 4 * n * (m + 8) + 4 * n * (n + 8) + 8192;
+    room -= 4 * n * (m + 64) + 4 * n * (n + 64) + 8192;
     if (room < 0) return std::max(i, 1);
   }
   return count;

@@ -37,7 +37,8 @@ def svd64(u, iterations=5):
 
 SHAPES = [[(1, 1)], [(1, 7), (7, 1), (2, 2)], [(64, 64)], [(63, 65), (65, 63)], [(33, 300)] * 3, [(300, 33)] * 2 + [(33, 300)], [(256, 256)] * 2,
           [(257, 255)], [(512, 700), (129, 129), (512, 700)], [(1000, 333), (333, 1000)], [(8 + 3 * i, 40 + 5 * i) for i in range(11)], [(16, 2050)],
-          [(31, 17)] * 70, [(800, 801)], [(1025, 513), (513, 1030)]]
+          [(31, 17)] * 70, [(800, 801)], [(1025, 513), (513, 1030)], [(300, 5000)], [(20, 9000), (9000, 20)], [(700, 2500), (40, 40), (90, 4100)],
+          [(1536, 1600)] * 4, [(100 + i, 300) for i in range(9)]]
 
 
 @pytest.mark.parametrize("shapes", [s for s in SHAPES if s[0][0] * s[0][1] < 200000])
