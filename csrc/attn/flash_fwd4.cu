@@ -34,6 +34,7 @@
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "packed.cuh"
+#include "packed_fwd_groups.cuh"
 
 namespace zb {
 
@@ -614,12 +615,16 @@ extern "C" int zb_flash_fwd4(const void* qkv, void* out, float* lse, int B, int 
 }
 
 // Sequences of different lengths (packed.cu): qkv [T, (Hq + 2 Hkv) D], out [T, Hq D], lse [Hq, T]; tokens of no sequence get
-// zeros and -inf.  bounds, order_pairs: of zb_pack_sequences for T tokens.
-extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const void* bounds, const void* order_pairs, int T, int Hq,
-                                  int Hkv, int D, int causal, int window, float softmax_scale, int* status, cudaStream_t stream) {
+// zeros and -inf.  bounds, order_pairs, order_tiles: of zb_pack_sequences for T tokens.
+extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const void* bounds, const void* order_pairs,
+                                  const void* order_tiles, int T, int Hq, int Hkv, int D, int causal, int window, float softmax_scale, int* status, cudaStream_t stream) {
   using namespace zb;
   if (T <= 0 || Hq <= 0) return 0;
   if (int rc = packed_check(T, Hq, Hkv, D)) return rc;
+  if (D == 64 && Hq / Hkv % 2 == 0)
+    return packed_fwd_groups(static_cast<const __nv_bfloat16*>(qkv), static_cast<__nv_bfloat16*>(out), lse, static_cast<const int2*>(bounds),
+                             static_cast<const PackedPair*>(order_pairs), static_cast<const PackedTile*>(order_tiles), T, Hq, Hkv, causal,
+                             window, softmax_scale * 1.4426950408889634f, status, stream);
   AttnFwd4Params p = {};
   p.O = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;

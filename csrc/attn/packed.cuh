@@ -72,15 +72,15 @@ __device__ __forceinline__ KeyRange query_range(int2 first, int2 last, int k0, i
   return r;
 }
 
-// Rows [from, 128) of a tile of 128 rows (64-column blocks of 128-byte rows) become zeros, for the products that a whole warp is
+// Rows [from, ROWS) of a tile of ROWS rows (64-column blocks of 128-byte rows) become zeros, for the products that a whole warp is
 // about to issue.  Only the tile that the last sequence ends in has any: what lies behind it may be anything.
-template <int D>
+template <int D, int ROWS = 128>
 __device__ __forceinline__ void clear_tail_rows(uint32_t tile, int from, int lane) {
-  if (from >= 128) return;   // (the same for the whole warp)
+  if (from >= ROWS) return;   // (the same for the whole warp)
 #pragma unroll 1
-  for (int i = max(from, 0) * 8 + lane; i < 128 * 8; i += 32)
+  for (int i = max(from, 0) * 8 + lane; i < ROWS * 8; i += 32)
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) st_shared_v4(tile + uint32_t(b * 128 * 128 + i * 16), 0u, 0u, 0u, 0u);
+    for (int b = 0; b < D / 64; ++b) st_shared_v4(tile + uint32_t(b * ROWS * 128 + i * 16), 0u, 0u, 0u, 0u);
   fence_proxy_async_smem();
   __syncwarp();
 }

@@ -66,7 +66,7 @@ struct Entry {
   int (*embedding_by_token_workspace)(int, int, long*);
   int (*embedding_by_token)(const long*, const void*, void*, void*, void*, int, int, int, int, int, float, int, cudaStream_t);
   int (*adamw_list)(const void*, int, int, float, float, float, float, float, float, float, cudaStream_t);
-  int (*packed_attn_fwd)(const void*, void*, float*, const void*, const void*, int, int, int, int, int, int, float, int*, cudaStream_t);
+  int (*packed_attn_fwd)(const void*, void*, float*, const void*, const void*, const void*, int, int, int, int, int, int, float, int*, cudaStream_t);
   int (*packed_attn_bwd)(const void*, const void*, const void*, const float*, void*, float*, const void*, const void*, const void*, int, int,
                          int, int, int, int, float, int*, cudaStream_t);
   int (*rope_at)(void*, const float*, const int*, const int*, int, int, int, int, int, long, int, cudaStream_t);
@@ -970,22 +970,24 @@ struct Packed {
     return dense(qkv, BF16) && qkv->dim() == 2 && qkv->size(0) == T && qkv->size(1) == (Hq + 2 * Hkv) * D && fits(qkv->size(1)) &&
            status_of(*qkv) != nullptr && dense(bounds, at::kInt) && bounds->numel() == (T + 255) / 256 * 512 && on(bounds, *qkv);
   }
-  bool order(const Tensor* t, int64_t n) const { return dense(t, at::kInt) && t->numel() == n && on(t, *qkv); }
+  bool order(const Tensor* t, int64_t rows, int64_t words) const {   // records of 256 or 128 rows
+    return dense(t, at::kInt) && t->dim() == 2 && t->size(0) == (T + rows - 1) / rows && t->size(1) == words && on(t, *qkv);
+  }
 };
-// packed_attn_fwd(qkv, bounds, order_pairs, T, Hq, Hkv, D, causal, window) -> (out, lse)
+// packed_attn_fwd(qkv, bounds, order_pairs, order_tiles, T, Hq, Hkv, D, causal, window) -> (out, lse)
 PyObject* packed_attn_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  ZB_ARGS(9)
+  ZB_ARGS(10)
   Packed a = {tensor_of(args[0]), tensor_of(args[1])};
-  const Tensor* pairs = tensor_of(args[2]);
-  if (!a.take(args + 3) || !a.order(pairs, (a.T + 255) / 256 * 12)) Py_RETURN_NONE;
+  const Tensor *pairs = tensor_of(args[2]), *tiles = tensor_of(args[3]);
+  if (!a.take(args + 4) || !a.order(pairs, 256, 12) || !a.order(tiles, 128, 8)) Py_RETURN_NONE;
   Tensor out = fresh({a.T, a.Hq * a.D}, *a.qkv, BF16), lse = fresh({a.Hq, a.T}, *a.qkv, F32);
   const float scale = float(1.0 / std::sqrt(double(a.D)));
   int* status = status_of(*a.qkv);
   const cudaStream_t s = stream();
   if (!launch("packed_attn_fwd", 1, [&] {
         return lib.packed_attn_fwd(ptr(a.qkv), out.data_ptr(), static_cast<float*>(lse.data_ptr()), ptr(a.bounds),
-                                   ptr(pairs), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window),
+                                   ptr(pairs), ptr(tiles), int(a.T), int(a.Hq), int(a.Hkv), int(a.D), a.causal, int(a.window),
                                    scale, status, s);
       }))
     return nullptr;
@@ -1002,7 +1004,7 @@ PyObject* packed_attn_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   ZB_ARGS(13)
   Packed a = {tensor_of(args[1]), tensor_of(args[4])};
   const Tensor *d_o = tensor_of(args[0]), *o = tensor_of(args[2]), *lse = tensor_of(args[3]), *tiles = tensor_of(args[5]), *keys = tensor_of(args[6]);
-  if (!a.take(args + 7) || !a.order(tiles, (a.T + 127) / 128 * 8) || !a.order(keys, (a.T + 127) / 128 * 8)) Py_RETURN_NONE;
+  if (!a.take(args + 7) || !a.order(tiles, 128, 8) || !a.order(keys, 128, 8)) Py_RETURN_NONE;
   for (const Tensor* t : {d_o, o})
     if (!dense(t, BF16) || t->dim() != 2 || t->size(0) != a.T || t->size(1) != a.Hq * a.D || !on(t, *a.qkv)) Py_RETURN_NONE;
   if (!dense(lse, F32) || lse->dim() != 2 || lse->size(0) != a.Hq || lse->size(1) != a.T || !on(lse, *a.qkv)) Py_RETURN_NONE;

@@ -32,15 +32,15 @@ def test_packed_attention(ops, T, Hq, Hkv, D, causal, window):
     qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g, device="cuda").bfloat16()
     do = torch.randn(T, Hq * D, generator=g, device="cuda").bfloat16()
     pk = ops.pack_sequences(torch.tensor([0, 70, 71, T - 9], dtype=torch.int32, device="cuda"), T)
-    native = ops._packed_attn_fwd(qkv, pk.bounds, pk.order_pairs, T, Hq, Hkv, D, causal, window)
+    native = ops._packed_attn_fwd(qkv, pk.bounds, pk.order_pairs, pk.order_tiles, T, Hq, Hkv, D, causal, window)
     wrapped, n = _counted(ops, lambda: ops.k.packed_attn_fwd(qkv, pk, Hq, Hkv, D, causal, window))
     assert _same(native, wrapped) and n == 1
     args = do, qkv, *wrapped
     native, n = _counted(ops, lambda: ops._packed_attn_bwd(*args, pk.bounds, pk.order_tiles, pk.order_keys, T, Hq, Hkv, D, causal, window))
     wrapped, m = _counted(ops, lambda: ops.k.packed_attn_bwd(*args, pk, Hq, Hkv, D, causal, window))
     assert _same(native, wrapped) and n == m == 3
-    fwd = lambda **w: ops._packed_attn_fwd(*{**dict(qkv=qkv, bounds=pk.bounds, order=pk.order_pairs, T=T, Hq=Hq, Hkv=Hkv, D=D, causal=causal, window=window), **w}.values())  # noqa: E731
-    for wrong in (dict(qkv=qkv.float()), dict(qkv=qkv[:-1]), dict(qkv=qkv.cpu()), dict(bounds=pk.bounds[:-1]), dict(order=pk.order_pairs.long()), dict(T=T + 1),
+    fwd = lambda **w: ops._packed_attn_fwd(*{**dict(qkv=qkv, bounds=pk.bounds, order=pk.order_pairs, tiles=pk.order_tiles, T=T, Hq=Hq, Hkv=Hkv, D=D, causal=causal, window=window), **w}.values())  # noqa: E731
+    for wrong in (dict(qkv=qkv.float()), dict(qkv=qkv[:-1]), dict(qkv=qkv.cpu()), dict(bounds=pk.bounds[:-1]), dict(order=pk.order_pairs.long()), dict(T=T + 1), dict(tiles=pk.order_pairs),
                   dict(Hkv=0), dict(D=32), dict(window=-1), dict(causal=False, window=3), dict(order=None)):
         assert fwd(**wrong) is None
     with pytest.raises(ValueError):

@@ -1,5 +1,7 @@
 """Attention over packed sequences: against the formulas in 64 bits sequence by sequence, against differences, and what is refused."""
 import math
+import pathlib
+import re
 
 import pytest
 import torch
@@ -86,6 +88,10 @@ CASES = [  # T, lengths, query heads, key heads, width, causal, window
     (900, [900], 8, 2, 64, True, 1), (511, [400, 111], 2, 2, 64, True, 400), (384, [384], 3, 1, 64, False, 0),
     (600, [129, 60, 127, 200], 6, 2, 128, False, 0), (1027, [50, 700, 13, 260], 4, 4, 64, False, 0), (200, [], 4, 2, 128, False, 0),
     (1500, [1400], 2, 2, 128, True, 0), (2000, [3] * 600, 4, 1, 64, False, 0),
+    # heads of 64 in groups: four or two of them side by side, and the odd groups that are not
+    (1, [1], 4, 1, 64, True, 0), (65, [63, 2], 4, 1, 64, True, 0), (129, [1, 64, 64], 8, 2, 64, False, 0), (1100, [1000, 77], 8, 1, 64, True, 0),
+    (1031, [130, 700, 191], 4, 2, 64, True, 0), (640, [100, 90, 0, 260], 2, 1, 64, True, 37), (900, [64, 64, 500, 200], 12, 2, 64, True, 150), (520, [510], 6, 3, 64, False, 0),
+    (1300, [1300], 16, 2, 64, True, 0),
 ]
 
 
@@ -165,21 +171,39 @@ def test_refusals_cpu(wrapper):
             wrapper.pack_sequences(offsets, T)
     T, Hq, Hkv, D = 6, 4, 2, 64
     qkv, do = _inputs(T, Hq, Hkv, D)
-    order = torch.zeros(1, dtype=torch.int32)
-    pk = packed.PackedSequences(T, torch.zeros(256, 2, dtype=torch.int32), torch.zeros(T, dtype=torch.int32), order, order, order)
+    tiles = torch.zeros(1, 8, dtype=torch.int32)
+    pk = packed.PackedSequences(T, torch.zeros(256, 2, dtype=torch.int32), torch.zeros(T, dtype=torch.int32), torch.zeros(1, 12, dtype=torch.int32), tiles, tiles)
     ok = dict(qkv=qkv, pk=pk, Hq=Hq, Hkv=Hkv, D=D)
     calls = [(wrapper.packed_attn_fwd, ok, []),
              (wrapper.packed_attn_bwd, ok | dict(do=do, o=do, lse=torch.zeros(Hq, T)),
               [dict(do=do[:3]), dict(o=do[:, :64]), dict(do=do.t().contiguous().t()), dict(lse=torch.zeros(T, Hq)), dict(lse=torch.zeros(Hq, T).double())])]
     for call, good, more in calls:
         for wrong in [dict(qkv=qkv[:5]), dict(qkv=qkv.t().contiguous().t()), dict(Hkv=3), dict(Hkv=0), dict(Hq=0), dict(D=32), dict(window=-1),
-                      dict(window=4, causal=False), dict(pk=packed.pack(offsets, T))] + more:
+                      dict(window=4, causal=False), dict(pk=packed.pack(offsets, T)), dict(pk=pk._replace(bounds=pk.bounds[:-1])),
+                      dict(pk=pk._replace(order_keys=tiles.long())), dict(pk=pk._replace(order_pairs=tiles)), dict(pk=pk._replace(tokens=5))] + more:
             with pytest.raises(ValueError):
                 call(**{**good, **wrong})
         with pytest.raises(TypeError):
             call(**{**good, "qkv": qkv.float()})
     with pytest.raises(ValueError):
         get_ops("ref").packed_attn_fwd(qkv, packed.pack(offsets, T), Hq, Hkv, D, False, 4)
+
+
+def test_the_issuer_of_four_chains_walks_as_a_warp_cpu():
+    """As in the kernels of equal sequences: every wait is the warp's, every issue is followed by a warp barrier, nothing is read ahead of chain_wait."""
+    text = (pathlib.Path(__file__).resolve().parent.parent / "csrc/attn/packed_fwd_groups.cuh").read_text()
+    body = text.split("const bool elected = elect_one();")[1]
+    body = body[:body.index("// ----")]
+    assert not re.search(r"\bmbar_wait\(", body)
+    for m in re.finditer(r"if \([^()\n]*\belected\) (\{|[^\n{]*\n)", body):
+        end = m.end()
+        if m.group(1) == "{":
+            depth = 1
+            while depth:
+                depth += {"{": 1, "}": -1}.get(body[end], 0)
+                end += 1
+        assert re.sub(r"//[^\n]*", "", body[end:]).split()[0] == "__syncwarp();"
+    assert text.index("chain_wait();") < text.index("load_packed(") and not re.search(r"__ldg|ld_nc|__restrict__", text)
 
 
 # ------------------------------------------------------------------------------------------------------------------ on the GPU
@@ -240,7 +264,7 @@ def test_forward_and_backward(ops, case):
 @pytest.mark.parametrize("D", [64, 128])
 def test_equal_sequences_as_a_batch(ops, D):
     """Sequences of 256 tokens packed: the bits of the batch of equal sequences."""
-    B, S, Hq, Hkv = 5, 256, 4, 2
+    B, S, Hq, Hkv = 5, 256, 4, 2 if D == 128 else 4         # (heads of 64 in groups have a kernel with other tiles)
     qkv, do = (x.cuda() for x in _inputs(B * S, Hq, Hkv, D))
     pk = ops.pack_sequences(_offsets([S] * B).cuda(), B * S)
     out, lse = ops.packed_attn_fwd(qkv, pk, Hq, Hkv, D)

@@ -358,7 +358,7 @@ class Sm100Ops(_EpilogueOps, _LaterOps):
         return self.k.pack_sequences(offsets, T)
 
     def packed_attn_fwd(self, qkv, pk, Hq, Hkv, D, causal=True, window=0):
-        r = self._packed_attn_fwd(qkv, pk.bounds, pk.order_pairs, pk.tokens, Hq, Hkv, D, causal, window)
+        r = self._packed_attn_fwd(qkv, pk.bounds, pk.order_pairs, pk.order_tiles, pk.tokens, Hq, Hkv, D, causal, window)
         return self.k.packed_attn_fwd(qkv, pk, Hq, Hkv, D, causal, window) if r is None else r
 
     def packed_attn_bwd(self, do, qkv, o, lse, pk, Hq, Hkv, D, causal=True, window=0):

@@ -56,7 +56,7 @@ _SIGNATURES = {
     "zb_flash_fwd4": "pppiiiiiiifipipip", "zb_flash_bwd3": "ppppppiiiiiiifpipip",
     "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
     "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
-    "zb_pack_sequences": "piipppppp", "zb_packed_attn_fwd": "pppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
+    "zb_pack_sequences": "piipppppp", "zb_packed_attn_fwd": "ppppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
     "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pilp", "zb_newton_schulz": "piiffiffiffflplppp",
     "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
@@ -866,7 +866,10 @@ def _packed_operands(qkv, pk, Hq, Hkv, D, causal, window):
     _need(Hq > 0 and Hkv > 0 and Hq % Hkv == 0 and D in (64, 128), f"{Hq} query heads, {Hkv} key heads of {D}: heads of 64 or 128 in whole groups")
     _need(qkv.shape == (pk.tokens, (Hq + 2 * Hkv) * D) and qkv.is_contiguous(),
           f"qkv {tuple(qkv.shape)}: expected contiguous rows of ({Hq} + 2 x {Hkv}) x {D}, one for each of {pk.tokens} tokens")
-    _need(pk.order_pairs is not None and pk.bounds.device == qkv.device, f"the packing is for another backend or device ({pk.bounds.device}, qkv on {qkv.device})")
+    T = pk.tokens
+    _need(0 <= T <= MOST_TOKENS and all(t is not None and t.dtype == torch.int32 and t.is_contiguous() and t.device == qkv.device and t.shape == shape for t, shape in (
+        (pk.bounds, (-(-T // 256) * 256, 2)), (pk.order_pairs, (-(-T // 256), 12)), (pk.order_tiles, (-(-T // 128), 8)), (pk.order_keys, (-(-T // 128), 8)))),
+        f"the packing is not one of {T} tokens made for {qkv.device} (`pack_sequences`)")
 
 
 def packed_attn_fwd(qkv, pk: PackedSequences, Hq: int, Hkv: int, D: int, causal: bool = True, window: int = 0, scale: Optional[float] = None):
@@ -875,7 +878,7 @@ def packed_attn_fwd(qkv, pk: PackedSequences, Hq: int, Hkv: int, D: int, causal:
     T = pk.tokens
     out = torch.empty(T, Hq * D, dtype=qkv.dtype, device=qkv.device)
     lse = torch.empty(Hq, T, dtype=torch.float32, device=qkv.device)
-    _check(lib().zb_packed_attn_fwd(_a(qkv), _a(out), _a(lse), _a(pk.bounds), _a(pk.order_pairs), T, Hq, Hkv, D, int(causal), _window(window, T),
+    _check(lib().zb_packed_attn_fwd(_a(qkv), _a(out), _a(lse), _a(pk.bounds), _a(pk.order_pairs), _a(pk.order_tiles), T, Hq, Hkv, D, int(causal), _window(window, T),
                                     1.0 / math.sqrt(D) if scale is None else scale, _a(status_word(qkv.device)), _stream()), "packed_attn_fwd")
     return out, lse
 
