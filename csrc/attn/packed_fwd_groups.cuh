@@ -5,8 +5,8 @@
 // to itself (2 x 4096 tokens, 32 / 8 heads: 3700 clocks for two tiles of 128 x 128 where the exponentials need 2048).  Here four
 // chains of 128 rows share the unit, with key tiles of 64 so that scores and output of all of them fit tensor memory (4 x (64 + 64) columns).
 // The chains are heads of one group at the same rows (four, or two at two tiles of rows), so they read the same K and V tiles, begin and end
-// together, and a CTA has 128 rows of every sequence it meets, not 256.  4096 x 2 tokens, 32 / 8 heads: 227 -> @LONG us; 8192 tokens in
-// documents of some 700, 32 / 4 heads: 152 -> @DOCS us.
+// together, and a CTA has 128 rows of every sequence it meets, not 256.  4096 x 2 tokens, 32 / 8 heads: 227 -> 192 us; 8192 tokens in
+// documents of some 700, 32 / 4 heads: 154 -> 113 us.
 //
 // Per chain and key tile j:  S = Q K_j^T (SS, fp32 in TMEM);  P = exp2(S c - m c), 128 softmax threads, a row each, over the first 32
 // columns of S as bf16;  O += P V_j (TS).  One warp issues, in the order PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1) ..., and waits for data
@@ -143,63 +143,76 @@ packed_fwd_groups_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gri
       }
     } else if (warp == 16) {
       // ------------------------------ MMA issuer (all chains) ------------------------------
+      // Chains and products are unrolled and places in the ring counted along: with a loop over chains (operands formed product by product) or chains
+      // taken as their weights come in, the issuing itself bounds the kernel (2 x 4096 tokens: 192 us unrolled, 220 and 422).
       const bool elected = elect_one();
       constexpr uint32_t idesc_s = umma_idesc_bf16(BM, BN, false, false);
       constexpr uint32_t idesc_o = umma_idesc_bf16(BM, D, false, true);
+      constexpr uint64_t KV_STEP = Cfg::KV_BYTES >> 4;      // of a descriptor, to the next entry of the ring
+      const uint64_t q_desc = umma_desc_kmajor(smem_u32(sQ)), k_desc = umma_desc_kmajor(smem_u32(sR)), v_desc = umma_desc_mnmajor(smem_u32(sR), BN * 128);
       bool ok = true;
-      auto has = [&](int c, int j) { return j >= lo_of(c) && j < hi_of(c); };
-      auto issue_qk = [&](int c, int j, int slot) -> bool {
-        if (j == lo_of(c)) {
-          if (!mbar_wait_warp(&q_full[c], 0, wctx, ST_TIMEOUT_FULL)) return false;
-          tc_fence_after();
-        }
-        const uint32_t q_addr = smem_u32(sQ + c * Cfg::Q_BYTES), k_addr = smem_u32(sR + slot * Cfg::KV_BYTES);
+      auto has = [&](int c, int j) { return TILES == 1 || (j >= lo_of(c) && j < hi_of(c)); };
+      auto issue_qk = [&](int c, uint64_t k_at) {
         if (elected) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            umma_f16_ss(tmem_base + uint32_t(c * 64), umma_desc_kmajor(q_addr + kk * 32), umma_desc_kmajor(k_addr + kk * 32), idesc_s,
-                        kk != 0 ? 1u : 0u);
+            umma_f16_ss(tmem_base + uint32_t(c * 64), q_desc + uint64_t(c * (Cfg::Q_BYTES >> 4) + kk * 2), k_at + uint64_t(kk * 2), idesc_s, kk != 0 ? 1u : 0u);
           umma_commit(&s_full[c]);
         }
         __syncwarp();
-        return true;
+      };
+      int slot = 0;                 // the ring's entry that comes next
+      uint32_t phase = 0;
+      auto next_entry = [&] {
+        if (++slot == NSLOT) { slot = 0; phase ^= 1; }
       };
       if (n_tiles > 0) {
         ok = mbar_wait_warp(&r_full[0], 0, wctx, ST_TIMEOUT_FULL);
-        tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < CHAINS && ok; ++c)
-          if (has(c, j_lo)) ok = issue_qk(c, j_lo, 0);
+#pragma unroll
+        for (int c = 0; c < CHAINS; ++c)
+          if (ok && has(c, j_lo)) {
+            ok = mbar_wait_warp(&q_full[c], 0, wctx, ST_TIMEOUT_FULL);
+            tc_fence_after();
+            if (ok) issue_qk(c, k_desc);
+          }
         if (ok && elected) umma_commit(&r_empty[0]);
         __syncwarp();
+        next_entry();
       }
-      for (int i = 0; i < n_tiles && ok; ++i) {
-        const int j = j_lo + i, tv = 2 * i + 1, tk = 2 * i + 2;
-        const int vslot = tv % NSLOT, kslot = tk % NSLOT;
-        const bool more = i + 1 < n_tiles;
-        if (!mbar_wait_warp(&r_full[vslot], uint32_t(tv / NSLOT) & 1, wctx, ST_TIMEOUT_FULL)) { ok = false; break; }
-        if (more && !mbar_wait_warp(&r_full[kslot], uint32_t(tk / NSLOT) & 1, wctx, ST_TIMEOUT_FULL)) { ok = false; break; }
+      for (int j = j_lo; j < j_hi && ok; ++j) {
+        const bool more = j + 1 < j_hi;
+        const int vslot = slot;
+        if (!mbar_wait_warp(&r_full[vslot], phase, wctx, ST_TIMEOUT_FULL)) { ok = false; break; }
+        next_entry();
+        const int kslot = slot;
+        if (more && !mbar_wait_warp(&r_full[kslot], phase, wctx, ST_TIMEOUT_FULL)) { ok = false; break; }
+        next_entry();
         tc_fence_after();
-        const uint32_t v_addr = smem_u32(sR + vslot * Cfg::KV_BYTES);
-        clear_tail_rows<D, BN>(v_addr, total - j * BN, lane);   // their weights are 0, but 0 times a NaN is one
-#pragma unroll 1
+        clear_tail_rows<D, BN>(smem_u32(sR + vslot * Cfg::KV_BYTES), total - j * BN, lane);   // their weights are 0, but 0 times a NaN is one
+        const uint64_t v_at = v_desc + uint64_t(vslot) * KV_STEP, k_at = k_desc + uint64_t(kslot) * KV_STEP;
+#pragma unroll
         for (int c = 0; c < CHAINS; ++c) {
-          if (has(c, j)) {
-            if (!mbar_wait_warp(&p_full[c], uint32_t(j - lo_of(c)) & 1, wctx, ST_TIMEOUT_MISC)) { ok = false; break; }
+          if (ok && has(c, j)) {
+            ok = mbar_wait_warp(&p_full[c], uint32_t(j - lo_of(c)) & 1, wctx, ST_TIMEOUT_MISC);
             tc_fence_after();
-            if (elected) {
+            if (ok && elected) {
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)
-                umma_f16_ts(tmem_base + uint32_t(256 + c * 64), tmem_base + uint32_t(c * 64 + kk * 8), umma_desc_mnmajor(v_addr + kk * 2048, BN * 128),
-                            idesc_o, j != lo_of(c) || kk != 0 ? 1u : 0u);
+                umma_f16_ts(tmem_base + uint32_t(256 + c * 64), tmem_base + uint32_t(c * 64 + kk * 8), v_at + uint64_t(kk * 128), idesc_o,
+                            j != lo_of(c) || kk != 0 ? 1u : 0u);
               if (j == hi_of(c) - 1) umma_commit(&o_done[c]);
             }
             __syncwarp();
           }
-          if (more && has(c, j + 1) && !issue_qk(c, j + 1, kslot)) { ok = false; break; }
+          if (ok && more && has(c, j + 1)) {
+            if (TILES > 1 && j + 1 == lo_of(c)) {
+              ok = mbar_wait_warp(&q_full[c], 0, wctx, ST_TIMEOUT_FULL);
+              tc_fence_after();
+            }
+            if (ok) issue_qk(c, k_at);
+          }
         }
-        if (!ok) break;
-        if (elected) {
+        if (ok && elected) {
           umma_commit(&r_empty[vslot]);
           if (more) umma_commit(&r_empty[kslot]);
         }
