@@ -270,6 +270,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       constexpr uint32_t idesc_dq = umma_idesc_bf16(128, D == 128 ? 128 : D, true, true);
       const uint32_t k_addr = smem_u32(sK), v_addr = smem_u32(sV), ds_addr = smem_u32(sDS);
       const uint32_t r_dp = tmem_base + Cfg::DP_COL;
+      const uint64_t k_desc = umma_desc_kmajor(k_addr), v_desc = umma_desc_kmajor(v_addr);
       auto r_s = [&](int it) { return tmem_base + (NSB == 2 && (it & 1) ? uint32_t(Cfg::S1_COL) : 0u); };
       bool ok = mbar_wait_warp(k_full, 0, wctx, ST_TIMEOUT_FULL);
       [[maybe_unused]] int tile_a = i_lo, tile_b = i_lo;   // PACKED: query tiles of the next A and the next B
@@ -283,11 +284,12 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       auto issue_a = [&](int it) {  // S^T = K Q^T
         clear_next(smem_u32(sQ + (it % QS) * Cfg::TILE_BYTES), tile_a);
         if (elected) {
-          const uint32_t q_addr = smem_u32(sQ + (it % QS) * Cfg::TILE_BYTES), d = r_s(it);
+          const uint64_t q_desc = umma_desc_kmajor(smem_u32(sQ + (it % QS) * Cfg::TILE_BYTES));
+          const uint32_t d = r_s(it);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = uint32_t(kk / 4) * BLK + uint32_t(kk % 4) * 32;
-            umma_f16_ss(d, umma_desc_kmajor(k_addr + off), umma_desc_kmajor(q_addr + off), idesc_s, kk != 0 ? 1u : 0u);
+            umma_f16_ss(d, umma_desc_add(k_desc, off), umma_desc_add(q_desc, off), idesc_s, kk != 0 ? 1u : 0u);
           }
           umma_commit(&s_full[it % NSB]);
         }
@@ -296,10 +298,11 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       auto issue_b = [&](uint32_t do_addr) {  // dP^T = V dO^T
         clear_next(do_addr, tile_b);
         if (elected) {
+          const uint64_t do_desc = umma_desc_kmajor(do_addr);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = uint32_t(kk / 4) * BLK + uint32_t(kk % 4) * 32;
-            umma_f16_ss(r_dp, umma_desc_kmajor(v_addr + off), umma_desc_kmajor(do_addr + off), idesc_s, kk != 0 ? 1u : 0u);
+            umma_f16_ss(r_dp, umma_desc_add(v_desc, off), umma_desc_add(do_desc, off), idesc_s, kk != 0 ? 1u : 0u);
           }
           umma_commit(dp_full);
         }
@@ -320,7 +323,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
       for (int it = 0; it < n_iters && ok; ++it) {
         const int st = it % QS;
-        const uint32_t q_addr = smem_u32(sQ + st * Cfg::TILE_BYTES), do_addr = smem_u32(sDO + st * Cfg::TILE_BYTES);
+        const uint64_t q_desc = umma_desc_mnmajor(smem_u32(sQ + st * Cfg::TILE_BYTES), BLK), do_desc = umma_desc_mnmajor(smem_u32(sDO + st * Cfg::TILE_BYTES), BLK);
         if (NSB == 2 && it + 1 < n_iters) {   // its buffer last held P^T of step it - 1, read by the D queued before this
           const int sn = (it + 1) % QS;
           if (!mbar_wait_warp(&q_full[sn], uint32_t((it + 1) / QS) & 1, wctx, ST_TIMEOUT_FULL)) break;
@@ -341,7 +344,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
           for (int kk = 0; kk < BM / 16; ++kk) {
             const uint32_t acol = uint32_t(kk / 4) * 64 + uint32_t(kk % 4) * 8;
-            umma_f16_ts(tmem_base + Cfg::DV_COL, r_s(it) + acol, umma_desc_mnmajor(do_addr + kk * 2048, BLK), idesc_dkv,
+            umma_f16_ts(tmem_base + Cfg::DV_COL, r_s(it) + acol, umma_desc_add(do_desc, kk * 2048), idesc_dkv,
                         (it | kk) != 0 ? 1u : 0u);
           }
           umma_commit(&do_empty[st]);     // B_i and D_i are dO_i's readers
@@ -366,7 +369,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
           for (int kk = 0; kk < BM / 16; ++kk) {
             const uint32_t acol = uint32_t(kk / 4) * 64 + uint32_t(kk % 4) * 8;
-            umma_f16_ts(tmem_base + Cfg::DK_COL, r_dp + acol, umma_desc_mnmajor(q_addr + kk * 2048, BLK), idesc_dkv,
+            umma_f16_ts(tmem_base + Cfg::DK_COL, r_dp + acol, umma_desc_add(q_desc, kk * 2048), idesc_dkv,
                         (it | kk) != 0 ? 1u : 0u);
           }
           umma_commit(&q_empty[st]);

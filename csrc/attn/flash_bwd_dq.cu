@@ -165,18 +165,19 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       const bool elected = elect_one();
       constexpr uint32_t idesc_s = umma_idesc_bf16(BM, BN, false, false);   // K-major A and B
       constexpr uint32_t idesc_dq = umma_idesc_bf16(BM, D, false, true);    // A from TMEM, B = K tile [keys][d] (N-major)
-      const uint32_t q_addr = smem_u32(sQ), do_addr = smem_u32(sDO);
+      const uint32_t do_addr = smem_u32(sDO);
+      const uint64_t q_desc = umma_desc_kmajor(smem_u32(sQ)), do_desc = umma_desc_kmajor(do_addr);
       auto k_of = [&](int i) { return smem_u32(sK + (i % NK) * Cfg::TILE_BYTES); };
       auto v_of = [&](int i) { return smem_u32(sV + (i % NV) * Cfg::TILE_BYTES); };
       auto issue_s = [&](int i) {    // S_i = Q K_i^T into S[i & 1]
         // PACKED: what lies behind the last sequence (K, V, dO) meets weights of 0 in products, and 0 times a NaN is one
         if constexpr (PACKED) clear_tail_rows<D>(k_of(i), total - (j_lo + i) * BN, lane);
         if (elected) {
-          const uint32_t k_addr = k_of(i);
+          const uint64_t k_desc = umma_desc_kmajor(k_of(i));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = uint32_t(kk / 4) * BLK + uint32_t(kk % 4) * 32;
-            umma_f16_ss(tmem_base + uint32_t((i & 1) * 128), umma_desc_kmajor(q_addr + off), umma_desc_kmajor(k_addr + off),
+            umma_f16_ss(tmem_base + uint32_t((i & 1) * 128), umma_desc_add(q_desc, off), umma_desc_add(k_desc, off),
                         idesc_s, kk != 0 ? 1u : 0u);
           }
           umma_commit(&s_full[i & 1]);
@@ -186,11 +187,11 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       auto issue_dp = [&](int i) {   // dP_i = dO V_i^T
         if constexpr (PACKED) clear_tail_rows<D>(v_of(i), total - (j_lo + i) * BN, lane);
         if (elected) {
-          const uint32_t v_addr = v_of(i);
+          const uint64_t v_desc = umma_desc_kmajor(v_of(i));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = uint32_t(kk / 4) * BLK + uint32_t(kk % 4) * 32;
-            umma_f16_ss(tmem_base + Cfg::DP_COL, umma_desc_kmajor(do_addr + off), umma_desc_kmajor(v_addr + off), idesc_s,
+            umma_f16_ss(tmem_base + Cfg::DP_COL, umma_desc_add(do_desc, off), umma_desc_add(v_desc, off), idesc_s,
                         kk != 0 ? 1u : 0u);
           }
           umma_commit(dp_full);
@@ -217,13 +218,13 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         tc_fence_after();
         // dQ += dS_i K_i (reduction over the 128 keys; the bf16 A operand sits in the first 32 columns of each
         // 64-column half of S[i & 1])
-        const uint32_t k_addr = k_of(i);
+        const uint64_t k_desc = umma_desc_mnmajor(k_of(i), BLK);
         const uint32_t s_col = tmem_base + uint32_t((i & 1) * 128);
         if (elected) {
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk) {
             const uint32_t acol = uint32_t(kk / 4) * 64 + uint32_t(kk % 4) * 8;
-            umma_f16_ts(tmem_base + Cfg::DQ_COL, s_col + acol, umma_desc_mnmajor(k_addr + kk * 2048, BLK), idesc_dq,
+            umma_f16_ts(tmem_base + Cfg::DQ_COL, s_col + acol, umma_desc_add(k_desc, kk * 2048), idesc_dq,
                         (i | kk) != 0 ? 1u : 0u);
           }
           umma_commit(&k_empty[i % NK]);     // S_i (queued earlier) and dQ_i are K_i's readers

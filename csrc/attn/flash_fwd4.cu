@@ -249,13 +249,13 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
             if (!mbar_wait_warp(&q_full[c], 0, wctx, ST_TIMEOUT_FULL)) return false;
             tc_fence_after();
           }
-          const uint32_t q_addr = smem_u32(sQ + c * Cfg::TILE_BYTES), k_addr = smem_u32(sR + slot * Cfg::TILE_BYTES);
+          const uint64_t q_desc = umma_desc_kmajor(smem_u32(sQ + c * Cfg::TILE_BYTES)), k_desc = umma_desc_kmajor(smem_u32(sR + slot * Cfg::TILE_BYTES));
           const uint32_t s_col = tmem_base + uint32_t(c * 128);
           if (elected) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = uint32_t(kk / 4) * BLK + uint32_t(kk % 4) * 32;
-              umma_f16_ss(s_col, umma_desc_kmajor(q_addr + off), umma_desc_kmajor(k_addr + off), idesc_s, kk != 0 ? 1u : 0u);
+              umma_f16_ss(s_col, umma_desc_add(q_desc, off), umma_desc_add(k_desc, off), idesc_s, kk != 0 ? 1u : 0u);
             }
             umma_commit(&s_full[c]);
           }
@@ -284,6 +284,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
           tr(TR_MMA_V_READY);
           bool k_ready = false;
           const uint32_t v_addr = smem_u32(sR + vslot * Cfg::TILE_BYTES);
+          const uint64_t v_desc = umma_desc_mnmajor(v_addr, BLK);
           if constexpr (PACKED) clear_tail_rows<D>(v_addr, total - j * BN, lane);   // their weights are 0, but 0 times a NaN is one
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
@@ -301,7 +302,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 #pragma unroll
                   for (int k4 = 0; k4 < 4; ++k4) {
                     const int kk = h * 4 + k4;
-                    umma_f16_ts(o_col, s_col + uint32_t(kk * 8), umma_desc_mnmajor(v_addr + kk * 16 * 128, BLK), idesc_o,
+                    umma_f16_ts(o_col, s_col + uint32_t(kk * 8), umma_desc_add(v_desc, kk * 16 * 128), idesc_o,
                                 (pv_done[c] | kk) != 0 ? 1u : 0u);
                   }
                 }

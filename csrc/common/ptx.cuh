@@ -366,6 +366,9 @@ __device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t
   d |= uint64_t(2) << 61;
   return d;
 }
+// The descriptor of a place `bytes` further on (a multiple of 16).  An issuer forms a tile's descriptor once and goes on by additions: formed
+// product by product they are five instructions each, which the issuing of short products waits for.
+__device__ __forceinline__ uint64_t umma_desc_add(uint64_t desc, uint32_t bytes) { return desc + uint64_t(bytes >> 4); }
 // K-major tile: rows of 64 bf16 (128 B); 8-row groups are 1024 B apart.
 __device__ __forceinline__ uint64_t umma_desc_kmajor(uint32_t smem_addr) {
   return umma_desc_sw128(smem_addr, 16, 1024);

@@ -187,10 +187,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) n
           if (!mbar_wait_warp(&full[stage], phase, wctx, ST_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * Cfg::STAGE_BYTES), sb = sa + Cfg::A_BYTES;
+          const uint64_t a_desc = umma_desc_kmajor(sa), b_desc = umma_desc_sw128(sb, b_lbo, 1024);
           if (elected) {
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk)
-              umma_f16_ss_pair(d_tmem, umma_desc_kmajor(sa + kk * 32), umma_desc_sw128(sb + kk * b_step, b_lbo, 1024), idesc,
+              umma_f16_ss_pair(d_tmem, umma_desc_add(a_desc, kk * 32), umma_desc_add(b_desc, kk * b_step), idesc,
                                kb != 0 || kk != 0 ? 1u : 0u);
             umma_commit_pair(&empty[stage]);
           }
