@@ -147,14 +147,6 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   };
 
-  const bool early = PACKED && later_wave();
-  [[maybe_unused]] PackedTile mine = {};
-  if constexpr (PACKED) {
-    if (early) {
-      chain_wait();
-      mine = load_packed(packed.tiles + blockIdx.y);
-    }
-  }
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     mbar_init(k_full, 1);
@@ -181,11 +173,11 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   if constexpr (!DQ) {
-    if (!early) chain_wait();
+    chain_wait();
     chain_trigger();   // behind the wait: the dQ kernel starts on this, under the last CTAs here (chain_late in ptx.cuh)
   }
   if constexpr (PACKED) {
-    if (!early) mine = load_packed(packed.tiles + blockIdx.y);
+    const PackedTile mine = load_packed(packed.tiles + blockIdx.y);
     kv0 = mine.tile * BN;
     total = mine.total;
     const KeyRange r = query_range(mine.first, mine.last, kv0, p.causal, p.window);

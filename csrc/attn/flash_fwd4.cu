@@ -144,15 +144,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     j_lo = act1 ? (act0 ? min(lo[0], lo[1]) : lo[1]) : lo[0];
     n_tiles = max(max(act0 ? hi[0] : 0, act1 ? hi[1] : 0) - j_lo, 0);
   };
-  const bool early = PACKED && later_wave();
-  if constexpr (PACKED) {
-    if (early) {
-      chain_wait();
-      mine = load_packed(p.packed.pairs + blockIdx.y);
-    }
-  } else {
-    tile_ranges();
-  }
+  if constexpr (!PACKED) tile_ranges();
   WaitCtx wctx{abort_flag, p.status};
 
   // ---- trace ----
@@ -192,9 +184,9 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   chain_trigger();
-  if (!early) chain_wait();
+  chain_wait();
   if constexpr (PACKED) {
-    if (!early) mine = load_packed(p.packed.pairs + blockIdx.y);
+    mine = load_packed(p.packed.pairs + blockIdx.y);
     tile_ranges();
   }
 

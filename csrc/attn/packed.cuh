@@ -11,9 +11,7 @@ namespace zb {
 
 constexpr int PACK_PAD = 256;
 
-// A tile (or pair of tiles) as it is dealt out, with all that a CTA needs before it knows its loads: read in one go.  Number by number out of
-// the bounds, behind the tile's own number, a CTA began 0.5 us later (16 x 1024 tokens, 32 / 8 heads of 128, fourteen waves: 224 us
-// against 214 of equal sequences without bounds).
+// A tile (or pair of tiles) as it is dealt out, with all that a CTA needs before it knows its loads: read in one go.
 struct alignas(16) PackedTile {
   int2 first, last;         // bounds of its first and last row
   int tile, total;          // total: the end of the last sequence
@@ -37,12 +35,6 @@ __device__ __forceinline__ T load_packed(const T* p) {
   for (int i = 0; i < int(sizeof(T) / 16); ++i) to[i] = ld_v4(reinterpret_cast<const uint4*>(p) + i);
   return r;
 }
-// Whether this CTA is not among the first on the GPU: the kernel before is most likely done when it starts, so its wait costs nothing and what
-// it reads first can come ahead of the set-up of barriers and tensor memory.
-__device__ __forceinline__ bool later_wave() {
-  return blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z) >= 148u;
-}
-
 inline int packed_rows(int T) { return (T + PACK_PAD - 1) / PACK_PAD * PACK_PAD; }   // entries of bounds
 
 // Sizes that the packed kernels take: tiles are the grid's second dimension, at most 65535 of 128 rows.
