@@ -240,3 +240,22 @@ def test_alignment_streams_graphs_and_repeats(ops):
     empty = torch.zeros(0, 5, device="cuda")
     assert ops.orthogonalize([empty, g[0]])[0].shape == (0, 5)
     ops.muon_step([empty], [empty.clone()], [empty.clone()], [None], lr=1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("turned", [False, True])
+def test_offsets_that_pass_32_bits(ops, turned):
+    """16 entries, each the only one of its row and column, the last of all among them: one iteration takes each by its polynomial."""
+    n, m = 40000, 53999
+    shape = (m, n) if turned else (n, m)
+    assert n * m > 2 ** 31
+    u = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    rows, cols = (torch.linspace(3, size - 1, 16, device="cuda").long() for size in shape)
+    u[rows, cols] = 2.0
+    a, b, c = muon.COEFFICIENTS
+    s = 1 / 4                # 2 / ||U||
+    got = ops.orthogonalize([u], 1)[0]
+    want = a * s + b * s ** 3 + c * s ** 5
+    assert ((got[rows, cols].double() - want).abs() <= (FROBENIUS + HALF) * want).all()
+    assert int((got != 0).sum()) == 16
+    ops.k.check_status()

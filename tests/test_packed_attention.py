@@ -329,3 +329,28 @@ def test_no_tokens(ops):
     out, lse = ops.packed_attn_fwd(qkv, pk, 2, 1, 64)
     assert out.shape == (0, 128) and lse.shape == (2, 0)
     assert ops.packed_attn_bwd(out, qkv, out, lse, pk, 2, 1, 64).shape == qkv.shape
+
+
+@pytest.mark.gpu
+def test_offsets_that_pass_32_bits(ops):
+    """Rows on both sides of element 2^31 of qkv, and the last: the same bits as of their sequences alone, which lie on the same tiles.
+    (Gradients of keys and values only nearly: a short batch divides a group's query heads among more CTAs, so sums go in another order.)"""
+    n, count, Hq, Hkv, D = 1024, 342, 48, 1, 128
+    T = n * count
+    assert T * Hq * D > 2 ** 31
+    torch.manual_seed(0)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16, device="cuda")
+    do = torch.randn(T, Hq * D, dtype=torch.bfloat16, device="cuda")
+    pk = ops.pack_sequences(torch.arange(count + 1, dtype=torch.int32, device="cuda") * n, T)
+    out, lse = ops.packed_attn_fwd(qkv, pk, Hq, Hkv, D)
+    grad = ops.packed_attn_bwd(do, qkv, out, lse, pk, Hq, Hkv, D)
+    one = ops.pack_sequences(torch.tensor([0, n], dtype=torch.int32, device="cuda"), n)
+    for i in (0, 2 ** 31 // qkv.shape[1] // n, count - 1):
+        at = slice(i * n, i * n + n)
+        o, s = ops.packed_attn_fwd(qkv[at], one, Hq, Hkv, D)
+        assert torch.equal(o, out[at]) and torch.equal(s, lse[:, at])
+        dq = slice(0, Hq * D)
+        assert torch.equal(ops.packed_attn_bwd(do[at], qkv[at], o, s, one, Hq, Hkv, D)[:, dq], grad[at][:, dq])
+        want, off, size = backward64(do[at], qkv[at], o, s, [n], Hq, Hkv, D, True, 0)
+        assert ((grad[at].double() - want).abs() <= HALF * (off + want.abs()) + HALF ** 2 * off + FP32 * size).all()
+    ops.k.check_status()

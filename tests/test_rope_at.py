@@ -138,3 +138,17 @@ def test_strides_streams_graphs_and_positions_outside(ops):
     assert torch.equal(got, ops.rope_at_(buf.cuda(), cs, outside.clamp(0, 49), heads, d, sections))
     assert ops.rope_at_(buf[:0].cuda(), cs, positions[:, :0].contiguous(), heads, d, sections).shape == (0, heads * d)
     assert torch.equal(ops.rope_at_(buf.cuda(), cs, positions, 0, d, sections).cpu(), buf)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [128, 90])
+def test_offsets_that_pass_32_bits(ops, d):
+    T, heads, sections = 300000, 60 * 128 // d, [d // 4, d // 2 - d // 4]
+    assert T * heads * d > 2 ** 31
+    torch.manual_seed(0)
+    buf = torch.randn(T, heads * d, dtype=torch.bfloat16, device="cuda")
+    cs, positions = torch.randn(500, d, device="cuda"), torch.randint(0, 500, (2, T), dtype=torch.int32, device="cuda")
+    near = 2 ** 31 // (heads * d)
+    rows = torch.tensor([0, near - 1, near, near + 1, T - 1], device="cuda")
+    want = ops.rope_at_(buf[rows], cs, positions[:, rows].contiguous(), heads, d, sections)
+    assert torch.equal(ops.rope_at_(buf, cs, positions, heads, d, sections)[rows], want)
