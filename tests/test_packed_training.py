@@ -114,6 +114,22 @@ def test_refused_batches():
     assert tr.pack({"inputs": batch["inputs"]}) is None
 
 
+def test_replays_take_the_packing():
+    from zorse_b200.utils.replay import replay_check
+
+    tr = Trainer(_cfg(), TrainerOptions(schedule="1f1b", ops="ref", model_overrides={"layers": 2}, documents=9))
+    batch = tr.synthetic_batch()
+    inputs, targets, _ = tr.to_device(batch)
+    rep = replay_check(tr, inputs, targets, packed=tr.pack(batch))
+    one = Trainer(_cfg(), TrainerOptions(schedule="1f1b", ops="ref", model_overrides={"layers": 2}, documents=9))
+    want = float(one.train_step(inputs, targets, one.pack(batch)))
+    assert rep["identical"] and rep["loss"] == (want, want)
+    plain = Trainer(_cfg(), TrainerOptions(schedule="1f1b", ops="ref", model_overrides={"layers": 2}))
+    assert float(plain.train_step(inputs, targets)) != want
+    with pytest.raises(ValueError, match="documents"):
+        Trainer(_cfg(), TrainerOptions(schedule="1f1b", ops="ref", documents=-3))
+
+
 # ------------------------------------------------------------------------------------------------------------------ Muon
 def _engine(device="cpu", **kw):
     spec = registry.get_spec("tiny_llama", vocab=512, layers=2, kv_heads=2, **SMALL)

@@ -139,7 +139,7 @@ def main(argv=None) -> int:
     if args.replay_check:
         from ..utils.replay import replay_check
 
-        rep = replay_check(tr, inputs, targets)
+        rep = replay_check(tr, inputs, targets, packed=packed)
         log.info(f"replay check: identical={rep['identical']} loss={rep['loss']} "
                  f"differing units={[(d['gid'], d['kind'], d['max_abs_diff']) for d in rep['differing_units']]}",
                  leader_only=False)

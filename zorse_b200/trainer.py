@@ -63,6 +63,8 @@ class Trainer:
             raise ValueError("--offload_model_params requires --optimizer_in_backwards")
         if opt.optimizer not in ("adam", "adamw", "muon"):
             raise ValueError(f"optimizer is adam, adamw or muon, not {opt.optimizer!r}")
+        if opt.documents < 0:
+            raise ValueError(f"documents of {opt.documents} tokens")
         if opt.collectives == "fused":
             opt.optimizer_in_backward = True  # the fused reduce-scatter kernel applies Adam itself
         self.cfg, self.opt = cfg, opt

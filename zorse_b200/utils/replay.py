@@ -44,17 +44,17 @@ def compare(a: list[dict], b: list[dict]) -> list[dict]:
     return diffs
 
 
-def replay_check(trainer, inputs, targets, tolerance: float = 0.0) -> dict:
-    """Steps once, rewinds, steps again. Leaves the trainer one step further (second run's state).
+def replay_check(trainer, inputs, targets, tolerance: float = 0.0, packed=None) -> dict:
+    """Steps once, rewinds, steps again (`packed`: of `Trainer.pack`). Leaves the trainer one step further (second run's state).
     Returns {"identical", "within_tolerance", "differing_units", "loss"}."""
     before = snapshot(trainer)
     step0 = trainer.step_idx
-    l1 = trainer.train_step(inputs, targets)
+    l1 = trainer.train_step(inputs, targets, packed)
     first = snapshot(trainer)
     l1 = None if l1 is None else float(l1)
     restore(trainer, before)
     trainer.step_idx = step0
-    l2 = trainer.train_step(inputs, targets)
+    l2 = trainer.train_step(inputs, targets, packed)
     second = snapshot(trainer)
     l2 = None if l2 is None else float(l2)
     diffs = compare(first, second)
