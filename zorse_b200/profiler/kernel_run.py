@@ -7,7 +7,8 @@ cases: gemm_fwd | gemm_dgrad | gemm_wgrad | gemm_act_fwd | gemm_act_bwd | gemm_r
        flash_bwd | flash_bwd3 | flash_bwd3_dkv | flash_bwd3_dq (flash_bwd: the default version; the last three also as
        flash64_bwd3... on grouped heads of 64) | rmsnorm | rmsnorm_bwd | layernorm_bwd | rope | swiglu_fwd | swiglu_bwd |
        embedding_fwd | embedding_bwd | adam | ce | qk_norm_rope_fwd | qk_norm_rope_bwd | embedding_scaled | embedding_by_token |
-       adamw_list | adamw_list8 | moment_values
+       adamw_list | adamw_list8 | moment_values | pack_sequences | packed_attn_fwd | packed_attn_bwd (the last two also as packed64_attn_... on
+       grouped heads of 64) | rope_at | orthogonalize | muon_step
 Prints the median CUDA-event time of the repetitions (a 256 MB write between them keeps operands out of L2).
 """
 from __future__ import annotations
@@ -125,6 +126,28 @@ def main(argv=None):
         table, dout, dtable = rnd(32000, 4096), rnd(32768, 4096), torch.zeros(32000, 4096, device=dev)
         fn = (lambda: k.embedding_scaled(ids, table, scale=64.0)) if case.endswith("scaled") else (
             lambda: k.embedding_by_token(ids, dout, dtable, scale=64.0))
+    elif case in ("pack_sequences", "packed_attn_fwd", "packed_attn_bwd", "packed64_attn_fwd", "packed64_attn_bwd", "rope_at"):
+        T, Hq, Hkv, D = (16384, 32, 4, 64) if "64" in case else (16384, 32, 8, 128)
+        ends = torch.arange(1, 12, device=dev) * 1501            # documents of 1501 tokens, the last shorter
+        offsets = torch.cat([ends[:1] - 1501, ends.clamp(max=T)]).to(torch.int32)
+        pk = k.pack_sequences(offsets, T)
+        qkv, do = rnd(T, (Hq + 2 * Hkv) * D), rnd(T, Hq * D)
+        if case == "pack_sequences":
+            fn = lambda: k.pack_sequences(offsets, T)
+        elif case == "rope_at":
+            from zorse_b200.ops.ref import rope_table
+
+            cs = rope_table(4096, D, 1e4, dev)
+            fn = lambda: k.rope_at_(qkv, cs, pk.positions, Hq + Hkv, D)
+        else:
+            out, lse = k.packed_attn_fwd(qkv, pk, Hq, Hkv, D)
+            fn = ((lambda: k.packed_attn_fwd(qkv, pk, Hq, Hkv, D)) if case.endswith("fwd") else
+                  (lambda: k.packed_attn_bwd(do, qkv, out, lse, pk, Hq, Hkv, D)))
+    elif case in ("orthogonalize", "muon_step"):
+        g = [rnd(r, c) for r, c in [(1024, 1024)] * 32 + [(4096, 1024), (1024, 4096)] * 8]    # the matrices of 8 blocks of 1024
+        p, m = [x.float() for x in g], [x.float() for x in g]
+        p16 = [torch.empty_like(x) for x in g]
+        fn = (lambda: k.orthogonalize(g)) if case == "orthogonalize" else (lambda: k.muon_step(p, m, g, p16, lr=1e-3))
     elif case in ("adamw_list", "adamw_list8", "moment_values"):
         from zorse_b200.ops.moments import Moments8
 
