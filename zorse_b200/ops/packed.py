@@ -1,7 +1,8 @@
 """Packed batches: sequences of different lengths, one after another, in one stream of T tokens (csrc/attn/packed.cu).
 
 `PackedSequences` is made once for a batch and used by every layer.  Tokens behind the last sequence belong to none: attention gives
-them zeros (and -inf for the log-sum-exp), and whatever they hold reaches nobody.
+them zeros (and -inf for the log-sum-exp), and whatever they hold reaches nobody.  A NaN or an infinity in a sequence can reach its
+neighbours in the batch: a weight of 0 times it is NaN.
 """
 from __future__ import annotations
 
