@@ -11,8 +11,13 @@
 // tiles each, one by one a launch would leave most of the GPU idle.
 //
 // Operands are fp16, sums fp32 in tensor memory.  All values are bounded (singular values stay below 1.21), so the range of bf16 is
-// not needed and its eight bits would cost: relative error of X after five iterations 1.0e-2 with bf16 and 1.0e-3 with fp16 (512 x
-// 512 to 1024 x 1024, noise and few strong directions alike).  X is held times 2^round(log2(sqrt m)), so its entries are near 1 at the end,
+// not needed and its eight bits would cost: relative error of X after five iterations 1.0e-2 with bf16 and 1.0e-3 with fp16 (noise of 512 x
+// 512 to 1024 x 1024).  What rounding leaves where a matrix has nothing is a singular value like others and grows by a = 3.4 an iteration, 485 times in
+// five, so X itself has to be held more exactly than the products read it: eight more bits of it go from product to product beside it
+// (ns_remainders) in all iterations but the last two, into a X alone, since B takes nothing from where X has nothing.  Relative errors (1024 x 1024)
+// without them and with them: rank 1 0.15 and 3.0e-3, 16 0.045 and 2.7e-3, 64 0.024 and 2.6e-3, 256 8.6e-3 and 2.3e-3; singular values as
+// 1 / k 3.7e-3 and 7e-4, 1 / k^2 0.021 and 1.4e-3; noise 1.0e-3 either way.  They cost 3 to 8 % (24 blocks of 1024 6600 -> 6830 us, 16 matrices
+// of 512 199 -> 214); more bits of the last two iterations' X would take 1e-3 off ranks below 64.  X is held times 2^round(log2(sqrt m)), so its entries are near 1 at the end,
 // A and B times 64, so that what the first iteration's small values round to stays far below what they add.
 //
 // Around the products: one pass over gradient and momentum with the sum of squares, one that scales, turns and rounds into the
@@ -50,8 +55,10 @@ struct NsPassMatrix {
   const void* g;
   __nv_bfloat16* out;
   __half* x;              // first the scaled matrix, at the end the result: [n, ld]
+  uint8_t* rem;           // remainders of the scaled matrix, or null
   double* sums;           // [parts]
   long ld;
+  int rem_cols;
   int rows, cols, parts, tiles_c, first;   // first: of the blocks of a launch
   int g_f32, wide;        // wide: rows start on 16 bytes in every type
   float scale, step;      // X is held times scale; muon: what the result is multiplied with
@@ -178,6 +185,12 @@ __global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant_
   const double by = s == 0.0 ? 0.0 : double(t.scale) / sqrt(s);
   const float low = float(frexp(by, &e) * 2.0);
   const float half = exp2f(float((e - 1) / 2)), rest = exp2f(float(e - 1 - (e - 1) / 2)) * low;
+  auto put = [&](int r, int c, float2 x01, float2 x23) {     // of X
+    const uint2 h = make_uint2(pack_half2(x01.x, x01.y), pack_half2(x23.x, x23.y));
+    *reinterpret_cast<uint2*>(t.x + size_t(r) * t.ld + c) = h;
+    if (t.rem != nullptr)
+      *reinterpret_cast<uint32_t*>(t.rem + ns_rem_at(size_t(r >> 5) * t.rem_cols + (c >> 6), r, c)) = ns_remainders(x01, x23, h.x, h.y);
+  };
   const int tiles = (t.rows + 63) / 64 * t.tiles_c, first = (int(blockIdx.x) - t.first) * a.span;
 #pragma unroll 1
   for (int tile = first; tile < min(first + a.span, tiles); ++tile) {
@@ -213,7 +226,7 @@ __global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant_
 #pragma unroll
         for (int j = 0; j < 4; ++j) tile_s[ty + 16 * k][tx * 4 + j] = u[k][j];
       } else if (r < t.rows && c < t.cols) {      // (rows of the workspace are padded to 64)
-        *reinterpret_cast<uint2*>(t.x + size_t(r) * t.ld + c) = make_uint2(pack_half2(u[k][0], u[k][1]), pack_half2(u[k][2], u[k][3]));
+        put(r, c, make_float2(u[k][0], u[k][1]), make_float2(u[k][2], u[k][3]));
       }
     }
     if (!turned) continue;
@@ -222,9 +235,8 @@ __global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant_
     for (int k = 0; k < 4; ++k) {
       const int cc = c0 + ty + 16 * k, r = r0 + tx * 4;
       if (cc < t.cols && r < t.rows)
-        *reinterpret_cast<uint2*>(t.x + size_t(cc) * t.ld + r) =
-            make_uint2(pack_half2(tile_s[tx * 4][ty + 16 * k], tile_s[tx * 4 + 1][ty + 16 * k]),
-                       pack_half2(tile_s[tx * 4 + 2][ty + 16 * k], tile_s[tx * 4 + 3][ty + 16 * k]));
+        put(cc, r, make_float2(tile_s[tx * 4][ty + 16 * k], tile_s[tx * 4 + 1][ty + 16 * k]),
+            make_float2(tile_s[tx * 4 + 2][ty + 16 * k], tile_s[tx * 4 + 3][ty + 16 * k]));
     }
     __syncthreads();
   }
@@ -298,11 +310,14 @@ enum : int { NS_X0 = 0, NS_X1 = 1, NS_A = 2, NS_B = 3, NS_BUFFERS = 4 };   // X 
 struct NsShape {
   long n, m;                       // short and long side
   std::vector<int> members;        // of the list
-  size_t at[NS_BUFFERS];           // places in the workspace
+  size_t at[NS_BUFFERS], rem;      // places in the workspace
   // Rows start on 128-byte lines, so that a row of a box is one line and not parts of two: lists of 3 x 1000 x 333 and 4097 x 641 and the
   // like 310 -> 265 us.
   long ld(int buffer) const { return ((buffer < NS_A ? m : n) + 63) / 64 * 64; }
   long cols(int buffer) const { return buffer < NS_A ? m : n; }
+  long rem_rows() const { return (n + 31) / 32; }      // boxes of remainders of one matrix
+  long rem_cols() const { return (m + 63) / 64; }
+  size_t rem_bytes() const { return size_t(rem_rows()) * rem_cols() * NS_REM_BOX; }
 };
 struct NsPlan {
   std::vector<NsShape> shapes;     // long sides first
@@ -321,12 +336,14 @@ static NsPlan ns_plan(const NsMatrix* t, int count) {
   for (int i = 0; i < count; ++i) {
     const long n = std::min(t[i].rows, t[i].cols), m = std::max(t[i].rows, t[i].cols);
     auto s = std::find_if(plan.shapes.begin(), plan.shapes.end(), [&](const NsShape& x) { return x.n == n && x.m == m; });
-    if (s == plan.shapes.end()) s = plan.shapes.insert(s, NsShape{n, m, {}, {}});
+    if (s == plan.shapes.end()) s = plan.shapes.insert(s, NsShape{n, m, {}, {}, 0});
     s->members.push_back(i);
   }
   std::stable_sort(plan.shapes.begin(), plan.shapes.end(), [](const NsShape& a, const NsShape& b) { return a.m > b.m; });
-  for (NsShape& s : plan.shapes)
+  for (NsShape& s : plan.shapes) {
     for (int i = 0; i < NS_BUFFERS; ++i) s.at[i] = take(s.members.size() * s.n * s.ld(i) * 2);
+    s.rem = take(s.members.size() * s.rem_bytes());
+  }
   for (int i = 0; i < count; ++i) {
     const long parts = (t[i].rows * t[i].cols + 4095) / 4096;
     plan.parts.push_back(int(std::min<long>(parts, NS_PARTS)));
@@ -337,21 +354,25 @@ static NsPlan ns_plan(const NsMatrix* t, int count) {
 
 static float ns_scale(long m) { return exp2f(float(std::min(13l, std::lround(0.5 * std::log2(double(m)))))); }
 
-// out = alpha P P^T + beta R + diag I (symmetric), or alpha P X + beta R; numbers of buffers, add < 0: no R.
+// out = alpha P P^T + beta R + diag I (symmetric), or alpha P X + beta R + gamma (R + its remainder); numbers of buffers, add < 0: no R.
 struct NsStep {
   bool symmetric;
   int p, q, add, out;
-  float alpha, beta, diag;
+  float alpha, beta, diag, gamma;
+  int remainders;         // 1: R's are read, 2: the result's are kept
 };
+// X of all iterations but the last two keeps what its rounding to fp16 leaves over (ns_remainders).
+constexpr bool ns_keeps_remainder(int iteration, int iterations) { return iteration + 2 < iterations; }
 // Launch by launch.  B goes with 2 I added and X with a - 2: once singular values are near 1, B is nearly -2.7 I, most of which a takes
 // away again, rounding errors excepted.  (1.43e-3 -> 0.95e-3 for 512 x 1376 noise, 1.64e-3 -> 0.69e-3 for 8 x 600, never more.)  (Two iterations of long matrices taken as one, X2 = q(A1) q(A) X0 with A1 = q(A) A q(A), save 3 n^2 m - 3 n^3 operations,
 // but q(A1) q(A) is 11.9 I less as much along a direction that holds most of a matrix: 1.4e-2 of a matrix of ones instead of 1e-4.)
 static std::vector<NsStep> ns_program(int iterations, float a, float b, float c) {
   std::vector<NsStep> steps;
   for (int i = 0, x = NS_X0; i < iterations; ++i, x = 1 - x) {
-    steps.push_back({true, x, x, -1, NS_A, 1.f, 0.f, 0.f});
-    steps.push_back({true, NS_A, NS_A, NS_A, NS_B, c, b, 2.f});
-    steps.push_back({false, NS_B, x, x, 1 - x, 1.f, a - 2.f, 0.f});
+    const bool more = ns_keeps_remainder(i, iterations);
+    steps.push_back({true, x, x, -1, NS_A, 1.f, 0.f, 0.f, 0.f, 0});
+    steps.push_back({true, NS_A, NS_A, NS_A, NS_B, c, b, 2.f, 0.f, 0});
+    steps.push_back({false, NS_B, x, x, 1 - x, 1.f, more ? -2.f : a - 2.f, 0.f, more ? a : 0.f, more + 2 * ns_keeps_remainder(i + 1, iterations)});
   }
   return steps;
 }
@@ -405,6 +426,11 @@ static int ns_products(const NsPlan& plan, char* ws, const std::vector<NsStep>& 
         g.alpha = e.alpha * (e.p < NS_A ? NS_A_SCALE / (scale * scale) : 1.f / NS_A_SCALE);
         g.beta = e.beta;
         g.diag = e.diag * NS_A_SCALE;
+        g.gamma = e.gamma;
+        g.remainders = e.remainders;
+        g.rem = reinterpret_cast<uint8_t*>(ws + s.rem);
+        g.rem_rows = int(s.rem_rows());
+        g.rem_cols = int(s.rem_cols());
         g.tiles_m = (g.M + NsCfg::BM - 1) / NsCfg::BM;
         const long columns = (g.N + NsCfg::BN - 1) / NsCfg::BN, count = long(s.members.size());
         const long tiles = e.symmetric ? long(g.tiles_m) * (g.tiles_m + 1) / 2 : g.tiles_m * columns;
@@ -440,7 +466,7 @@ static int ns_pass_launch(const NsPass<NS_MATRICES>& all, unsigned blocks, cudaS
 
 // One of the passes over all matrices; PASS 0: sums, 1: scale, 2: apply.
 template <int PASS>
-static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRICES>& common, float lr, char* ws, int x, cudaStream_t stream, int* launches) {
+static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRICES>& common, float lr, char* ws, int x, bool remainders, cudaStream_t stream, int* launches) {
   NsPass<NS_MATRICES> a = common;
   a.count = 0;
   long all = 0;
@@ -467,6 +493,8 @@ static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRIC
       e.g = t[i].g;
       e.out = t[i].out;
       e.x = reinterpret_cast<__half*>(ws + s.at[x]) + k * s.n * s.ld(NS_X0);
+      e.rem = remainders ? reinterpret_cast<uint8_t*>(ws + s.rem) + k * s.rem_bytes() : nullptr;
+      e.rem_cols = int(s.rem_cols());
       e.sums = reinterpret_cast<double*>(ws + plan.sums[i]);
       e.ld = s.ld(NS_X0);
       e.rows = int(t[i].rows);
@@ -501,7 +529,7 @@ static int ns_together(const NsMatrix* t, int count, long limit) {
   double room = double(limit);
   for (int i = 0; i < count; ++i) {
     const double n = double(std::min(t[i].rows, t[i].cols)), m = double(std::max(t[i].rows, t[i].cols));
-    room -= 4 * n * (m + 64) + 4 * n * (n + 64) + 8192;
+    room -= 4 * n * (m + 64) + 4 * n * (n + 64) + (n + 32) * (m + 64) + 8192;
     if (room < 0) return std::max(i, 1);
   }
   return count;
@@ -552,10 +580,10 @@ int zb_newton_schulz(const void* table, int count, int muon, float lr, float mom
       n = ns_together(t + i, count - i, limit);
       const NsPlan plan = ns_plan(t + i, n);
       if (bytes < long(plan.bytes)) ZB_FAIL(-4, "newton_schulz: %ld bytes of workspace, %zu are needed", bytes, plan.bytes);
-      int rc = ns_pass<0>(plan, t + i, pass, lr, ws, NS_X0, stream, launches);
-      if (!rc) rc = ns_pass<1>(plan, t + i, pass, lr, ws, NS_X0, stream, launches);
+      int rc = ns_pass<0>(plan, t + i, pass, lr, ws, NS_X0, false, stream, launches);
+      if (!rc) rc = ns_pass<1>(plan, t + i, pass, lr, ws, NS_X0, ns_keeps_remainder(0, iterations), stream, launches);
       if (!rc) rc = ns_products(plan, ws, program, status, stream, launches);
-      if (!rc) rc = ns_pass<2>(plan, t + i, pass, lr, ws, iterations & 1 ? NS_X1 : NS_X0, stream, launches);
+      if (!rc) rc = ns_pass<2>(plan, t + i, pass, lr, ws, iterations & 1 ? NS_X1 : NS_X0, false, stream, launches);
       if (rc) return rc;
     }
     return 0;

@@ -1,7 +1,7 @@
 // The products of the Newton-Schulz iterations (newton_schulz.cu): fp16 operands, fp32 sums, all matrices of up to NS_GROUPS shapes in one
 // launch.  Two forms, by shape:
 //     symmetric   out = alpha P P^T + beta R + diag I
-//     plain       out = alpha P X + beta R            P symmetric, X [n, m]
+//     plain       out = alpha P X + beta R + gamma (R + its remainder)      P symmetric, X [n, m]
 // Of a symmetric result only the tiles on and above the diagonal are formed; the others are stored as well, turned over.  A tile on the
 // diagonal has the same rows on both sides, which are loaded once (8 blocks of 1024: X X^T 99.7 -> 98.2 us, A A 56.4 -> 55.0; 24 blocks, at the
 // power limit, 7680 -> 7390).
@@ -20,6 +20,7 @@
 #include "../common/ptx.cuh"
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace zb {
 
@@ -46,6 +47,10 @@ struct alignas(64) NsGroup {
   int symmetric;
   int first;              // its first item
   float alpha, beta, diag;
+  float gamma;            // plain, with R's remainder
+  int remainders;         // 1: of R are read, 2: of the result are written (over those of R, by the thread that read them)
+  int rem_rows, rem_cols; // boxes of the remainders of one matrix
+  uint8_t* rem;
 };
 template <int GROUPS>      // (a launch with few shapes has few parameters to send: 2 of 8 shapes' 5.6 KB)
 struct NsParams {
@@ -63,6 +68,27 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+
+// Remainders: eight more bits of a value behind its fp16 form, as the difference of the two as whole numbers.  fp16 keeps 10 of fp32's 23 bits of a
+// mantissa, so rounding moves the number by at most 2^12, and a byte holds that in steps of 2^5.  (Values below fp16's normal numbers are
+// further off and keep what a byte can: they are small against the rest.)  A box of 32 rows and 64 columns lies together, 16 columns
+// of a row in one piece and the rows behind one another: the products read and write it 512 bytes a warp, without shared memory.
+constexpr int NS_REM_BOX = 32 * 64;
+__device__ __forceinline__ size_t ns_rem_at(size_t box, int row, int col) { return box * NS_REM_BOX + (col & 48) * 32 + (row & 31) * 16 + (col & 15); }
+__device__ __forceinline__ uint32_t ns_remainders(float2 x01, float2 x23, uint32_t h01, uint32_t h23) {
+  const float2 a = unpack_half2(h01), b = unpack_half2(h23);
+  auto q = [](float x, float h) { return (__float_as_int(x) - __float_as_int(h) + 16) >> 5; };
+  uint32_t hi, all;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(q(x23.y, b.y)), "r"(q(x23.x, b.x)));
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(all) : "r"(q(x01.y, a.y)), "r"(q(x01.x, a.x)), "r"(hi));
+  return all;
+}
+template <int K>      // byte K of the word belongs to h
+__device__ __forceinline__ float ns_with_remainder(float h, uint32_t word) {
+  int q;      // the byte with its sign in the other three
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(q) : "r"(word), "n"(K | (K | 8) << 4 | (K | 8) << 8 | (K | 8) << 12));
+  return __int_as_float(__float_as_int(h) + q * 32);
+}
 
 template <int GROUPS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) newton_schulz_kernel(const __grid_constant__ NsParams<GROUPS> p) {
@@ -228,7 +254,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) n
       const int n_boxes = row0 < g.M ? min(BN / 64, (g.N - n0 + 63) / 64) : 0;
       const int mine = (n_boxes - h + 1) >> 1;
       const int buf = local & 1;
-      const float alpha = g.alpha, beta = g.beta, diag = g.diag;
+      const float alpha = g.alpha, beta = g.beta, diag = g.diag, gamma = g.gamma;
+      const bool rem_in = (g.remainders & 1) != 0, rem_out = (g.remainders & 2) != 0;
+      auto rem_box = [&](int u) {   // of this thread's row in box u
+        const size_t at = (size_t(it.matrix) * g.rem_rows + (row0 >> 5)) * g.rem_cols + (n0 >> 6) + h + 2 * u;
+        return reinterpret_cast<uint4*>(g.rem + ns_rem_at(at, lane, 0));
+      };
+      uint32_t rem[16];          // of this thread's 64 columns of a box, four a word
+      auto load_rem = [&](int u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 v = ld_v4(rem_box(u) + 32 * k);
+          rem[4 * k] = v.x; rem[4 * k + 1] = v.y; rem[4 * k + 2] = v.z; rem[4 * k + 3] = v.w;
+        }
+      };
+      if (rem_in && mine > 0) load_rem(0);
       const bool add = beta != 0.f, turned = g.symmetric && it.tm != it.tn;
       auto load_box = [&](int u) {   // lane 0; every store from its place has left
         mbar_expect_tx(&my_full[u], Cfg::BOX_BYTES);
@@ -248,82 +288,104 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) n
       };
       bool ok = true;
       if (mine <= 0) release_tmem();
+      // (two forms: with the remainders' branches inside the loop each of fifteen small products took 2.4 us longer, not only those with some)
+      auto boxes_out = [&](auto with_remainders) {
+        constexpr bool REM = decltype(with_remainders)::value;
 #pragma unroll 1
-      for (int u = 0; u < mine; ++u) {
-        const int col0 = n0 + (h + 2 * u) * 64;
-        const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + (h + 2 * u) * 64);
-        uint32_t r[32], s[32];
-        tmem_ld32(t_addr, r);
-        tmem_ld32(t_addr + 32u, s);
-        if (BOXES == 1 && u == 1 && lane == 0) {
-          bulk_wait_read<0>();
-          if (add) load_box(1);
-        }
-        tmem_wait_ld();
-        if (u == mine - 1) release_tmem();
-        else __syncwarp();
-        uint8_t* box = my_boxes + (u & (BOXES - 1)) * Cfg::BOX_BYTES;
-        const uint32_t row_at = smem_u32(box) + uint32_t(lane) * 128;
-        if (add) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&my_full[u], (phases >> u) & 1, wctx, ST_TIMEOUT_FULL));
-          if (!ok) break;
-          phases ^= 1u << u;
-        }
-        // the one column of this box that lies on the diagonal in this thread's row
-        const int diag_at = it.tm == it.tn && (row0 & ~63) == col0 ? (row0 & 32) + lane : -1;
-        uint32_t o[32];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t at = row_at + uint32_t((j ^ (lane & 7)) << 4);
-          uint32_t x[4] = {0u, 0u, 0u, 0u};
+        for (int u = 0; u < mine; ++u) {
+          const int col0 = n0 + (h + 2 * u) * 64;
+          const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(buf * BN + (h + 2 * u) * 64);
+          uint32_t r[32], s[32];
+          tmem_ld32(t_addr, r);
+          tmem_ld32(t_addr + 32u, s);
+          if (BOXES == 1 && u == 1 && lane == 0) {
+            bulk_wait_read<0>();
+            if (add) load_box(1);
+          }
+          tmem_wait_ld();
+          if (u == mine - 1) release_tmem();
+          else __syncwarp();
+          uint8_t* box = my_boxes + (u & (BOXES - 1)) * Cfg::BOX_BYTES;
+          const uint32_t row_at = smem_u32(box) + uint32_t(lane) * 128;
           if (add) {
-            const uint4 v = ld_shared_v4(at);
-            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            ok = __all_sync(0xffffffffu, mbar_wait(&my_full[u], (phases >> u) & 1, wctx, ST_TIMEOUT_FULL));
+            if (!ok) break;
+            phases ^= 1u << u;
           }
+          // the one column of this box that lies on the diagonal in this thread's row
+          const int diag_at = it.tm == it.tn && (row0 & ~63) == col0 ? (row0 & 32) + lane : -1;
+          uint32_t o[32];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int e = (j & 3) * 8 + 2 * w;
-            float lo = __uint_as_float(j < 4 ? r[e] : s[e]) * alpha, hi = __uint_as_float(j < 4 ? r[e + 1] : s[e + 1]) * alpha;
-            const float2 more = unpack_half2(x[w]);
-            lo = fmaf(beta, more.x, lo);
-            hi = fmaf(beta, more.y, hi);
-            if (diag_at >= 0) {
-              lo += diag_at == j * 8 + 2 * w ? diag : 0.f;
-              hi += diag_at == j * 8 + 2 * w + 1 ? diag : 0.f;
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t at = row_at + uint32_t((j ^ (lane & 7)) << 4);
+            uint32_t x[4] = {0u, 0u, 0u, 0u};
+            if (add) {
+              const uint4 v = ld_shared_v4(at);
+              x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
             }
-            o[j * 4 + w] = pack_half2(lo, hi);
-          }
-          st_shared_v4(at, o[j * 4], o[j * 4 + 1], o[j * 4 + 2], o[j * 4 + 3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.c, box, col0, row0, it.matrix);
-          bulk_commit();
-          // turned boxes leave from the first place: what it holds (this box, or the turned one before it) has been read by then
-          if (turned) {
-            if (u == 0 || BOXES == 1) bulk_wait_read<0>();
-            else bulk_wait_read<1>();
-          }
-        }
-        if (turned) {
-          // Two lanes trade halves, so that each has two rows of one column: 64 rows of 32 of the turned box, 128 bytes a store.
-          __syncwarp();
-          const uint32_t to = smem_u32(my_boxes) + uint32_t(lane & 1) * 64 + uint32_t(lane >> 1) * 4;
+            float2 v[4];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, o[j], 1);
-            const uint32_t v = lane & 1 ? __byte_perm(other, o[j], 0x7632) : __byte_perm(o[j], other, 0x5410);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + uint32_t(j * 128)), "r"(v) : "memory");
+            for (int w = 0; w < 4; ++w) {
+              const int e = (j & 3) * 8 + 2 * w;
+              float lo = __uint_as_float(j < 4 ? r[e] : s[e]) * alpha, hi = __uint_as_float(j < 4 ? r[e + 1] : s[e + 1]) * alpha;
+              const float2 more = unpack_half2(x[w]);
+              lo = fmaf(beta, more.x, lo);
+              hi = fmaf(beta, more.y, hi);
+              if (REM) {
+                const uint32_t word = rem[j * 2 + (w >> 1)];
+                lo = fmaf(gamma, (w & 1) ? ns_with_remainder<2>(more.x, word) : ns_with_remainder<0>(more.x, word), lo);
+                hi = fmaf(gamma, (w & 1) ? ns_with_remainder<3>(more.y, word) : ns_with_remainder<1>(more.y, word), hi);
+              }
+              if (diag_at >= 0) {
+                lo += diag_at == j * 8 + 2 * w ? diag : 0.f;
+                hi += diag_at == j * 8 + 2 * w + 1 ? diag : 0.f;
+              }
+              o[j * 4 + w] = pack_half2(lo, hi);
+              v[w] = make_float2(lo, hi);
+            }
+            if (REM && rem_out) {
+              rem[j * 2] = ns_remainders(v[0], v[1], o[j * 4], o[j * 4 + 1]);
+              rem[j * 2 + 1] = ns_remainders(v[2], v[3], o[j * 4 + 2], o[j * 4 + 3]);
+            }
+            st_shared_v4(at, o[j * 4], o[j * 4 + 1], o[j * 4 + 2], o[j * 4 + 3]);
           }
+          if (REM && rem_out) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) rem_box(u)[32 * k] = make_uint4(rem[4 * k], rem[4 * k + 1], rem[4 * k + 2], rem[4 * k + 3]);
+          }
+          if (REM && u + 1 < mine) load_rem(u + 1);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.t, my_boxes, row0, col0, it.matrix);
+            if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.c, box, col0, row0, it.matrix);
             bulk_commit();
+            // turned boxes leave from the first place: what it holds (this box, or the turned one before it) has been read by then
+            if (turned) {
+              if (u == 0 || BOXES == 1) bulk_wait_read<0>();
+              else bulk_wait_read<1>();
+            }
+          }
+          if (turned) {
+            // Two lanes trade halves, so that each has two rows of one column: 64 rows of 32 of the turned box, 128 bytes a store.
+            __syncwarp();
+            const uint32_t to = smem_u32(my_boxes) + uint32_t(lane & 1) * 64 + uint32_t(lane >> 1) * 4;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, o[j], 1);
+              const uint32_t v = lane & 1 ? __byte_perm(other, o[j], 0x7632) : __byte_perm(o[j], other, 0x5410);
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + uint32_t(j * 128)), "r"(v) : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (zb_in_bounds(row0 < g.M && col0 < g.N, p.status, 2)) tma_store_3d(&g.t, my_boxes, row0, col0, it.matrix);
+              bulk_commit();
+            }
           }
         }
-      }
+      };
+      if (rem_in) boxes_out(std::true_type());
+      else boxes_out(std::false_type());
       if (!ok) break;
     }
   }

@@ -616,7 +616,7 @@ def moment_values(moments, dtype=torch.float32):
     return out
 
 
-# Matrices of a list are taken together as far as their workspace (4 bytes an element, 4 a pair of rows of the short side) stays below this:
+# Matrices of a list are taken together as far as their workspace (5 bytes an element, 4 a pair of rows of the short side) stays below this:
 # enough tiles for many waves.
 NEWTON_SCHULZ_BYTES = 1 << 30
 
