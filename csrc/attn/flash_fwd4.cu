@@ -487,7 +487,8 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     ok = __all_sync(0xffffffffu, ok);
     tr(TR_EPI_BEGIN);
     tc_fence_after();
-    const float inv_l = (l_run > 0.f) ? 1.f / l_run : 0.f;
+    const bool any = PACKED ? l_run != 0.f : l_run > 0.f;      // (PACKED: NaN stays NaN)
+    const float inv_l = any ? 1.f / l_run : 0.f;
     // O leaves through the chain's Q tile, whose last reader is done, and TMA, which drops the rows behind the sequence
     const uint32_t orow = smem_u32(sQ) + uint32_t(c) * Cfg::TILE_BYTES + uint32_t(t) * 128;
 #pragma unroll 1
@@ -520,7 +521,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (ok && row < p.S && p.lse != nullptr) {
       const float m_eff = (m_run == -INFINITY) ? 0.f : m_run;
       p.lse[(size_t(batch) * p.Hq + head) * p.S + row] =
-          (l_run > 0.f) ? (m_eff * scale + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+          any ? (m_eff * scale + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
     }
     if ((warp & 3) == 0 && lane == 0) bulk_wait_read<0>();
     tr(TR_EPI_END);

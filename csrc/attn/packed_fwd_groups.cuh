@@ -312,7 +312,7 @@ packed_fwd_groups_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gri
     if (ok && my_tiles > 0) ok = mbar_wait(&o_done[c], 0, wctx, ST_TIMEOUT_MISC);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-    const float inv_l = (l_run > 0.f) ? 1.f / l_run : 0.f;
+    const float inv_l = l_run != 0.f ? 1.f / l_run : 0.f;      // (NaN stays NaN)
     // O leaves through the chain's Q tile, whose last reader is done, and TMA, which drops the rows behind the batch
     const uint32_t orow = smem_u32(sQ) + uint32_t(c * Cfg::Q_BYTES) + uint32_t(t) * 128;
 #pragma unroll 1
@@ -341,7 +341,7 @@ packed_fwd_groups_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gri
     }
     if (ok && row < p.T)
       p.lse[size_t(head) * p.T + row] =
-          (l_run > 0.f) ? ((m_run == -INFINITY ? 0.f : m_run) * scale + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
+          l_run != 0.f ? ((m_run == -INFINITY ? 0.f : m_run) * scale + log2f(l_run)) * 0.6931471805599453f : -INFINITY;
     if ((warp & 3) == 0 && lane == 0) bulk_wait_read<0>();
   }
 
