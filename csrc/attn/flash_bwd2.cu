@@ -695,7 +695,7 @@ flash_bwd2_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (CL == 4 && which != (cl_rank >> 1)) continue;    // ranks 0 and 1: alternate row halves of dK, 2 and 3: of dV
       if (CL == 4 && ((warp & 3) >> 1) != (cl_rank & 1)) continue;
       const uint32_t col0 = which == 0 ? Cfg::DK_COL : Cfg::DV_COL;
-      const float mul = !DQ && which == 0 ? p.scale : 1.f;   // the two-kernel form leaves dS unscaled
+      const float mul = PACKED && total < 0 ? PACKED_NAN : !DQ && which == 0 ? p.scale : 1.f;   // the two-kernel form leaves dS unscaled
       const uint32_t row = smem_u32(which == 0 ? sK : sV) + uint32_t(t) * 128;
 #pragma unroll 1
       for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {

@@ -326,6 +326,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
     if (ok && n > 0) ok = mbar_wait(dq_done, 0, wctx, ST_TIMEOUT_MISC);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
+    const float mul = PACKED && total < 0 ? PACKED_NAN : p.scale;
     // through the place of Q, whose last reader is done, and TMA (see flash_bwd2.cu)
 #pragma unroll 1
     for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
@@ -338,7 +339,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
         for (int k = 0; k < 32; ++k) r[k] = 0u;
       }
 #pragma unroll
-      for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * p.scale);
+      for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * mul);
       const uint32_t at = smem_u32(sQ) + uint32_t(c >> 1) * BLK + uint32_t(t) * 128;
 #pragma unroll
       for (int v4 = 0; v4 < 4; ++v4)

@@ -354,7 +354,7 @@ flash_fwd4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       all_lo = p.window > 0 ? max(last_begin, q0 + BM - p.window) : last_begin;
       all_hi = min(first_end, p.causal ? q0 + 1 : p.S);
     }
-    float m_run = -INFINITY, l_run = 0.f;  // m_run in raw (unscaled) score units
+    float m_run = -INFINITY, l_run = PACKED && total < 0 ? PACKED_NAN : 0.f;  // m_run in raw (unscaled) score units
     bool ok = true;
     for (int i = 0; i < my_tiles; ++i) {
       const int kv0 = (my_lo + i) * BN;

@@ -10,11 +10,12 @@
 namespace zb {
 
 constexpr int PACK_PAD = 256;
+#define PACKED_NAN __uint_as_float(0x7fc00000u)
 
 // A tile (or pair of tiles) as it is dealt out, with all that a CTA needs before it knows its loads: read in one go.
 struct alignas(16) PackedTile {
   int2 first, last;         // bounds of its first and last row
-  int tile, total;          // total: the end of the last sequence
+  int tile, total;          // total: the end of the last sequence; -1: the offsets did not rise, and results are NaN
   int unused[2];
 };
 struct alignas(16) PackedPair {

@@ -233,7 +233,7 @@ packed_fwd_groups_kernel(const __grid_constant__ CUtensorMap tmap_q, const __gri
     const int last_begin = TILES == 1 || c < HEADS ? last[0].x : last[TILES - 1].x, first_end = TILES == 1 || c < HEADS ? first[0].y : first[TILES - 1].y;
     const int all_lo = p.window > 0 ? max(last_begin, q0 + BM - p.window) : last_begin, all_hi = p.causal ? min(first_end, q0 + 1) : first_end;
     const float scale = p.scale_log2;
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run = -INFINITY, l_run = total < 0 ? PACKED_NAN : 0.f;
     bool ok = true;
     for (int i = 0; i < my_tiles; ++i) {
       const int kv0 = (my_lo + i) * BN;

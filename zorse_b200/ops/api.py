@@ -137,7 +137,9 @@ class RefOps(_EpilogueOps, _LaterOps):
 
     # ---- packed batches: sequences of different lengths, one after another -----------------
     def pack_sequences(self, offsets, T):
-        """What the calls below need to know of sequences [offsets[i], offsets[i + 1]) in T tokens; once for all layers of a batch."""
+        """What the calls below need to know of sequences [offsets[i], offsets[i + 1]) in T tokens; once for all layers of a batch.
+        Offsets that do not rise from 0 to at most T are refused here and by `Trainer.pack`; the kernels, which wait for nothing, answer
+        them with NaN."""
         return packed.pack(offsets, T)
 
     def packed_attn_fwd(self, qkv, pk, Hq, Hkv, D, causal=True, window=0):

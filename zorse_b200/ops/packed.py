@@ -13,6 +13,7 @@ import torch
 
 MOST_TOKENS = 65535 * 128
 MOST_AXES = 4
+PACK_SCAN = 4096      # sequences whose offsets every block of the plan looks at (csrc/attn/packed.cu)
 
 
 class PackedSequences(NamedTuple):

@@ -23,7 +23,7 @@ import torch
 
 from .moments import BLOCK as MOMENT_BLOCK
 from .muon import COEFFICIENTS as NEWTON_SCHULZ
-from .packed import MOST_AXES, MOST_TOKENS, PackedSequences, check_window
+from .packed import MOST_AXES, MOST_TOKENS, PACK_SCAN, PackedSequences, check_window
 
 _LIB_PATH = Path(__file__).resolve().parents[1] / "_C" / "libzorse_sm100.so"
 _lib = None
@@ -56,7 +56,7 @@ _SIGNATURES = {
     "zb_flash_fwd4": "pppiiiiiiifipipip", "zb_flash_bwd3": "ppppppiiiiiiifpipip",
     "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
     "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
-    "zb_pack_sequences": "piipppppp", "zb_packed_attn_fwd": "ppppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
+    "zb_pack_sequences": "piippppppp", "zb_packed_attn_fwd": "ppppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
     "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pilp", "zb_newton_schulz": "piiffiffiffflplppp",
     "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
@@ -845,17 +845,19 @@ def flash_bwd(do, qkv, o, lse, B: int, S: int, Hq: int, Hkv: int, D: int, causal
 # --------------------------------------------------------------------------- packed sequences
 def pack_sequences(offsets, T: int) -> PackedSequences:
     """What attention and rotation need to know of sequences that lie one after another in T tokens: sequence i has the tokens
-    [offsets[i], offsets[i + 1]).  offsets: int32 on the device, from 0 up, not falling; nothing waits for the GPU, so their values
-    are not checked (others than these give results of no meaning, within the batch)."""
+    [offsets[i], offsets[i + 1]).  offsets: int32 on the device, from 0 up to at most T, not falling.  Nothing waits for the GPU, so
+    others than these are not refused here: attention over their packing, forward and backward, is NaN throughout."""
     _need(offsets.dtype == torch.int32 and offsets.dim() == 1 and offsets.is_contiguous() and 1 <= offsets.numel() < 2 ** 31,
           f"offsets {tuple(offsets.shape)}, {offsets.dtype}: expected int32 [sequences + 1]")
     _on_current(offsets, "offsets")
     _need(0 <= T <= MOST_TOKENS, f"{T} tokens: at most {MOST_TOKENS}")
     dev, pairs, tiles = offsets.device, -(-T // 256), -(-T // 128)
     bounds = torch.empty(pairs * 256, 2, dtype=torch.int32, device=dev)
-    rest = torch.empty(12 * pairs + 16 * tiles + T, dtype=torch.int32, device=dev).split([12 * pairs, 8 * tiles, 8 * tiles, T])
+    rest = torch.empty(12 * pairs + 16 * tiles + T + 1, dtype=torch.int32, device=dev).split([12 * pairs, 8 * tiles, 8 * tiles, T, 1])
     orders = rest[0].view(pairs, 12), rest[1].view(tiles, 8), rest[2].view(tiles, 8)
-    _check(lib().zb_pack_sequences(_a(offsets), offsets.numel() - 1, T, _a(bounds), _a(rest[3]), *(_a(t) for t in orders), _stream()), "pack_sequences")
+    _check(lib().zb_pack_sequences(_a(offsets), offsets.numel() - 1, T, _a(bounds), _a(rest[3]), *(_a(t) for t in orders), _a(rest[4]), _stream()), "pack_sequences")
+    global _launches
+    _launches += T > 0 and offsets.numel() - 1 > PACK_SCAN     # (their values are looked at by a kernel of its own)
     return PackedSequences(T, bounds, rest[3], *orders)
 
 
