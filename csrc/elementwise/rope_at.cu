@@ -146,8 +146,8 @@ extern "C" int zb_rope_at(void* buf, const float* cs, const int* positions, cons
     if (blocks > 0x7fffffffL) ZB_FAIL(-1, "rope_at: %d tokens of %d heads", T, heads);
     ZB_CUDA_OK(launch_pass(rope_at_kernel<HEADS>, dim3(unsigned(blocks)), 256, 0, stream, p, sign));
   } else {
-    const long blocks = (long(T) * heads * (d / 2) + 255) / 256;
-    ZB_CUDA_OK(launch_pass(rope_at_pairs_kernel, dim3(unsigned(blocks < 148 * 64 ? blocks : 148 * 64)), 256, 0, stream, p, sign));
+    const long blocks = (long(T) * heads * (d / 2) + 255) / 256, most = 64l * num_sms();
+    ZB_CUDA_OK(launch_pass(rope_at_pairs_kernel, dim3(unsigned(blocks < most ? blocks : most)), 256, 0, stream, p, sign));
   }
   return 0;
 }

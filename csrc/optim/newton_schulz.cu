@@ -471,7 +471,7 @@ static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRIC
   a.count = 0;
   long all = 0;
   for (const NsShape& s : plan.shapes) all += long(s.members.size()) * ((s.n + 63) / 64) * ((s.m + 63) / 64);
-  a.span = int(std::min(4l, std::max(1l, all / (2 * 148 * 6))));      // two rounds of blocks on all SMs at the least
+  a.span = int(std::min(4l, std::max(1l, all / (2 * num_sms() * 6))));      // two rounds of blocks on all SMs at the least
   long blocks = 0;
   auto flush = [&]() -> int {
     if (a.count == 0) return 0;
