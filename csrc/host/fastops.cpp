@@ -71,7 +71,7 @@ struct Entry {
                          int, int, int, int, float, int*, cudaStream_t);
   int (*rope_at)(void*, const float*, const int*, const int*, int, int, int, int, int, long, int, cudaStream_t);
   int (*newton_schulz_workspace)(const void*, int, long, long*);
-  int (*newton_schulz)(const void*, int, int, float, float, int, float, float, int, float, float, float, long, void*, long, int*, int*,
+  int (*newton_schulz)(const void*, int, int, float, float, int, float, float, int, float, float, float, float, long, void*, long, int*, int*,
                        cudaStream_t);
   const char* (*last_error)();
 };
@@ -1069,7 +1069,7 @@ bool any_matrix(const Tensor* t, const Tensor& like) {   // contiguous, of a typ
 }
 // 1: done, 0: not for here, -1: error set
 int newton_schulz(c10::SmallVectorImpl<NsMatrix>& table, const Tensor& like, bool muon, const double (&h)[4], bool nesterov, int64_t iterations,
-                  const double (&abc)[3], int64_t limit) {   // h: lr, momentum, keep, grad_scale
+                  const double (&abc)[4], int64_t limit) {   // h: lr, momentum, keep, grad_scale; abc: coefficients and the step's size
   int* status = status_of(like);
   if (status == nullptr || iterations < 1 || iterations > 100) return 0;
   long bytes = 0;
@@ -1079,21 +1079,21 @@ int newton_schulz(c10::SmallVectorImpl<NsMatrix>& table, const Tensor& like, boo
   int n = 0;
   if (!launch("newton_schulz", 0, [&] {
         return lib.newton_schulz(table.data(), int(table.size()), muon, float(h[0]), float(h[1]), nesterov, float(h[2]), float(h[3]),
-                                 int(iterations), float(abc[0]), float(abc[1]), float(abc[2]), limit, ws.data_ptr(), bytes, &n, status, s);
+                                 int(iterations), float(abc[0]), float(abc[1]), float(abc[2]), float(abc[3]), limit, ws.data_ptr(), bytes, &n, status, s);
       }))
     return -1;
   launches += n;
   return 1;
 }
-// orthogonalize(mats, iterations, (a, b, c), limit) -> the results
+// orthogonalize(mats, iterations, (a, b, c, size), limit) -> the results
 PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   ZB_ARGS(4)
   const Py_ssize_t n = PyList_Check(args[0]) ? PyList_GET_SIZE(args[0]) : 0;
   int64_t iterations, limit;
-  double abc[3];
-  if (n == 0 || !int_arg(args[1], iterations) || !int_arg(args[3], limit) || !PyTuple_Check(args[2]) || PyTuple_GET_SIZE(args[2]) != 3) Py_RETURN_NONE;
-  for (int i = 0; i < 3; ++i)
+  double abc[4];
+  if (n == 0 || !int_arg(args[1], iterations) || !int_arg(args[3], limit) || !PyTuple_Check(args[2]) || PyTuple_GET_SIZE(args[2]) != 4) Py_RETURN_NONE;
+  for (int i = 0; i < 4; ++i)
     if (!float_arg(PyTuple_GET_ITEM(args[2], i), abc[i])) Py_RETURN_NONE;
   const Tensor* first = tensor_of(PyList_GET_ITEM(args[0], 0));
   if (!gradient(first) || !here(*first)) Py_RETURN_NONE;
@@ -1117,19 +1117,19 @@ PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return list;
   END_HANDLE_TH_ERRORS
 }
-// muon_step(p, m, g, p16, lr, momentum, weight_decay, nesterov, iterations, grad_scale, (a, b, c), limit) -> True; lists
+// muon_step(p, m, g, p16, lr, momentum, weight_decay, nesterov, iterations, grad_scale, (a, b, c, size), limit) -> True; lists
 PyObject* muon_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   ZB_ARGS(12)
   const Py_ssize_t n = PyList_Check(args[0]) ? PyList_GET_SIZE(args[0]) : 0;
   auto list = [&](PyObject* o) { return PyList_Check(o) && PyList_GET_SIZE(o) == n; };
-  double lr, momentum, decay, grad_scale, abc[3];
+  double lr, momentum, decay, grad_scale, abc[4];
   int64_t iterations, limit;
   if (n == 0 || !list(args[1]) || !list(args[2]) || !list(args[3]) || !float_arg(args[4], lr) || !float_arg(args[5], momentum) ||
       !float_arg(args[6], decay) || !int_arg(args[8], iterations) || !float_arg(args[9], grad_scale) || !PyTuple_Check(args[10]) ||
-      PyTuple_GET_SIZE(args[10]) != 3 || !int_arg(args[11], limit) || !(momentum >= 0 && momentum < 1))
+      PyTuple_GET_SIZE(args[10]) != 4 || !int_arg(args[11], limit) || !(momentum >= 0 && momentum < 1))
     Py_RETURN_NONE;
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i < 4; ++i)
     if (!float_arg(PyTuple_GET_ITEM(args[10], i), abc[i])) Py_RETURN_NONE;
   const Tensor* first = tensor_of(PyList_GET_ITEM(args[0], 0));
   if (!dense(first, F32) || !here(*first)) Py_RETURN_NONE;

@@ -466,7 +466,7 @@ static int ns_pass_launch(const NsPass<NS_MATRICES>& all, unsigned blocks, cudaS
 
 // One of the passes over all matrices; PASS 0: sums, 1: scale, 2: apply.
 template <int PASS>
-static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRICES>& common, float lr, char* ws, int x, bool remainders, cudaStream_t stream, int* launches) {
+static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRICES>& common, float step, char* ws, int x, bool remainders, cudaStream_t stream, int* launches) {
   NsPass<NS_MATRICES> a = common;
   a.count = 0;
   long all = 0;
@@ -507,7 +507,7 @@ static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRIC
       const uintptr_t b16 = reinterpret_cast<uintptr_t>(e.out) | (e.g_f32 ? 0 : reinterpret_cast<uintptr_t>(e.g));
       e.wide = e.cols % 4 == 0 && (f32 & 15) == 0 && (b16 & 7) == 0;
       e.scale = scale;
-      e.step = (common.muon ? lr * 0.2f * sqrtf(float(s.m)) : 1.f) / scale;
+      e.step = (common.muon ? step * sqrtf(float(s.m)) : 1.f) / scale;
       const long tiles = long((e.rows + 63) / 64) * e.tiles_c;
       blocks += PASS == 0 ? e.parts : PASS == 1 ? (tiles + a.span - 1) / a.span : tiles;
       if (a.count == NS_MATRICES)
@@ -557,10 +557,10 @@ int zb_newton_schulz_workspace(const void* table, int count, long limit, long* b
   }
 }
 
-// table: `count` NsMatrix, none of them empty.  muon: p and m are stepped with lr, momentum (nesterov: the gradient looks ahead by it), the
+// table: `count` NsMatrix, none of them empty.  muon: p and m are stepped with lr times `size` sqrt(long side), momentum (nesterov: the gradient looks ahead by it), the
 // gradient times grad_scale, and keep = 1 - lr weight_decay; else the orthogonalised matrices go to `out`.  a, b, c: coefficients.
 int zb_newton_schulz(const void* table, int count, int muon, float lr, float momentum, int nesterov, float keep, float grad_scale, int iterations,
-                     float a, float b, float c, long limit, void* workspace, long bytes, int* launches, int* status, cudaStream_t stream) {
+                     float a, float b, float c, float size, long limit, void* workspace, long bytes, int* launches, int* status, cudaStream_t stream) {
   using namespace zb;
   try {
     const NsMatrix* t = static_cast<const NsMatrix*>(table);
@@ -580,10 +580,10 @@ int zb_newton_schulz(const void* table, int count, int muon, float lr, float mom
       n = ns_together(t + i, count - i, limit);
       const NsPlan plan = ns_plan(t + i, n);
       if (bytes < long(plan.bytes)) ZB_FAIL(-4, "newton_schulz: %ld bytes of workspace, %zu are needed", bytes, plan.bytes);
-      int rc = ns_pass<0>(plan, t + i, pass, lr, ws, NS_X0, false, stream, launches);
-      if (!rc) rc = ns_pass<1>(plan, t + i, pass, lr, ws, NS_X0, ns_keeps_remainder(0, iterations), stream, launches);
+      int rc = ns_pass<0>(plan, t + i, pass, lr * size, ws, NS_X0, false, stream, launches);
+      if (!rc) rc = ns_pass<1>(plan, t + i, pass, lr * size, ws, NS_X0, ns_keeps_remainder(0, iterations), stream, launches);
       if (!rc) rc = ns_products(plan, ws, program, status, stream, launches);
-      if (!rc) rc = ns_pass<2>(plan, t + i, pass, lr, ws, iterations & 1 ? NS_X1 : NS_X0, false, stream, launches);
+      if (!rc) rc = ns_pass<2>(plan, t + i, pass, lr * size, ws, iterations & 1 ? NS_X1 : NS_X0, false, stream, launches);
       if (rc) return rc;
     }
     return 0;

@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 
 from .moments import BLOCK as MOMENT_BLOCK
-from .muon import COEFFICIENTS as NEWTON_SCHULZ
+from .muon import COEFFICIENTS, SCALE
 from .packed import MOST_AXES, MOST_TOKENS, PACK_SCAN, PackedSequences, check_window
 
 _LIB_PATH = Path(__file__).resolve().parents[1] / "_C" / "libzorse_sm100.so"
@@ -57,7 +57,7 @@ _SIGNATURES = {
     "zb_qk_norm_rope_fwd": "ppppppiiiiiillfp", "zb_qk_norm_rope_workspace": "iiiip", "zb_qk_norm_rope_bwd": "pppppppppiiiiillip",
     "zb_embedding_scaled": "ppppiiiiifp", "zb_embedding_by_token_workspace": "iip", "zb_embedding_by_token": "pppppiiiiifip",
     "zb_pack_sequences": "piippppppp", "zb_packed_attn_fwd": "ppppppiiiiiifpp", "zb_packed_attn_bwd": "pppppppppiiiiiifpp",
-    "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pilp", "zb_newton_schulz": "piiffiffiffflplppp",
+    "zb_rope_at": "ppppiiiiilip", "zb_newton_schulz_workspace": "pilp", "zb_newton_schulz": "piiffiffifffflplppp",
     "zb_adamw_list": "piifffffffp", "zb_moment_values": "pppppplip",
 }
 _CTYPES = {"p": c_void_p, "i": c_int, "l": c_long, "f": c_float}
@@ -619,6 +619,7 @@ def moment_values(moments, dtype=torch.float32):
 # Matrices of a list are taken together as far as their workspace (5 bytes an element, 4 a pair of rows of the short side) stays below this:
 # enough tiles for many waves.
 NEWTON_SCHULZ_BYTES = 1 << 30
+NEWTON_SCHULZ = (*COEFFICIENTS, SCALE)
 
 
 def _newton_schulz(table, muon: bool, iterations: int, dev, lr=0.0, momentum=0.0, nesterov=False, keep=1.0, grad_scale=1.0) -> None:
