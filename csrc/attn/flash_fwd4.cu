@@ -615,7 +615,7 @@ extern "C" int zb_packed_attn_fwd(const void* qkv, void* out, float* lse, const 
   using namespace zb;
   if (T <= 0 || Hq <= 0) return 0;
   if (int rc = packed_check(T, Hq, Hkv, D)) return rc;
-  if (D == 64 && Hq / Hkv % 2 == 0)
+  if (D == 64 && Hq / Hkv % 2 == 0 && groups_pay(T, Hq, Hkv))
     return packed_fwd_groups(static_cast<const __nv_bfloat16*>(qkv), static_cast<__nv_bfloat16*>(out), lse, static_cast<const int2*>(bounds),
                              static_cast<const PackedPair*>(order_pairs), static_cast<const PackedTile*>(order_tiles), T, Hq, Hkv, causal,
                              window, softmax_scale * 1.4426950408889634f, status, stream);

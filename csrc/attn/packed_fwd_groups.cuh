@@ -382,6 +382,18 @@ inline int launch_groups(const __nv_bfloat16* qkv, __nv_bfloat16* out, int Hkv, 
   return 0;
 }
 
+// Whether the four chains are the faster form (heads of 64 in even groups); `pairs`: CTAs that the kernel of two chains (flash_fwd4.cu) would have.  Of a
+// CTA by itself the two chains are done 1.3 to 2 times sooner, which decides where all CTAs run at once or one long sequence goes on
+// behind the rest; with several rounds of CTAs the exponential unit decides.  The lengths are not known here, so by `pairs` alone.  us of four
+// chains / two:  groups of 4 and 8, `pairs` of up to 128 12.3 / 10.3 to 30.7 / 20.5; 256 14.6 / 24.6 and 20.5 / 28.7 for documents of 90 and
+// 300 tokens, 30.8 / 36.9 of 700, 65 / 43 and 102 / 60 for one of 2047 and 4096; 512 and more 32.8 / 49.2, 203 / 278, one of 8192 196 / 204 and
+// 366 / 400.  Groups of 2, 6 and 10 (two heads a CTA, so two tiles of rows): `pairs` of 128 36 / 21; 320 and 384 32.8 / 36.9 and 43 / 49, one of 4096
+// 125 / 80 and 125 / 93; 512 37 / 49, one of 4096 124 / 117; 1024 and 2048 86 / 107 and 241 / 278, one of 8192 444 / 400.
+inline bool groups_pay(int T, int Hq, int Hkv) {
+  const long pairs = long(Hq) * ((T + 255) / 256);
+  return pairs > (Hq / Hkv % 4 == 0 ? 1l : 3l) * num_sms();
+}
+
 // Hq / Hkv even; heads of 64.
 inline int packed_fwd_groups(const __nv_bfloat16* qkv, __nv_bfloat16* out, float* lse, const int2* bounds, const PackedPair* pairs,
                       const PackedTile* tiles, int T, int Hq, int Hkv, int causal, int window, float scale_log2, int* status,
