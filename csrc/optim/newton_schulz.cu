@@ -36,7 +36,7 @@ namespace zb {
 constexpr float NS_A_SCALE = 64.f;   // what is n x n is held times this
 
 // --------------------------------------------------------------------------------------------- passes before and behind
-constexpr int NS_MATRICES = 64;      // of a launch of a pass; 12 where there are no more
+constexpr int NS_MATRICES = 64;      // of a launch of a pass
 constexpr int NS_PARTS = 256;        // sums of squares of one matrix, at most
 
 // What a caller hands over for each matrix.
@@ -63,17 +63,15 @@ struct NsPassMatrix {
   int g_f32, wide;        // wide: rows start on 16 bytes in every type
   float scale, step;      // X is held times scale; muon: what the result is multiplied with
 };
-template <int MATRICES>
 struct NsPass {
-  NsPassMatrix t[MATRICES];
+  NsPassMatrix t[NS_MATRICES];
   int count;
   float momentum, grad_scale, keep;
   int nesterov, muon;
   int span;               // tiles of a block that scales
 };
 
-template <int N>
-__device__ __forceinline__ int ns_find(const NsPass<N>& a, int block) {
+__device__ __forceinline__ int ns_find(const NsPass& a, int block) {
   int lo = 0, hi = a.count;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -94,12 +92,10 @@ __device__ __forceinline__ float ns_load1(const void* base, bool f32, size_t at)
   return f32 ? static_cast<const float*>(base)[at] : __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
 }
 // The update from the scaled gradient and the new momentum.
-template <int N>
-__device__ __forceinline__ float ns_update(const NsPass<N>& a, float g, float m) { return a.nesterov ? fmaf(a.momentum, m, g) : m; }
+__device__ __forceinline__ float ns_update(const NsPass& a, float g, float m) { return a.nesterov ? fmaf(a.momentum, m, g) : m; }
 
 // Momentum (written back) and the sum of squares of the update; a block has an equal part of its matrix's elements.
-template <int N>
-__global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ NsPass<N> a) {
+__global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ NsPass a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
@@ -164,10 +160,9 @@ __global__ void __launch_bounds__(256) ns_sums_kernel(const __grid_constant__ Ns
 
 // Tiles of 64 x 64, `span` a block: the update times scale / norm in fp16, turned over where the matrix has more rows than columns.  All of a
 // tile's loads are asked for before the first is used, and a block finds its matrix and factor once for up to four tiles: 101 million
-// elements of 48 matrices (bf16 gradients, 8 bytes an element in all) 227 -> 175 us (198 with one tile a block); with five blocks an SM instead of
-// six 180, with four 205.
-template <int N>
-__global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant__ NsPass<N> a) {
+// elements of 48 matrices (bf16 gradients, 8 bytes an element in all) 227 -> 175 us (198 with one tile a block).  With the remainders, 9 bytes an
+// element, 203 (207 with five blocks an SM instead of six, which spares the 130 bytes that spill, and 228 with four).
+__global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant__ NsPass a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
@@ -243,8 +238,7 @@ __global__ void __launch_bounds__(256, 6) ns_scale_kernel(const __grid_constant_
 }
 
 // Tiles of 64 x 64: the result in bf16, or the step of the parameters.
-template <int N>
-__global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ NsPass<N> a) {
+__global__ void __launch_bounds__(256) ns_apply_kernel(const __grid_constant__ NsPass a) {
   chain_trigger();
   chain_wait();
   const NsPassMatrix& t = a.t[ns_find(a, blockIdx.x)];
@@ -405,7 +399,7 @@ static int ns_products(const NsPlan& plan, char* ws, const std::vector<NsStep>& 
     // the longest reductions first: the last wave of a launch is then of short ones
     std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return plan.shapes[i].cols(e.p) > plan.shapes[j].cols(e.p); });
     for (size_t first = 0; first < order.size(); first += NS_GROUPS) {
-      NsParams<NS_GROUPS> p;
+      NsParams p;
       p.status = status;
       p.groups = p.items = 0;
       for (size_t k = first; k < std::min(first + NS_GROUPS, order.size()); ++k) {
@@ -447,27 +441,10 @@ static int ns_products(const NsPlan& plan, char* ws, const std::vector<NsStep>& 
   return 0;
 }
 
-template <int PASS, int N>
-static int ns_pass_launch(const NsPass<NS_MATRICES>& all, unsigned blocks, cudaStream_t stream) {
-  NsPass<N> a;
-  std::copy(all.t, all.t + all.count, a.t);
-  a.count = all.count;
-  a.momentum = all.momentum;
-  a.grad_scale = all.grad_scale;
-  a.keep = all.keep;
-  a.nesterov = all.nesterov;
-  a.muon = all.muon;
-  a.span = all.span;
-  if (PASS == 0) ZB_CUDA_OK(launch_pass(ns_sums_kernel<N>, dim3(blocks), 256, 0, stream, a));
-  else if (PASS == 1) ZB_CUDA_OK(launch_pass(ns_scale_kernel<N>, dim3(blocks), 256, 0, stream, a));
-  else ZB_CUDA_OK(launch_pass(ns_apply_kernel<N>, dim3(blocks), 256, 0, stream, a));
-  return 0;
-}
-
 // One of the passes over all matrices; PASS 0: sums, 1: scale, 2: apply.
 template <int PASS>
-static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRICES>& common, float step, char* ws, int x, bool remainders, cudaStream_t stream, int* launches) {
-  NsPass<NS_MATRICES> a = common;
+static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, float step, char* ws, int x, bool remainders, cudaStream_t stream, int* launches) {
+  NsPass a = common;
   a.count = 0;
   long all = 0;
   for (const NsShape& s : plan.shapes) all += long(s.members.size()) * ((s.n + 63) / 64) * ((s.m + 63) / 64);
@@ -476,8 +453,8 @@ static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass<NS_MATRIC
   auto flush = [&]() -> int {
     if (a.count == 0) return 0;
     if (blocks > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: %ld blocks", blocks);
-    const int rc = a.count <= 12 ? ns_pass_launch<PASS, 12>(a, unsigned(blocks), stream) : ns_pass_launch<PASS, NS_MATRICES>(a, unsigned(blocks), stream);
-    if (rc) return rc;
+    const auto kernel = PASS == 0 ? ns_sums_kernel : PASS == 1 ? ns_scale_kernel : ns_apply_kernel;
+    ZB_CUDA_OK(launch_pass(kernel, dim3(unsigned(blocks)), 256, 0, stream, a));
     ++*launches;
     a.count = 0;
     blocks = 0;
@@ -568,7 +545,7 @@ int zb_newton_schulz(const void* table, int count, int muon, float lr, float mom
     if (count <= 0) return 0;
     if (int rc = ns_check(t, count)) return rc;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) ZB_FAIL(-4, "newton_schulz: the workspace is not on a 16-byte boundary");
-    NsPass<NS_MATRICES> pass = {};
+    NsPass pass = {};
     pass.momentum = momentum;
     pass.grad_scale = grad_scale;
     pass.keep = keep;

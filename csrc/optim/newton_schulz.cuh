@@ -30,7 +30,8 @@ struct NsCfg {
   static constexpr int BM = 256, BN = 256, BK = 64, HALF_N = 128;
   static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = HALF_N * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
   // Shared memory is split at launch: a second box for each epilogue warp, or a sixth stage for long reductions, under which the
-  // epilogue has time.
+  // epilogue has time.  us with five stages / six, always:  12 matrices of 128 and 512 98.3 / 100.3, 16 of 512 157.7 / 161.6, 16 of 256 x 4096
+  // (reductions of 256 mostly) 331 / 341, 8 of 1024 292 / 289, 4 of 2048 687 / 658, 2 of 4096 2500 / 2420.
   static constexpr int EP_WARPS = 8, BOX_BYTES = 32 * 128, MAX_STAGES = 6;
   static constexpr int RING_BYTES = MAX_STAGES * STAGE_BYTES + EP_WARPS * BOX_BYTES;
   static constexpr int LONG_K = 2048;
@@ -52,9 +53,8 @@ struct alignas(64) NsGroup {
   int rem_rows, rem_cols; // boxes of the remainders of one matrix
   uint8_t* rem;
 };
-template <int GROUPS>      // (a launch with few shapes has few parameters to send: 2 of 8 shapes' 5.6 KB)
 struct NsParams {
-  NsGroup g[GROUPS];
+  NsGroup g[NS_GROUPS];
   int groups, items;
   int stages;             // 6 with one box a warp, 5 with two
   int* status;
@@ -90,8 +90,7 @@ __device__ __forceinline__ float ns_with_remainder(float h, uint32_t word) {
   return __int_as_float(__float_as_int(h) + q * 32);
 }
 
-template <int GROUPS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) newton_schulz_kernel(const __grid_constant__ NsParams<GROUPS> p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) newton_schulz_kernel(const __grid_constant__ NsParams p) {
   using Cfg = NsCfg;
   constexpr int BK = Cfg::BK, BN = Cfg::BN, EP_WARPS = Cfg::EP_WARPS;
   const int STAGES = p.stages, BOXES = Cfg::MAX_STAGES + 1 - STAGES;
@@ -405,22 +404,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NsCfg::THREADS, 1) n
   }
 }
 
-template <int GROUPS>
-inline int ns_launch_few(const NsParams<NS_GROUPS>& all, cudaStream_t stream) {
-  NsParams<GROUPS> p;
-  std::copy(all.g, all.g + all.groups, p.g);
-  p.groups = all.groups;
-  p.items = all.items;
-  p.stages = all.stages;
-  p.status = all.status;
+inline int ns_launch(const NsParams& p, cudaStream_t stream) {
   static SharedLimit limit;
-  ZB_CUDA_OK(limit.raise(newton_schulz_kernel<GROUPS>, NsCfg::SMEM_BYTES));
+  ZB_CUDA_OK(limit.raise(newton_schulz_kernel, NsCfg::SMEM_BYTES));
   const int pairs = std::min(num_sms() / 2, p.items);
-  ZB_CUDA_OK(launch_chained(newton_schulz_kernel<GROUPS>, dim3(2 * pairs), NsCfg::THREADS, NsCfg::SMEM_BYTES, stream, 0, p));
+  ZB_CUDA_OK(launch_chained(newton_schulz_kernel, dim3(2 * pairs), NsCfg::THREADS, NsCfg::SMEM_BYTES, stream, 0, p));
   return 0;
-}
-inline int ns_launch(const NsParams<NS_GROUPS>& p, cudaStream_t stream) {
-  return p.groups <= 2 ? ns_launch_few<2>(p, stream) : ns_launch_few<NS_GROUPS>(p, stream);
 }
 
 }  // namespace zb
