@@ -4,7 +4,8 @@
 //     A = X X^T,   B = b A + c A A,   X <- a X + B X
 // an odd polynomial of the singular values that drives them all towards 1 without an SVD.  Three products an iteration; A and A A
 // are symmetric, so only their tiles on and above the diagonal are formed and every other one is stored a second time, turned
-// over: 2 n^2 m + n^3 / 2 ... n^2 m + n^3 + 2 n^2 m floating-point operations instead of 4 n^2 m + 2 n^3.
+// over: down to 3 n^2 m + n^3 floating-point operations instead of 4 n^2 m + 2 n^3.  (Tiles on the diagonal are formed whole: of t x t tiles, t = n / 256
+// rounded up, t (t + 1) / 2 are formed, all of them for n of up to 256.)
 //
 // Every matrix of the list takes part in each launch: those of one shape lie one behind the other in the workspace under one tensor
 // map, and the tiles of up to GROUPS shapes are dealt to persistent CTA pairs.  A model's matrices of 512 to 1024 columns have 3 to 10
@@ -21,8 +22,8 @@
 // A and B times 64, so that what the first iteration's small values round to stays far below what they add.
 //
 // Around the products: one pass over gradient and momentum with the sum of squares, one that scales, turns and rounds into the
-// workspace, and one that applies the result (momentum and scale come from fp32, sums of squares are held in 64 bits: no gradient is too
-// small or too large for them).
+// workspace, and one that applies the result (momentum and scale come from fp32, sums of squares are held in 64 bits: no normal number of fp32 is too
+// small or too large for them; below those, 1.2e-38, values count as zeros).
 #include "../common/host.h"
 #include "../common/ptx.cuh"
 #include "newton_schulz.cuh"

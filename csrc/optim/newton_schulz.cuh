@@ -12,8 +12,9 @@
 // boxes loaded two at a time and the turned tiles stored from registers a tile took 14 us (26 thousand clocks) to leave, more than the
 // 8 thousand of a reduction of 1024.
 //
-// Bound by the tensor pipe, and under load by the power limit: 4 x 4096 x 4096 and 3 x 4096 x 11008 take 448 us for X X^T (1850 TFLOP/s of the half
-// that is formed), 281 for A A (1710) and 818 for B X (2030) run one by one; 8 blocks of 1024 keep the pipe busy for 85, 67 and 81 %.
+// Bound by the tensor pipe, and under load by the power limit: 4 x 4096 x 4096 and 3 x 4096 x 11008 take 601 us for X X^T (1380 TFLOP/s of the half
+// that is needed), 351 for A A (1370) and 1085 for B X (1530; 1126 with remainders), launch by launch under a profiler; 8 blocks of 1024 keep the pipe
+// busy for 86 and 69 %, and in B X for 81 % without remainders (137 us) and 69 % with them (160 us: the epilogue has twice as many instructions).
 #pragma once
 #include "../common/host.h"
 #include "../common/pair.cuh"

@@ -11,6 +11,10 @@ All math goes through an ops backend (`ops/api.py`): `sm100` kernels or the PyTo
 oracle.  Tensors are `[tokens, features]`; `ctx["B"]`, `ctx["S"]` give the microbatch
 geometry.  `ctx["packed"]` (`ops/packed.py`): its B S tokens are one stream of sequences of different lengths, each of which
 attends to itself alone and counts its positions from 0.
+
+A packed microbatch rounds to bf16 more often than the same sequences as a batch.  The turn by positions is a pass of its own, as the projection's
+epilogue and the head norms take places by t mod S alone: queries and keys are rounded ahead of it and behind it, by half a step (2^-8 of a value)
+twice instead of once, and with head norms their gradients too.  A scaled embedding is rounded before its learned position is added, and after.
 """
 from __future__ import annotations
 

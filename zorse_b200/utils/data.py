@@ -105,7 +105,8 @@ def pack_documents(documents, microbatches: int, B: int, S: int, ignore_index: i
     """A batch for `Trainer.train_step_from_host` from token documents (1-D int64 tensors) of any lengths: inputs and targets [M, B, S] and
     "offsets" [M, n + 1].  Documents lie one after another in each microbatch's B S tokens; one that does not fit goes on in the next
     microbatch as a sequence of its own.  Targets are the document's next tokens; the last token of each part and what is left
-    over are ignored.  Documents that no microbatch has room for are left out."""
+    over are ignored.  Documents that no microbatch has room for are left out.  Loss and gradients are means over all B S places of a microbatch, as
+    they are for batches of equal sequences: ignored ones count as 0, so many short documents and a padded end make both smaller."""
     T = B * S
     x, y = torch.full((microbatches, T), pad, dtype=torch.int64), torch.full((microbatches, T), ignore_index, dtype=torch.int64)
     ends = [[0] for _ in range(microbatches)]
