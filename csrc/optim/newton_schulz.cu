@@ -454,8 +454,10 @@ static int ns_pass(const NsPlan& plan, const NsMatrix* t, const NsPass& common, 
   auto flush = [&]() -> int {
     if (a.count == 0) return 0;
     if (blocks > 0x7fffffffL) ZB_FAIL(-1, "newton_schulz: %ld blocks", blocks);
-    const auto kernel = PASS == 0 ? ns_sums_kernel : PASS == 1 ? ns_scale_kernel : ns_apply_kernel;
-    ZB_CUDA_OK(launch_pass(kernel, dim3(unsigned(blocks)), 256, 0, stream, a));
+    const dim3 grid{unsigned(blocks)};
+    if (PASS == 0) ZB_CUDA_OK(launch_pass(ns_sums_kernel, grid, 256, 0, stream, a));
+    else if (PASS == 1) ZB_CUDA_OK(launch_pass(ns_scale_kernel, grid, 256, 0, stream, a));
+    else ZB_CUDA_OK(launch_pass(ns_apply_kernel, grid, 256, 0, stream, a));
     ++*launches;
     a.count = 0;
     blocks = 0;
