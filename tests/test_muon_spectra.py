@@ -99,3 +99,21 @@ def test_many_shapes_side_by_side(ops):
     shapes = [(33, 70), (70, 33), (64, 64), (31, 65), (257, 130), (5, 700), (33, 70), (1, 3), (96, 1030), (40, 40), (65, 63)]
     mats = [_matrix("r1", *s, seed=i).cuda() for i, s in enumerate(shapes)]
     assert all(torch.equal(x, ops.orthogonalize([u])[0]) for u, x in zip(mats, ops.orthogonalize(mats)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("turned", [False, True])
+def test_remainders_that_pass_32_bits(ops, turned):
+    """A block of rank 1 at the far corner of a matrix of more than 2^31 elements: as exact as by itself."""
+    n, m, k = 40000, 53999, 300
+    shape = (m, n) if turned else (n, m)
+    assert n * m > 2 ** 31
+    block = _matrix("r1", k, k).bfloat16()
+    u = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    u[-k:, -k:] = block.cuda()
+    got = ops.orthogonalize([u])[0]
+    want, bound = exact_and_bound(block.float())
+    off = float((got[-k:, -k:].cpu().double() - want).norm() / want.norm())
+    assert off <= math.hypot(bound, 2.0 ** -8 / math.sqrt(3)), (off, bound)
+    assert int(got.count_nonzero()) == int(got[-k:, -k:].count_nonzero())
+    ops.k.check_status()
