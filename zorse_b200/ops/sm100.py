@@ -862,7 +862,7 @@ def pack_sequences(offsets, T: int) -> PackedSequences:
     return PackedSequences(T, bounds, rest[3], *orders)
 
 
-def _packed_operands(qkv, pk, Hq, Hkv, D, causal, window):
+def _packed_operands(qkv, pk, Hq, Hkv, D, causal, window, scale):
     _bf16(qkv, "qkv")
     _on_current(qkv, "qkv")
     check_window(causal, window)
@@ -873,23 +873,26 @@ def _packed_operands(qkv, pk, Hq, Hkv, D, causal, window):
     _need(0 <= T <= MOST_TOKENS and all(t is not None and t.dtype == torch.int32 and t.is_contiguous() and t.device == qkv.device and t.shape == shape for t, shape in (
         (pk.bounds, (-(-T // 256) * 256, 2)), (pk.order_pairs, (-(-T // 256), 12)), (pk.order_tiles, (-(-T // 128), 8)), (pk.order_keys, (-(-T // 128), 8)))),
         f"the packing is not one of {T} tokens made for {qkv.device} (`pack_sequences`)")
+    # (the kernels keep maxima of the scores as they are and hide by -inf: times 0 that is NaN, and times a negative number the largest)
+    _need(scale is None or 1e-37 <= scale <= 1e37, f"scale {scale}: a positive number, from 1e-37 to 1e37 (a normal one in fp32)")
+    return 1.0 / math.sqrt(D) if scale is None else scale
 
 
 def packed_attn_fwd(qkv, pk: PackedSequences, Hq: int, Hkv: int, D: int, causal: bool = True, window: int = 0, scale: Optional[float] = None):
     """Attention of every token over its own sequence: (out [T, Hq D], lse [Hq, T]).  Tokens of no sequence get zeros and -inf."""
-    _packed_operands(qkv, pk, Hq, Hkv, D, causal, window)
+    scale = _packed_operands(qkv, pk, Hq, Hkv, D, causal, window, scale)
     T = pk.tokens
     out = torch.empty(T, Hq * D, dtype=qkv.dtype, device=qkv.device)
     lse = torch.empty(Hq, T, dtype=torch.float32, device=qkv.device)
     _check(lib().zb_packed_attn_fwd(_a(qkv), _a(out), _a(lse), _a(pk.bounds), _a(pk.order_pairs), _a(pk.order_tiles), T, Hq, Hkv, D, int(causal), _window(window, T),
-                                    1.0 / math.sqrt(D) if scale is None else scale, _a(status_word(qkv.device)), _stream()), "packed_attn_fwd")
+                                    scale, _a(status_word(qkv.device)), _stream()), "packed_attn_fwd")
     return out, lse
 
 
 def packed_attn_bwd(do, qkv, o, lse, pk: PackedSequences, Hq: int, Hkv: int, D: int, causal: bool = True, window: int = 0,
                     scale: Optional[float] = None):
     """Gradient of the packed projection from the output's (o, lse: what the forward pass returned); zeros for tokens of no sequence."""
-    _packed_operands(qkv, pk, Hq, Hkv, D, causal, window)
+    scale = _packed_operands(qkv, pk, Hq, Hkv, D, causal, window, scale)
     _bf16(do, "do"); _bf16(o, "o")
     T = pk.tokens
     _need(do.shape == o.shape == (T, Hq * D) and do.is_contiguous() and o.is_contiguous() and do.device == o.device == qkv.device,
@@ -900,7 +903,7 @@ def packed_attn_bwd(do, qkv, o, lse, pk: PackedSequences, Hq: int, Hkv: int, D: 
     dqkv = torch.empty_like(qkv)
     _check(lib().zb_packed_attn_bwd(_a(do), _a(qkv), _a(o), _a(lse), _a(dqkv), _a(stats), _a(pk.bounds), _a(pk.order_tiles),
                                     _a(pk.order_keys), T, Hq, Hkv, D, int(causal), _window(window, T),
-                                    1.0 / math.sqrt(D) if scale is None else scale, _a(status_word(qkv.device)), _stream()), "packed_attn_bwd")
+                                    scale, _a(status_word(qkv.device)), _stream()), "packed_attn_bwd")
     global _launches
     _launches += 2     # statistics, dQ
     return dqkv
