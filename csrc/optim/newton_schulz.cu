@@ -17,7 +17,7 @@
 // five, so X itself has to be held more exactly than the products read it: eight more bits of it go from product to product beside it
 // (ns_remainders) in all iterations but the last two, into a X alone, since B takes nothing from where X has nothing.  Relative errors (1024 x 1024)
 // without them and with them: rank 1 0.15 and 3.0e-3, 16 0.045 and 2.7e-3, 64 0.024 and 2.6e-3, 256 8.6e-3 and 2.3e-3; singular values as
-// 1 / k 3.7e-3 and 7e-4, 1 / k^2 0.021 and 1.4e-3; noise 1.0e-3 either way.  They cost 3 to 8 % (24 blocks of 1024 6600 -> 6830 us, 16 matrices
+// 1 / k 3.7e-3 and 7e-4, 1 / k^2 0.021 and 1.4e-3; noise 1.0e-3 either way (of a handful of entries, 2 x 2 to 3 x 5, 2e-3 on average and up to 1e-2).  They cost 3 to 8 % (24 blocks of 1024 6600 -> 6830 us, 16 matrices
 // of 512 199 -> 214); more bits of the last two iterations' X would take 1e-3 off ranks below 64.  X is held times 2^round(log2(sqrt m)), so its entries are near 1 at the end,
 // A and B times 64, so that what the first iteration's small values round to stays far below what they add.
 //
